@@ -26,10 +26,14 @@ HEADERS = (os.path.join(CSRC, "mvs_common.h"), os.path.join(CSRC, "sweep_common.
 # -fno-slp-vectorize: v_pk_fma_f32 retires two results in 5-7 cycles (scripts/micro/pk_fma.hip), no
 # faster than two v_fma_f32, and the vectoriser pays for its pairs with register moves (85 per tap
 # iteration of the prob kernel): prob 0.36 -> 0.33 ms, conv9 0.145 -> 0.134 ms without it.
+# -packed-fp32-ops: no v_pk_add / mul / fma_f32 anywhere (hipcc forms them from plain float2 / float4 code even without the SLP
+# vectoriser: 687 of them in sweep, conv_bf16x6, cas_hypo, regress and cvp_glue before the flag).  Some of their forms have given
+# wrong results on MI355X now and then; the scalar forms round alike.  (The host pass warns that it does not know the feature:
+# harmless.)
 # -fvisibility=hidden: only what include/mvs_hip.h (and, tuning build, mvs_hip_tuning.h) declares leaves the library (the
 # mvs:: launchers leaked as 64 extra text symbols)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-ffp-contract=off",
-         "-fno-fast-math", "-fno-slp-vectorize", "-Wall", "-Wno-unused-function"]
+         "-fno-fast-math", "-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function"]
 
 
 # sources compiled WITH the SLP vectoriser (v_pk_fma_f32 / v_pk_mul_f32 pairs); MVS_BUILD_SLP="a,b" overrides for experiments
