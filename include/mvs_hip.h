@@ -91,7 +91,9 @@ extern "C" {
  * 103 (0.1.3): the hand-over of the variance volume as fp16 pieces -- mvs_costvol_variance_fwd_ws3_f32 / _handover_bytes,
  * mvs_conv3d_c8p_f16x3_f32, mvs_conv3d_c8_handed_f16x3_f32, mvs_c8p_bytes, mvs_c8_to_c8p_f32, mvs_conv3d_f16x3_pack_veto_word, mvs_costreg_fwd4_f32; a launch
  * under a run-only-if word that has no kernel honouring it now fails with MVS_EUNSUPPORTED instead of running unconditionally;
- * mvs_costreg_tail_guarded_f16_f32 needs prob's packed weights.  Nothing a 102 caller sized or packed changes. */
+ * mvs_costreg_tail_guarded_f16_f32 needs prob's packed weights.  Nothing a 102 caller sized or packed changes.
+ * 104 (0.1.4): mvs_act8_*, mvs_bn_train_*_act8_f32, mvs_lookup_rows_*, mvs_linear_ce_* added (the training operators at the end of
+ * this file; they take bfloat16 and float16 too).  Nothing a 103 caller sized or packed changes. */
 int mvs_version(void);
 /* Text of the last error on the calling thread ("" if none). */
 const char *mvs_last_error_string(void);
@@ -691,6 +693,60 @@ int mvs_interleave2x2_f32(const float *classes, int N, int H, int W, int C, floa
  * can sit inside a captured HIP graph.  (The eval default evaluates these with the reference's own float32 LAPACK
  * call on the host, stream-ordered.) */
 int mvs_rot_trans_f32(const float *proj_matrices, int B, int V, float *rot_trans, void *stream);
+
+/* ---- training operators that keep no large tensor ------------------------------------------------------------------
+ * Element types of their operands (the entry points above are float32 throughout). */
+#define MVS_DTYPE_F32 0
+#define MVS_DTYPE_BF16 1
+#define MVS_DTYPE_F16 2
+
+/* An activation held in 8 bits for the backward pass.  The n values of a contiguous tensor are cut into blocks of 32 (the last
+ * may be shorter); block b has one power of two 2^k, k the smallest >= -126 with round(max|x| / 2^k) <= 127, stored as
+ * scales[b] = k + 127; a value is codes[i] = round-to-nearest-even(x / 2^k).  A block with an Inf or NaN has scales[b] = 255 and
+ * reads back as NaN throughout.  Reading back: codes[i] * 2^k, at most the largest finite number of the output type.
+ * codes: n bytes, scales: ceil(n / 32) bytes.  The 8-bit form does not depend on the type it was made from. */
+int mvs_act8_quantize(const void *x, int dtype, int64_t n, signed char *codes, unsigned char *scales, void *stream);
+int mvs_act8_dequantize(const signed char *codes, const unsigned char *scales, int64_t n, int dtype, void *out, void *stream);
+/* mvs_bn_train_fwd_groups_f32 that also writes its input in that form, in the pass that writes y, and (relu != 0) the ReLU's mask:
+ * bit i of mask[b] (32-bit words, ceil(G N C / 32) of them; NULL without the ReLU) = the normalised value i of block b is > 0.
+ * The backward pass reads codes, scales and mask where mvs_bn_train_bwd_groups_f32 reads x: the normalised input is that of the
+ * 8-bit form, the mask the forward's own.  x, codes and mask cover the G N rows as one tensor (blocks may span two groups). */
+int mvs_bn_train_fwd_act8_f32(const float *x, const float *weight, const float *bias, const float *skip, int G, int64_t N, int C,
+                              float eps, float momentum, int relu, float *running_mean, float *running_var,
+                              long long *num_batches_tracked, float *save_mean, float *save_invstd, float *y,
+                              signed char *codes, unsigned char *scales, unsigned *mask, void *workspace,
+                              size_t workspace_bytes, void *stream);
+int mvs_bn_train_bwd_act8_f32(const float *grad_y, const signed char *codes, const unsigned char *scales, const unsigned *mask,
+                              const float *weight, const float *save_mean, const float *save_invstd, int G, int64_t N, int C,
+                              float *grad_x, float *grad_weight, float *grad_bias, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
+/* Rows of a table by index, times `scale`: out[i] = scale * table[index[i]], computed in float32 and rounded once.  table
+ * [rows, C], out [n, C] contiguous, of one type; index int64.  An index outside [0, rows) names no row: out[i] = 0 and no
+ * gradient.  The gradient (grad_table overwritten) is summed in float32 in the order of i -- the indices are sorted, stably, in
+ * the workspace; no atomics, so equal calls give equal bits. */
+int mvs_lookup_rows_fwd(const void *table, int dtype, int64_t rows, int C, const int64_t *index, int64_t n, float scale, void *out,
+                        void *stream);
+size_t mvs_lookup_rows_workspace_bytes(int64_t rows, int C, int64_t n);
+int mvs_lookup_rows_bwd(const void *grad_out, int dtype, const int64_t *index, int64_t n, int64_t rows, int C, float scale,
+                        void *grad_table, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Softmax cross entropy of n rows against a table of V rows without the logits: l[i][v] = scale * <x[i], weight[v]>,
+ * loss_i = logsumexp_v l[i][v] - l[i][target[i]].  x [n, C], weight [V, C] contiguous, of one type, 16-byte aligned; target int64.
+ * A row whose target is ignore_index has loss 0 and no gradient, whatever x holds there; a target outside [0, V) otherwise makes
+ * the row's loss NaN.  Products are summed in float32 (float32 operands: on the float32 matrix pipe), losses are float32.
+ * reduction: 0 none (loss [n]), 1 mean over the rows kept (0 / 0 = NaN if there are none; gradients are then zero), 2 sum.
+ * lse [n] and kept [1] (the number of rows kept, as a float) are for the backward pass.
+ * Backward: grad_loss [n] (reduction 0) or [1]; grad_x [n, C] and grad_weight [V, C] in the operands' type, either may be NULL.
+ * The logits are formed again, a piece of the table at a time; the workspace (mvs_linear_ce_workspace_bytes; backward != 0 for
+ * the backward pass, with need_x / need_w for the gradients asked for) holds a piece's gradient and no more. */
+size_t mvs_linear_ce_workspace_bytes(int64_t n, int64_t V, int C, int dtype, int backward, int need_x, int need_w);
+int mvs_linear_ce_fwd(const void *x, const void *weight, int dtype, const int64_t *target, int64_t n, int64_t V, int C, float scale,
+                      int64_t ignore_index, int reduction, float *loss, float *lse, float *kept, void *workspace,
+                      size_t workspace_bytes, void *stream);
+int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, const int64_t *target, const float *lse, const float *kept,
+                      const float *grad_loss, int64_t n, int64_t V, int C, float scale, int64_t ignore_index, int reduction,
+                      void *grad_x, void *grad_weight, void *workspace, size_t workspace_bytes, void *stream);
 
 #if defined(__GNUC__) || defined(__clang__)
 #pragma GCC visibility pop

@@ -23,6 +23,11 @@ MVS_LAYOUT_C8P = 6
 MVS_LAYOUT_C8PT = 7
 MVS_LAYOUT_C8PH = 8
 
+MVS_DTYPE_F32 = 0
+MVS_DTYPE_BF16 = 1
+MVS_DTYPE_F16 = 2
+DTYPES = {torch.float32: MVS_DTYPE_F32, torch.bfloat16: MVS_DTYPE_BF16, torch.float16: MVS_DTYPE_F16}
+
 _c_f = ctypes.c_void_p   # device pointers travel as integers
 _c_i = ctypes.c_int
 _c_l = ctypes.c_int64
@@ -139,6 +144,19 @@ _SIGS = {
     "mvs_conv2d_supported": (_c_i, [_c_i] * 4),
     "mvs_softmax_regress_conf_f32": (_c_i, [_c_f, _c_f] + [_c_i] * 6 + [_c_f] * 4),
     "mvs_softmax_regress_bwd_f32": (_c_i, [_c_f, _c_f, _c_i, _c_f] + [_c_i] * 4 + [_c_f, _c_f]),
+    "mvs_act8_quantize": (_c_i, [_c_f, _c_i, _c_l, _c_f, _c_f, _c_f]),
+    "mvs_act8_dequantize": (_c_i, [_c_f, _c_f, _c_l, _c_i, _c_f, _c_f]),
+    "mvs_bn_train_fwd_act8_f32": (_c_i, [_c_f] * 4 + [_c_i, _c_l, _c_i, ctypes.c_float, ctypes.c_float, _c_i] + [_c_f] * 10
+                                  + [ctypes.c_size_t, _c_f]),
+    "mvs_bn_train_bwd_act8_f32": (_c_i, [_c_f] * 7 + [_c_i, _c_l, _c_i] + [_c_f] * 4 + [ctypes.c_size_t, _c_f]),
+    "mvs_lookup_rows_fwd": (_c_i, [_c_f, _c_i, _c_l, _c_i, _c_f, _c_l, ctypes.c_float, _c_f, _c_f]),
+    "mvs_lookup_rows_workspace_bytes": (ctypes.c_size_t, [_c_l, _c_i, _c_l]),
+    "mvs_lookup_rows_bwd": (_c_i, [_c_f, _c_i, _c_f, _c_l, _c_l, _c_i, ctypes.c_float, _c_f, _c_f, ctypes.c_size_t, _c_f]),
+    "mvs_linear_ce_workspace_bytes": (ctypes.c_size_t, [_c_l, _c_l] + [_c_i] * 5),
+    "mvs_linear_ce_fwd": (_c_i, [_c_f, _c_f, _c_i, _c_f, _c_l, _c_l, _c_i, ctypes.c_float, _c_l, _c_i] + [_c_f] * 4
+                          + [ctypes.c_size_t, _c_f]),
+    "mvs_linear_ce_bwd": (_c_i, [_c_f, _c_f, _c_i] + [_c_f] * 4 + [_c_l, _c_l, _c_i, ctypes.c_float, _c_l, _c_i] + [_c_f] * 3
+                          + [ctypes.c_size_t, _c_f]),
 }
 
 # only in the tuning build (include/mvs_hip_tuning.h; MVS_HIP_TUNING=1 loads libmvs_hip_tuning.so)
@@ -214,6 +232,17 @@ def ptr(t):
         raise MvsHipError("mvs_amd ops need device (HIP) tensors; got a CPU tensor")
     if t.dtype != torch.float32 or not t.is_contiguous():
         raise MvsHipError(f"expected contiguous float32, got {t.dtype} contiguous={t.is_contiguous()}")
+    return any_ptr(t)
+
+
+def any_ptr(t):
+    """Device pointer of a contiguous tensor of any type on the current device, or None (the caller has checked its type)."""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise MvsHipError("mvs_amd ops need device (HIP) tensors; got a CPU tensor")
+    if not t.is_contiguous():
+        raise MvsHipError("expected a contiguous tensor")
     if t.device.index != torch.cuda.current_device():
         # kernels launch on the CURRENT device and its current stream (stream() below): a tensor
         # of another GPU would be dereferenced there.  nn.DataParallel sets the device per replica.

@@ -10,7 +10,15 @@
 // The ReLU mask is recomputed from x (z = bn(x) > 0), so neither z nor the mask is stored.
 // Per-channel sums are carried in fp64 (per thread, per block and across blocks): var =
 // E[x^2] - mean^2 is then safe at N ~ 4e6, and the result does not depend on the grid.
-#include "mvs_common.h"
+//
+// HELD (mvs_bn_train_*_act8_f32): the backward pass has x in 8 bits (act8.h) and the ReLU's mask as a bit per value.  The apply
+// pass of the forward writes both while it has x in registers: 1.16 bytes kept per value instead of 4, and the backward's two
+// passes read 1.16 + 4 bytes instead of 8.  The mask is the forward's own, not recomputed from the codes: within half a step of
+// the corner the codes do not know the sign, and a wrong mask bit costs the gradient its whole value there, where a rounded
+// x costs it a part in 250 of the projection term only.
+#include <initializer_list>
+
+#include "act8.h"
 
 namespace mvs {
 
@@ -28,12 +36,24 @@ struct BnArgs {
     // view (mvsnet.py:146), so a batch of views [V*B, h, w, C] is V groups; blockIdx.y = group; mean / invstd / coef are
     // [G][C] / [G][2][C], partial is [G][gridDim.x][2][C]
     int G;
+    // HELD: written by the forward's apply pass, read by the backward in place of x
+    signed char *codes;
+    unsigned char *scales;
+    unsigned *mask;                  // NULL: no ReLU
 };
+
+// x of float4 element e, from its codes; `keep`: the four mask bits
+__device__ __forceinline__ float4 held4(const BnArgs &a, int64_t e, unsigned &keep) {
+    const unsigned q = reinterpret_cast<const unsigned *>(a.codes)[e];
+    const float step = act8_step(a.scales[e >> 3]);
+    keep = a.mask ? a.mask[e >> 3] >> (unsigned)(4 * (e & 7)) : 15u;
+    return make_float4(act8_value(q, 0, step), act8_value(q, 1, step), act8_value(q, 2, step), act8_value(q, 3, step));
+}
 
 __device__ __forceinline__ float4 ld4(const float *p, int64_t e) { return reinterpret_cast<const float4 *>(p)[e]; }
 
 // MODE 0: sum x, sum x^2.  MODE 1: sum dz, sum dz (x - mean), dz = dy masked by z > 0.
-template <int MODE>
+template <int MODE, bool HELD = false>
 __global__ __launch_bounds__(256) void bn_reduce_kernel(BnArgs a) {
     __shared__ double red[8][256];
     const int Q = a.C >> 2, tid = threadIdx.x, q = tid % Q, grp = blockIdx.y;
@@ -43,7 +63,7 @@ __global__ __launch_bounds__(256) void bn_reduce_kernel(BnArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             mean[j] = a.mean[grp * a.C + q * 4 + j]; istd[j] = a.invstd[grp * a.C + q * 4 + j];
-            w[j] = a.weight[q * 4 + j]; b[j] = a.bias[q * 4 + j];
+            if (!HELD) { w[j] = a.weight[q * 4 + j]; b[j] = a.bias[q * 4 + j]; }
         }
     }
     double s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
@@ -54,13 +74,14 @@ __global__ __launch_bounds__(256) void bn_reduce_kernel(BnArgs a) {
     constexpr int U = 4;
     for (int64_t el = (int64_t)blockIdx.x * 256 + tid; el < a.nq; el += step * U) {
         float4 xv[U], gv[U];
+        unsigned keep[U];
         bool ok[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t eu = el + u * step;
             ok[u] = eu < a.nq;
             const int64_t e = g0 + (ok[u] ? eu : el);
-            xv[u] = ld4(a.x, e);
+            xv[u] = HELD ? held4(a, e, keep[u]) : ld4(a.x, e);
             if (MODE == 1) gv[u] = ld4(a.dy, e);
         }
 #pragma unroll
@@ -76,7 +97,7 @@ __global__ __launch_bounds__(256) void bn_reduce_kernel(BnArgs a) {
                 for (int j = 0; j < 4; ++j) {
                     const float xm = xs[j] - mean[j];
                     const float z = xm * istd[j] * w[j] + b[j];
-                    const float dz = (a.relu && !(z > 0.0f)) ? 0.0f : gs[j];
+                    const float dz = (HELD ? !(keep[u] >> j & 1) : (a.relu && !(z > 0.0f))) ? 0.0f : gs[j];
                     s0[j] += (double)dz; s1[j] += (double)dz * (double)xm;
                 }
             }
@@ -146,7 +167,7 @@ __global__ __launch_bounds__(1024) void bn_finalize_kernel(const double *__restr
 
 // MODE 0: y = relu((x - mean) invstd w + b) [+ skip].
 // MODE 1: dx = (dz - k2 - (x - mean) k1) invstd w.
-template <int MODE>
+template <int MODE, bool HELD = false>
 __global__ __launch_bounds__(256) void bn_apply_kernel(BnArgs a) {
     const int Q = a.C >> 2, tid = threadIdx.x, q = tid % Q, grp = blockIdx.y;
     const int64_t g0 = (int64_t)grp * a.nq;
@@ -154,14 +175,15 @@ __global__ __launch_bounds__(256) void bn_apply_kernel(BnArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = q * 4 + j;
-        mean[j] = a.mean[grp * a.C + c]; istd[j] = a.invstd[grp * a.C + c]; w[j] = a.weight[c]; b[j] = a.bias[c];
+        mean[j] = a.mean[grp * a.C + c]; istd[j] = a.invstd[grp * a.C + c]; w[j] = a.weight[c]; b[j] = HELD ? 0.f : a.bias[c];
         k1[j] = MODE == 1 ? a.coef[(grp * 2 + 0) * a.C + c] : 0.f;
         k2[j] = MODE == 1 ? a.coef[(grp * 2 + 1) * a.C + c] : 0.f;
     }
     const int64_t step = (int64_t)gridDim.x * 256;
     for (int64_t el = (int64_t)blockIdx.x * 256 + tid; el < a.nq; el += step) {
         const int64_t e = g0 + el;
-        const float4 xv = ld4(a.x, e);
+        unsigned keep = 15u;
+        const float4 xv = HELD ? held4(a, e, keep) : ld4(a.x, e);
         const float xs[4] = {xv.x, xv.y, xv.z, xv.w};
         float o[4];
         if (MODE == 0) {
@@ -181,11 +203,80 @@ __global__ __launch_bounds__(256) void bn_apply_kernel(BnArgs a) {
             for (int j = 0; j < 4; ++j) {
                 const float xm = xs[j] - mean[j];
                 const float z = xm * istd[j] * w[j] + b[j];
-                const float dz = (a.relu && !(z > 0.0f)) ? 0.0f : gs[j];
+                const float dz = (HELD ? !(keep >> j & 1) : (a.relu && !(z > 0.0f))) ? 0.0f : gs[j];
                 o[j] = (dz - k2[j] - xm * k1[j]) * istd[j] * w[j];
             }
         }
         reinterpret_cast<float4 *>(a.out)[e] = make_float4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+// The forward's apply pass that also writes the checkpoint.  Blocks of 32 values are cut across the whole tensor, so a block may
+// span two groups (N * C not a multiple of 32): the pass runs over all groups' float4 elements as one range, 8 lanes per block,
+// and a lane takes the statistics of the group its element is in.
+template <bool GROUPS>
+__global__ __launch_bounds__(256) void bn_apply_act8_kernel(BnArgs a) {
+    constexpr int U = 4;
+    const int Q = a.C >> 2, tid = threadIdx.x, c0 = tid % Q * 4;      // (256 and the groups' sizes are multiples of Q)
+    const float4 w = *reinterpret_cast<const float4 *>(a.weight + c0), b = *reinterpret_cast<const float4 *>(a.bias + c0);
+    const int64_t total = a.nq * a.G;
+    for (int64_t base = (int64_t)blockIdx.x * 256 * U; base < total; base += (int64_t)gridDim.x * 256 * U) {
+        int grp = 0;
+        int64_t next = a.nq;                                            // first element of the group behind `grp`
+        if (GROUPS) { grp = (int)((base + tid) / a.nq); next = (grp + 1) * a.nq; }
+        float4 mean = make_float4(0, 0, 0, 0), istd = mean;
+        if (grp < a.G) {
+            mean = *reinterpret_cast<const float4 *>(a.mean + grp * a.C + c0);
+            istd = *reinterpret_cast<const float4 *>(a.invstd + grp * a.C + c0);
+        }
+        float4 xv[U], sv[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t e = base + u * 256 + tid;
+            if (e < total) {
+                xv[u] = ld4(a.x, e);
+                if (a.skip) sv[u] = ld4(a.skip, e);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t e = base + u * 256 + tid;
+            const bool here = e < total;
+            if (GROUPS && here && e >= next) {
+                while (e >= next) { ++grp; next += a.nq; }
+                mean = *reinterpret_cast<const float4 *>(a.mean + grp * a.C + c0);
+                istd = *reinterpret_cast<const float4 *>(a.invstd + grp * a.C + c0);
+            }
+            const float xs[4] = {here ? xv[u].x : 0.f, here ? xv[u].y : 0.f, here ? xv[u].z : 0.f, here ? xv[u].w : 0.f};
+            const float ms[4] = {mean.x, mean.y, mean.z, mean.w}, is[4] = {istd.x, istd.y, istd.z, istd.w};
+            const float ws[4] = {w.x, w.y, w.z, w.w}, bs[4] = {b.x, b.y, b.z, b.w};
+            unsigned amax = 0, keep = 0;
+            float o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                amax = max(amax, __float_as_uint(xs[j]) & 0x7fffffffu);
+                const float z = (xs[j] - ms[j]) * is[j] * ws[j] + bs[j];
+                o[j] = (a.relu && z <= 0.0f) ? 0.0f : z;
+                if (here && z > 0.0f) keep |= 1u << j;
+            }
+            keep <<= 4 * (tid & 7);
+#pragma unroll
+            for (int s = 1; s < 8; s <<= 1) {
+                amax = umax_xor(amax, s);
+                keep |= (unsigned)__shfl_xor((int)keep, s);
+            }
+            if (!here) continue;
+            const unsigned byte = act8_scale_byte(amax);
+            const float inv = byte == kAct8Nan ? 0.0f : act8_inverse(byte);
+            reinterpret_cast<unsigned *>(a.codes)[e] =
+                byte == kAct8Nan ? 0u : act8_pack4(act8_code(xs[0], inv), act8_code(xs[1], inv), act8_code(xs[2], inv), act8_code(xs[3], inv));
+            if ((tid & 7) == 0) {
+                a.scales[e >> 3] = (unsigned char)byte;
+                if (a.mask) a.mask[e >> 3] = keep;
+            }
+            if (a.skip) { o[0] += sv[u].x; o[1] += sv[u].y; o[2] += sv[u].z; o[3] += sv[u].w; }
+            reinterpret_cast<float4 *>(a.out)[e] = make_float4(o[0], o[1], o[2], o[3]);
+        }
     }
 }
 
@@ -281,4 +372,84 @@ extern "C" int mvs_bn_train_bwd_f32(const float *grad_y, const float *x, const f
                                     size_t workspace_bytes, void *stream) {
     return mvs_bn_train_bwd_groups_f32(grad_y, x, weight, bias, save_mean, save_invstd, 1, N, C, relu, grad_x, grad_weight,
                                        grad_bias, workspace, workspace_bytes, stream);
+}
+
+static bool bn_aligned16(std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if (reinterpret_cast<uintptr_t>(p) & 15) return false;
+    return true;
+}
+
+extern "C" int mvs_bn_train_fwd_act8_f32(const float *x, const float *weight, const float *bias, const float *skip, int G, int64_t N,
+                                         int C, float eps, float momentum, int relu, float *running_mean, float *running_var,
+                                         long long *num_batches_tracked, float *save_mean, float *save_invstd, float *y,
+                                         signed char *codes, unsigned char *scales, unsigned *mask, void *workspace,
+                                         size_t workspace_bytes, void *stream) {
+    if (!x || !weight || !bias || !save_mean || !save_invstd || !y || !codes || !scales || (relu != 0) != (mask != nullptr) || !workspace ||
+        N <= 0 || G < 1 || G > kBnMaxGroups) {
+        set_error("mvs_bn_train_fwd_act8_f32: invalid argument (1 <= groups <= %d, a mask with the ReLU and only then)", kBnMaxGroups);
+        return MVS_EINVAL;
+    }
+    if (!bn_channels_ok(C)) {
+        set_error("mvs_bn_train_fwd_act8_f32: C=%d (channels-last rows of 8, 16, 32 or 64)", C);
+        return MVS_EUNSUPPORTED;
+    }
+    if (!bn_aligned16({x, weight, bias, skip, save_mean, save_invstd, y, codes, mask})) {
+        set_error("mvs_bn_train_fwd_act8_f32: the tensors are to be aligned to 16 bytes");
+        return MVS_EINVAL;
+    }
+    if (workspace_bytes < mvs_bn_train_workspace_bytes(C)) {
+        set_error("mvs_bn_train_fwd_act8_f32: workspace too small");
+        return MVS_EWORKSPACE;
+    }
+    hipStream_t st = as_stream(stream);
+    BnArgs a = {};
+    a.x = x; a.skip = skip; a.weight = weight; a.bias = bias; a.mean = save_mean; a.invstd = save_invstd;
+    a.out = y; a.partial = static_cast<double *>(workspace); a.nq = N * (C / 4); a.C = C; a.relu = relu; a.G = G;
+    a.codes = codes; a.scales = scales; a.mask = mask;
+    const unsigned g = bn_grid(a.nq, G);
+    hipLaunchKernelGGL((bn_reduce_kernel<0>), dim3(g, G), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((bn_finalize_kernel<0>), dim3(1), dim3(1024), 0, st, a.partial, (int)g, C, G, (double)N, eps,
+                       momentum, (const float *)nullptr, save_mean, save_invstd, running_mean, running_var,
+                       num_batches_tracked);
+    const unsigned ga = (unsigned)min((int64_t)8 * kBnBlocks, (a.nq * G + 1023) / 1024);
+    if (G > 1) hipLaunchKernelGGL((bn_apply_act8_kernel<true>), dim3(ga), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((bn_apply_act8_kernel<false>), dim3(ga), dim3(256), 0, st, a);
+    return check_launch("mvs_bn_train_fwd_act8_f32");
+}
+
+extern "C" int mvs_bn_train_bwd_act8_f32(const float *grad_y, const signed char *codes, const unsigned char *scales, const unsigned *mask,
+                                         const float *weight, const float *save_mean, const float *save_invstd, int G, int64_t N, int C,
+                                         float *grad_x, float *grad_weight, float *grad_bias, void *workspace,
+                                         size_t workspace_bytes, void *stream) {
+    if (!grad_y || !codes || !scales || !weight || !save_mean || !save_invstd || !grad_x || !grad_weight || !grad_bias || !workspace ||
+        N <= 0 || G < 1 || G > kBnMaxGroups) {
+        set_error("mvs_bn_train_bwd_act8_f32: invalid argument (1 <= groups <= %d)", kBnMaxGroups);
+        return MVS_EINVAL;
+    }
+    if (!bn_channels_ok(C)) {
+        set_error("mvs_bn_train_bwd_act8_f32: C=%d (channels-last rows of 8, 16, 32 or 64)", C);
+        return MVS_EUNSUPPORTED;
+    }
+    if (!bn_aligned16({grad_y, codes, mask, grad_x})) {
+        set_error("mvs_bn_train_bwd_act8_f32: the tensors are to be aligned to 16 bytes");
+        return MVS_EINVAL;
+    }
+    if (workspace_bytes < mvs_bn_train_workspace_bytes(C)) {
+        set_error("mvs_bn_train_bwd_act8_f32: workspace too small");
+        return MVS_EWORKSPACE;
+    }
+    hipStream_t st = as_stream(stream);
+    BnArgs a = {};
+    a.dy = grad_y; a.weight = weight; a.mean = save_mean; a.invstd = save_invstd;
+    a.out = grad_x; a.partial = static_cast<double *>(workspace); a.nq = N * (C / 4); a.C = C; a.G = G;
+    a.codes = const_cast<signed char *>(codes); a.scales = const_cast<unsigned char *>(scales); a.mask = const_cast<unsigned *>(mask);
+    float *coef = reinterpret_cast<float *>(a.partial + (size_t)kBnBlocks * 2 * C);
+    a.coef = coef;
+    const unsigned g = bn_grid(a.nq, G);
+    hipLaunchKernelGGL((bn_reduce_kernel<1, true>), dim3(g, G), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((bn_finalize_kernel<1>), dim3(1), dim3(1024), 0, st, a.partial, (int)g, C, G, (double)N, 0.f, 0.f,
+                       save_invstd, grad_weight, grad_bias, coef, (float *)nullptr, (long long *)nullptr);
+    hipLaunchKernelGGL((bn_apply_kernel<1, true>), dim3(4 * g, G), dim3(256), 0, st, a);
+    return check_launch("mvs_bn_train_bwd_act8_f32");
 }

@@ -137,8 +137,8 @@ static int launch_transpose(const float *in, float *out, int B, int R, int64_t S
 using namespace mvs;
 
 // the changelog is in include/mvs_hip.h above mvs_version(): 0.1.1 re-query the *_f16*_packed_bytes sizes, 0.1.2 re-query
-// mvs_costreg_workspace_bytes, 0.1.3 the hand-over entry points
-extern "C" int mvs_version(void) { return 103; /* 0.1.3 */ }
+// mvs_costreg_workspace_bytes, 0.1.3 the hand-over entry points, 0.1.4 the training operators that keep no large tensor
+extern "C" int mvs_version(void) { return 104; /* 0.1.4 */ }
 extern "C" const char *mvs_last_error_string(void) { return g_err; }
 extern "C" const char *mvs_arch(void) { return "gfx950"; }
 

@@ -1,0 +1,47 @@
+// Element types of the entry points that take more than float32 (MVS_DTYPE_*): widened to float, rounded to nearest even once.
+#pragma once
+#include "mvs_common.h"
+
+namespace mvs {
+
+struct bf16_t { unsigned short bits; };
+struct f16_t { _Float16 v; };
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(bf16_t x) { return __uint_as_float((unsigned)x.bits << 16); }
+__device__ __forceinline__ float to_float(f16_t x) { return (float)x.v; }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16_t from_float<bf16_t>(float x) {
+    const __bf16 b = (__bf16)x;      // (v_cvt_pk_bf16_f32: nearest even, NaN stays one)
+    return bf16_t{__builtin_bit_cast(unsigned short, b)};
+}
+template <>
+__device__ __forceinline__ f16_t from_float<f16_t>(float x) { return f16_t{(_Float16)x}; }
+
+// largest finite value of a type
+template <typename T> struct DtypeMax;
+template <> struct DtypeMax<float> { static constexpr float value = 3.4028234663852886e38f; };
+template <> struct DtypeMax<bf16_t> { static constexpr float value = 3.3895313892515355e38f; };
+template <> struct DtypeMax<f16_t> { static constexpr float value = 65504.0f; };
+
+// VEC elements moved as one access
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
+
+inline size_t dtype_size(int dtype) { return dtype == MVS_DTYPE_F32 ? 4 : (dtype == MVS_DTYPE_BF16 || dtype == MVS_DTYPE_F16) ? 2 : 0; }
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace mvs
+
+// f(T()) for the element type that `dtype` names; `dtype` has been checked
+#define MVS_DTYPE_DISPATCH(dtype, T, ...)                                   \
+    do {                                                                    \
+        if ((dtype) == MVS_DTYPE_F32) { using T = float; __VA_ARGS__; }     \
+        else if ((dtype) == MVS_DTYPE_BF16) { using T = mvs::bf16_t; __VA_ARGS__; } \
+        else { using T = mvs::f16_t; __VA_ARGS__; }                         \
+    } while (0)

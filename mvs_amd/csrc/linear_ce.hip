@@ -1,0 +1,669 @@
+// Softmax cross entropy of rows against a large table, without the logits:  l = scale x W^T,  loss_n = lse(l_n) - l_n[t_n].
+//
+//   forward    a tile of logits lives in the matrix cores' accumulators and leaves as one (max, sum of exponentials) per row and
+//              tile; a second launch joins a row's tiles.  2 N V C operations, (N + V) C elements read.
+//   backward   dl = (p - 1[t]) g needs the logits again: a piece of the table at a time (N * piece <= 2^26, so that what it writes
+//              stays in the last-level cache), one launch forms the tile's logits once more and writes dl and its transpose,
+//              rounded to the operands' type; two products follow, dx += dl W and dW = dl^T x.  6 N V C operations: 8 in all, of
+//              which 6 are the definition's and 2 buy the N V logits not being kept.
+//
+// All four products are one kernel shape: C[m][n] = sum_k A[m][k] B[n][k] with both operands contiguous along k -- x, W, dl and dl^T
+// are so by themselves, W^T and x^T are written by a transposing pass (W piece by piece).  A workgroup owns a BM x BN tile and
+// walks k in 128-byte steps: rows of both operands go from memory to LDS by DMA, two stages, the 16-byte chunks of a row exchanged by
+// its low three bits (chunk ^ row & 7) so that the fragment reads of 16 rows spread over the banks; a lane's 16-byte chunk is one
+// 16x16x32 fragment (16 bits) or four 16x16x4 ones (float32: lane group g holds k = 4 g + j for the j-th, on both sides).
+// m runs over table rows or channels, n over the rows of x or of W: a lane of the accumulator then holds four consecutive m of one
+// n, so a row's softmax statistics reduce within the lane first, and results leave as vectors.
+//
+// Numbers: sums, statistics and exponentials in float32, exponents in base 2 (one rounding of scale * log2 e per logit, the same
+// one in both passes, so a row's p sum to one).  16-bit dl: float16 carries it times 2^14 (|p - 1| <= 1: no overflow, and p down to
+// 4e-9 keeps a normal number's precision), the row's gradient factor is applied after the product in float32 (dx) or, relative to
+// the largest one, before the rounding (dW) -- 1 / N of a mean never reaches a 16-bit number.
+#include <type_traits>
+
+#include "dtype.h"
+
+namespace mvs {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kRowBytes = 128;                  // bytes of k per stage and row
+
+__device__ __forceinline__ void mma16(f32x4_t &c, u32x4_t a, u32x4_t b, float) {
+    const f32x4_t fa = __builtin_bit_cast(f32x4_t, a), fb = __builtin_bit_cast(f32x4_t, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[j], fb[j], c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(f32x4_t &c, u32x4_t a, u32x4_t b, bf16_t) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(f32x4_t &c, u32x4_t a, u32x4_t b, f16_t) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// dl is carried times this
+template <typename T> struct GradUnit { static constexpr float value = 1.0f; };
+template <> struct GradUnit<f16_t> { static constexpr float value = 16384.0f; };
+
+// One operand of a product: rows of `ld` bytes, the last of them `rows - 1` (a tile's rows beyond it read that one again)
+struct Operand {
+    const char *p;
+    int64_t ld, rows;
+};
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct Tile {
+    static constexpr int BM = BM_, BN = BN_, WAVES_M = WM_, WAVES_N = WN_, WAVES = WM_ * WN_, THREADS = 64 * WAVES;
+    static constexpr int TM = BM / WAVES_M / 16, TN = BN / WAVES_N / 16;
+    static constexpr int STAGE = (BM + BN) * kRowBytes;
+    static constexpr int COPIES = (BM + BN) / 8;                 // wave-wide copies of 8 rows
+    static constexpr int PER_WAVE = (COPIES + WAVES - 1) / WAVES;
+    static_assert(COPIES % WAVES == 0 || COPIES < WAVES || PER_WAVE > 0, "");
+};
+
+// acc[tm][tn] += the tile (m0, n0) of A B^T over `steps` 128-byte steps of k
+template <typename T, typename X>
+__device__ __forceinline__ void tile_product(const Operand &a, const Operand &b, int64_t m0, int64_t n0, int64_t k_byte0, int steps, char *lds,
+                                             f32x4_t (&acc)[X::TM][X::TN]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
+    const unsigned lds_base = (unsigned)(uintptr_t)lds;
+    // copy c moves the tile rows 8 c .. 8 c + 7 (A's, then B's): lane i = row 8 c + i / 8, LDS chunk i % 8
+    const int r8 = lane >> 3, chunk = (lane & 7) ^ r8;
+    const char *from[X::PER_WAVE];
+#pragma unroll
+    for (int i = 0; i < X::PER_WAVE; ++i) {
+        const int c = wave + i * X::WAVES;
+        const bool of_a = c < X::BM / 8;
+        const int64_t row = of_a ? m0 + c * 8 + r8 : n0 + (c - X::BM / 8) * 8 + r8;
+        const Operand &o = of_a ? a : b;
+        from[i] = o.p + (row < o.rows ? row : o.rows - 1) * o.ld + k_byte0 + chunk * 16;
+    }
+    auto copy = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < X::PER_WAVE; ++i) {
+            const int c = wave + i * X::WAVES;
+            if (X::COPIES % X::WAVES == 0 || c < X::COPIES) {
+                glds16(from[i], lds_base + (unsigned)(stage * X::STAGE + c * 1024));
+                from[i] += kRowBytes;
+            }
+        }
+    };
+    const int frow = lane & 15, fk = lane >> 4;
+    const int swz0 = (fk ^ (frow & 7)) * 16, swz1 = ((4 + fk) ^ (frow & 7)) * 16;
+    const int a_row = (wm * (X::BM / X::WAVES_M) + frow) * kRowBytes, b_row = (X::BM + wn * (X::BN / X::WAVES_N) + frow) * kRowBytes;
+    copy(0);
+    for (int s = 0; s < steps; ++s) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                         // stage s has landed for everybody, and nobody reads the other one any more
+        if (s + 1 < steps) copy((s + 1) & 1);
+        const char *stage = lds + (s & 1) * X::STAGE;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int swz = half ? swz1 : swz0;
+            u32x4_t fa[X::TM], fb[X::TN];
+#pragma unroll
+            for (int i = 0; i < X::TM; ++i) fa[i] = *reinterpret_cast<const u32x4_t *>(stage + a_row + i * 16 * kRowBytes + swz);
+#pragma unroll
+            for (int j = 0; j < X::TN; ++j) fb[j] = *reinterpret_cast<const u32x4_t *>(stage + b_row + j * 16 * kRowBytes + swz);
+#pragma unroll
+            for (int i = 0; i < X::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < X::TN; ++j) mma16(acc[i][j], fa[i], fb[j], T());
+        }
+    }
+}
+
+// Which tile a workgroup owns: the XCDs take consecutive runs of the list (each has its own L2), and the list walks 8 m-tiles wide
+// columns of the grid, so that the tiles an XCD works on share rows of both operands.
+__device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn) {
+    const int64_t total = tiles_m * tiles_n, per = total >> 3, extra = total & 7, xcd = id & 7;
+    const int64_t at = xcd * per + (xcd < extra ? xcd : extra) + (id >> 3);
+    const int64_t band = at / (8 * tiles_n), wide = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8, in = at - band * 8 * tiles_n;
+    tm = band * 8 + in % wide;
+    tn = in / wide;
+}
+
+__device__ __forceinline__ bool ce_kept(int64_t target, int64_t ignore) { return target != ignore; }
+
+struct CeArgs {
+    Operand w, x;                       // table piece and rows, padded along k
+    int steps;                          // 128-byte steps of k
+    int64_t n, v_total, v0, v_count;    // rows; table; this piece
+    int64_t tiles_m, tiles_n, ignore;
+    float scale2;                       // scale * log2 e
+    const int64_t *target;
+    // forward
+    float2 *part;                       // [tile_m][n]: max, sum
+    float *own;                         // [n]: the target's logit (base 2)
+    // backward
+    const float *lse2, *ratio;
+    void *dl, *dlt;                     // [n][ld_dl], [v][ld_dlt]; either may be NULL
+    int64_t ld_dl, ld_dlt;
+};
+
+template <typename T, typename X>
+__global__ __launch_bounds__(X::THREADS) void ce_stats_kernel(CeArgs a) {
+    extern __shared__ __align__(1024) char lds[];
+    int64_t tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    const int64_t m0 = tm * X::BM, n0 = tn * X::BN;
+    f32x4_t acc[X::TM][X::TN] = {};
+    tile_product<T, X>(a.w, a.x, m0, n0, 0, a.steps, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
+    const int64_t v_lane = m0 + wm * (X::BM / X::WAVES_M) + (lane >> 4) * 4;
+    float2 stat[X::TN];
+#pragma unroll
+    for (int j = 0; j < X::TN; ++j) {
+        const int64_t n = n0 + wn * (X::BN / X::WAVES_N) + j * 16 + (lane & 15);
+        const int64_t t = n < a.n ? a.target[n] : -1;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < X::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t v = v_lane + i * 16 + r;
+                const float l = v < a.v_total ? acc[i][j][r] * a.scale2 : -INFINITY;
+                acc[i][j][r] = l;
+                top = fmaxf(top, l);
+                if (v == t && v < a.v_total) a.own[n] = l;
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float base = top == -INFINITY ? 0.0f : top;      // (a tile of -Inf alone sums to 0; Inf - Inf and NaN make the sum NaN)
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < X::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(acc[i][j][r] - base);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        stat[j] = make_float2(top, sum);
+    }
+    // the waves of one n range, through LDS
+    float2 *s = reinterpret_cast<float2 *>(lds);
+    __syncthreads();
+    if (lane < 16)
+#pragma unroll
+        for (int j = 0; j < X::TN; ++j) s[wm * X::BN + wn * (X::BN / X::WAVES_N) + j * 16 + lane] = stat[j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < X::BN; c += X::THREADS) {
+        if (n0 + c >= a.n) continue;
+        float2 r = s[c];
+#pragma unroll
+        for (int w = 1; w < X::WAVES_M; ++w) {
+            const float2 o = s[w * X::BN + c];
+            const float top = fmaxf(r.x, o.x), base = top == -INFINITY ? 0.0f : top;
+            r = make_float2(top, r.y * __builtin_amdgcn_exp2f(r.x - base) + o.y * __builtin_amdgcn_exp2f(o.x - base));
+        }
+        a.part[tm * a.n + n0 + c] = r;
+    }
+}
+
+// Joins a row's tiles: 16 rows x 16 tiles at a time per workgroup.
+__global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__ part, int64_t tiles, int64_t n, int64_t v_total,
+                                                      const int64_t *__restrict__ target, int64_t ignore, const float *__restrict__ own,
+                                                      float *__restrict__ lse2, float *__restrict__ loss) {
+    __shared__ float2 s[256];
+    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+    float2 r = make_float2(-INFINITY, 0.0f);
+    auto join = [](float2 p, float2 q) {
+        const float top = fmaxf(p.x, q.x), base = top == -INFINITY ? 0.0f : top;
+        return make_float2(top, p.y * __builtin_amdgcn_exp2f(p.x - base) + q.y * __builtin_amdgcn_exp2f(q.x - base));
+    };
+    if (row < n)
+        for (int64_t t = threadIdx.x >> 4; t < tiles; t += 16) r = join(r, part[t * n + row]);
+    s[threadIdx.x] = r;
+    __syncthreads();
+    if (threadIdx.x < 16 && row < n) {
+        for (int t = 1; t < 16; ++t) r = join(r, s[t * 16 + threadIdx.x]);
+        const int64_t t = target[row];
+        const bool kept = ce_kept(t, ignore), named = t >= 0 && t < v_total;
+        const float l = r.x + __builtin_amdgcn_logf(r.y);      // (base 2)
+        lse2[row] = kept && !named ? __uint_as_float(0x7fc00000u) : l;
+        loss[row] = !kept ? 0.0f : !named ? __uint_as_float(0x7fc00000u) : (l - own[row]) * kLn2;
+    }
+}
+
+// sum of the rows' losses and how many were kept, in a fixed order, by one workgroup
+__global__ __launch_bounds__(1024) void ce_total_kernel(const float *__restrict__ rows, const int64_t *__restrict__ target, int64_t n, int64_t ignore,
+                                                        int reduction, float *__restrict__ loss, float *__restrict__ kept) {
+    __shared__ double sums[16], counts[16];
+    double sum = 0.0, count = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        sum += (double)rows[i];
+        count += ce_kept(target[i], ignore) ? 1.0 : 0.0;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) { sum += __shfl_xor(sum, o); count += __shfl_xor(count, o); }
+    if ((threadIdx.x & 63) == 0) { sums[threadIdx.x >> 6] = sum; counts[threadIdx.x >> 6] = count; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) { sum += sums[w]; count += counts[w]; }
+        *kept = (float)count;
+        if (reduction == 1) *loss = (float)(sum / count);
+        if (reduction == 2) *loss = (float)sum;
+    }
+}
+
+// ---- backward
+// a row's factor g_n (0 for an ignored one), and its ratio to the largest magnitude; factors[2 n] = that magnitude
+__global__ __launch_bounds__(1024) void ce_factors_kernel(const float *__restrict__ grad_loss, const float *__restrict__ kept,
+                                                          const int64_t *__restrict__ target, int64_t n, int64_t ignore, int reduction,
+                                                          float *__restrict__ factors) {
+    __shared__ float tops[16];
+    float common = reduction == 0 ? 0.0f : grad_loss[0];
+    if (reduction == 1) common = common / *kept;
+    auto factor = [&](int64_t i) { return !ce_kept(target[i], ignore) ? 0.0f : reduction == 0 ? grad_loss[i] : common; };
+    float top = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, __builtin_fabsf(factor(i)));
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 16; ++w) top = fmaxf(top, tops[w]);
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        const float g = factor(i);
+        factors[i] = g;
+        factors[n + i] = g == 0.0f ? 0.0f : g / top;
+    }
+    if (threadIdx.x == 0) factors[2 * n] = top;
+}
+
+template <typename T, typename X>
+__global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
+    extern __shared__ __align__(1024) char lds[];
+    int64_t tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    const int64_t m0 = tm * X::BM, n0 = tn * X::BN;      // (m0 within the piece)
+    f32x4_t acc[X::TM][X::TN] = {};
+    tile_product<T, X>(a.w, a.x, m0, n0, 0, a.steps, lds, acc);
+    constexpr float unit = GradUnit<T>::value;
+    constexpr int PITCH = X::BN * (int)sizeof(T) + 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
+    const int m_lane = wm * (X::BM / X::WAVES_M) + (lane >> 4) * 4;
+    __syncthreads();      // the stages have been read: LDS holds the transpose from here on
+#pragma unroll
+    for (int j = 0; j < X::TN; ++j) {
+        const int nl = wn * (X::BN / X::WAVES_N) + j * 16 + (lane & 15);
+        const int64_t n = n0 + nl;
+        const int64_t t = n < a.n ? a.target[n] : a.ignore;
+        const bool kept = n < a.n && ce_kept(t, a.ignore);
+        const float lse2 = kept ? a.lse2[n] : 0.0f, ratio = kept ? a.ratio[n] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < X::TM; ++i) {
+            Pack<T, 4> out;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int ml = m_lane + i * 16 + r;
+                const bool real = kept && m0 + ml < a.v_count;
+                const float p = __builtin_amdgcn_exp2f(acc[i][j][r] * a.scale2 - lse2);
+                const float d = real ? (a.v0 + m0 + ml == t ? p - 1.0f : p) * unit : 0.0f;
+                out.v[r] = from_float<T>(d);
+                if (a.dlt) *reinterpret_cast<T *>(lds + ml * PITCH + nl * (int)sizeof(T)) = from_float<T>(real ? d * ratio : 0.0f);
+            }
+            const int64_t m = m0 + m_lane + i * 16;
+            if (a.dl && n < a.n && m < a.ld_dl) *reinterpret_cast<Pack<T, 4> *>(static_cast<T *>(a.dl) + n * a.ld_dl + m) = out;
+        }
+    }
+    if (!a.dlt) return;
+    __syncthreads();
+    constexpr int PER16 = 16 / (int)sizeof(T), CHUNKS = X::BN / PER16;
+    for (int c = threadIdx.x; c < X::BM * CHUNKS; c += X::THREADS) {
+        const int ml = c / CHUNKS, nc = c % CHUNKS * PER16;
+        if (m0 + ml < a.v_count && n0 + nc < a.ld_dlt)
+            *reinterpret_cast<u32x4_t *>(static_cast<T *>(a.dlt) + (m0 + ml) * a.ld_dlt + n0 + nc) =
+                *reinterpret_cast<const u32x4_t *>(lds + ml * PITCH + nc * (int)sizeof(T));
+    }
+}
+
+// out[n][m] (+)= factor * sum_k A[m][k] B[n][k]; blockIdx.y = part of k
+struct CeProduct {
+    Operand a, b;
+    int steps, steps_per_part;
+    int64_t m, n, tiles_m, tiles_n;
+    float *sums;            // float32 sums [part][n][ld_sums] (added to if `add`), or NULL: `out` is written
+    int64_t ld_sums;
+    int add;
+    void *out;              // [n][m] of T
+    const float *top;       // `out` = sum * *top * factor
+    float factor;
+};
+
+template <typename T, typename X>
+__global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
+    extern __shared__ __align__(1024) char lds[];
+    int64_t tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    const int64_t m0 = tm * X::BM, n0 = tn * X::BN;
+    const int first = blockIdx.y * a.steps_per_part, steps = min(a.steps_per_part, a.steps - first);
+    f32x4_t acc[X::TM][X::TN] = {};
+    tile_product<T, X>(a.a, a.b, m0, n0, (int64_t)first * kRowBytes, steps, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
+    const float f = a.sums ? 1.0f : *a.top * a.factor;
+#pragma unroll
+    for (int j = 0; j < X::TN; ++j) {
+        const int64_t n = n0 + wn * (X::BN / X::WAVES_N) + j * 16 + (lane & 15);
+        if (n >= a.n) continue;
+#pragma unroll
+        for (int i = 0; i < X::TM; ++i) {
+            const int64_t m = m0 + wm * (X::BM / X::WAVES_M) + i * 16 + (lane >> 4) * 4;
+            if (m >= a.m) continue;
+            if (a.sums) {      // (rows of ld_sums floats, a multiple of 4: the padding behind m may be written)
+                f32x4_t *to = reinterpret_cast<f32x4_t *>(a.sums + ((int64_t)blockIdx.y * a.n + n) * a.ld_sums + m);
+                *to = a.add ? *to + acc[i][j] : acc[i][j];
+            } else {
+                T *to = static_cast<T *>(a.out) + n * a.m + m;
+                Pack<T, 4> o;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o.v[r] = from_float<T>(acc[i][j][r] * f);
+                if ((a.m & 3) == 0) *reinterpret_cast<Pack<T, 4> *>(to) = o;
+                else
+                    for (int r = 0; r < 4; ++r) if (m + r < a.m) to[r] = o.v[r];
+            }
+        }
+    }
+}
+
+// dx[n][c] = g_n * factor * the parts' sums, in order
+template <typename T>
+__global__ __launch_bounds__(256) void ce_finish_kernel(const float *__restrict__ sums, int parts, int64_t n, int C, int64_t ld, const float *__restrict__ g,
+                                                        float factor, T *__restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n * C) return;
+    const int64_t row = i / C, c = i - row * C;
+    float s = 0.0f;
+    for (int p = 0; p < parts; ++p) s += sums[((int64_t)p * n + row) * ld + c];
+    const float f = g[row];
+    out[i] = from_float<T>(f == 0.0f ? 0.0f : s * f * factor);
+}
+
+// out[c][r] = in[r][c] for c < C, zero for r in [R, ld_out) and where the row's target is `ignore` (targets == NULL: nowhere)
+template <typename T>
+__global__ __launch_bounds__(256) void ce_transpose_kernel(const T *__restrict__ in, int64_t R, int C, int64_t ld_in, const int64_t *__restrict__ target,
+                                                           int64_t ignore, T *__restrict__ out, int64_t ld_out) {
+    __shared__ T tile[64][64 + 4 / sizeof(T)];
+    const int64_t r0 = (int64_t)blockIdx.x * 64;
+    const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    for (int r = ty; r < 64; r += 4) {
+        const int64_t row = r0 + r;
+        const bool here = row < R && c0 + tx < C && (!target || ce_kept(target[row], ignore));
+        tile[r][tx] = here ? in[row * ld_in + c0 + tx] : from_float<T>(0.0f);
+    }
+    __syncthreads();
+    for (int c = ty; c < 64; c += 4)
+        if (c0 + c < C && r0 + tx < ld_out) out[(int64_t)(c0 + c) * ld_out + r0 + tx] = tile[tx][c];
+}
+
+// out[r][0 .. Cp) = in[r][0 .. C), zeros
+template <typename T>
+__global__ __launch_bounds__(256) void ce_pad_kernel(const T *__restrict__ in, int64_t R, int C, T *__restrict__ out, int Cp) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= R * Cp) return;
+    const int64_t r = i / Cp;
+    const int c = (int)(i - r * Cp);
+    out[i] = c < C ? in[r * C + c] : from_float<T>(0.0f);
+}
+
+// ---- host side
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+struct CePlan {
+    int es;                          // element size
+    int Cp;                          // C padded to whole 128-byte steps
+    bool pad;                        // the operands are copied to rows of Cp
+    int64_t piece, np, c4;           // backward: table rows per piece, rows padded to 128 bytes of dl^T, C rounded up to 4
+    int parts;                       // of k in dx's product
+    size_t xp, wp;                   // byte offsets
+    size_t part, own, rows;          // forward
+    size_t factors, dl, dlt, wt, xt, sums;
+    size_t total;
+};
+
+using TileBig = Tile<128, 128, 2, 2>;
+
+static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, bool need_x, bool need_w) {
+    CePlan p = {};
+    p.es = (int)dtype_size(dtype);
+    const int step = kRowBytes / p.es;
+    p.Cp = (int)round_up(C, step);
+    p.pad = p.Cp != C;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
+    if (p.pad) {
+        p.xp = take((size_t)n * p.Cp * p.es);
+        p.wp = take((size_t)V * p.Cp * p.es);
+    }
+    if (!backward) {
+        p.part = take((size_t)ceil_div(V, TileBig::BM) * n * sizeof(float2));
+        p.own = take((size_t)n * 4);
+        p.rows = take((size_t)n * 4);
+    } else {
+        // the piece: dl of at most 2^26 values, whole tiles
+        p.piece = ((int64_t)1 << 26) / (n > 0 ? n : 1) / 256 * 256;
+        if (p.piece < 256) p.piece = 256;
+        if (p.piece > round_up(V, 256)) p.piece = round_up(V, 256);
+        p.np = round_up(n, step);
+        p.c4 = round_up(C, 4);
+        p.factors = take((size_t)(2 * n + 1) * 4);
+        if (need_x) {
+            p.dl = take((size_t)n * p.piece * p.es);
+            p.wt = take((size_t)C * p.piece * p.es);
+            const int64_t tiles = ceil_div(C, TileBig::BM) * ceil_div(n, TileBig::BN), steps = round_up(V < p.piece ? V : p.piece, step) / step;
+            // parts of k: enough workgroups for the chip's 256 CUs twice over, at least 8 steps each
+            int64_t parts = ceil_div(512, tiles > 0 ? tiles : 1);
+            if (parts > steps / 8) parts = steps / 8;
+            if (parts < 1) parts = 1;
+            p.parts = (int)ceil_div(steps, ceil_div(steps, parts));      // (as many as get work; a smaller last piece then has no more)
+            p.sums = take((size_t)p.parts * n * p.c4 * 4);
+        }
+        if (need_w) {
+            p.dlt = take((size_t)p.piece * p.np * p.es);
+            p.xt = take((size_t)C * p.np * p.es);
+        }
+    }
+    p.total = at;
+    return p;
+}
+
+static int ce_check(const char *who, const void *x, const void *w, int dtype, const int64_t *target, int64_t n, int64_t V, int C, int reduction,
+                    const void *workspace, size_t workspace_bytes, size_t need) {
+    if (n < 0 || V < 1 || C < 1 || dtype_size(dtype) == 0 || !w || (n > 0 && (!x || !target)) || reduction < 0 || reduction > 2 || !workspace) {
+        set_error("%s: invalid argument (n=%lld, V=%lld, C=%d, dtype=%d, reduction=%d)", who, (long long)n, (long long)V, C, dtype, reduction);
+        return MVS_EINVAL;
+    }
+    if (!aligned16(x) || !aligned16(w) || !aligned16(workspace)) {
+        set_error("%s: x, weight and the workspace are to be aligned to 16 bytes", who);
+        return MVS_EINVAL;
+    }
+    if (n > ((int64_t)1 << 30) || V > ((int64_t)1 << 30) || C > (1 << 20) || ceil_div(n, 64) * ceil_div(V, 64) > 0x7fffffff) {
+        set_error("%s: n=%lld, V=%lld (at most 2^30 each, n V / 4096 below 2^31), C=%d (at most 2^20)", who, (long long)n, (long long)V, C);
+        return MVS_EUNSUPPORTED;
+    }
+    if (workspace_bytes < need) {
+        set_error("%s: workspace too small (%zu of %zu bytes)", who, workspace_bytes, need);
+        return MVS_EWORKSPACE;
+    }
+    return MVS_OK;
+}
+
+// LDS of a kernel: the two stages, or what its epilogue lays there
+template <typename X>
+static unsigned ce_lds(size_t epilogue) { return (unsigned)(epilogue > 2 * (size_t)X::STAGE ? epilogue : 2 * (size_t)X::STAGE); }
+
+// (more than 64 KiB of dynamic LDS has to be asked for, once per kernel and device)
+template <typename F>
+static bool ce_allow_lds(F kernel, unsigned bytes) {
+    return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
+}
+
+template <typename T>
+static void ce_pad(const void *in, int64_t R, int C, char *out, int Cp, hipStream_t st) {
+    if (R > 0)
+        hipLaunchKernelGGL((ce_pad_kernel<T>), dim3((unsigned)ceil_div(R * Cp, 256)), dim3(256), 0, st, static_cast<const T *>(in), R, C,
+                           reinterpret_cast<T *>(out), Cp);
+}
+
+template <typename T, typename X>
+static int ce_forward(const CePlan &p, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, int64_t ignore,
+                      int reduction, float *loss, float *lse, float *kept, char *ws, hipStream_t st) {
+    if (n > 0) {
+        CeArgs a = {};
+        a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
+        a.x = Operand{static_cast<const char *>(x), (int64_t)p.Cp * p.es, n};
+        if (p.pad) {
+            ce_pad<T>(x, n, C, ws + p.xp, p.Cp, st);
+            ce_pad<T>(w, V, C, ws + p.wp, p.Cp, st);
+            a.x.p = ws + p.xp;
+            a.w.p = ws + p.wp;
+        }
+        a.steps = p.Cp * p.es / kRowBytes;
+        a.n = n; a.v_total = V; a.v_count = V; a.ignore = ignore;
+        a.tiles_m = ceil_div(V, X::BM); a.tiles_n = ceil_div(n, X::BN);
+        a.scale2 = scale * kLog2e;
+        a.target = target;
+        a.part = reinterpret_cast<float2 *>(ws + p.part);
+        a.own = reinterpret_cast<float *>(ws + p.own);
+        float *rows = reduction == 0 ? loss : reinterpret_cast<float *>(ws + p.rows);
+        const unsigned bytes = ce_lds<X>((size_t)X::WAVES_M * X::BN * sizeof(float2));
+        if (!ce_allow_lds(ce_stats_kernel<T, X>, bytes)) return check_launch("mvs_linear_ce_fwd");
+        hipLaunchKernelGGL((ce_stats_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), bytes, st, a);
+        hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(256), 0, st, a.part, a.tiles_m, n, V, target, ignore, a.own, lse, rows);
+        hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, rows, target, n, ignore, reduction, loss, kept);
+    } else {
+        hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, (const float *)nullptr, target, n, ignore, reduction, loss, kept);
+    }
+    return check_launch("mvs_linear_ce_fwd");
+}
+
+template <typename T, typename X>
+static int ce_backward(const CePlan &p, const void *x, const void *w, const int64_t *target, const float *lse, const float *kept, const float *grad_loss,
+                       int64_t n, int64_t V, int C, float scale, int64_t ignore, int reduction, void *grad_x, void *grad_w, char *ws, hipStream_t st) {
+    const int step = kRowBytes / p.es;
+    float *factors = reinterpret_cast<float *>(ws + p.factors);
+    hipLaunchKernelGGL(ce_factors_kernel, dim3(1), dim3(1024), 0, st, grad_loss, kept, target, n, ignore, reduction, factors);
+    CeArgs a = {};
+    a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
+    a.x = Operand{static_cast<const char *>(x), (int64_t)p.Cp * p.es, n};
+    if (p.pad) {
+        ce_pad<T>(x, n, C, ws + p.xp, p.Cp, st);
+        ce_pad<T>(w, V, C, ws + p.wp, p.Cp, st);
+        a.x.p = ws + p.xp;
+        a.w.p = ws + p.wp;
+    }
+    const char *w_rows = a.w.p;
+    a.steps = p.Cp * p.es / kRowBytes;
+    a.n = n; a.v_total = V; a.ignore = ignore;
+    a.tiles_n = ceil_div(n, X::BN);
+    a.scale2 = scale * kLog2e;
+    a.target = target; a.lse2 = lse; a.ratio = factors + n;
+    a.dl = grad_x ? ws + p.dl : nullptr;
+    a.dlt = grad_w ? ws + p.dlt : nullptr;
+    a.ld_dlt = p.np;
+    const float factor = scale / GradUnit<T>::value;
+    const unsigned grad_lds = ce_lds<X>((size_t)X::BM * (X::BN * sizeof(T) + 16)), product_lds = ce_lds<X>(0);
+    if (!ce_allow_lds(ce_grad_kernel<T, X>, grad_lds) || !ce_allow_lds(ce_product_kernel<T, X>, product_lds)) return check_launch("mvs_linear_ce_bwd");
+    if (grad_w)      // x^T once; ignored rows as zeros, whatever they hold
+        hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(p.np, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
+                           reinterpret_cast<const T *>(a.x.p), n, C, (int64_t)p.Cp, target, ignore, reinterpret_cast<T *>(ws + p.xt), p.np);
+    for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+        const int64_t count = V - v0 < p.piece ? V - v0 : p.piece, k = round_up(count, step);
+        a.w.p = w_rows + v0 * p.Cp * p.es;
+        a.w.rows = count;
+        a.v0 = v0; a.v_count = count; a.ld_dl = k;
+        a.tiles_m = ceil_div(count, X::BM);
+        hipLaunchKernelGGL((ce_grad_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), grad_lds, st, a);
+        if (grad_x) {
+            hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(k, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
+                               reinterpret_cast<const T *>(a.w.p), count, C, (int64_t)p.Cp, (const int64_t *)nullptr, ignore,
+                               reinterpret_cast<T *>(ws + p.wt), k);
+            CeProduct d = {};
+            d.a = Operand{ws + p.wt, k * p.es, C};
+            d.b = Operand{ws + p.dl, k * p.es, n};
+            d.steps = (int)(k / step);
+            d.steps_per_part = (int)ceil_div(d.steps, p.parts);
+            d.m = C; d.n = n; d.tiles_m = ceil_div(C, X::BM); d.tiles_n = ceil_div(n, X::BN);
+            d.sums = reinterpret_cast<float *>(ws + p.sums); d.ld_sums = p.c4;
+            d.add = v0 > 0;
+            // (a smaller last piece may have fewer parts of k: the sums of the others stay as they are)
+            hipLaunchKernelGGL((ce_product_kernel<T, X>), dim3((unsigned)(d.tiles_m * d.tiles_n), (unsigned)ceil_div(d.steps, d.steps_per_part)),
+                               dim3(X::THREADS), product_lds, st, d);
+        }
+        if (grad_w) {
+            CeProduct d = {};
+            d.a = Operand{ws + p.xt, p.np * p.es, C};
+            d.b = Operand{ws + p.dlt, p.np * p.es, count};
+            d.steps = (int)(p.np / step);
+            d.steps_per_part = d.steps;
+            d.m = C; d.n = count; d.tiles_m = ceil_div(C, X::BM); d.tiles_n = ceil_div(count, X::BN);
+            d.out = static_cast<T *>(grad_w) + v0 * C;
+            d.top = factors + 2 * n; d.factor = factor;
+            hipLaunchKernelGGL((ce_product_kernel<T, X>), dim3((unsigned)(d.tiles_m * d.tiles_n)), dim3(X::THREADS), product_lds, st, d);
+        }
+    }
+    if (grad_x) {
+        hipLaunchKernelGGL((ce_finish_kernel<T>), dim3((unsigned)ceil_div(n * C, 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums), p.parts, n, C,
+                           p.c4, factors, factor, static_cast<T *>(grad_x));
+    }
+    return check_launch("mvs_linear_ce_bwd");
+}
+
+// a gradient of no rows
+__global__ __launch_bounds__(256) void ce_zero_kernel(unsigned short *__restrict__ p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
+}  // namespace mvs
+
+using namespace mvs;
+
+extern "C" size_t mvs_linear_ce_workspace_bytes(int64_t n, int64_t V, int C, int dtype, int backward, int need_x, int need_w) {
+    if (n < 0 || V < 1 || C < 1 || dtype_size(dtype) == 0) return 0;
+    return ce_plan(n, V, C, dtype, backward != 0, need_x != 0, need_w != 0).total + 256;
+}
+
+extern "C" int mvs_linear_ce_fwd(const void *x, const void *weight, int dtype, const int64_t *target, int64_t n, int64_t V, int C, float scale,
+                                 int64_t ignore_index, int reduction, float *loss, float *lse, float *kept, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    const int rc = ce_check("mvs_linear_ce_fwd", x, weight, dtype, target, n, V, C, reduction, workspace, workspace_bytes,
+                            mvs_linear_ce_workspace_bytes(n, V, C, dtype, 0, 0, 0));
+    if (rc != MVS_OK) return rc;
+    if (!kept || (!loss && (reduction != 0 || n > 0)) || (!lse && n > 0)) {
+        set_error("mvs_linear_ce_fwd: loss, lse and kept are needed");
+        return MVS_EINVAL;
+    }
+    const CePlan p = ce_plan(n, V, C, dtype, false, false, false);
+    MVS_DTYPE_DISPATCH(dtype, T, {
+        return ce_forward<T, TileBig>(p, x, weight, target, n, V, C, scale, ignore_index, reduction, loss, lse, kept, static_cast<char *>(workspace),
+                                      as_stream(stream));
+    });
+}
+
+extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, const int64_t *target, const float *lse, const float *kept,
+                                 const float *grad_loss, int64_t n, int64_t V, int C, float scale, int64_t ignore_index, int reduction,
+                                 void *grad_x, void *grad_weight, void *workspace, size_t workspace_bytes, void *stream) {
+    const int rc = ce_check("mvs_linear_ce_bwd", x, weight, dtype, target, n, V, C, reduction, workspace, workspace_bytes,
+                            mvs_linear_ce_workspace_bytes(n, V, C, dtype, 1, grad_x != nullptr, grad_weight != nullptr));
+    if (rc != MVS_OK) return rc;
+    if (n == 0) {
+        if (grad_weight)
+            hipLaunchKernelGGL(ce_zero_kernel, dim3(1024), dim3(256), 0, as_stream(stream), static_cast<unsigned short *>(grad_weight),
+                               V * C * (int64_t)(dtype_size(dtype) / 2));
+        return check_launch("mvs_linear_ce_bwd");
+    }
+    if (!lse || !kept || !grad_loss || (!grad_x && !grad_weight)) {
+        set_error("mvs_linear_ce_bwd: lse, kept, grad_loss and a gradient to compute are needed");
+        return MVS_EINVAL;
+    }
+    const CePlan p = ce_plan(n, V, C, dtype, true, grad_x != nullptr, grad_weight != nullptr);
+    MVS_DTYPE_DISPATCH(dtype, T, {
+        return ce_backward<T, TileBig>(p, x, weight, target, lse, kept, grad_loss, n, V, C, scale, ignore_index, reduction, grad_x, grad_weight,
+                                       static_cast<char *>(workspace), as_stream(stream));
+    });
+}

@@ -67,3 +67,37 @@ def depth_regression(p, depth_values):
     if depth_values.dim() == 2:
         depth_values = depth_values.view(*depth_values.shape, 1, 1)
     return torch.sum(p * depth_values, 1)
+
+
+def matching_cells(depth, src_proj, ref_proj, mask=None):
+    """The source view's feature cell that every reference cell's point falls on: depth [B,h,w] of the reference view at feature
+    resolution, projection matrices [B,4,4] as in homo_warping -> int64 [B, h*w], y * w + x of the nearest cell, -1 where the point
+    lies behind the camera or outside the map, where depth is not positive and where mask ([B,h,w]) is not > 0.5."""
+    B, h, w = depth.shape
+    rt = ops.rot_trans_all(torch.stack((ref_proj, src_proj), 1), "device")[0].view(B, 3, 4)
+    y, x = torch.meshgrid(torch.arange(h, device=depth.device, dtype=torch.float32), torch.arange(w, device=depth.device, dtype=torch.float32), indexing="ij")
+    ray = torch.stack((x, y, torch.ones_like(x)), -1).view(1, h * w, 3, 1)
+    p = (rt[:, None, :, :3] * ray.transpose(2, 3)).sum(-1) * depth.reshape(B, h * w, 1) + rt[:, None, :, 3]
+    u, v = torch.round(p[..., 0] / p[..., 2]), torch.round(p[..., 1] / p[..., 2])
+    seen = (depth.reshape(B, h * w) > 0) & (p[..., 2] > 0) & (u >= 0) & (u <= w - 1) & (v >= 0) & (v <= h - 1)
+    if mask is not None:
+        seen = seen & (mask.reshape(B, h * w) > 0.5)
+    cell = torch.where(seen, v * w + u, torch.full_like(u, -1.0))
+    return cell.to(torch.int64)
+
+
+def feature_matching_loss(ref_fea, src_fea, ref_cells, src_cells, temperature=1.0):
+    """Cross entropy of finding a point's cell in the source view by its feature in the reference view: over the pairs (point) of
+    ref_cells, src_cells [B,P] (cell numbers y * w + x; -1 on either side: no such pair), the softmax of <ref feature, source
+    feature> / temperature over ALL cells of the source map, averaged over the pairs there are (NaN if there is none).
+    ref_fea, src_fea [B,C,h,w]; differentiable in both.  The [P, h*w] scores are never stored (ops.linear_cross_entropy), several
+    points may share a cell (ops.lookup_rows)."""
+    B, C, h, w = src_fea.shape
+    total = 0.0
+    for b in range(B):
+        rows = [f[b].permute(1, 2, 0).reshape(-1, C) for f in (ref_fea, src_fea)]
+        paired = (ref_cells[b] >= 0) & (src_cells[b] >= 0)
+        target = torch.where(paired, src_cells[b], torch.full_like(src_cells[b], -100))
+        total = total + ops.linear_cross_entropy(ops.lookup_rows(rows[0], ref_cells[b]), rows[1], target, scale=1.0 / temperature,
+                                                 reduction="sum")
+    return total / ((ref_cells >= 0) & (src_cells >= 0)).sum()

@@ -24,7 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import ops
-from .module import ConvBnReLU, ConvBnReLU3D
+from .module import ConvBnReLU, ConvBnReLU3D, feature_matching_loss, matching_cells
 
 
 class FeatureNet(nn.Module):
@@ -82,18 +82,19 @@ class FeatureNet(nn.Module):
     def hip_supported(self):
         return all(p["packed"] is not None for p in self._hip_params())
 
-    def forward_train_hip(self, img_nchw, groups=1):
+    def forward_train_hip(self, img_nchw, groups=1, act8=False):
         """Autograd path on the HIP 2D kernels, forward and both gradients (mvs_amd/train_ops.py: no MIOpen):
         [N,3,H,W] -> [N,H/4,W/4,32] channels-last, batch-statistics BatchNorm (fused HIP op) as in forward().
         groups: the N images are that many consecutive blocks (the V views of a sample batch, view-major), each normalised
         with its own batch statistics and counted as one update of the running statistics -- the reference's V calls
-        `self.feature(imgs[:, v])` (mvsnet.py:146) as ONE launch per layer (round 4: a third of the launches of a step)."""
+        `self.feature(imgs[:, v])` (mvsnet.py:146) as ONE launch per layer (round 4: a third of the launches of a step).
+        act8: the layers keep their inputs for the backward pass in 8 bits (ops.act8_quantize)."""
         from ..train_ops import conv2d_bn_relu_cl, conv2d_cl
-        x = conv2d_bn_relu_cl(img_nchw, self.conv0.conv, self.conv0.bn, 1, planar=True, groups=groups)
+        x = conv2d_bn_relu_cl(img_nchw, self.conv0.conv, self.conv0.bn, 1, planar=True, groups=groups, act8=act8)
         for name, stride in self._PLAN[1:]:
             m = getattr(self, name)
-            x = conv2d_bn_relu_cl(x, m.conv, m.bn, stride, groups=groups)
-        return conv2d_cl(x, self.feature.weight, 1) + self.feature.bias      # [N,H/4,W/4,32] channels-last
+            x = conv2d_bn_relu_cl(x, m.conv, m.bn, stride, groups=groups, act8=act8)
+        return conv2d_cl(x, self.feature.weight, 1, act8=act8) + self.feature.bias      # [N,H/4,W/4,32] channels-last
 
     def forward_train_cl(self, img_nchw):
         """Autograd path in channels-last: torch's conv2d (MIOpen NHWC kernels, forward and both
@@ -202,21 +203,22 @@ class CostRegNet(nn.Module):
         return self.prob(x)
 
     # -- autograd path on the HIP conv kernels (forward + input gradients), channels-last
-    def forward_train_hip(self, x_cl, conv0_raw=None):
+    def forward_train_hip(self, x_cl, conv0_raw=None, act8=False):
         """x_cl [B,D,H,W,32] -> cost [B,D,H,W]; same graph as forward() (mvsnet.py:83-93).  conv0_raw: conv0's output
-        before BatchNorm from ops.variance_conv0_autograd (then x_cl is not used)."""
+        before BatchNorm from ops.variance_conv0_autograd (then x_cl is not used).  act8: the layers keep their inputs for the
+        backward pass in 8 bits (ops.act8_quantize)."""
         from ..train_ops import conv3d_cl, conv_bn_relu_cl
 
         def blk(name, t, stride=1):
             m = getattr(self, name)
-            return conv_bn_relu_cl(t, m.conv, m.bn, False, stride, tag=name)
+            return conv_bn_relu_cl(t, m.conv, m.bn, False, stride, tag=name, act8=act8)
 
         def up(name, t, skip):
             m = getattr(self, name)
-            return conv_bn_relu_cl(t, m[0], m[1], True, 2, skip=skip, tag=name)
+            return conv_bn_relu_cl(t, m[0], m[1], True, 2, skip=skip, tag=name, act8=act8)
 
         if conv0_raw is not None and self.conv0.bn.training and self.conv0.bn.momentum is not None:
-            c0 = ops.bn_relu_cl(conv0_raw, self.conv0.bn)
+            c0 = ops.bn_relu_cl(conv0_raw, self.conv0.bn, act8=act8)
         else:
             c0 = blk("conv0", x_cl)
         c2 = blk("conv2", blk("conv1", c0, 2))
@@ -225,7 +227,7 @@ class CostRegNet(nn.Module):
         t = up("conv7", t, c4)     # c4 + relu(bn(deconv))
         t = up("conv9", t, c2)
         t = up("conv11", t, c0)
-        return (conv3d_cl(t, self.prob.weight, tag="prob") + self.prob.bias).squeeze(-1)
+        return (conv3d_cl(t, self.prob.weight, tag="prob", act8=act8) + self.prob.bias).squeeze(-1)
 
     # -- inference path: HIP kernels, BN folded to a per-channel affine
     def _layers(self):
@@ -371,6 +373,11 @@ class MVSNet(nn.Module):
         # True: the V per-view FeatureNet calls of a training step run as ONE batch with per-view BatchNorm statistics
         # (FeatureNet.forward_train_hip(groups=V)); False: V calls, as the reference's loop (A/B)
         self.train_feature_batched = True
+        # True: a training step keeps its activations for the backward pass in 8 bits (blocks of 32 values with a power of two each,
+        # ops.act8_quantize): the convolutions' and BatchNorms' inputs and the variance volume, about a quarter of the bytes.  The
+        # forward pass is the same bit for bit; the gradients are those of the rounded activations.  Needs train_impl = "hip"
+        # (and train_feature_impl = "hip" for FeatureNet's layers); layers on torch's kernels keep float32.
+        self.train_act8 = False
         self._feature_cl = False
         self.feature = FeatureNet()
         self.cost_regularization = CostRegNet()
@@ -416,11 +423,11 @@ class MVSNet(nn.Module):
                     if self.train_feature_batched:
                         # the V per-view calls as one batch of V groups (view-major): per-view BatchNorm statistics, one launch per layer
                         Bn = imgs.shape[0]
-                        fall = self.feature.forward_train_hip(imgs.transpose(0, 1).reshape(V * Bn, *imgs.shape[2:]), groups=V)
+                        fall = self.feature.forward_train_hip(imgs.transpose(0, 1).reshape(V * Bn, *imgs.shape[2:]), groups=V, act8=self.train_act8)
                         feats_stacked = fall.reshape(V, Bn, *fall.shape[1:])                           # [V,B,h,w,C]
                         feats_cl = list(feats_stacked.unbind(0))
                     else:
-                        feats_cl = [self.feature.forward_train_hip(imgs[:, v]) for v in range(V)]   # [B,h,w,C]
+                        feats_cl = [self.feature.forward_train_hip(imgs[:, v], act8=self.train_act8) for v in range(V)]   # [B,h,w,C]
                     feats = [f.permute(0, 3, 1, 2) for f in feats_cl]
                 elif self.train_feature_impl == "torch_cl" and self.feature.training:
                     if not self._feature_cl:   # weights in NHWC once, not re-laid-out by every conv2d call
@@ -450,16 +457,16 @@ class MVSNet(nn.Module):
                 if C == 32 and self.training and self.train_conv0_fused and ops.conv_split_enabled() and bn0.training and bn0.momentum is not None:
                     # warp + variance -> conv0 as one autograd node: the volume stays 8-channel blocked for the bf16 kernel
                     c0 = ops.variance_conv0_autograd(f16[0], f16[1:], rts, depth_values,
-                                                     self.cost_regularization.conv0.conv.weight, self.align_corners)
-                    cost = self.cost_regularization.forward_train_hip(None, conv0_raw=c0)
+                                                     self.cost_regularization.conv0.conv.weight, self.align_corners, act8=self.train_act8)
+                    cost = self.cost_regularization.forward_train_hip(None, conv0_raw=c0, act8=self.train_act8)
                 else:
                     var = ops.costvol_variance_c16_autograd(f16[0], f16[1:], rts, depth_values, self.align_corners)
-                    cost = self.cost_regularization.forward_train_hip(var)
+                    cost = self.cost_regularization.forward_train_hip(var, act8=self.train_act8)
             else:
                 var = ops.costvol_variance(feats[0], torch.stack(feats[1:]), rts, depth_values,
                                            self.align_corners)          # [B,32,D,h,w]
                 if self.train_impl == "hip":
-                    cost = self.cost_regularization.forward_train_hip(var.permute(0, 2, 3, 4, 1))
+                    cost = self.cost_regularization.forward_train_hip(var.permute(0, 2, 3, 4, 1), act8=self.train_act8)
                 else:
                     cost = self.cost_regularization(var).squeeze(1)
         else:
@@ -548,6 +555,24 @@ class MVSNet(nn.Module):
         if self.refine:
             out["refined_depth"] = self.refine_network(imgs[:, 0], depth)
         return out
+
+
+    def matching_loss(self, imgs, proj_matrices, depth, mask=None, temperature=0.1):
+        """Supervision of FeatureNet alone, from the depth the reference view is trained on: every reference cell with a depth has to
+        find its cell in each source view among all of them (feature_matching_loss over matching_cells), averaged over the source
+        views.  imgs [B,V,3,H,W], proj_matrices [B,V,4,4], depth and mask [B,H/4,W/4].  Add it to mvsnet_loss, or train on it first;
+        training mode, FeatureNet's HIP layers (each view with its own batch statistics, as in forward())."""
+        if not (self.training and self.feature.hip_supported()):
+            raise ops.MvsHipError("matching_loss: a training step on FeatureNet's HIP layers (model.train())")
+        if imgs.shape[1] != proj_matrices.shape[1] or imgs.shape[1] < 2:
+            raise ops.MvsHipError(f"matching_loss: {imgs.shape[1]} images and {proj_matrices.shape[1]} projection matrices, two views at least")
+        B, V = imgs.shape[:2]
+        fea = self.feature.forward_train_hip(imgs.transpose(0, 1).reshape(V * B, *imgs.shape[2:]), groups=V, act8=self.train_act8)
+        fea = fea.reshape(V, B, *fea.shape[1:]).permute(0, 1, 4, 2, 3)             # [V,B,C,h,w] views of channels-last maps
+        here = torch.arange(fea.shape[3] * fea.shape[4], device=fea.device).expand(B, -1)
+        losses = [feature_matching_loss(fea[0], fea[v], here, matching_cells(depth, proj_matrices[:, v], proj_matrices[:, 0], mask), temperature)
+                  for v in range(1, V)]
+        return torch.stack(losses).mean()
 
 
 def mvsnet_loss(depth_est, depth_gt, mask):

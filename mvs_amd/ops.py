@@ -9,10 +9,11 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import (MVS_LAYOUT_C4, MVS_LAYOUT_C8, MVS_LAYOUT_C16, MVS_LAYOUT_NCHW, MVS_LAYOUT_NHWC, MvsHipError, check, ptr,
-                   stream)
+from ._lib import (DTYPES, MVS_LAYOUT_C4, MVS_LAYOUT_C8, MVS_LAYOUT_C16, MVS_LAYOUT_NCHW, MVS_LAYOUT_NHWC, MvsHipError, any_ptr, check,
+                   ptr, stream)
 
 _I = ctypes.c_int
 
@@ -1563,7 +1564,7 @@ class _VarianceConv0(torch.autograd.Function):
     kernel's backward on that."""
 
     @staticmethod
-    def forward(ctx, ref16, srcs16, rts, depth_values, weight, align_corners):
+    def forward(ctx, ref16, srcs16, rts, depth_values, weight, align_corners, act8=False):
         ref16, srcs16, depth_values = _f32c(ref16), _f32c(srcs16), _f32c(depth_values)
         if _depth_mode(depth_values) != 0:
             raise MvsHipError("the fused variance -> conv0 training op takes [B,D] depth planes")
@@ -1578,23 +1579,28 @@ class _VarianceConv0(torch.autograd.Function):
         split_stage_names.add("train.conv0.fwd")
         with stage("train.conv0.fwd"):
             out = conv3d_c8_f16x3(var, pks, amax) if f16 else conv3d_c8_split(var, pks, None, None, None, False)
-        ctx.save_for_backward(ref16, srcs16, rts, depth_values, var, weight)
-        ctx.ac = int(align_corners)
+        held = act8_quantize(var) if act8 and ctx.needs_input_grad[4] else None
+        ctx.save_for_backward(ref16, srcs16, rts, depth_values, weight, *((var,) if held is None else (held.codes, held.scales)))
+        ctx.ac, ctx.var_shape = int(align_corners), var.shape
         ctx.var_absmax = amax          # (None on the bf16 path)
         return out
 
     @staticmethod
     def backward(ctx, g):
-        ref16, srcs16, rts, depth_values, var, weight = ctx.saved_tensors
+        ref16, srcs16, rts, depth_values, weight, *kept = ctx.saved_tensors
         g = _f32c(g)
         w = weight.detach()
         gw = g_ref = g_src = None
         g_absmax = None                # max |g|: the operand scale of both two-piece kernels below, one pass
         if ctx.needs_input_grad[4]:
             with stage("train.conv0.wgrad"):
-                if ctx.var_absmax is not None and wgrad_f16_enabled():
+                var, var_absmax = kept[0], ctx.var_absmax
+                if len(kept) == 2:      # held in 8 bits: rounded values, whose largest magnitude may be half a step above the volume's
+                    var = act8_dequantize(Act8(*kept, ctx.var_shape, torch.float32))
+                    var_absmax = absmax(var) if var_absmax is not None else None
+                if var_absmax is not None and wgrad_f16_enabled():
                     g_absmax = absmax(g)
-                    gw = conv3d_wgrad_c8_f16(var, ctx.var_absmax, g, g_absmax)
+                    gw = conv3d_wgrad_c8_f16(var, var_absmax, g, g_absmax)
                 if gw is None:
                     gw = conv3d_wgrad_c8(var, g)
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
@@ -1614,12 +1620,13 @@ class _VarianceConv0(torch.autograd.Function):
                     ptr(gvar), ptr(ref16), ptr(srcs16), ptr(rts), ptr(depth_values), 0, B, V, G * 16, D, H, W,
                     ctx.ac, MVS_LAYOUT_C16, MVS_LAYOUT_NHWC, ptr(g_ref), ptr(g_src), stream()),
                     "mvs_costvol_variance_bwd_f32")
-        return g_ref, g_src, None, None, gw, None
+        return g_ref, g_src, None, None, gw, None, None
 
 
-def variance_conv0_autograd(ref16, srcs16, rts, depth_values, conv0_weight, align_corners=False):
-    """ref16 [B,C/16,H,W,16]; srcs16 [V-1,B,C/16,H,W,16]; conv0_weight (8,C,3,3,3) -> conv0's raw output [B,D,H,W,8]."""
-    return _VarianceConv0.apply(ref16, srcs16, rts, depth_values, conv0_weight, align_corners)
+def variance_conv0_autograd(ref16, srcs16, rts, depth_values, conv0_weight, align_corners=False, act8=False):
+    """ref16 [B,C/16,H,W,16]; srcs16 [V-1,B,C/16,H,W,16]; conv0_weight (8,C,3,3,3) -> conv0's raw output [B,D,H,W,8].  act8: the
+    variance volume is kept for conv0's weight gradient in 8 bits (the other gradients do not read it)."""
+    return _VarianceConv0.apply(ref16, srcs16, rts, depth_values, conv0_weight, align_corners, act8)
 
 
 def conv2d_wgrad(x, g_cl, ksize, stride, planar=False):
@@ -1704,6 +1711,63 @@ def cas_depth_hypotheses(prev_depth, ndepth, interval, full_hw, stage_hw):
     return out
 
 
+# ------------------------------------------------------------ activations in 8 bits
+ACT8_BLOCK = 32
+
+
+def _aligned16(t):
+    """t, or a copy of it where a view begins off 16 bytes (the kernels' vector accesses)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _dtype_code(t, who):
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise MvsHipError(f"{who}: takes float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+class Act8:
+    """A tensor held in 8 bits: `codes` (int8, one per value in contiguous order), `scales` (uint8, one per block of 32 values),
+    the `shape` and `dtype` it was made from.  `nbytes`: what it keeps, 1.03 bytes per value."""
+    __slots__ = ("codes", "scales", "shape", "dtype")
+
+    def __init__(self, codes, scales, shape, dtype):
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, tuple(shape), dtype
+
+    @classmethod
+    def empty_for(cls, x):
+        n = x.numel()
+        return cls(torch.empty((n,), device=x.device, dtype=torch.int8),
+                   torch.empty(((n + ACT8_BLOCK - 1) // ACT8_BLOCK,), device=x.device, dtype=torch.uint8), x.shape, x.dtype)
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+
+def act8_quantize(x):
+    """x (float32, bfloat16 or float16, any shape) -> Act8.  Blocks of 32 consecutive values (contiguous order, the last one may be
+    shorter) share a power of two 2^k, the smallest with round(max|x| / 2^k) <= 127 (k >= -126); a value is
+    round-to-nearest-even(x / 2^k), off by at most half a step.  A block that holds an Inf or NaN reads back as NaN: a poisoned
+    activation stays one.  No gradient passes through (what a backward pass reads is a constant to it)."""
+    code = _dtype_code(x, "act8_quantize")
+    x = x.detach().contiguous()
+    held = Act8.empty_for(x)
+    check(_lib.load().mvs_act8_quantize(any_ptr(x), code, x.numel(), any_ptr(held.codes), any_ptr(held.scales), stream()), "mvs_act8_quantize")
+    return held
+
+
+def act8_dequantize(held, dtype=None):
+    """The values that an Act8 stands for, in the type it was made from (or `dtype`): codes times their block's power of two,
+    exact in float32 and bfloat16, at most the type's largest finite number."""
+    out = torch.empty(held.shape, device=held.codes.device, dtype=held.dtype if dtype is None else dtype)
+    code = _dtype_code(out, "act8_dequantize")
+    check(_lib.load().mvs_act8_dequantize(any_ptr(held.codes), any_ptr(held.scales), out.numel(), code, any_ptr(out), stream()),
+          "mvs_act8_dequantize")
+    return out
+
+
 class _BnReluCL(torch.autograd.Function):
     """Training-mode BatchNorm + optional ReLU + optional skip add on channels-last rows
     (mvs_bn_train_fwd_f32 / mvs_bn_train_bwd_f32); running statistics are updated in place."""
@@ -1751,14 +1815,70 @@ class _BnReluCL(torch.autograd.Function):
         return gx, gw, gb, (gy if ctx.has_skip else None), None, None, None, None, None, None, None
 
 
-def bn_relu_cl(x, bn, relu=True, skip=None, groups=1):
+class _BnReluAct8CL(torch.autograd.Function):
+    """_BnReluCL that keeps its input in 8 bits (act8_quantize's form, written by the pass that writes the output) and the ReLU's
+    mask as a bit per value: mvs_bn_train_fwd_act8_f32 / mvs_bn_train_bwd_act8_f32."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, skip, running_mean, running_var, nbt, momentum, eps, relu, groups):
+        x = _aligned16(_f32c(x))
+        C = x.shape[-1]
+        if x.shape[0] % groups:
+            raise MvsHipError(f"bn_relu_cl: leading dimension {x.shape[0]} is not a multiple of groups={groups}")
+        N = x.numel() // C // groups
+        lib = _lib.load()
+        nbytes = int(lib.mvs_bn_train_workspace_bytes(C))
+        if nbytes == 0:
+            raise MvsHipError(f"bn_relu_cl: C={C} not supported")
+        ws = torch.empty((nbytes // 4,), device=x.device, dtype=torch.float32)
+        w, b = _aligned16(_f32c(weight.detach())), _aligned16(_f32c(bias.detach()))
+        sk = _aligned16(_f32c(skip)) if skip is not None else None
+        mean = torch.empty((groups, C), device=x.device, dtype=torch.float32)
+        invstd = torch.empty_like(mean)
+        y = torch.empty_like(x)
+        held = Act8.empty_for(x)
+        mask = torch.empty(held.scales.shape, device=x.device, dtype=torch.int32) if relu else None
+        check(lib.mvs_bn_train_fwd_act8_f32(ptr(x), ptr(w), ptr(b), ptr(sk), int(groups), N, C, float(eps), float(momentum), int(relu),
+                                            ptr(running_mean), ptr(running_var), any_ptr(nbt), ptr(mean), ptr(invstd), ptr(y),
+                                            any_ptr(held.codes), any_ptr(held.scales), any_ptr(mask), ptr(ws), nbytes, stream()),
+              "mvs_bn_train_fwd_act8_f32")
+        ctx.save_for_backward(held.codes, held.scales, mask, w, mean, invstd)
+        ctx.has_skip, ctx.groups = skip is not None, int(groups)
+        ctx.mark_non_differentiable(*[t for t in (running_mean, running_var, nbt) if t is not None])
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        codes, scales, mask, w, mean, invstd = ctx.saved_tensors
+        gy = _aligned16(_f32c(gy))
+        C = gy.shape[-1]
+        N = gy.numel() // C // ctx.groups
+        lib = _lib.load()
+        nbytes = int(lib.mvs_bn_train_workspace_bytes(C))
+        ws = torch.empty((nbytes // 4,), device=gy.device, dtype=torch.float32)
+        gx = torch.empty_like(gy)
+        gw, gb = torch.empty_like(w), torch.empty_like(w)
+        check(lib.mvs_bn_train_bwd_act8_f32(ptr(gy), any_ptr(codes), any_ptr(scales), any_ptr(mask), ptr(w), ptr(mean), ptr(invstd),
+                                            ctx.groups, N, C, ptr(gx), ptr(gw), ptr(gb), ptr(ws), nbytes, stream()),
+              "mvs_bn_train_bwd_act8_f32")
+        return gx, gw, gb, (gy if ctx.has_skip else None), None, None, None, None, None, None, None
+
+
+def bn_relu_cl(x, bn, relu=True, skip=None, groups=1, act8=False):
     """relu(bn(x)) [+ skip] with batch statistics for a channels-last tensor [..., C] and an
     nn.BatchNorm module in training mode (momentum must be a number, affine + running stats).
     groups: x[0] splits into that many consecutive blocks, each normalised with its OWN statistics; the running statistics are
     updated once per block, in order -- what `groups` separate calls of the module would do (the reference's per-view FeatureNet
-    calls, mvsnet.py:146, as one batch)."""
+    calls, mvsnet.py:146, as one batch).
+    act8: x is kept for the backward pass in 8 bits (act8_quantize) and the ReLU's mask as bits, 1.16 bytes per value instead of 4.
+    The output is the same; the gradients are those of the normalised 8-bit values (exact in dL/dbias, within half a step of a
+    block's scale -- at most 1 / 127 of its largest magnitude -- where they use x)."""
     if bn.momentum is None or bn.weight is None:
         raise MvsHipError("bn_relu_cl: needs an affine BatchNorm with a numeric momentum")
+    if act8:
+        return _BnReluAct8CL.apply(x, bn.weight, bn.bias, skip, bn.running_mean, bn.running_var, bn.num_batches_tracked,
+                                   bn.momentum, bn.eps, relu, groups)
     return _BnReluCL.apply(x, bn.weight, bn.bias, skip, bn.running_mean, bn.running_var, bn.num_batches_tracked,
                            bn.momentum, bn.eps, relu, groups)
 
@@ -1948,3 +2068,116 @@ class _SoftmaxRegress(torch.autograd.Function):
 def softmax_regress_conf(cost, depth_values, clamp_idx=False, want_prob=False):
     """cost [B,D,H,W] -> (depth [B,H,W], photometric confidence [B,H,W], prob or None)."""
     return _SoftmaxRegress.apply(cost, depth_values, clamp_idx, want_prob)
+
+
+# ------------------------------------------------------------ rows by index, and a loss against a large table
+class _LookupRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, scale):
+        rows, C = table.shape
+        t = table.detach().contiguous()
+        out = torch.empty((*index.shape, C), device=t.device, dtype=t.dtype)
+        check(_lib.load().mvs_lookup_rows_fwd(any_ptr(t), DTYPES[t.dtype], rows, C, any_ptr(index), index.numel(), scale, any_ptr(out), stream()),
+              "mvs_lookup_rows_fwd")
+        ctx.save_for_backward(index)
+        ctx.cfg = (rows, C, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        index, = ctx.saved_tensors
+        rows, C, scale = ctx.cfg
+        g = g.contiguous()
+        n = index.numel()
+        lib = _lib.load()
+        nbytes = int(lib.mvs_lookup_rows_workspace_bytes(rows, C, n))
+        ws = torch.empty((nbytes,), device=g.device, dtype=torch.uint8)
+        grad = torch.empty((rows, C), device=g.device, dtype=g.dtype)
+        check(lib.mvs_lookup_rows_bwd(any_ptr(g), DTYPES[g.dtype], any_ptr(index), n, rows, C, scale, any_ptr(grad), any_ptr(ws), nbytes,
+                                      stream()), "mvs_lookup_rows_bwd")
+        return grad, None, None
+
+
+def lookup_rows(table, index, scale=1.0):
+    """scale * table[index]: table [rows, C] (float32, bfloat16 or float16), index of whole numbers in any shape -> [*index.shape, C].
+    The product is rounded once.  An index outside [0, rows) names no row (a point that projects outside the map): a row of zeros,
+    no gradient.  The table's gradient is dense, summed in float32 in the order of the indices (sorted, stably; no atomics): equal
+    calls give equal bits however often an index repeats."""
+    _dtype_code(table, "lookup_rows")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise MvsHipError(f"lookup_rows: the table is [rows, C], got {tuple(table.shape)}")
+    if index.dtype not in (torch.int64, torch.int32):
+        raise MvsHipError(f"lookup_rows: the index holds int64 or int32, got {index.dtype}")
+    if index.device != table.device:
+        raise MvsHipError(f"lookup_rows: index on {index.device}, table on {table.device}")
+    return _LookupRows.apply(table, index.to(torch.int64).contiguous(), float(scale))
+
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, scale, ignore_index, reduction):
+        n, C = x.shape
+        V = weight.shape[0]
+        xd, wd = _aligned16(x.detach().contiguous()), _aligned16(weight.detach().contiguous())
+        code = DTYPES[xd.dtype]
+        lib = _lib.load()
+        nbytes = int(lib.mvs_linear_ce_workspace_bytes(n, V, C, code, 0, 0, 0))
+        ws = torch.empty((nbytes,), device=xd.device, dtype=torch.uint8)
+        loss = torch.empty((n,) if reduction == 0 else (), device=xd.device, dtype=torch.float32)
+        state = torch.empty((n + 1,), device=xd.device, dtype=torch.float32)      # the rows' lse, and how many rows were kept
+        check(lib.mvs_linear_ce_fwd(any_ptr(xd), any_ptr(wd), code, any_ptr(target), n, V, C, scale, ignore_index, reduction, any_ptr(loss),
+                                    any_ptr(state[:n]), any_ptr(state[n:]), any_ptr(ws), nbytes, stream()), "mvs_linear_ce_fwd")
+        ctx.save_for_backward(xd, wd, target, state)
+        ctx.cfg = (scale, ignore_index, reduction)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w, target, state = ctx.saved_tensors
+        scale, ignore_index, reduction = ctx.cfg
+        n, C = x.shape
+        V = w.shape[0]
+        need_x, need_w = ctx.needs_input_grad[:2]
+        lib = _lib.load()
+        g = _f32c(g)
+        code = DTYPES[x.dtype]
+        nbytes = int(lib.mvs_linear_ce_workspace_bytes(n, V, C, code, 1, int(need_x), int(need_w)))
+        ws = torch.empty((nbytes,), device=x.device, dtype=torch.uint8)
+        gx = torch.empty_like(x) if need_x else None
+        gw = torch.empty_like(w) if need_w else None
+        check(lib.mvs_linear_ce_bwd(any_ptr(x), any_ptr(w), code, any_ptr(target), any_ptr(state[:n]), any_ptr(state[n:]), ptr(g), n, V, C,
+                                    scale, ignore_index, reduction, any_ptr(gx), any_ptr(gw), any_ptr(ws), nbytes, stream()),
+              "mvs_linear_ce_bwd")
+        return gx, gw, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of the logits scale * x @ weight.T, which are never stored: x [..., C], weight [V, C] of one type
+    (float32, bfloat16, float16), target [...] of class numbers -> the mean over the rows kept, the sum, or ("none") each row's
+    loss, in float32 -- torch.nn.functional.cross_entropy(scale * x @ weight.T, target, ignore_index=..., reduction=...) without the
+    [rows, V] tensor, forward or backward.  scale is one over a temperature.
+    A row with target == ignore_index has loss 0 and leaves no trace in a gradient, whatever x holds there (the mean over no row at
+    all is 0 / 0 = NaN, its gradients zero); any other target outside [0, V) makes its row's loss and the gradients NaN.
+    Products are summed in float32.  For 16-bit operands the backward pass rounds each logit's gradient to that type before its two
+    products (half a unit in the last place of each term, of either sign); float32 stays float32 throughout."""
+    _dtype_code(x, "linear_cross_entropy")
+    if weight.dtype != x.dtype:
+        raise MvsHipError(f"linear_cross_entropy: x is {x.dtype}, weight {weight.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise MvsHipError(f"linear_cross_entropy: x is [..., C] and weight [V, C], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if tuple(target.shape) != tuple(x.shape[:-1]):
+        raise MvsHipError(f"linear_cross_entropy: target {tuple(target.shape)} does not fit x {tuple(x.shape)}")
+    if target.dtype not in (torch.int64, torch.int32):
+        raise MvsHipError(f"linear_cross_entropy: the target holds int64 or int32, got {target.dtype}")
+    if not (x.device == weight.device == target.device):
+        raise MvsHipError(f"linear_cross_entropy: x on {x.device}, weight on {weight.device}, target on {target.device}")
+    if reduction not in _REDUCTIONS:
+        raise MvsHipError(f"linear_cross_entropy: reduction is 'none', 'mean' or 'sum', got {reduction!r}")
+    loss = _LinearCrossEntropy.apply(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1).to(torch.int64).contiguous(), float(scale),
+                                     int(ignore_index), _REDUCTIONS[reduction])
+    return loss.reshape(target.shape) if reduction == "none" else loss

@@ -145,11 +145,28 @@ def prepare_step(feature, costreg):
         _dgrad3(costreg.prob.weight, False, 1)
 
 
+def _save_input(ctx, x, weight, act8):
+    """What a convolution keeps for its backward pass: the weight and its input -- in float32, or (act8) as 8-bit codes and scales
+    (ops.act8_quantize), a quarter of the bytes.  Only the weight gradient reads the input; the input gradient does not."""
+    ctx.x_shape = x.shape
+    if act8 and ctx.needs_input_grad[1]:
+        held = ops.act8_quantize(x)
+        ctx.save_for_backward(weight, held.codes, held.scales)
+    else:
+        ctx.save_for_backward(weight, x)
+
+
+def _saved_input(ctx):
+    """The input again: float32 values of the 8-bit form live for the length of the weight gradient's launch only."""
+    kept = ctx.saved_tensors[1:]
+    return kept[0] if len(kept) == 1 else ops.act8_dequantize(ops.Act8(*kept, ctx.x_shape, torch.float32))
+
+
 class _Conv3dCL(torch.autograd.Function):
     """x [B,D,H,W,Ci] -> raw convolution output [B,Do,Ho,Wo,Co] (no bias, no affine)."""
 
     @staticmethod
-    def forward(ctx, x, weight, transposed, stride, tag):
+    def forward(ctx, x, weight, transposed, stride, tag, act8=False):
         x = x.contiguous()
         w = weight.detach().contiguous()
         # (split-operand bf16 kernels where the shape has one)
@@ -159,13 +176,13 @@ class _Conv3dCL(torch.autograd.Function):
         with ops.stage(f"train.{tag}.fwd"):
             out = ops.conv3d(x, w, None, None, None, False, transposed, stride, channels_last=True,
                              packed=packed)
-        ctx.save_for_backward(x, weight)
+        _save_input(ctx, x, weight, act8)
         ctx.cfg = (transposed, stride, tag)
         return out
 
     @staticmethod
     def backward(ctx, g):
-        x, weight = ctx.saved_tensors
+        xshape, weight = ctx.x_shape, ctx.saved_tensors[0]
         transposed, stride, tag = ctx.cfg
         g = g.contiguous()
         w = weight.detach()
@@ -178,7 +195,7 @@ class _Conv3dCL(torch.autograd.Function):
                 with ops.stage(f"train.{tag}.dgrad"):
                     gx = ops.conv3d(g, wt, channels_last=True, packed=pk)
             elif not transposed:
-                if any(s % 2 for s in x.shape[1:4]):
+                if any(s % 2 for s in xshape[1:4]):
                     raise ops.MvsHipError("stride-2 conv backward needs even D, H, W")
                 wc = w.contiguous()                                            # (Co,Ci,k) as a deconv weight
                 pk = _dgrad3(weight, False, 2)
@@ -193,8 +210,8 @@ class _Conv3dCL(torch.autograd.Function):
                     gx = ops.conv3d(g, wc, stride=stride, channels_last=True, packed=pk)
         if ctx.needs_input_grad[1]:
             with ops.stage(f"train.{tag}.wgrad"):
-                gw = _wgrad(x, g, transposed, stride, weight.shape)
-        return gx, gw, None, None, None
+                gw = _wgrad(_saved_input(ctx), g, transposed, stride, weight.shape)
+        return gx, gw, None, None, None, None
 
 
 _SPLIT = 16384   # voxels per split-K slice
@@ -243,19 +260,20 @@ def _wgrad(x, g, transposed, stride, wshape):
     return gw
 
 
-def conv3d_cl(x, weight, transposed=False, stride=1, tag="conv3d"):
-    return _Conv3dCL.apply(x, weight, transposed, stride, tag)
+def conv3d_cl(x, weight, transposed=False, stride=1, tag="conv3d", act8=False):
+    """act8: the input is kept for the weight gradient in 8 bits (ops.act8_quantize)."""
+    return _Conv3dCL.apply(x, weight, transposed, stride, tag, act8)
 
 
-def conv_bn_relu_cl(x, conv, bn, transposed=False, stride=1, skip=None, tag="conv3d"):
+def conv_bn_relu_cl(x, conv, bn, transposed=False, stride=1, skip=None, tag="conv3d", act8=False):
     """ConvBnReLU3D / deconv block of the reference (module.py:26-33, mvsnet.py:66-79) in
     channels-last with batch statistics when bn.training (running stats are updated); `skip`
     is added after the ReLU (mvsnet.py:89-91).  BatchNorm + ReLU + skip are one fused HIP op
-    when the channel count has a kernel, torch ops otherwise."""
-    y = conv3d_cl(x, conv.weight, transposed, stride, tag)
+    when the channel count has a kernel, torch ops otherwise.  act8: both of them keep their inputs in 8 bits."""
+    y = conv3d_cl(x, conv.weight, transposed, stride, tag, act8)
     C = y.shape[-1]
     if bn.training and C in (8, 16, 32, 64) and bn.momentum is not None and bn.weight is not None:
-        return ops.bn_relu_cl(y, bn, True, skip)
+        return ops.bn_relu_cl(y, bn, True, skip, act8=act8)
     out = _bn_relu_torch(y, bn)
     return out if skip is None else skip + out
 
@@ -299,27 +317,27 @@ class _Conv2dCL(torch.autograd.Function):
     output parity) + mvs_interleave2x2_f32; the weight gradient is mvs_conv2d_wgrad_f32."""
 
     @staticmethod
-    def forward(ctx, x, weight, stride, planar):
+    def forward(ctx, x, weight, stride, planar, act8=False):
         x = x.contiguous()
         w = weight.detach().contiguous()
         cout, cin, k, _ = w.shape
         pk = _pk2(weight, stride)
         with ops.stage("train.feature.fwd"):
             out = ops.conv2d(x, pk, cin, cout, k, stride, None, None, False, planar=planar)
-        ctx.save_for_backward(x, weight)
+        _save_input(ctx, x, weight, act8 and not planar)      # (the image is the caller's: keeping it costs nothing)
         ctx.cfg = (stride, planar)
         return out
 
     @staticmethod
     def backward(ctx, g):
-        x, weight = ctx.saved_tensors
+        xshape, weight = ctx.x_shape, ctx.saved_tensors[0]
         stride, planar = ctx.cfg
         g = g.contiguous()
         w = weight.detach()
         cout, cin, k, _ = w.shape
         gx = gw = None
         if ctx.needs_input_grad[0]:
-            H, W = (x.shape[2], x.shape[3]) if planar else (x.shape[1], x.shape[2])
+            H, W = (xshape[2], xshape[3]) if planar else (xshape[1], xshape[2])
             with ops.stage("train.feature.dgrad"):
                 if stride == 1 and ops.conv2d_supported(cout, cin, k, 1) and not planar:
                     pk = _dgrad2_s1(weight)
@@ -337,22 +355,24 @@ class _Conv2dCL(torch.autograd.Function):
                     gx = gx if planar else gx.permute(0, 2, 3, 1).contiguous()
         if ctx.needs_input_grad[1]:
             with ops.stage("train.feature.wgrad"):
-                gw = ops.conv2d_wgrad(x, g, k, stride, planar)
-        return gx, gw, None, None
+                gw = ops.conv2d_wgrad(_saved_input(ctx), g, k, stride, planar)
+        return gx, gw, None, None, None
 
 
-def conv2d_cl(x, weight, stride=1, planar=False):
-    return _Conv2dCL.apply(x, weight, stride, planar)
+def conv2d_cl(x, weight, stride=1, planar=False, act8=False):
+    """act8: the input (a planar image apart) is kept for the weight gradient in 8 bits (ops.act8_quantize)."""
+    return _Conv2dCL.apply(x, weight, stride, planar, act8)
 
 
-def conv2d_bn_relu_cl(x, conv, bn, stride=1, planar=False, groups=1):
+def conv2d_bn_relu_cl(x, conv, bn, stride=1, planar=False, groups=1, act8=False):
     """ConvBnReLU of the reference (module.py:6-13) in channels-last: the HIP convolution + the fused HIP BatchNorm
     (batch statistics when bn.training, running statistics updated) + ReLU.  groups: the images of x are that many
-    consecutive blocks (views), each with its own batch statistics -- `groups` calls of the reference's module as one."""
-    y = conv2d_cl(x, conv.weight, stride, planar)
+    consecutive blocks (views), each with its own batch statistics -- `groups` calls of the reference's module as one.  act8: the
+    convolution and the BatchNorm keep their inputs in 8 bits."""
+    y = conv2d_cl(x, conv.weight, stride, planar, act8)
     C = y.shape[-1]
     if bn.training and C in (8, 16, 32, 64) and bn.momentum is not None and bn.weight is not None:
-        return ops.bn_relu_cl(y, bn, groups=groups)
+        return ops.bn_relu_cl(y, bn, groups=groups, act8=act8)
     outs = []
     for yg in y.chunk(groups, 0):       # torch ops: one module call per group, as the reference
         y2 = F.batch_norm(yg.reshape(-1, C), bn.running_mean, bn.running_var, bn.weight, bn.bias,

@@ -1,0 +1,494 @@
+"""The training operators that keep no large tensor, on the GPU, against plain implementations in 64 bits.
+
+Tolerances are error bounds: u = 2^-24 (float32 rounding), h = half a unit in the last place of the operand type (finfo.eps / 2)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from mvs_amd import ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def half_ulp(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(*shape, seed=0):
+    return torch.randn(*shape, generator=gen(seed), device="cuda")
+
+
+# ------------------------------------------------------------------ activations in 8 bits
+def act8_by_definition(x):
+    """(codes, scales) from the definition, in 64 bits on the host."""
+    v = x.detach().double().cpu().numpy().reshape(-1)
+    n = v.size
+    v = np.concatenate([v, np.zeros(-n % 32)]).reshape(-1, 32)
+    codes, scales = np.zeros(v.shape, np.int8), np.zeros(len(v), np.uint8)
+    for b, row in enumerate(v):
+        if not np.isfinite(row).all():
+            scales[b] = 255
+            continue
+        most, k = np.abs(row).max(), -126
+        if most > 0:
+            k = max(-126, int(math.floor(math.log2(most))) - 8)
+        while np.rint(most * 2.0 ** -k) > 127:
+            k += 1
+        codes[b], scales[b] = np.rint(row * 2.0 ** -k), k + 127
+    return codes.reshape(-1)[:n], scales
+
+
+def values_of(codes, scales, shape):
+    step = np.where(scales == 255, np.nan, 2.0 ** (scales.astype(np.float64) - 127))
+    return torch.from_numpy(codes.astype(np.float64) * np.repeat(step, 32)[:codes.size]).reshape(shape)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1,), (7,), (31,), (32,), (33,), (64, 8), (5, 77), (3, 1024), (2, 5, 7, 16), (65, 1031)])
+def test_act8_is_its_definition_bit_for_bit(shape, dtype):
+    x = (randn(*shape, seed=len(shape)) * torch.exp(2 * randn(*shape, seed=3))).to(dtype)
+    held = ops.act8_quantize(x)
+    codes, scales = act8_by_definition(x)
+    assert np.array_equal(held.codes.cpu().numpy(), codes) and np.array_equal(held.scales.cpu().numpy(), scales)
+    back = ops.act8_dequantize(held)
+    assert back.dtype == dtype and back.shape == x.shape and held.nbytes == x.numel() + -(-x.numel() // 32)
+    assert torch.equal(back.cpu(), values_of(codes, scales, shape).to(dtype))
+    for other in TYPES:
+        assert torch.equal(ops.act8_dequantize(held, other).cpu().double().clamp(-1e30, 1e30),
+                           values_of(codes, scales, shape).clamp(-torch.finfo(other).max, torch.finfo(other).max).to(other).double().clamp(-1e30, 1e30))
+
+
+def test_act8_extreme_values():
+    big = torch.finfo(torch.float32).max
+    rows = [[0.0] * 32, [big] * 32, [-big] + [1.0] * 31, [1e-45] * 32, [1e-38, -3e-39] * 16, [127.0, 127.49, -127.49, 0.5, 1.5, 2.5, -0.5, -1.5] * 4,
+            [127.5, 0.5] * 16, [255.0 / 128, 1.0] * 16, [2.0 ** -120] * 32, [-0.0] * 32]
+    x = torch.tensor(rows, device="cuda")
+    held = ops.act8_quantize(x)
+    codes, scales = act8_by_definition(x)
+    assert np.array_equal(held.codes.cpu().numpy(), codes) and np.array_equal(held.scales.cpu().numpy(), scales)
+    back = ops.act8_dequantize(held)
+    assert torch.isfinite(back).all() and float(back[1, 0]) == big
+    h = torch.full((64,), 65504.0, device="cuda", dtype=torch.float16)
+    assert torch.equal(ops.act8_dequantize(ops.act8_quantize(h)), h)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_act8_a_poisoned_block_reads_back_as_nan_and_no_other(bad, dtype):
+    x = randn(100, seed=1).to(dtype)
+    x[40] = bad
+    x[99] = bad
+    back = ops.act8_dequantize(ops.act8_quantize(x))
+    assert torch.isnan(back[32:64]).all() and torch.isnan(back[96:]).all() and torch.isfinite(back[:32]).all() and torch.isfinite(back[64:96]).all()
+
+
+def test_act8_strides_offsets_and_empty_tensors():
+    x = randn(64, 40, seed=5)
+    for view in (x.t(), x[:, ::2], x[1:, 1:], x.reshape(-1)[3:], x.half().reshape(-1)[1:]):
+        a, b = ops.act8_quantize(view), ops.act8_quantize(view.clone(memory_format=torch.contiguous_format))
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+        assert torch.equal(ops.act8_dequantize(a), ops.act8_dequantize(b))
+    empty = ops.act8_quantize(torch.empty(0, 8, device="cuda"))
+    assert ops.act8_dequantize(empty).shape == (0, 8) and empty.nbytes == 0
+
+
+def bn_by_formula(x, held, gy, w, b, skip, relu, groups, eps):
+    """y and the gradients in 64 bits; x [G, N, C]; the backward sees `held` (the values of the 8-bit form) and the forward's mask."""
+    x, gy, w, b = x.double(), gy.double(), w.double(), b.double()
+    mean, var = x.mean(1, keepdim=True), x.var(1, keepdim=True, unbiased=False)
+    inv = 1 / torch.sqrt(var + eps)
+    z = (x - mean) * inv * w + b
+    y = torch.relu(z) if relu else z
+    dz = gy * (z > 0) if relu else gy
+    hat = (held.double() - mean) * inv
+    dx = w * inv * (dz - dz.mean(1, keepdim=True) - hat * (dz * hat).mean(1, keepdim=True))
+    return y + (skip.double() if skip is not None else 0), dx, (dz * hat).sum((0, 1)), dz.sum((0, 1)), z, (dz, hat, inv, w)
+
+
+@pytest.mark.parametrize("relu", [True, False])
+@pytest.mark.parametrize("C,N,groups,skip", [(8, 1, 1, False), (8, 7, 3, True), (8, 1000, 1, True), (16, 333, 2, False), (32, 65, 5, True), (64, 129, 1, False),
+                                            (8, 5003, 3, True)])
+def test_bn_act8_against_the_formula(C, N, groups, skip, relu):
+    x = randn(groups, N, C, seed=1) * 2 + randn(C, seed=2)
+    bn, plain = torch.nn.BatchNorm2d(C).cuda().train(), torch.nn.BatchNorm2d(C).cuda().train()
+    with torch.no_grad():
+        bn.weight.copy_(1 + 0.3 * randn(C, seed=3))
+        bn.bias.copy_(0.5 * randn(C, seed=4))
+    plain.load_state_dict(bn.state_dict())
+    with torch.no_grad():      # off the ReLU's corner, where either gradient is right
+        mean, var = x.double().mean(1, keepdim=True), x.double().var(1, keepdim=True, unbiased=False)
+        z = (x - mean) / torch.sqrt(var + bn.eps) * bn.weight + bn.bias
+        x = x + 0.05 * (z.abs() < 1e-4).float()
+    sk = randn(groups, N, C, seed=6) if skip else None
+    gy = randn(groups, N, C, seed=7)
+    leaves = [x.clone().requires_grad_(), bn.weight, bn.bias] + ([sk.clone().requires_grad_()] if skip else [])
+    y = ops.bn_relu_cl(leaves[0], bn, relu=relu, skip=leaves[3] if skip else None, groups=groups, act8=True)
+    grads = torch.autograd.grad(y, leaves, gy)
+    # the output and the running statistics are those of the block that keeps float32
+    assert torch.equal(y, ops.bn_relu_cl(x, plain, relu=relu, skip=sk, groups=groups))
+    assert torch.equal(bn.running_mean, plain.running_mean) and torch.equal(bn.running_var, plain.running_var)
+    assert int(bn.num_batches_tracked) == groups
+    held = ops.act8_dequantize(ops.act8_quantize(x))
+    want_y, want_dx, want_dw, want_db, _, (dz, hat, inv, w) = bn_by_formula(x, held, gy, bn.weight.detach(), bn.bias.detach(), sk, relu, groups, bn.eps)
+    if skip:
+        assert torch.equal(grads[3], gy)
+    if N == 1:
+        # one row: the variance is 0, x - mean a rounding of 0 and 1 / sqrt(eps) = 316 multiplies whatever the codes are off by
+        # -- the formula's dx is 0 only for held == x; what is asserted is that dL/dbias does not depend on it
+        assert torch.allclose(grads[2].double(), want_db, atol=4 * U * float(gy.abs().sum()))
+        return
+    # dx = inv w (dz - k2 - xm k1): about ten float32 roundings of terms of these magnitudes, mean and inv rounded once each (the
+    # mean's rounding moves hat by u |mean| inv)
+    n = dz.shape[1]
+    shift = x.double().abs().amax() * inv
+    scale = w.abs() * inv * (dz.abs() + dz.abs().mean(1, keepdim=True) + (hat.abs() + shift) * (dz * hat).abs().mean(1, keepdim=True)
+                             + hat.abs() * (dz.abs() * shift).mean(1, keepdim=True))
+    assert ((grads[0].double() - want_dx).abs() <= 16 * U * scale).all()
+    assert ((grads[1].double() - want_dw).abs() <= 16 * U * (dz.abs() * (hat.abs() + shift)).sum((0, 1))).all()
+    assert ((grads[2].double() - want_db).abs() <= 4 * U * dz.abs().sum((0, 1))).all()
+
+
+def test_bn_act8_keeps_a_third_of_the_memory():
+    x = randn(1, 200_000, 8, seed=1).requires_grad_()
+    bn = torch.nn.BatchNorm2d(8).cuda().train()
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.numel() * t.element_size()) or t, lambda t: t):
+        ops.bn_relu_cl(x, bn, act8=True)
+    assert sum(kept) < 1.2 * x.numel()
+
+
+# ------------------------------------------------------------------ rows by index
+def lookup_bound(table, index, g, scale):
+    """The gradient in 64 bits, and the error bound of a float32 sum of a row's k terms, rounded to the type once."""
+    ok = (index >= 0) & (index < table.shape[0])
+    at = torch.where(ok, index, 0)
+    g = torch.where(ok.unsqueeze(-1), g.double(), torch.zeros((), dtype=torch.float64, device=g.device))
+    C = table.shape[1]
+    want, mag = (torch.zeros(table.shape, dtype=torch.float64, device="cuda").index_put_((at.reshape(-1),), t.reshape(-1, C), accumulate=True)
+                 for t in (g, g.abs()))
+    count = torch.zeros(table.shape[0], dtype=torch.float64, device="cuda").index_put_((at.reshape(-1),), ok.double().reshape(-1), accumulate=True)
+    bound = abs(scale) * mag * (count.unsqueeze(1) + 2) * U + half_ulp(table.dtype) * abs(scale) * mag + torch.finfo(table.dtype).smallest_normal
+    return want * scale, bound
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,C,n", [(1, 1, 1), (1, 8, 50), (5, 3, 17), (100, 8, 1), (64, 32, 64), (65, 33, 200), (1000, 257, 333), (20480, 32, 1021),
+                                      (300, 2048, 129), (7, 64, 9000), (5000, 16, 20011), (40000, 40, 8193)])
+def test_lookup_rows_and_its_gradient(rows, C, n, dtype):
+    table = randn(rows, C, seed=rows).to(dtype).requires_grad_()
+    index = torch.randint(rows, (n,), generator=gen(n), device="cuda")
+    index[::3] = int(index[0])                                  # one index makes up a third: its run spans many pieces
+    if n > 4:
+        index[1], index[3] = -1, rows                       # these name no row
+    scale = 1.7
+    out = ops.lookup_rows(table, index, scale)
+    ok = (index >= 0) & (index < rows)
+    # The product of a float32 scale and a 16-bit value takes up to 35 bits.  A multiplication in float32 and one rounding to the type
+    # give (1 + u)(1 + h) at worst, a multiply-and-round instruction (float16 has one) 1 + h: both are within h + u + h u of the
+    # exact product, plus half the spacing of the type's subnormal numbers
+    want = table.detach()[torch.where(ok, index, 0)].double() * float(np.float32(scale)) * ok.unsqueeze(1)
+    h = half_ulp(dtype)
+    assert ((out.double() - want).abs() <= (h + U + h * U) * want.abs() + torch.finfo(dtype).smallest_normal * h).all()
+    assert (out[~ok] == 0).all()
+    g = randn(n, C, seed=2).to(dtype)
+    grad, = torch.autograd.grad(out, table, g, retain_graph=True)
+    want, bound = lookup_bound(table, index, g, scale)
+    assert ((grad.double() - want).abs() <= bound).all()
+    untouched = torch.ones(rows, dtype=torch.bool, device="cuda")
+    untouched[index[ok]] = False
+    assert (grad[untouched] == 0).all()
+    again, = torch.autograd.grad(out, table, g)
+    assert torch.equal(grad, again)
+
+
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 30000])
+def test_lookup_rows_gradient_order_is_the_indices_order(n):
+    """Equal keys are summed in their order: with terms 2^24, 1, ..., 1, -2^24 any other order gives another float32 sum."""
+    index = torch.full((n,), 3, device="cuda")
+    index[:16] = torch.tensor([3, 1] * 8, device="cuda")
+    table = torch.zeros(5, 4, device="cuda", requires_grad=True)
+    g = torch.zeros(n, 4, device="cuda")
+    g[1], g[3:15:2], g[15] = 2.0 ** 24, 1.0, -2.0 ** 24      # index 1's eight terms: 2^24 + 1 + ... (each lost) - 2^24 = 0
+    grad, = torch.autograd.grad(ops.lookup_rows(table, index), table, g)
+    assert (grad[1] == 0).all() and (grad[[0, 2, 4]] == 0).all()
+
+
+def test_lookup_rows_shapes_strides_and_empty():
+    table = randn(50, 16, seed=1)
+    index = torch.randint(50, (4, 6), generator=gen(2), device="cuda")
+    for t in (table, randn(16, 50, seed=3).t(), randn(50, 32, seed=4)[:, ::2], randn(51, 16, seed=5)[1:], randn(50, 17, seed=6)[:, 1:]):
+        for i in (index, index.t(), index.to(torch.int32), index[:, :1]):
+            leaf = t.detach().requires_grad_()
+            out = ops.lookup_rows(leaf, i, 0.5)
+            assert torch.equal(out, t[i.long()] * 0.5)
+            grad, = torch.autograd.grad(out, leaf, torch.ones_like(out))
+            assert torch.equal(grad[:, 0], 0.5 * torch.bincount(i.long().reshape(-1), minlength=50).float())
+    leaf = table.clone().requires_grad_()
+    out = ops.lookup_rows(leaf, torch.empty(0, dtype=torch.int64, device="cuda"))
+    assert out.shape == (0, 16)
+    grad, = torch.autograd.grad(out, leaf, torch.empty(0, 16, device="cuda"))
+    assert (grad == 0).all()
+
+
+# ------------------------------------------------------------------ cross entropy against a large table
+def ce_case(n, V, C, dtype, ignored=0.2, sharp=1.0, seed=0):
+    w = randn(V, C, seed=seed + 1) / math.sqrt(C)
+    t = torch.randint(V, (n,), generator=gen(seed + 2), device="cuda")
+    x = (randn(n, C, seed=seed + 3) + w[t] * 2).to(dtype)
+    t[torch.rand(n, generator=gen(seed + 4), device="cuda") < ignored] = -100
+    return x, w.to(dtype), t, sharp
+
+
+def ce_bounds(x, w, t, scale, ignore, g_row):
+    """Row losses and gradients in 64 bits (g_row: dL/dloss_n) with bounds of the kernels' error.
+    A logit: C products summed in float32, in any order, and the scale: (C + 4) u scale |x||w|^T =: d (base-2 scaling included).
+    A row's lse moves by at most the largest d of the row, its terms are summed in float32 (a tile's 128 terms, then tiles):
+    e = max d + (V / 128 + 160) u.  p: relative error 2 e + 8 u.  dl rounded to the type (h), its unit's smallest normal number
+    for float16.  The products: one float32 sum over V (or n) terms.  The result rounded once."""
+    dtype = x.dtype
+    xd, wd = x.double(), w.double()
+    kept = t != ignore
+    xd = torch.where(kept.unsqueeze(1), xd, torch.zeros((), dtype=torch.float64, device=x.device))
+    at = torch.where(kept, t, 0)
+    n, V, C = x.shape[0], w.shape[0], x.shape[1]
+    l = scale * (xd @ wd.t())
+    d = (C + 4) * U * abs(scale) * (xd.abs() @ wd.abs().t()) + 4 * U * l.abs()
+    e = d.amax(1, keepdim=True) + (V / 128 + 160) * U
+    lse = torch.logsumexp(l, 1, keepdim=True)
+    own = l.gather(1, at.unsqueeze(1))
+    loss = torch.where(kept, (lse - own).squeeze(1), torch.zeros((), dtype=torch.float64, device=x.device))
+    loss_bound = (2 * e + 4 * U * (lse.abs() + own.abs())).squeeze(1)
+    p = torch.exp(l - lse)
+    dl = p.clone()
+    dl[torch.arange(n, device=x.device), at] -= 1
+    h = half_ulp(dtype) if dtype != torch.float32 else U
+    tiny = 2.0 ** -25 / 16384 if dtype == torch.float16 else 0.0
+    dl_err = p * (2 * e + 8 * U) + 2 * h * dl.abs() + tiny
+    grow = (torch.where(kept, g_row.double(), torch.zeros((), dtype=torch.float64, device=x.device)) * scale).unsqueeze(1)
+    small = torch.finfo(dtype).smallest_normal * (2.0 ** -10 if dtype == torch.float16 else 1)
+    dx, dw = (dl * grow) @ wd, (dl * grow).t() @ xd
+    dx_bound = (dl_err * grow.abs()) @ wd.abs() + (V + 8) * U * (dl.abs() * grow.abs()) @ wd.abs()
+    dw_bound = (dl_err * grow.abs()).t() @ xd.abs() + (n + 8) * U * (dl.abs() * grow.abs()).t() @ xd.abs()
+    return loss, loss_bound, dx, dx_bound + half_ulp(dtype) * (dx.abs() + dx_bound) + small, dw, dw_bound + half_ulp(dtype) * (dw.abs() + dw_bound) + small
+
+
+def ce_check(x, w, t, scale, ignore=-100, reduction="mean", seed=9):
+    leaves = [x.detach().requires_grad_(), w.detach().requires_grad_()]
+    loss = ops.linear_cross_entropy(*leaves, t, scale=scale, ignore_index=ignore, reduction=reduction)
+    n, kept = x.shape[0], int((t != ignore).sum())
+    g = randn(n, seed=seed) if reduction == "none" else torch.tensor(0.7, device="cuda")
+    g_row = g if reduction == "none" else (g / kept if reduction == "mean" and kept else g).expand(n)
+    want, bound, dx, dx_bound, dw, dw_bound = ce_bounds(x, w, t, scale, ignore, g_row)
+    got_dx, got_dw = torch.autograd.grad(loss, leaves, g)
+    assert loss.dtype == torch.float32 and got_dx.dtype == x.dtype and got_dw.dtype == w.dtype
+    if reduction == "none":
+        assert ((loss.double() - want).abs() <= bound).all()
+    elif reduction == "sum":
+        assert abs(float(loss) - float(want.sum())) <= float(bound.sum()) + U * float(want.sum())
+    elif kept:
+        assert abs(float(loss) - float(want.sum() / kept)) <= float(bound.max()) + 2 * U * float(want.sum() / kept)
+    else:
+        assert math.isnan(float(loss))
+    assert ((got_dx.double() - dx).abs() <= dx_bound).all(), float(((got_dx.double() - dx).abs() / dx_bound).max())
+    assert ((got_dw.double() - dw).abs() <= dw_bound).all(), float(((got_dw.double() - dw).abs() / dw_bound).max())
+    assert (got_dx[t == ignore] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,C", [(1, 1, 1), (1, 2, 3), (2, 129, 8), (1, 1000, 64), (17, 130, 32), (64, 128, 33), (100, 257, 100), (129, 2000, 64),
+                                   (130, 511, 200), (33, 5000, 320), (300, 300, 16)])
+def test_linear_cross_entropy(n, V, C, dtype):
+    x, w, t, _ = ce_case(n, V, C, dtype, seed=n)
+    t[0] = min(t.clamp(min=0).max(), V - 1)
+    ce_check(x, w, t, 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_linear_cross_entropy_reductions_and_scales(reduction, dtype):
+    x, w, t, _ = ce_case(150, 700, 48, dtype, seed=5)
+    for scale in (1.0, 8.0, 0.125, -2.0):
+        ce_check(x, w, t, scale, reduction=reduction)
+    ce_check(x, w, t.clamp(min=3), 1.0, ignore=3, reduction=reduction)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_in_pieces_of_the_table(dtype):
+    """n V beyond 2^26: the backward pass walks the table in more than one piece, the last of them a ragged one."""
+    x, w, t, _ = ce_case(1025, 70001, 8, dtype, seed=6)
+    ce_check(x, w, t, 2.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_no_row_kept(dtype):
+    x, w, t, _ = ce_case(20, 50, 16, dtype, ignored=2.0)
+    for reduction in ("mean", "sum", "none"):
+        ce_check(x, w, t, 1.0, reduction=reduction)
+    x = torch.empty(0, 16, device="cuda", dtype=dtype, requires_grad=True)
+    w = w.detach().requires_grad_()
+    empty = torch.empty(0, dtype=torch.int64, device="cuda")
+    assert math.isnan(float(ops.linear_cross_entropy(x, w, empty)))
+    loss = ops.linear_cross_entropy(x, w, empty, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, (x, w))
+    assert float(loss) == 0 and gx.shape == (0, 16) and (gw == 0).all()
+    assert ops.linear_cross_entropy(x, w, empty, reduction="none").shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_linear_cross_entropy_what_an_ignored_row_holds_leaves_no_trace(bad, dtype):
+    x, w, t, _ = ce_case(70, 200, 40, dtype, seed=7)
+    t[3] = t[50] = -100
+    clean = x.clone()
+    clean[[3, 50]] = 0
+    x[3], x[50, 5] = bad, bad
+    res = []
+    for rows in (x, clean):
+        leaves = [rows.detach().requires_grad_(), w.detach().requires_grad_()]
+        loss = ops.linear_cross_entropy(*leaves, t)
+        res.append([loss.detach(), *torch.autograd.grad(loss, leaves)])
+    for a, b in zip(*res):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_poisoned_rows_show(dtype):
+    x, w, t, _ = ce_case(10, 200, 40, dtype, ignored=0.0, seed=8)
+    for bad_t in (-1, 200, 2 ** 40):
+        t2 = t.clone()
+        t2[4] = bad_t
+        leaves = [x.detach().requires_grad_(), w.detach().requires_grad_()]
+        loss = ops.linear_cross_entropy(*leaves, t2, reduction="none")
+        assert torch.isnan(loss[4]) and torch.isfinite(loss[[0, 1, 2, 3, 5, 6, 7, 8, 9]]).all()
+        gx, gw = torch.autograd.grad(loss.sum(), leaves)
+        assert torch.isnan(gx[4]).all() and torch.isfinite(gx[:4]).all() and torch.isnan(gw).all()
+    x2 = x.clone()
+    x2[2, 3] = float("nan")
+    loss = ops.linear_cross_entropy(x2, w, t, reduction="none")
+    assert torch.isnan(loss[2]) and torch.isfinite(loss[3:]).all()
+    # a table row of the type's lowest value: its logit is a large number of either sign or -Inf / Inf, as in torch
+    low = w.clone()
+    low[7] = torch.finfo(dtype).min
+    want = torch.nn.functional.cross_entropy((x.float().abs() @ low.float().t()), t.clamp(min=8), reduction="none")
+    got = ops.linear_cross_entropy(x.abs(), low, t.clamp(min=8), reduction="none")
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want)) and torch.allclose(got, want, rtol=1e-3, atol=1e-3)
+
+
+def test_linear_cross_entropy_one_gradient_at_a_time_and_shapes():
+    x, w, t, _ = ce_case(60, 300, 64, torch.bfloat16, seed=10)
+    both = torch.autograd.grad(ops.linear_cross_entropy(a := x.detach().requires_grad_(), b := w.detach().requires_grad_(), t), (a, b))
+    gx, = torch.autograd.grad(ops.linear_cross_entropy(a := x.detach().requires_grad_(), w, t), (a,))
+    gw, = torch.autograd.grad(ops.linear_cross_entropy(x, b := w.detach().requires_grad_(), t), (b,))
+    assert torch.equal(gx, both[0]) and torch.equal(gw, both[1])
+    flat = ops.linear_cross_entropy(x, w, t, reduction="none")
+    assert torch.equal(ops.linear_cross_entropy(x.view(6, 10, 64), w, t.view(6, 10), reduction="none"), flat.view(6, 10))
+    assert torch.equal(ops.linear_cross_entropy(x[0], w, t[0], reduction="none"), flat[0])
+    wide = torch.zeros(60, 130, device="cuda", dtype=x.dtype)
+    wide[:, 1:65] = x
+    assert torch.equal(ops.linear_cross_entropy(wide[:, 1:65], w, t.to(torch.int32), reduction="none"), flat)
+    assert torch.equal(ops.linear_cross_entropy(x, w.t().contiguous().t(), t, reduction="none"), flat)
+
+
+def test_linear_cross_entropy_against_differences():
+    x, w, t, _ = ce_case(12, 40, 8, torch.float32, seed=11)
+    leaves = [x.detach().requires_grad_(), w.detach().requires_grad_()]
+    grads = torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, scale=1.5, reduction="sum"), leaves)
+    step = 2.0 ** -6
+    for which, g in enumerate(grads):
+        for seed in range(3):
+            d = randn(*g.shape, seed=seed)
+            d /= d.norm()
+            ends = [float(ops.linear_cross_entropy(x + s * step * d if which == 0 else x, w + s * step * d if which else w, t, scale=1.5, reduction="sum"))
+                    for s in (1, -1)]
+            # second-order differences: the third derivative of the summed loss along a unit direction is below 12 * (1.5 |.|)^3
+            # with |.| <= 5 the largest row norm; float32 losses of about 50 are off by 2^-18
+            bound = 12 * (1.5 * 5) ** 3 * step ** 2 / 6 + 2.0 ** -17 / step
+            assert abs((ends[0] - ends[1]) / (2 * step) - float((g * d).sum())) <= bound
+
+
+# ------------------------------------------------------------------ together, other streams, graphs
+def _step(features, keys, points, cells, bn, act8=True):
+    """A training step as it uses them together: a BatchNorm block kept in 8 bits, the points' rows of its output, their loss
+    against every cell of the other view."""
+    f = ops.bn_relu_cl(features, bn, act8=act8)
+    rows = ops.lookup_rows(f.reshape(-1, f.shape[-1]), points)
+    loss = ops.linear_cross_entropy(rows, keys, cells, scale=4.0)
+    return loss, torch.autograd.grad(loss, (features, keys, bn.weight, bn.bias))
+
+
+def _step_inputs(seed):
+    f = randn(1, 40, 50, 32, seed=seed).requires_grad_()
+    keys = randn(2000, 32, seed=seed + 1).requires_grad_()
+    points = torch.randint(2000, (333,), generator=gen(seed + 2), device="cuda")
+    cells = torch.randint(2000, (333,), generator=gen(seed + 3), device="cuda")
+    cells[::7] = -100
+    return f, keys, points, cells
+
+
+def test_the_operators_together_follow_autograd_in_64_bits():
+    f, keys, points, cells = _step_inputs(1)
+    bn = torch.nn.BatchNorm2d(32).cuda().train()
+    loss, grads = _step(f, keys, points, cells, bn)
+    fd, kd = f.detach().double().requires_grad_(), keys.detach().double().requires_grad_()
+    wd, bd = bn.weight.detach().double().requires_grad_(), bn.bias.detach().double().requires_grad_()
+    y = torch.relu(torch.nn.functional.batch_norm(fd.reshape(-1, 32), None, None, wd, bd, True, 0.0, bn.eps))
+    want = torch.nn.functional.cross_entropy(4.0 * (y[points] @ kd.t()), cells)
+    wants = torch.autograd.grad(want, (fd, kd, wd, bd))
+    assert abs(float(loss) - float(want)) < 1e-5
+    # float32 products of 32 terms and a softmax at scale 4: 1e-5; the 8-bit block enters through the normalised input only, within
+    # half a step of its block's scale (1 / 254 of its largest magnitude, at most 5 standard deviations here): 2 % of the terms it is in
+    for got, ref, tol in zip(grads, wants, (5e-3, 1e-5, 2e-2, 1e-5)):
+        assert float((got.double() - ref).norm() / ref.norm()) < tol
+
+
+def test_another_stream():
+    side = torch.cuda.Stream()
+    f, keys, points, cells = _step_inputs(2)
+    bn = torch.nn.BatchNorm2d(32).cuda().train()
+    want = _step(f, keys, points, cells, bn)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = _step(f, keys, points, cells, bn)
+    side.synchronize()
+    for a, b in zip((want[0], *want[1]), (got[0], *got[1])):
+        assert torch.equal(a, b)
+
+
+def test_captured_and_replayed():
+    bufs = _step_inputs(3)
+    bn = torch.nn.BatchNorm2d(32).cuda().train()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            _step(*bufs, bn)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _step(*bufs, bn)
+    for seed in (4, 8, 12, 16):
+        new = _step_inputs(seed)
+        with torch.no_grad():
+            for b, v in zip(bufs, new):
+                b.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _step(*new, bn)
+        for a, b in zip((want[0], *want[1]), (out[0], *out[1])):
+            assert torch.equal(a, b), seed
+
+
+def test_double_backward_is_refused():
+    x, w, t, _ = ce_case(5, 20, 8, torch.float32, ignored=0.0)
+    leaf = x.detach().requires_grad_()
+    g, = torch.autograd.grad(ops.linear_cross_entropy(leaf, w, t), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), leaf)
