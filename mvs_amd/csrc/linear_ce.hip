@@ -19,41 +19,9 @@
 // one in both passes, so a row's p sum to one).  16-bit dl: float16 carries it times 2^14 (|p - 1| <= 1: no overflow, and p down to
 // 4e-9 keeps a normal number's precision), the row's gradient factor is applied after the product in float32 (dx) or, relative to
 // the largest one, before the rounding (dW) -- 1 / N of a mean never reaches a 16-bit number.
-#include <type_traits>
-
-#include "dtype.h"
+#include "linear_ce.h"
 
 namespace mvs {
-
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kRowBytes = 128;                  // bytes of k per stage and row
-
-__device__ __forceinline__ void mma16(f32x4_t &c, u32x4_t a, u32x4_t b, float) {
-    const f32x4_t fa = __builtin_bit_cast(f32x4_t, a), fb = __builtin_bit_cast(f32x4_t, b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[j], fb[j], c, 0, 0, 0);
-}
-__device__ __forceinline__ void mma16(f32x4_t &c, u32x4_t a, u32x4_t b, bf16_t) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ void mma16(f32x4_t &c, u32x4_t a, u32x4_t b, f16_t) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-}
-
-// dl is carried times this
-template <typename T> struct GradUnit { static constexpr float value = 1.0f; };
-template <> struct GradUnit<f16_t> { static constexpr float value = 16384.0f; };
-
-// One operand of a product: rows of `ld` bytes, the last of them `rows - 1` (a tile's rows beyond it read that one again)
-struct Operand {
-    const char *p;
-    int64_t ld, rows;
-};
 
 template <int BM_, int BN_, int WM_, int WN_>
 struct Tile {
@@ -127,8 +95,6 @@ __device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_m, int64_t til
     tm = band * 8 + in % wide;
     tn = in / wide;
 }
-
-__device__ __forceinline__ bool ce_kept(int64_t target, int64_t ignore) { return target != ignore; }
 
 struct CeArgs {
     Operand w, x;                       // table piece and rows, padded along k
@@ -370,21 +336,38 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
     }
 }
 
-// dx[n][c] = g_n * factor * the parts' sums, in order
-template <typename T>
-__global__ __launch_bounds__(256) void ce_finish_kernel(const float *__restrict__ sums, int parts, int64_t n, int C, int64_t ld, const float *__restrict__ g,
+// out[row][c] = f * factor * the parts' sums, in order; f = g[row] (dx: 0 for an ignored row, whose sums may be anything) or g[0] (dW)
+template <typename T, bool PER_ROW>
+__global__ __launch_bounds__(256) void ce_finish_kernel(const float *__restrict__ sums, int parts, int64_t rows, int C, int64_t ld, const float *__restrict__ g,
                                                         float factor, T *__restrict__ out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n * C) return;
-    const int64_t row = i / C, c = i - row * C;
-    float s = 0.0f;
-    for (int p = 0; p < parts; ++p) s += sums[((int64_t)p * n + row) * ld + c];
-    const float f = g[row];
-    out[i] = from_float<T>(f == 0.0f ? 0.0f : s * f * factor);
+    const int64_t quads = ld >> 2, i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads, c = (i - row * quads) * 4;
+    if (row >= rows) return;
+    const f32x4_t *from = reinterpret_cast<const f32x4_t *>(sums) + i;
+    const int64_t step = rows * quads;
+    f32x4_t s = from[0];
+    int p = 1;
+    for (; p + 8 <= parts; p += 8) {
+        f32x4_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = from[(p + j) * step];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; p < parts; ++p) s += from[p * step];
+    const float f = PER_ROW ? g[row] : g[0];
+    Pack<T, 4> o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o.v[r] = from_float<T>(PER_ROW && f == 0.0f ? 0.0f : s[r] * f * factor);
+    T *to = out + row * C + c;
+    if ((C & 3) == 0) *reinterpret_cast<Pack<T, 4> *>(to) = o;
+    else
+        for (int r = 0; r < 4; ++r) if (c + r < C) to[r] = o.v[r];
 }
 
-// out[c][r] = in[r][c] for c < C, zero for r in [R, ld_out) and where the row's target is `ignore` (targets == NULL: nowhere)
-template <typename T>
+// out[c][r] = in[r][c] for c < C, zero for r in [R, ld_out) and where the row's target is `ignore` (targets == NULL: nowhere).
+// LANES: every 32 rows in the order in which a lane of the narrow kernels holds them (linear_ce_narrow.hip): place 8 g + e holds row
+// 4 g + e for e < 4, 16 + 4 g + e - 4 for the others.
+template <typename T, bool LANES>
 __global__ __launch_bounds__(256) void ce_transpose_kernel(const T *__restrict__ in, int64_t R, int C, int64_t ld_in, const int64_t *__restrict__ target,
                                                            int64_t ignore, T *__restrict__ out, int64_t ld_out) {
     __shared__ T tile[64][64 + 4 / sizeof(T)];
@@ -397,7 +380,10 @@ __global__ __launch_bounds__(256) void ce_transpose_kernel(const T *__restrict__
     }
     __syncthreads();
     for (int c = ty; c < 64; c += 4)
-        if (c0 + c < C && r0 + tx < ld_out) out[(int64_t)(c0 + c) * ld_out + r0 + tx] = tile[tx][c];
+        if (c0 + c < C && r0 + tx < ld_out) {
+            const int r = LANES ? (tx & 32) + ((tx >> 3) & 3) * 4 + (tx & 3) + ((tx & 4) << 2) : tx;
+            out[(int64_t)(c0 + c) * ld_out + r0 + tx] = tile[r][c];
+        }
 }
 
 // out[r][0 .. Cp) = in[r][0 .. C), zeros
@@ -411,15 +397,15 @@ __global__ __launch_bounds__(256) void ce_pad_kernel(const T *__restrict__ in, i
 }
 
 // ---- host side
-static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-static int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
-
 struct CePlan {
     int es;                          // element size
     int Cp;                          // C padded to whole 128-byte steps
     bool pad;                        // the operands are copied to rows of Cp
     int64_t piece, np, c4;           // backward: table rows per piece, rows padded to 128 bytes of dl^T, C rounded up to 4
     int parts;                       // of k in dx's product
+    bool narrow;                     // linear_ce_narrow.hip
+    int64_t per_x, per_w;            // its rows of the table / of x per part
+    int parts_x, parts_w;
     size_t xp, wp;                   // byte offsets
     size_t part, own, rows;          // forward
     size_t factors, dl, dlt, wt, xt, sums;
@@ -440,17 +426,36 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
         p.xp = take((size_t)n * p.Cp * p.es);
         p.wp = take((size_t)V * p.Cp * p.es);
     }
+    p.narrow = ce_narrow(p.Cp, p.es);
+    p.c4 = round_up(C, 4);
+    if (p.narrow && n > 0) {
+        // parts of the rows that are walked: enough workgroups for the chip's 256 CUs four times over, at least 256 rows each
+        auto split = [](int64_t fixed, int64_t moving, int64_t &per, int &parts) {
+            const int64_t want = ceil_div(1024, ceil_div(fixed, kNarrowRows));
+            per = round_up(ceil_div(moving, want), 64);
+            if (per < 256) per = 256;
+            parts = (int)ceil_div(moving, per);
+        };
+        split(n, V, p.per_x, p.parts_x);
+        split(V, n, p.per_w, p.parts_w);
+    }
     if (!backward) {
-        p.part = take((size_t)ceil_div(V, TileBig::BM) * n * sizeof(float2));
+        p.part = take((size_t)(p.narrow ? p.parts_x : ceil_div(V, TileBig::BM)) * n * sizeof(float2));
         p.own = take((size_t)n * 4);
         p.rows = take((size_t)n * 4);
+    } else if (p.narrow) {
+        p.np = round_up(n, 64);
+        p.factors = take((size_t)(2 * n + 1) * 4);
+        if (need_x) p.wt = take((size_t)C * round_up(V, 64) * p.es);
+        if (need_w) p.xt = take((size_t)C * p.np * p.es);
+        const size_t sx = need_x ? (size_t)p.parts_x * n : 0, sw = need_w ? (size_t)p.parts_w * V : 0;
+        p.sums = take((sx > sw ? sx : sw) * p.c4 * 4);      // (one after the other)
     } else {
         // the piece: dl of at most 2^26 values, whole tiles
         p.piece = ((int64_t)1 << 26) / (n > 0 ? n : 1) / 256 * 256;
         if (p.piece < 256) p.piece = 256;
         if (p.piece > round_up(V, 256)) p.piece = round_up(V, 256);
         p.np = round_up(n, step);
-        p.c4 = round_up(C, 4);
         p.factors = take((size_t)(2 * n + 1) * 4);
         if (need_x) {
             p.dl = take((size_t)n * p.piece * p.es);
@@ -511,7 +516,7 @@ static void ce_pad(const void *in, int64_t R, int C, char *out, int Cp, hipStrea
 }
 
 template <typename T, typename X>
-static int ce_forward(const CePlan &p, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, int64_t ignore,
+static int ce_forward(const CePlan &p, int dtype, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, int64_t ignore,
                       int reduction, float *loss, float *lse, float *kept, char *ws, hipStream_t st) {
     if (n > 0) {
         CeArgs a = {};
@@ -531,9 +536,18 @@ static int ce_forward(const CePlan &p, const void *x, const void *w, const int64
         a.part = reinterpret_cast<float2 *>(ws + p.part);
         a.own = reinterpret_cast<float *>(ws + p.own);
         float *rows = reduction == 0 ? loss : reinterpret_cast<float *>(ws + p.rows);
+        if (p.narrow) {
+            NarrowArgs b = {};
+            b.fixed = a.x; b.moving = a.w; b.per_part = p.per_x; b.scale2 = a.scale2; b.target = target; b.ignore = ignore;
+            b.part = a.part; b.own = a.own;
+            a.tiles_m = p.parts_x;
+            const int rc = ce_narrow_stats(dtype, p.Cp * p.es, b, p.parts_x, st);
+            if (rc != MVS_OK) return rc;
+        } else {
         const unsigned bytes = ce_lds<X>((size_t)X::WAVES_M * X::BN * sizeof(float2));
         if (!ce_allow_lds(ce_stats_kernel<T, X>, bytes)) return check_launch("mvs_linear_ce_fwd");
         hipLaunchKernelGGL((ce_stats_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), bytes, st, a);
+        }
         hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(256), 0, st, a.part, a.tiles_m, n, V, target, ignore, a.own, lse, rows);
         hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, rows, target, n, ignore, reduction, loss, kept);
     } else {
@@ -543,7 +557,7 @@ static int ce_forward(const CePlan &p, const void *x, const void *w, const int64
 }
 
 template <typename T, typename X>
-static int ce_backward(const CePlan &p, const void *x, const void *w, const int64_t *target, const float *lse, const float *kept, const float *grad_loss,
+static int ce_backward(const CePlan &p, int dtype, const void *x, const void *w, const int64_t *target, const float *lse, const float *kept, const float *grad_loss,
                        int64_t n, int64_t V, int C, float scale, int64_t ignore, int reduction, void *grad_x, void *grad_w, char *ws, hipStream_t st) {
     const int step = kRowBytes / p.es;
     float *factors = reinterpret_cast<float *>(ws + p.factors);
@@ -557,6 +571,37 @@ static int ce_backward(const CePlan &p, const void *x, const void *w, const int6
         a.x.p = ws + p.xp;
         a.w.p = ws + p.wp;
     }
+    const float factor = scale / GradUnit<T>::value;
+    auto finish = [&](bool of_table, int parts) {
+        const int64_t rows = of_table ? V : n;
+        const dim3 grid((unsigned)ceil_div(rows * (p.c4 / 4), 256));
+        const float *sums = reinterpret_cast<const float *>(ws + p.sums);
+        if (of_table) hipLaunchKernelGGL((ce_finish_kernel<T, false>), grid, dim3(256), 0, st, sums, parts, rows, C, p.c4, factors + 2 * n, factor, static_cast<T *>(grad_w));
+        else hipLaunchKernelGGL((ce_finish_kernel<T, true>), grid, dim3(256), 0, st, sums, parts, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));
+    };
+    if (p.narrow) {
+        constexpr bool lanes = sizeof(T) == 2;
+        NarrowArgs b = {};
+        b.scale2 = scale * kLog2e; b.target = target; b.ignore = ignore; b.lse2 = lse; b.ratio = factors + n;
+        b.sums = reinterpret_cast<float *>(ws + p.sums); b.ld_sums = p.c4; b.C = C;
+        for (int of_table = 0; of_table < 2; ++of_table) {
+            if (!(of_table ? grad_w : grad_x)) continue;
+            const int64_t rows = of_table ? n : V, ld = round_up(rows, 64);      // the rows walked
+            char *t = ws + (of_table ? p.xt : p.wt);
+            b.fixed = of_table ? a.w : a.x;
+            b.moving = of_table ? a.x : a.w;
+            b.moving_t = Operand{t, ld * p.es, C};
+            b.per_part = of_table ? p.per_w : p.per_x;
+            const int parts = of_table ? p.parts_w : p.parts_x;
+            hipLaunchKernelGGL((ce_transpose_kernel<T, lanes>), dim3((unsigned)(ld / 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
+                               reinterpret_cast<const T *>(b.moving.p), rows, C, (int64_t)p.Cp, of_table ? target : (const int64_t *)nullptr, ignore,
+                               reinterpret_cast<T *>(t), ld);
+            const int rc = ce_narrow_grad(dtype, p.Cp * p.es, of_table, b, parts, st);
+            if (rc != MVS_OK) return rc;
+            finish(of_table, parts);
+        }
+        return check_launch("mvs_linear_ce_bwd");
+    }
     const char *w_rows = a.w.p;
     a.steps = p.Cp * p.es / kRowBytes;
     a.n = n; a.v_total = V; a.ignore = ignore;
@@ -566,11 +611,10 @@ static int ce_backward(const CePlan &p, const void *x, const void *w, const int6
     a.dl = grad_x ? ws + p.dl : nullptr;
     a.dlt = grad_w ? ws + p.dlt : nullptr;
     a.ld_dlt = p.np;
-    const float factor = scale / GradUnit<T>::value;
     const unsigned grad_lds = ce_lds<X>((size_t)X::BM * (X::BN * sizeof(T) + 16)), product_lds = ce_lds<X>(0);
     if (!ce_allow_lds(ce_grad_kernel<T, X>, grad_lds) || !ce_allow_lds(ce_product_kernel<T, X>, product_lds)) return check_launch("mvs_linear_ce_bwd");
     if (grad_w)      // x^T once; ignored rows as zeros, whatever they hold
-        hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(p.np, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
+        hipLaunchKernelGGL((ce_transpose_kernel<T, false>), dim3((unsigned)ceil_div(p.np, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
                            reinterpret_cast<const T *>(a.x.p), n, C, (int64_t)p.Cp, target, ignore, reinterpret_cast<T *>(ws + p.xt), p.np);
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
         const int64_t count = V - v0 < p.piece ? V - v0 : p.piece, k = round_up(count, step);
@@ -580,7 +624,7 @@ static int ce_backward(const CePlan &p, const void *x, const void *w, const int6
         a.tiles_m = ceil_div(count, X::BM);
         hipLaunchKernelGGL((ce_grad_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), grad_lds, st, a);
         if (grad_x) {
-            hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(k, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
+            hipLaunchKernelGGL((ce_transpose_kernel<T, false>), dim3((unsigned)ceil_div(k, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
                                reinterpret_cast<const T *>(a.w.p), count, C, (int64_t)p.Cp, (const int64_t *)nullptr, ignore,
                                reinterpret_cast<T *>(ws + p.wt), k);
             CeProduct d = {};
@@ -607,10 +651,7 @@ static int ce_backward(const CePlan &p, const void *x, const void *w, const int6
             hipLaunchKernelGGL((ce_product_kernel<T, X>), dim3((unsigned)(d.tiles_m * d.tiles_n)), dim3(X::THREADS), product_lds, st, d);
         }
     }
-    if (grad_x) {
-        hipLaunchKernelGGL((ce_finish_kernel<T>), dim3((unsigned)ceil_div(n * C, 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums), p.parts, n, C,
-                           p.c4, factors, factor, static_cast<T *>(grad_x));
-    }
+    if (grad_x) finish(false, p.parts);
     return check_launch("mvs_linear_ce_bwd");
 }
 
@@ -640,7 +681,7 @@ extern "C" int mvs_linear_ce_fwd(const void *x, const void *weight, int dtype, c
     }
     const CePlan p = ce_plan(n, V, C, dtype, false, false, false);
     MVS_DTYPE_DISPATCH(dtype, T, {
-        return ce_forward<T, TileBig>(p, x, weight, target, n, V, C, scale, ignore_index, reduction, loss, lse, kept, static_cast<char *>(workspace),
+        return ce_forward<T, TileBig>(p, dtype, x, weight, target, n, V, C, scale, ignore_index, reduction, loss, lse, kept, static_cast<char *>(workspace),
                                       as_stream(stream));
     });
 }
@@ -663,7 +704,7 @@ extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, c
     }
     const CePlan p = ce_plan(n, V, C, dtype, true, grad_x != nullptr, grad_weight != nullptr);
     MVS_DTYPE_DISPATCH(dtype, T, {
-        return ce_backward<T, TileBig>(p, x, weight, target, lse, kept, grad_loss, n, V, C, scale, ignore_index, reduction, grad_x, grad_weight,
+        return ce_backward<T, TileBig>(p, dtype, x, weight, target, lse, kept, grad_loss, n, V, C, scale, ignore_index, reduction, grad_x, grad_weight,
                                        static_cast<char *>(workspace), as_stream(stream));
     });
 }

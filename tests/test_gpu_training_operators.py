@@ -304,7 +304,8 @@ def ce_check(x, w, t, scale, ignore=-100, reduction="mean", seed=9):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,V,C", [(1, 1, 1), (1, 2, 3), (2, 129, 8), (1, 1000, 64), (17, 130, 32), (64, 128, 33), (100, 257, 100), (129, 2000, 64),
-                                   (130, 511, 200), (33, 5000, 320), (300, 300, 16)])
+                                   (130, 511, 200), (33, 5000, 320), (300, 300, 16), (1, 3, 130), (2, 1000, 257), (129, 129, 129), (70, 300, 1000),
+                                   (257, 400, 128), (1, 5000, 512), (1500, 10, 32), (2000, 1000, 160)])
 def test_linear_cross_entropy(n, V, C, dtype):
     x, w, t, _ = ce_case(n, V, C, dtype, seed=n)
     t[0] = min(t.clamp(min=0).max(), V - 1)
@@ -321,9 +322,10 @@ def test_linear_cross_entropy_reductions_and_scales(reduction, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_linear_cross_entropy_in_pieces_of_the_table(dtype):
-    """n V beyond 2^26: the backward pass walks the table in more than one piece, the last of them a ragged one."""
-    x, w, t, _ = ce_case(1025, 70001, 8, dtype, seed=6)
+@pytest.mark.parametrize("C", [8, 130])
+def test_linear_cross_entropy_in_pieces_of_the_table(dtype, C):
+    """n V beyond 2^26: the backward pass walks the table in more than one piece (wide rows), the last of them a ragged one."""
+    x, w, t, _ = ce_case(1025, 70001, C, dtype, seed=6)
     ce_check(x, w, t, 2.0)
 
 
