@@ -232,17 +232,6 @@ def ptr(t):
         raise MvsHipError("mvs_amd ops need device (HIP) tensors; got a CPU tensor")
     if t.dtype != torch.float32 or not t.is_contiguous():
         raise MvsHipError(f"expected contiguous float32, got {t.dtype} contiguous={t.is_contiguous()}")
-    return any_ptr(t)
-
-
-def any_ptr(t):
-    """Device pointer of a contiguous tensor of any type on the current device, or None (the caller has checked its type)."""
-    if t is None:
-        return None
-    if not t.is_cuda:
-        raise MvsHipError("mvs_amd ops need device (HIP) tensors; got a CPU tensor")
-    if not t.is_contiguous():
-        raise MvsHipError("expected a contiguous tensor")
     if t.device.index != torch.cuda.current_device():
         # kernels launch on the CURRENT device and its current stream (stream() below): a tensor
         # of another GPU would be dereferenced there.  nn.DataParallel sets the device per replica.

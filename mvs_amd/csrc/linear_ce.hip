@@ -217,28 +217,10 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(const float *__restrict_
 }
 
 // ---- backward
-// a row's factor g_n (0 for an ignored one), and its ratio to the largest magnitude; factors[2 n] = that magnitude
-__global__ __launch_bounds__(1024) void ce_factors_kernel(const float *__restrict__ grad_loss, const float *__restrict__ kept,
-                                                          const int64_t *__restrict__ target, int64_t n, int64_t ignore, int reduction,
-                                                          float *__restrict__ factors) {
+__global__ __launch_bounds__(1024) void ce_factors_kernel(const float *grad_loss, const float *kept, const int64_t *target, int64_t n, int64_t ignore,
+                                                          int reduction, float *factors) {
     __shared__ float tops[16];
-    float common = reduction == 0 ? 0.0f : grad_loss[0];
-    if (reduction == 1) common = common / *kept;
-    auto factor = [&](int64_t i) { return !ce_kept(target[i], ignore) ? 0.0f : reduction == 0 ? grad_loss[i] : common; };
-    float top = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, __builtin_fabsf(factor(i)));
-#pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 16; ++w) top = fmaxf(top, tops[w]);
-    for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        const float g = factor(i);
-        factors[i] = g;
-        factors[n + i] = g == 0.0f ? 0.0f : g / top;
-    }
-    if (threadIdx.x == 0) factors[2 * n] = top;
+    ce_factors(grad_loss, kept, target, n, ignore, reduction, factors, tops);
 }
 
 template <typename T, typename X>
@@ -336,38 +318,13 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
     }
 }
 
-// out[row][c] = f * factor * the parts' sums, in order; f = g[row] (dx: 0 for an ignored row, whose sums may be anything) or g[0] (dW)
-template <typename T, bool PER_ROW>
-__global__ __launch_bounds__(256) void ce_finish_kernel(const float *__restrict__ sums, int parts, int64_t rows, int C, int64_t ld, const float *__restrict__ g,
-                                                        float factor, T *__restrict__ out) {
-    const int64_t quads = ld >> 2, i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads, c = (i - row * quads) * 4;
-    if (row >= rows) return;
-    const f32x4_t *from = reinterpret_cast<const f32x4_t *>(sums) + i;
-    const int64_t step = rows * quads;
-    f32x4_t s = from[0];
-    int p = 1;
-    for (; p + 8 <= parts; p += 8) {
-        f32x4_t v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = from[(p + j) * step];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[j];
-    }
-    for (; p < parts; ++p) s += from[p * step];
-    const float f = PER_ROW ? g[row] : g[0];
-    Pack<T, 4> o;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) o.v[r] = from_float<T>(PER_ROW && f == 0.0f ? 0.0f : s[r] * f * factor);
-    T *to = out + row * C + c;
-    if ((C & 3) == 0) *reinterpret_cast<Pack<T, 4> *>(to) = o;
-    else
-        for (int r = 0; r < 4; ++r) if (c + r < C) to[r] = o.v[r];
+template <typename T>
+__global__ __launch_bounds__(256) void ce_finish_kernel(const float *sums, int parts, int64_t rows, int C, int64_t ld, const float *g, float factor, T *out) {
+    ce_finish<T, true>(sums, parts, rows, C, ld, g, factor, out, blockIdx.x);
 }
 
 // out[c][r] = in[r][c] for c < C, zero for r in [R, ld_out) and where the row's target is `ignore` (targets == NULL: nowhere).
-// LANES: every 32 rows in the order in which a lane of the narrow kernels holds them (linear_ce_narrow.hip): place 8 g + e holds row
-// 4 g + e for e < 4, 16 + 4 g + e - 4 for the others.
-template <typename T, bool LANES>
+template <typename T>
 __global__ __launch_bounds__(256) void ce_transpose_kernel(const T *__restrict__ in, int64_t R, int C, int64_t ld_in, const int64_t *__restrict__ target,
                                                            int64_t ignore, T *__restrict__ out, int64_t ld_out) {
     __shared__ T tile[64][64 + 4 / sizeof(T)];
@@ -380,10 +337,7 @@ __global__ __launch_bounds__(256) void ce_transpose_kernel(const T *__restrict__
     }
     __syncthreads();
     for (int c = ty; c < 64; c += 4)
-        if (c0 + c < C && r0 + tx < ld_out) {
-            const int r = LANES ? (tx & 32) + ((tx >> 3) & 3) * 4 + (tx & 3) + ((tx & 4) << 2) : tx;
-            out[(int64_t)(c0 + c) * ld_out + r0 + tx] = tile[r][c];
-        }
+        if (c0 + c < C && r0 + tx < ld_out) out[(int64_t)(c0 + c) * ld_out + r0 + tx] = tile[tx][c];
 }
 
 // out[r][0 .. Cp) = in[r][0 .. C), zeros
@@ -399,16 +353,19 @@ __global__ __launch_bounds__(256) void ce_pad_kernel(const T *__restrict__ in, i
 // ---- host side
 struct CePlan {
     int es;                          // element size
-    int Cp;                          // C padded to whole 128-byte steps
-    bool pad;                        // the operands are copied to rows of Cp
-    int64_t piece, np, c4;           // backward: table rows per piece, rows padded to 128 bytes of dl^T, C rounded up to 4
-    int parts;                       // of k in dx's product
     bool narrow;                     // linear_ce_narrow.hip
-    int64_t per_x, per_w;            // its rows of the table / of x per part
-    int parts_x, parts_w;
-    size_t xp, wp;                   // byte offsets
+    int Cp;                          // C padded to whole 128-byte steps (narrow: to 32 elements)
+    bool pad;                        // the operands are copied to rows of Cp (narrow: and into pieces)
+    int64_t c4;                      // C rounded up to 4
+    size_t xp, wp;                   // byte offsets: those copies
     size_t part, own, rows;          // forward
-    size_t factors, dl, dlt, wt, xt, sums;
+    int64_t tiles;                   // statistics per row
+    // backward
+    int64_t piece, np;               // table rows per piece; n padded to 128 bytes of dl^T
+    int parts;                       // of k in dx's product
+    int64_t per_x, per_w;            // narrow: rows of the table / of x per part
+    int parts_x, parts_w;
+    size_t factors, dl, dlt, wt, xt, sums, sums_w;
     size_t total;
 };
 
@@ -417,17 +374,18 @@ using TileBig = Tile<128, 128, 2, 2>;
 static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, bool need_x, bool need_w) {
     CePlan p = {};
     p.es = (int)dtype_size(dtype);
-    const int step = kRowBytes / p.es;
-    p.Cp = (int)round_up(C, step);
-    p.pad = p.Cp != C;
+    p.narrow = ce_narrow(C, dtype);
+    p.c4 = round_up(C, 4);
+    const int step = kRowBytes / p.es, planes = ce_planes(dtype);
+    p.Cp = (int)round_up(C, p.narrow ? 32 : step);
+    p.pad = p.Cp != C || (p.narrow && planes > 1);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
     if (p.pad) {
-        p.xp = take((size_t)n * p.Cp * p.es);
-        p.wp = take((size_t)V * p.Cp * p.es);
+        const size_t row = (size_t)p.Cp * (p.narrow ? 2 * planes : p.es);
+        p.xp = take((size_t)n * row);
+        p.wp = take((size_t)V * row);
     }
-    p.narrow = ce_narrow(p.Cp, p.es);
-    p.c4 = round_up(C, 4);
     if (p.narrow && n > 0) {
         // parts of the rows that are walked: enough workgroups for the chip's 256 CUs four times over, at least 256 rows each
         auto split = [](int64_t fixed, int64_t moving, int64_t &per, int &parts) {
@@ -440,16 +398,20 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
         split(V, n, p.per_w, p.parts_w);
     }
     if (!backward) {
-        p.part = take((size_t)(p.narrow ? p.parts_x : ceil_div(V, TileBig::BM)) * n * sizeof(float2));
+        p.tiles = p.narrow ? p.parts_x : ceil_div(V, TileBig::BM);
+        p.part = take((size_t)p.tiles * n * sizeof(float2));
         p.own = take((size_t)n * 4);
         p.rows = take((size_t)n * 4);
     } else if (p.narrow) {
-        p.np = round_up(n, 64);
         p.factors = take((size_t)(2 * n + 1) * 4);
-        if (need_x) p.wt = take((size_t)C * round_up(V, 64) * p.es);
-        if (need_w) p.xt = take((size_t)C * p.np * p.es);
-        const size_t sx = need_x ? (size_t)p.parts_x * n : 0, sw = need_w ? (size_t)p.parts_w * V : 0;
-        p.sums = take((sx > sw ? sx : sw) * p.c4 * 4);      // (one after the other)
+        if (need_x) {
+            p.wt = take((size_t)C * planes * round_up(V, 64) * 2);
+            p.sums = take((size_t)p.parts_x * n * p.c4 * 4);
+        }
+        if (need_w) {
+            p.xt = take((size_t)C * planes * round_up(n, 64) * 2);
+            p.sums_w = take((size_t)p.parts_w * V * p.c4 * 4);
+        }
     } else {
         // the piece: dl of at most 2^26 values, whole tiles
         p.piece = ((int64_t)1 << 26) / (n > 0 ? n : 1) / 256 * 256;
@@ -475,6 +437,18 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
     }
     p.total = at;
     return p;
+}
+
+// the arguments of the narrow kernels that both passes share
+static NarrowArgs ce_narrow_args(const CePlan &p, int dtype, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale,
+                                 int64_t ignore, char *ws) {
+    NarrowArgs a = {};
+    a.x = NarrowOperand{x, p.pad ? ws + p.xp : const_cast<char *>(static_cast<const char *>(x)), nullptr, n, p.pad};
+    a.w = NarrowOperand{w, p.pad ? ws + p.wp : const_cast<char *>(static_cast<const char *>(w)), nullptr, V, p.pad};
+    a.C = C; a.Cp = p.Cp; a.planes = ce_planes(dtype);
+    a.per_x = p.per_x; a.per_w = p.per_w; a.parts_x = p.parts_x; a.parts_w = p.parts_w;
+    a.scale2 = scale * kLog2e; a.target = target; a.ignore = ignore; a.ld_sums = p.c4;
+    return a;
 }
 
 static int ce_check(const char *who, const void *x, const void *w, int dtype, const int64_t *target, int64_t n, int64_t V, int C, int reduction,
@@ -516,48 +490,53 @@ static void ce_pad(const void *in, int64_t R, int C, char *out, int Cp, hipStrea
 }
 
 template <typename T, typename X>
-static int ce_forward(const CePlan &p, int dtype, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, int64_t ignore,
-                      int reduction, float *loss, float *lse, float *kept, char *ws, hipStream_t st) {
-    if (n > 0) {
-        CeArgs a = {};
-        a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
-        a.x = Operand{static_cast<const char *>(x), (int64_t)p.Cp * p.es, n};
-        if (p.pad) {
-            ce_pad<T>(x, n, C, ws + p.xp, p.Cp, st);
-            ce_pad<T>(w, V, C, ws + p.wp, p.Cp, st);
-            a.x.p = ws + p.xp;
-            a.w.p = ws + p.wp;
-        }
-        a.steps = p.Cp * p.es / kRowBytes;
-        a.n = n; a.v_total = V; a.v_count = V; a.ignore = ignore;
-        a.tiles_m = ceil_div(V, X::BM); a.tiles_n = ceil_div(n, X::BN);
-        a.scale2 = scale * kLog2e;
-        a.target = target;
-        a.part = reinterpret_cast<float2 *>(ws + p.part);
-        a.own = reinterpret_cast<float *>(ws + p.own);
-        float *rows = reduction == 0 ? loss : reinterpret_cast<float *>(ws + p.rows);
-        if (p.narrow) {
-            NarrowArgs b = {};
-            b.fixed = a.x; b.moving = a.w; b.per_part = p.per_x; b.scale2 = a.scale2; b.target = target; b.ignore = ignore;
-            b.part = a.part; b.own = a.own;
-            a.tiles_m = p.parts_x;
-            const int rc = ce_narrow_stats(dtype, p.Cp * p.es, b, p.parts_x, st);
-            if (rc != MVS_OK) return rc;
-        } else {
-        const unsigned bytes = ce_lds<X>((size_t)X::WAVES_M * X::BN * sizeof(float2));
-        if (!ce_allow_lds(ce_stats_kernel<T, X>, bytes)) return check_launch("mvs_linear_ce_fwd");
-        hipLaunchKernelGGL((ce_stats_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), bytes, st, a);
-        }
-        hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(256), 0, st, a.part, a.tiles_m, n, V, target, ignore, a.own, lse, rows);
-        hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, rows, target, n, ignore, reduction, loss, kept);
-    } else {
-        hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, (const float *)nullptr, target, n, ignore, reduction, loss, kept);
+static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, char *ws, hipStream_t st) {
+    CeArgs a = {};
+    a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
+    a.x = Operand{static_cast<const char *>(x), (int64_t)p.Cp * p.es, n};
+    if (p.pad) {
+        ce_pad<T>(x, n, C, ws + p.xp, p.Cp, st);
+        ce_pad<T>(w, V, C, ws + p.wp, p.Cp, st);
+        a.x.p = ws + p.xp;
+        a.w.p = ws + p.wp;
     }
+    a.steps = p.Cp * p.es / kRowBytes;
+    a.n = n; a.v_total = V; a.v_count = V;
+    a.tiles_m = p.tiles; a.tiles_n = ceil_div(n, X::BN);
+    a.scale2 = scale * kLog2e;
+    a.target = target;
+    a.part = reinterpret_cast<float2 *>(ws + p.part);
+    a.own = reinterpret_cast<float *>(ws + p.own);
+    const unsigned bytes = ce_lds<X>((size_t)X::WAVES_M * X::BN * sizeof(float2));
+    if (!ce_allow_lds(ce_stats_kernel<T, X>, bytes)) return check_launch("mvs_linear_ce_fwd");
+    hipLaunchKernelGGL((ce_stats_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), bytes, st, a);
+    return check_launch("mvs_linear_ce_fwd");
+}
+
+static int ce_forward(int dtype, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, int64_t ignore,
+                      int reduction, float *loss, float *lse, float *kept, char *ws, hipStream_t st) {
+    const CePlan p = ce_plan(n, V, C, dtype, false, false, false);
+    float *rows = reduction == 0 ? loss : reinterpret_cast<float *>(ws + p.rows);
+    if (n > 0) {
+        float2 *part = reinterpret_cast<float2 *>(ws + p.part);
+        float *own = reinterpret_cast<float *>(ws + p.own);
+        int rc = MVS_OK;
+        if (p.narrow) {
+            NarrowArgs a = ce_narrow_args(p, dtype, x, w, target, n, V, C, scale, ignore, ws);
+            a.part = part; a.own = own;
+            rc = ce_narrow_forward(dtype, a, st);
+        } else {
+            MVS_DTYPE_DISPATCH(dtype, T, rc = (ce_wide_stats<T, TileBig>(p, x, w, target, n, V, C, scale, ws, st)));
+        }
+        if (rc != MVS_OK) return rc;
+        hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(256), 0, st, part, p.tiles, n, V, target, ignore, own, lse, rows);
+    }
+    hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, rows, target, n, ignore, reduction, loss, kept);
     return check_launch("mvs_linear_ce_fwd");
 }
 
 template <typename T, typename X>
-static int ce_backward(const CePlan &p, int dtype, const void *x, const void *w, const int64_t *target, const float *lse, const float *kept, const float *grad_loss,
+static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const int64_t *target, const float *lse, const float *kept, const float *grad_loss,
                        int64_t n, int64_t V, int C, float scale, int64_t ignore, int reduction, void *grad_x, void *grad_w, char *ws, hipStream_t st) {
     const int step = kRowBytes / p.es;
     float *factors = reinterpret_cast<float *>(ws + p.factors);
@@ -572,36 +551,6 @@ static int ce_backward(const CePlan &p, int dtype, const void *x, const void *w,
         a.w.p = ws + p.wp;
     }
     const float factor = scale / GradUnit<T>::value;
-    auto finish = [&](bool of_table, int parts) {
-        const int64_t rows = of_table ? V : n;
-        const dim3 grid((unsigned)ceil_div(rows * (p.c4 / 4), 256));
-        const float *sums = reinterpret_cast<const float *>(ws + p.sums);
-        if (of_table) hipLaunchKernelGGL((ce_finish_kernel<T, false>), grid, dim3(256), 0, st, sums, parts, rows, C, p.c4, factors + 2 * n, factor, static_cast<T *>(grad_w));
-        else hipLaunchKernelGGL((ce_finish_kernel<T, true>), grid, dim3(256), 0, st, sums, parts, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));
-    };
-    if (p.narrow) {
-        constexpr bool lanes = sizeof(T) == 2;
-        NarrowArgs b = {};
-        b.scale2 = scale * kLog2e; b.target = target; b.ignore = ignore; b.lse2 = lse; b.ratio = factors + n;
-        b.sums = reinterpret_cast<float *>(ws + p.sums); b.ld_sums = p.c4; b.C = C;
-        for (int of_table = 0; of_table < 2; ++of_table) {
-            if (!(of_table ? grad_w : grad_x)) continue;
-            const int64_t rows = of_table ? n : V, ld = round_up(rows, 64);      // the rows walked
-            char *t = ws + (of_table ? p.xt : p.wt);
-            b.fixed = of_table ? a.w : a.x;
-            b.moving = of_table ? a.x : a.w;
-            b.moving_t = Operand{t, ld * p.es, C};
-            b.per_part = of_table ? p.per_w : p.per_x;
-            const int parts = of_table ? p.parts_w : p.parts_x;
-            hipLaunchKernelGGL((ce_transpose_kernel<T, lanes>), dim3((unsigned)(ld / 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
-                               reinterpret_cast<const T *>(b.moving.p), rows, C, (int64_t)p.Cp, of_table ? target : (const int64_t *)nullptr, ignore,
-                               reinterpret_cast<T *>(t), ld);
-            const int rc = ce_narrow_grad(dtype, p.Cp * p.es, of_table, b, parts, st);
-            if (rc != MVS_OK) return rc;
-            finish(of_table, parts);
-        }
-        return check_launch("mvs_linear_ce_bwd");
-    }
     const char *w_rows = a.w.p;
     a.steps = p.Cp * p.es / kRowBytes;
     a.n = n; a.v_total = V; a.ignore = ignore;
@@ -614,7 +563,7 @@ static int ce_backward(const CePlan &p, int dtype, const void *x, const void *w,
     const unsigned grad_lds = ce_lds<X>((size_t)X::BM * (X::BN * sizeof(T) + 16)), product_lds = ce_lds<X>(0);
     if (!ce_allow_lds(ce_grad_kernel<T, X>, grad_lds) || !ce_allow_lds(ce_product_kernel<T, X>, product_lds)) return check_launch("mvs_linear_ce_bwd");
     if (grad_w)      // x^T once; ignored rows as zeros, whatever they hold
-        hipLaunchKernelGGL((ce_transpose_kernel<T, false>), dim3((unsigned)ceil_div(p.np, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
+        hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(p.np, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
                            reinterpret_cast<const T *>(a.x.p), n, C, (int64_t)p.Cp, target, ignore, reinterpret_cast<T *>(ws + p.xt), p.np);
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
         const int64_t count = V - v0 < p.piece ? V - v0 : p.piece, k = round_up(count, step);
@@ -624,7 +573,7 @@ static int ce_backward(const CePlan &p, int dtype, const void *x, const void *w,
         a.tiles_m = ceil_div(count, X::BM);
         hipLaunchKernelGGL((ce_grad_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), grad_lds, st, a);
         if (grad_x) {
-            hipLaunchKernelGGL((ce_transpose_kernel<T, false>), dim3((unsigned)ceil_div(k, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
+            hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(k, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
                                reinterpret_cast<const T *>(a.w.p), count, C, (int64_t)p.Cp, (const int64_t *)nullptr, ignore,
                                reinterpret_cast<T *>(ws + p.wt), k);
             CeProduct d = {};
@@ -651,7 +600,9 @@ static int ce_backward(const CePlan &p, int dtype, const void *x, const void *w,
             hipLaunchKernelGGL((ce_product_kernel<T, X>), dim3((unsigned)(d.tiles_m * d.tiles_n)), dim3(X::THREADS), product_lds, st, d);
         }
     }
-    if (grad_x) finish(false, p.parts);
+    if (grad_x)
+        hipLaunchKernelGGL((ce_finish_kernel<T>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
+                           p.parts, n, C, p.c4, factors, factor, static_cast<T *>(grad_x));
     return check_launch("mvs_linear_ce_bwd");
 }
 
@@ -679,11 +630,7 @@ extern "C" int mvs_linear_ce_fwd(const void *x, const void *weight, int dtype, c
         set_error("mvs_linear_ce_fwd: loss, lse and kept are needed");
         return MVS_EINVAL;
     }
-    const CePlan p = ce_plan(n, V, C, dtype, false, false, false);
-    MVS_DTYPE_DISPATCH(dtype, T, {
-        return ce_forward<T, TileBig>(p, dtype, x, weight, target, n, V, C, scale, ignore_index, reduction, loss, lse, kept, static_cast<char *>(workspace),
-                                      as_stream(stream));
-    });
+    return ce_forward(dtype, x, weight, target, n, V, C, scale, ignore_index, reduction, loss, lse, kept, static_cast<char *>(workspace), as_stream(stream));
 }
 
 extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, const int64_t *target, const float *lse, const float *kept,
@@ -703,8 +650,19 @@ extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, c
         return MVS_EINVAL;
     }
     const CePlan p = ce_plan(n, V, C, dtype, true, grad_x != nullptr, grad_weight != nullptr);
+    char *ws = static_cast<char *>(workspace);
+    if (p.narrow) {
+        NarrowArgs a = ce_narrow_args(p, dtype, x, weight, target, n, V, C, scale, ignore_index, ws);
+        a.lse2 = lse; a.grad_loss = grad_loss; a.kept = kept; a.reduction = reduction;
+        a.factors = reinterpret_cast<float *>(ws + p.factors);
+        if (grad_x) { a.w.trans = ws + p.wt; a.sums_x = reinterpret_cast<float *>(ws + p.sums); }
+        if (grad_weight) { a.x.trans = ws + p.xt; a.sums_w = reinterpret_cast<float *>(ws + p.sums_w); }
+        a.grad_x = grad_x; a.grad_w = grad_weight;
+        a.factor = scale / (dtype == MVS_DTYPE_F16 ? GradUnit<f16_t>::value : 1.0f);
+        return ce_narrow_backward(dtype, a, as_stream(stream));
+    }
     MVS_DTYPE_DISPATCH(dtype, T, {
-        return ce_backward<T, TileBig>(p, dtype, x, weight, target, lse, kept, grad_loss, n, V, C, scale, ignore_index, reduction, grad_x, grad_weight,
-                                       static_cast<char *>(workspace), as_stream(stream));
+        return (ce_wide_backward<T, TileBig>(p, x, weight, target, lse, kept, grad_loss, n, V, C, scale, ignore_index, reduction, grad_x, grad_weight, ws,
+                                             as_stream(stream)));
     });
 }

@@ -1,260 +1,292 @@
-// Cross entropy against a table for NARROW rows (at most 256 bytes: float32 C <= 64, 16 bits C <= 128), the shape of feature
-// matching: points of one view against all cells of another.
+// Cross entropy against a table for NARROW rows (float32 C <= 64, 16 bits C <= 128), the shape of feature matching: points of one
+// view against all cells of another.
 //
 // With so few operations per logit the piecewise scheme of linear_ce.hip is bound by writing and reading dl (20480 x 20480 x 32
 // float32: 6.7 GB, against 0.27 TFLOP in all).  Here dl never leaves the registers: a workgroup owns 128 rows, keeps them as matrix
-// fragments and walks the other operand 64 rows at a time through LDS (DMA, two stages).  Per 32 rows of it
+// fragments and walks the other operand through LDS (DMA, two stages).  Per 32 rows of it
 //     S[m][n] = <moving m, fixed n>      lane: n = lane & 15, m = 4 (lane >> 4) + r, two 16-row tiles
 //     dl      = (exp2(S scale2 - lse2) - [target]) ratio
-//     sums[c][n] += sum_m moving_t[c][m] dl[m][n]
+//     sums[c][n] += sum_m trans[c][m] dl[m][n]
 // and the second product takes dl from the accumulators as they lie: the order of k inside a matrix instruction is free if both
-// operands agree, and 4 g + r (float32: four instructions of k = 4, the r-th takes register r) or {4 g + 0..3, 16 + 4 g + 0..3}
-// (16 bits: one of k = 32) is the order the lanes hold.  The transposed copy is written in that order (ce_transpose_kernel).
-// dx: fixed = x, moving = the table.  dW: fixed = the table, moving = x, whose rows' statistics then run along m.
-// The forward pass is the first product alone with a running maximum and sum per lane.
-// Operations: 10 N V C forward and backward (the logits three times) instead of 8, all on chip.
+// operands agree, and {4 g + 0..3, 16 + 4 g + 0..3} is what lane group g holds of 32 rows.  The transposed copy is written in that
+// order.  dx: fixed = x, moving = the table.  dW: fixed = the table, moving = x, whose rows' statistics then run along m.  The forward
+// pass is the first product alone with a running maximum and sum per lane.
+//
+// float32 runs on the bfloat16 pipe: a value is three bfloat16 pieces of 8 bits each (24 in all: nothing is dropped), a product six
+// of the nine piece products -- the others are below 2^-24 of it -- summed in float32.  16 times the float32 pipe's rate over six
+// products.  dl is split the same way in the registers.
+//
+// Operations: 10 N V C forward and backward (the logits three times) instead of 8, all on chip.  A 32 x 32 block of logits costs a
+// wave 24 + 24 matrix instructions of 16 cycles (float32, C = 32, a gradient) and about as many cycles of exponentials and splitting.
 #include "linear_ce.h"
 
 namespace mvs {
 
-constexpr int kMoving = 64;      // rows of the moving operand per stage
-
-// RB: bytes of a row, 128 or 256
-template <typename T, int RB>
+// E: what the planes hold.  PL planes, KS 64-byte (32-element) steps of k per plane.
+template <typename E_, int PL_, int KS_>
 struct Narrow {
-    static constexpr int KSTEPS = RB / 64;                       // 64-byte fragments along k
-    static constexpr int CT = RB / (int)sizeof(T) / 16;          // 16-column tiles of the result
-    static constexpr int ROWS_B = kMoving * RB;                  // moving tile
-    static constexpr int TRANS_B = CT * 16 * kMoving * (int)sizeof(T);      // its transpose: the same bytes
-    static_assert(ROWS_B == TRANS_B, "");
+    using E = E_;
+    static constexpr int PL = PL_, KS = KS_;
+    static constexpr int CT = KS * 2;                            // 16-column tiles of the result
+    static constexpr int MR = PL * KS >= 6 ? 32 : 64;            // rows of the moving operand per stage (two workgroups' stages fit a CU)
+    static constexpr int RG = MR / 16, HALVES = MR / 32;
+    static constexpr int ROWS_COPIES = PL * KS * RG, TRANS_COPIES = PL * HALVES * CT;      // of 1024 bytes: 16 rows of 64
+    static constexpr int ROWS_B = ROWS_COPIES * 1024, TRANS_B = TRANS_COPIES * 1024;
 };
 
-// Copies `rows` rows of 128 bytes (byte `at` of each operand row on) to LDS, chunks exchanged by the row's low three bits; 4 waves.
-template <int ROWS>
-__device__ __forceinline__ void narrow_copy(const Operand &o, int64_t row0, int64_t at, unsigned lds_to) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r8 = lane >> 3, chunk = (lane & 7) ^ r8;
+__device__ __forceinline__ void mma_e(f32x4_t &c, u32x4_t a, u32x4_t b, bf16_t) { mma16(c, a, b, bf16_t()); }
+__device__ __forceinline__ void mma_e(f32x4_t &c, u32x4_t a, u32x4_t b, f16_t) { mma16(c, a, b, f16_t()); }
+
+// c += a b over planes, the smallest products first
+template <typename E, int PL>
+__device__ __forceinline__ void mma_planes(f32x4_t &c, const u32x4_t (&a)[PL], const u32x4_t (&b)[PL]) {
+    if constexpr (PL == 3) {
+        mma_e(c, a[2], b[0], E());
+        mma_e(c, a[1], b[1], E());
+        mma_e(c, a[0], b[2], E());
+        mma_e(c, a[1], b[0], E());
+        mma_e(c, a[0], b[1], E());
+    }
+    mma_e(c, a[0], b[0], E());
+}
+
+// LDS holds sub-tiles of rows of 64 bytes, two rows to a 128-byte line, the eight 16-byte chunks of a line exchanged by the line's
+// low three bits: 16 rows' fragments (one chunk each) then spread over all banks.  A wave's copy is 16 rows.
+__device__ __forceinline__ void narrow_copy16(const char *rows, int64_t ld, int64_t row0, int64_t last, int64_t at, unsigned lds_to) {
+    const int lane = threadIdx.x & 63, line = lane >> 3, in = (lane & 7) ^ line;
+    int64_t row = row0 + line * 2 + (in >> 2);
+    row = row < last ? row : last;
+    glds16(rows + row * ld + at + (in & 3) * 16, lds_to);
+}
+__device__ __forceinline__ int narrow_lane() {      // a lane's byte within a 16-row block of a sub-tile
+    const int ln = threadIdx.x & 15, fk = (threadIdx.x & 63) >> 4;
+    return (ln >> 1) * 128 + ((((ln & 1) * 4 + fk) ^ (ln >> 1)) * 16);
+}
+__device__ __forceinline__ u32x4_t narrow_frag(const char *sub, int block, int lane_at) {
+    return *reinterpret_cast<const u32x4_t *>(sub + block * 1024 + lane_at);
+}
+
+template <typename X>
+__device__ __forceinline__ void narrow_copy_rows(const NarrowOperand &o, int Cp, int64_t m0, unsigned to) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int i = 0; i < ROWS / 32; ++i) {
+    for (int i = 0; i < (X::ROWS_COPIES + 3) / 4; ++i) {
         const int c = wave + i * 4;
-        const int64_t row = row0 + c * 8 + r8;
-        glds16(o.p + (row < o.rows ? row : o.rows - 1) * o.ld + at + chunk * 16, lds_to + (unsigned)(c * 1024));
+        if (X::ROWS_COPIES % 4 != 0 && c >= X::ROWS_COPIES) break;
+        const int sub = c / X::RG, rg = c % X::RG, plane = sub / X::KS, k = sub % X::KS;
+        narrow_copy16(o.rows, (int64_t)X::PL * Cp * 2, m0 + rg * 16, o.count - 1, plane * Cp * 2 + k * 64, to + (unsigned)(c * 1024));
+    }
+}
+template <typename X>
+__device__ __forceinline__ void narrow_copy_trans(const NarrowOperand &o, int C, int64_t m0, unsigned to) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t mp = (o.count + 63) & ~(int64_t)63;
+#pragma unroll
+    for (int i = 0; i < (X::TRANS_COPIES + 3) / 4; ++i) {
+        const int c = wave + i * 4;
+        if (X::TRANS_COPIES % 4 != 0 && c >= X::TRANS_COPIES) break;
+        const int sub = c / X::CT, rg = c % X::CT, plane = sub / X::HALVES, half = sub % X::HALVES;
+        narrow_copy16(o.trans, X::PL * mp * 2, rg * 16, C - 1, plane * mp * 2 + m0 * 2 + half * 64, to + (unsigned)(c * 1024));
     }
 }
 
-// the 16-byte fragment of tile row `row` (16-row tile base + lane & 15) at 64-byte step `k`
-__device__ __forceinline__ u32x4_t narrow_frag(const char *tile, int row, int k, int rows_per_half) {
-    const int fk = (threadIdx.x & 63) >> 4, chunk = (k & 1) * 4 + fk;
-    return *reinterpret_cast<const u32x4_t *>(tile + (k >> 1) * rows_per_half * 128 + row * 128 + ((chunk ^ (row & 7)) * 16));
+// the fixed rows n0 .. n0 + 31 of a wave as fragments; `keep`: lanes whose row counts (others hold zeros)
+template <typename X>
+__device__ __forceinline__ void narrow_fixed(const NarrowOperand &o, int Cp, int64_t row, bool keep, u32x4_t (&f)[X::KS][X::PL]) {
+    const char *p = o.rows + (row < o.count ? row : o.count - 1) * ((int64_t)X::PL * Cp * 2) + ((threadIdx.x & 63) >> 4) * 16;
+#pragma unroll
+    for (int k = 0; k < X::KS; ++k)
+#pragma unroll
+        for (int q = 0; q < X::PL; ++q) {
+            f[k][q] = *reinterpret_cast<const u32x4_t *>(p + q * Cp * 2 + k * 64);
+            if (!keep) f[k][q] = u32x4_t{0, 0, 0, 0};
+        }
 }
 
-template <typename T, int RB>
-__global__ __launch_bounds__(256, 2) void narrow_stats_kernel(NarrowArgs a) {
-    using X = Narrow<T, RB>;
-    __shared__ __align__(1024) char lds[2][X::ROWS_B];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15;
-    const int64_t n0 = (int64_t)blockIdx.x * kNarrowRows + wave * 32;
-    const int64_t m_begin = (int64_t)blockIdx.y * a.per_part, m_end = min(a.moving.rows, m_begin + a.per_part);
-    const unsigned base = (unsigned)(uintptr_t)&lds[0][0];
-    auto copy = [&](int64_t m0, int stage) {
+// S of 32 moving rows (16-row blocks `block`, block + 1 of the stage) against the wave's 32 fixed rows
+template <typename X>
+__device__ __forceinline__ void narrow_first(const char *stage, int block, int lane_at, const u32x4_t (&fixed)[2][X::KS][X::PL], f32x4_t (&s)[2][2]) {
 #pragma unroll
-        for (int h = 0; h < RB / 128; ++h) narrow_copy<kMoving>(a.moving, m0, h * 128, base + (unsigned)(stage * X::ROWS_B + h * kMoving * 128));
-    };
-    copy(m_begin, 0);
-    u32x4_t fixed[2][X::KSTEPS];
-    int64_t target[2];
-    float top[2], sum[2];
+    for (int k = 0; k < X::KS; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u32x4_t a[X::PL];
+#pragma unroll
+            for (int q = 0; q < X::PL; ++q) a[q] = narrow_frag(stage + (q * X::KS + k) * X::RG * 1024, block + i, lane_at);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) mma_planes<typename X::E, X::PL>(s[i][j], a, fixed[j][k]);
+        }
+}
+
+// eight values of a lane, as they lie, as a fragment of each plane
+template <typename E, int PL>
+__device__ __forceinline__ void narrow_pieces(const f32x4_t &lo, const f32x4_t &hi, u32x4_t (&d)[PL]) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        float v0 = w < 2 ? lo[w * 2] : hi[w * 2 - 4], v1 = w < 2 ? lo[w * 2 + 1] : hi[w * 2 - 3];
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            const Pack<E, 2> p{{from_float<E>(v0), from_float<E>(v1)}};
+            d[q][w] = __builtin_bit_cast(unsigned, p);
+            if (q + 1 < PL) { v0 -= to_float(p.v[0]); v1 -= to_float(p.v[1]); }
+        }
+    }
+}
+
+template <typename X>
+__global__ __launch_bounds__(256) void narrow_stats_kernel(NarrowArgs a) {
+    __shared__ __align__(1024) char lds[2][X::ROWS_B];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, lane_at = narrow_lane();
+    const int64_t n0 = (int64_t)blockIdx.x * kNarrowRows + wave * 32, m_begin = (int64_t)blockIdx.y * a.per_x;
+    const int rows = (int)min(a.per_x, a.w.count - m_begin);
+    const unsigned base_lds = (unsigned)(uintptr_t)&lds[0][0];
+    narrow_copy_rows<X>(a.w, a.Cp, m_begin, base_lds);
+    // a negative scale is taken as its magnitude and negated rows: the largest logit is then that of the largest product
+    const float scale2 = __builtin_fabsf(a.scale2);
+    u32x4_t fixed[2][X::KS][X::PL];
+    int target[2];
+    float base[2], sum[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const int64_t n = n0 + j * 16 + ln, row = n < a.fixed.rows ? n : a.fixed.rows - 1;
+        const int64_t n = n0 + j * 16 + ln;
+        narrow_fixed<X>(a.x, a.Cp, n, true, fixed[j]);
+        if (a.scale2 < 0.0f)
 #pragma unroll
-        for (int k = 0; k < X::KSTEPS; ++k) fixed[j][k] = *reinterpret_cast<const u32x4_t *>(a.fixed.p + row * a.fixed.ld + k * 64 + (lane >> 4) * 16);
-        target[j] = n < a.fixed.rows ? a.target[n] : -1;
-        top[j] = -INFINITY;
+            for (int k = 0; k < X::KS; ++k)
+#pragma unroll
+                for (int q = 0; q < X::PL; ++q) fixed[j][k][q] ^= 0x80008000u;
+        const int64_t t = (n < a.x.count ? a.target[n] : -1) - m_begin;
+        target[j] = t >= 0 && t < rows ? (int)t : -1;
+        base[j] = -INFINITY;
         sum[j] = 0.0f;
     }
     int stage = 0;
-    for (int64_t m0 = m_begin; m0 < m_end; m0 += kMoving, stage ^= 1) {
+    for (int m = 0; m < rows; m += X::MR, stage ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (m0 + kMoving < m_end) copy(m0 + kMoving, stage ^ 1);
-        const char *tile = lds[stage];
+        if (m + X::MR < rows) narrow_copy_rows<X>(a.w, a.Cp, m_begin + m + X::MR, base_lds + (unsigned)((stage ^ 1) * X::ROWS_B));
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int64_t mh = m0 + half * 32;
-            if (mh >= m_end) break;
+        for (int half = 0; half < X::HALVES; ++half) {
+            const int mh = m + half * 32;
+            if (mh >= rows) break;
             f32x4_t s[2][2] = {};
-#pragma unroll
-            for (int k = 0; k < X::KSTEPS; ++k) {
-                u32x4_t f[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) f[i] = narrow_frag(tile, half * 32 + i * 16 + ln, k, kMoving);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) mma16(s[i][j], f[i], fixed[j][k], T());
-            }
-            const int64_t m_lane = mh + (lane >> 4) * 4;
+            narrow_first<X>(lds[stage], half * 2, lane_at, fixed, s);
+            const int m_lane = mh + (lane >> 4) * 4;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float l[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) l[e] = s[e >> 2][j][e & 3] * a.scale2;
-                if (mh + 32 > m_end) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) if (m_lane + (e >> 2) * 16 + (e & 3) >= m_end) l[e] = -INFINITY;
-                }
-                const int64_t d = target[j] - mh;
-                if (__ballot(d >= 0 && d < 32)) {
+                if (__ballot((unsigned)(target[j] - mh) < 32u)) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (m_lane + (e >> 2) * 16 + (e & 3) == target[j] && target[j] < m_end) a.own[n0 + j * 16 + ln] = l[e];
+                        if (m_lane + (e >> 2) * 16 + (e & 3) == target[j]) a.own[n0 + j * 16 + ln] = s[e >> 2][j][e & 3] * scale2;
                 }
-                float t = top[j];
+                // (rows behind the table's last one repeat it: they do not raise the maximum)
+                float top = s[0][j][0];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t = fmaxf(t, l[e]);
-                const float low = t == -INFINITY ? 0.0f : t;      // (-Inf alone sums to 0; Inf - Inf and NaN make the sum NaN)
+                for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e >> 2][j][e & 3]);
+                // (a lane whose logits are all -Inf sums to 0; Inf - Inf and NaN make the sum NaN)
+                const float next = fmaxf(base[j], top == -INFINITY ? -INFINITY : top * scale2), low = next == -INFINITY ? 0.0f : next;
                 float add = 0.0f;
+                if (mh + 32 <= rows) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) add += __builtin_amdgcn_exp2f(l[e] - low);
-                sum[j] = sum[j] * __builtin_amdgcn_exp2f(top[j] - low) + add;
-                top[j] = t;
+                    for (int e = 0; e < 8; ++e) add += __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][j][e & 3], scale2, -low));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (m_lane + (e >> 2) * 16 + (e & 3) < rows) add += __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][j][e & 3], scale2, -low));
+                }
+                sum[j] = __builtin_fmaf(sum[j], __builtin_amdgcn_exp2f(base[j] - low), add);
+                base[j] = next;
             }
         }
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        float t = fmaxf(top[j], __shfl_xor(top[j], 16));
+        float t = fmaxf(base[j], __shfl_xor(base[j], 16));
         t = fmaxf(t, __shfl_xor(t, 32));
-        float r = sum[j] * __builtin_amdgcn_exp2f(top[j] - (t == -INFINITY ? 0.0f : t));
+        float r = sum[j] * __builtin_amdgcn_exp2f(base[j] - (t == -INFINITY ? 0.0f : t));
         r += __shfl_xor(r, 16);
         r += __shfl_xor(r, 32);
         const int64_t n = n0 + j * 16 + ln;
-        if (lane < 16 && n < a.fixed.rows) a.part[(int64_t)blockIdx.y * a.fixed.rows + n] = make_float2(t, r);
+        if (lane < 16 && n < a.x.count) a.part[(int64_t)blockIdx.y * a.x.count + n] = make_float2(t, r);
     }
 }
 
-// out[c][n] += sum_m trans[c][m] s[m][n] over the 32 rows m of one half of a stage
-template <typename T, int CT>
-__device__ __forceinline__ void narrow_second(const char *trans, int half, const f32x4_t (&s)[2][2], f32x4_t (&out)[CT][2]) {
-    const int ln = threadIdx.x & 15;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)      // (64 bytes of the row: 16 m; half = the 128-byte half)
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const u32x4_t f = narrow_frag(trans, c * 16 + ln, half * 2 + i, CT * 16);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) mma16(out[c][j], f, __builtin_bit_cast(u32x4_t, s[i][j]), T());
-            }
-    } else {
-        u32x4_t d[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const Pack<T, 2> p{{from_float<T>(s[w >> 1][j][(w & 1) * 2]), from_float<T>(s[w >> 1][j][(w & 1) * 2 + 1])}};
-                d[j][w] = __builtin_bit_cast(unsigned, p);
-            }
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            const u32x4_t f = narrow_frag(trans, c * 16 + ln, half, CT * 16);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) mma16(out[c][j], f, d[j], T());
-        }
-    }
-}
+// statistics of a stage's moving rows (of_table), in LDS
+struct NarrowRows {
+    float lse[2][64], ratio[2][64];
+    int target[2][64];
+};
 
 // OF_TABLE: fixed = table rows, moving = rows of x (statistics along m); else fixed = rows of x, moving = table rows
-template <typename T, int RB, bool OF_TABLE>
-__global__ __launch_bounds__(256, 2) void narrow_grad_kernel(NarrowArgs a) {
-    using X = Narrow<T, RB>;
-    constexpr float unit = GradUnit<T>::value;
-    __shared__ __align__(1024) char lds[2][X::ROWS_B + X::TRANS_B];
-    __shared__ float row_lse[OF_TABLE ? 2 : 1][kMoving], row_ratio[OF_TABLE ? 2 : 1][kMoving];
-    __shared__ int row_target[OF_TABLE ? 2 : 1][kMoving];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, group = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * kNarrowRows + wave * 32;
-    const int64_t m_begin = (int64_t)blockIdx.y * a.per_part, m_end = min(a.moving.rows, m_begin + a.per_part);
-    const unsigned base = (unsigned)(uintptr_t)&lds[0][0];
-    // the transposed tile is CT * 16 rows of kMoving elements: one 128-byte half (16 bits) or two (float32)
-    constexpr int HALVES_T = kMoving * (int)sizeof(T) / 128;
-    auto copy = [&](int64_t m0, int stage) {
-        const unsigned to = base + (unsigned)(stage * (X::ROWS_B + X::TRANS_B));
-#pragma unroll
-        for (int h = 0; h < RB / 128; ++h) narrow_copy<kMoving>(a.moving, m0, h * 128, to + (unsigned)(h * kMoving * 128));
-#pragma unroll
-        for (int h = 0; h < HALVES_T; ++h)
-            narrow_copy<X::CT * 16>(a.moving_t, 0, m0 * (int64_t)sizeof(T) + h * 128, to + (unsigned)(X::ROWS_B + h * X::CT * 16 * 128));
+template <typename X, bool OF_TABLE>
+__device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOperand &fix, const NarrowOperand &mov, int64_t block, int64_t part, float unit,
+                                            char *lds, NarrowRows &row_stats) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, group = lane >> 4, lane_at = narrow_lane();
+    const int64_t per = OF_TABLE ? a.per_w : a.per_x, n0 = block * kNarrowRows + wave * 32, m_begin = part * per;
+    const int rows = (int)min(per, mov.count - m_begin);
+    const unsigned base_lds = (unsigned)(uintptr_t)lds;
+    auto copy = [&](int m, int stage) {
+        const unsigned to = base_lds + (unsigned)(stage * (X::ROWS_B + X::TRANS_B));
+        narrow_copy_rows<X>(mov, a.Cp, m_begin + m, to);
+        narrow_copy_trans<X>(mov, a.C, m_begin + m, to + (unsigned)X::ROWS_B);
     };
-    // statistics of the moving rows of a stage (OF_TABLE): thread t < kMoving's row; loaded ahead, stored with the stage
-    auto stats = [&](int64_t m0, float &lse, float &ratio, int &target) {
-        const int64_t m = m0 + threadIdx.x;
-        const bool kept = threadIdx.x < kMoving && m < m_end && ce_kept(a.target[m], a.ignore);
-        lse = kept ? a.lse2[m] : 0.0f;
-        ratio = kept ? a.ratio[m] * unit : 0.0f;
-        target = kept && a.target[m] >= 0 && a.target[m] < a.fixed.rows ? (int)a.target[m] : -1;
+    const float *ratios = a.factors + a.x.count;
+    float lse_next = 0.0f, ratio_next = 0.0f;
+    int target_next = -1;
+    auto stats = [&](int m) {      // thread t < MR's row of the stage, loaded a stage ahead
+        const int64_t row = m_begin + m + threadIdx.x;
+        const bool kept = threadIdx.x < X::MR && m + (int)threadIdx.x < rows && ce_kept(a.target[row], a.ignore);
+        lse_next = kept ? a.lse2[row] : 0.0f;
+        ratio_next = kept ? ratios[row] * unit : 0.0f;
+        target_next = kept ? (int)(a.target[row] >= 0 && a.target[row] < fix.count ? a.target[row] : -1) : -1;
     };
-    copy(m_begin, 0);
-    float lse_next, ratio_next;
-    int target_next;
-    if (OF_TABLE) stats(m_begin, lse_next, ratio_next, target_next);
-    u32x4_t fixed[2][X::KSTEPS];
-    int64_t target[2];
+    copy(0, 0);
+    if (OF_TABLE) stats(0);
+    u32x4_t fixed[2][X::KS][X::PL];
+    int target[2];
     float lse[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const int64_t n = n0 + j * 16 + ln, row = n < a.fixed.rows ? n : a.fixed.rows - 1;
-        const bool kept = OF_TABLE || (n < a.fixed.rows && ce_kept(a.target[row], a.ignore));
-#pragma unroll
-        for (int k = 0; k < X::KSTEPS; ++k) {
-            fixed[j][k] = *reinterpret_cast<const u32x4_t *>(a.fixed.p + row * a.fixed.ld + k * 64 + group * 16);
-            if (!kept) fixed[j][k] = u32x4_t{0, 0, 0, 0};      // (whatever an ignored row holds; its exponentials are of -Inf)
-        }
-        target[j] = OF_TABLE ? n : kept ? a.target[row] : -1;
-        lse[j] = OF_TABLE ? 0.0f : kept ? a.lse2[row] : INFINITY;
+        const int64_t n = n0 + j * 16 + ln, t = !OF_TABLE && n < fix.count ? a.target[n] : a.ignore;
+        const bool kept = OF_TABLE || ce_kept(t, a.ignore);
+        // (whatever an ignored row holds, its S are 0 and its exponentials those of -Inf)
+        narrow_fixed<X>(fix, a.Cp, n, kept, fixed[j]);
+        lse[j] = OF_TABLE ? 0.0f : kept ? a.lse2[n] : INFINITY;
+        target[j] = OF_TABLE ? (int)n : kept && t >= m_begin && t - m_begin < rows ? (int)(t - m_begin) : -1;
     }
     f32x4_t out[X::CT][2] = {};
     int stage = 0;
-    for (int64_t m0 = m_begin; m0 < m_end; m0 += kMoving, stage ^= 1) {
-        if (OF_TABLE && threadIdx.x < kMoving) {      // (last read two stages ago, a barrier in between)
-            row_lse[stage & (OF_TABLE ? 1 : 0)][threadIdx.x] = lse_next;
-            row_ratio[stage & (OF_TABLE ? 1 : 0)][threadIdx.x] = ratio_next;
-            row_target[stage & (OF_TABLE ? 1 : 0)][threadIdx.x] = target_next;
+    for (int m = 0; m < rows; m += X::MR, stage ^= 1) {
+        if (OF_TABLE && threadIdx.x < X::MR) {      // (last read two stages ago, a barrier in between)
+            row_stats.lse[stage][threadIdx.x] = lse_next;
+            row_stats.ratio[stage][threadIdx.x] = ratio_next;
+            row_stats.target[stage][threadIdx.x] = target_next;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (m0 + kMoving < m_end) {
-            copy(m0 + kMoving, stage ^ 1);
-            if (OF_TABLE) stats(m0 + kMoving, lse_next, ratio_next, target_next);
+        if (m + X::MR < rows) {
+            copy(m + X::MR, stage ^ 1);
+            if (OF_TABLE) stats(m + X::MR);
         }
-        const char *tile = lds[stage], *trans = tile + X::ROWS_B;
+        const char *tile = lds + stage * (X::ROWS_B + X::TRANS_B), *trans = tile + X::ROWS_B;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int64_t mh = m0 + half * 32;
-            if (mh >= m_end) break;
+        for (int half = 0; half < X::HALVES; ++half) {
+            const int mh = m + half * 32;
+            if (mh >= rows) break;
             f32x4_t s[2][2] = {};
-#pragma unroll
-            for (int k = 0; k < X::KSTEPS; ++k) {
-                u32x4_t f[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) f[i] = narrow_frag(tile, half * 32 + i * 16 + ln, k, kMoving);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) mma16(s[i][j], f[i], fixed[j][k], T());
-            }
+            narrow_first<X>(tile, half * 2, lane_at, fixed, s);
             if (OF_TABLE) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int at = half * 32 + i * 16 + group * 4;
-                    const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(&row_lse[stage][at]), r4 = *reinterpret_cast<const f32x4_t *>(&row_ratio[stage][at]);
-                    const u32x4_t t4 = *reinterpret_cast<const u32x4_t *>(&row_target[stage][at]);
+                    const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(&row_stats.lse[stage][at]), r4 = *reinterpret_cast<const f32x4_t *>(&row_stats.ratio[stage][at]);
+                    const u32x4_t t4 = *reinterpret_cast<const u32x4_t *>(&row_stats.target[stage][at]);
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            float d = __builtin_amdgcn_exp2f(s[i][j][r] * a.scale2 - l4[r]);
-                            if ((int)t4[r] == (int)(n0 + j * 16 + ln)) d -= 1.0f;
+                            float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][r], a.scale2, -l4[r]));
+                            if ((int)t4[r] == target[j]) d -= 1.0f;
                             s[i][j][r] = r4[r] == 0.0f ? 0.0f : d * r4[r];      // (an ignored row's S may be anything)
                         }
                 }
@@ -264,65 +296,198 @@ __global__ __launch_bounds__(256, 2) void narrow_grad_kernel(NarrowArgs a) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[i][j][r] = __builtin_amdgcn_exp2f(s[i][j][r] * a.scale2 - lse[j]);
-                    const int64_t d = target[j] - mh;
-                    if (__ballot(d >= 0 && d < 32)) {
+                        for (int r = 0; r < 4; ++r) s[i][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][r], a.scale2, -lse[j]));
+                    const int d = target[j] - mh;
+                    if (__ballot((unsigned)d < 32u)) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) if (d == i * 16 + group * 4 + r) s[i][j][r] -= 1.0f;
                     }
+                    if (unit != 1.0f)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[i][j][r] *= unit;
+                            for (int r = 0; r < 4; ++r) s[i][j][r] *= unit;
                 }
-                if (mh + 32 > m_end) {
+                if (mh + 32 > rows) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (mh + i * 16 + group * 4 + r >= m_end) s[i][0][r] = s[i][1][r] = 0.0f;
+                            if (mh + i * 16 + group * 4 + r >= rows) s[i][0][r] = s[i][1][r] = 0.0f;
                 }
             }
-            narrow_second<T, X::CT>(trans, half, s, out);
+            u32x4_t d[2][X::PL];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) narrow_pieces<typename X::E, X::PL>(s[0][j], s[1][j], d[j]);
+#pragma unroll
+            for (int c = 0; c < X::CT; ++c) {
+                u32x4_t f[X::PL];
+#pragma unroll
+                for (int q = 0; q < X::PL; ++q) f[q] = narrow_frag(trans + (q * X::HALVES + half) * X::CT * 1024, c, lane_at);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma_planes<typename X::E, X::PL>(out[c][j], f, d[j]);
+            }
         }
     }
+    float *sums = OF_TABLE ? a.sums_w : a.sums_x;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int64_t n = n0 + j * 16 + ln;
-        if (n >= a.fixed.rows) continue;
+        if (n >= fix.count) continue;
 #pragma unroll
         for (int c = 0; c < X::CT; ++c) {
-            const int64_t col = c * 16 + group * 4;
-            if (col < a.C) *reinterpret_cast<f32x4_t *>(a.sums + ((int64_t)blockIdx.y * a.fixed.rows + n) * a.ld_sums + col) = out[c][j];
+            const int col = c * 16 + group * 4;
+            if (col < a.C) *reinterpret_cast<f32x4_t *>(sums + (part * fix.count + n) * a.ld_sums + col) = out[c][j];
         }
     }
 }
 
-template <typename T, int RB>
-static void narrow_launch_stats(const NarrowArgs &a, int parts, hipStream_t st) {
-    hipLaunchKernelGGL((narrow_stats_kernel<T, RB>), dim3((unsigned)ceil_div(a.fixed.rows, kNarrowRows), (unsigned)parts), dim3(256), 0, st, a);
-}
-template <typename T, int RB>
-static void narrow_launch_grad(bool of_table, const NarrowArgs &a, int parts, hipStream_t st) {
-    const dim3 grid((unsigned)ceil_div(a.fixed.rows, kNarrowRows), (unsigned)parts);
-    if (of_table) hipLaunchKernelGGL((narrow_grad_kernel<T, RB, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((narrow_grad_kernel<T, RB, false>), grid, dim3(256), 0, st, a);
+// One launch for both gradients: the workgroups of dx, then those of dW.
+template <typename X>
+__global__ __launch_bounds__(256, 2) void narrow_grad_kernel(NarrowArgs a, int64_t blocks_x, int64_t groups_x, int64_t blocks_w, float unit) {
+    __shared__ __align__(1024) char lds[2 * (X::ROWS_B + X::TRANS_B)];
+    __shared__ NarrowRows row_stats;
+    const int64_t id = blockIdx.x;
+    if (id < groups_x) narrow_grad<X, false>(a, a.x, a.w, id % blocks_x, id / blocks_x, unit, lds, row_stats);
+    else narrow_grad<X, true>(a, a.w, a.x, (id - groups_x) % blocks_w, (id - groups_x) / blocks_w, unit, lds, row_stats);
 }
 
-int ce_narrow_stats(int dtype, int row_bytes, const NarrowArgs &a, int parts, hipStream_t st) {
-    MVS_DTYPE_DISPATCH(dtype, T, {
-        if (row_bytes == 128) narrow_launch_stats<T, 128>(a, parts, st);
-        else narrow_launch_stats<T, 256>(a, parts, st);
-    });
+// a value's pieces: 8 bits each, the first one cut instead of rounded where rounding would overflow
+template <typename E, int PL, typename T>
+__device__ __forceinline__ void pieces_of(T value, E (&p)[PL]) {
+    if constexpr (PL == 1) {
+        p[0] = value;
+    } else {
+        float v = value;
+        p[0] = from_float<E>(v);
+        if (__builtin_fabsf(v) > DtypeMax<E>::value && __builtin_fabsf(v) <= DtypeMax<float>::value) p[0].bits = (unsigned short)(__float_as_uint(v) >> 16);
+#pragma unroll
+        for (int q = 1; q < PL; ++q) {
+            v -= to_float(p[q - 1]);
+            p[q] = from_float<E>(v);
+        }
+    }
+}
+
+// Writes what the other kernels read of x (blockIdx.y = 0) and of the table (1): the rows in pieces and their transpose, 64 rows per
+// workgroup.  Backward: blockIdx.y = 2 works out the rows' factors (one workgroup).
+template <typename T, typename E, int PL>
+__global__ __launch_bounds__(256) void narrow_prepare_kernel(NarrowArgs a) {
+    __shared__ T tile[64][128 + 2];
+    __shared__ float tops[4];
+    const int tid = threadIdx.x;
+    if (blockIdx.y == 2) {
+        if (blockIdx.x == 0) ce_factors(a.grad_loss, a.kept, a.target, a.x.count, a.ignore, a.reduction, a.factors, tops);
+        return;
+    }
+    const NarrowOperand &o = blockIdx.y ? a.w : a.x;
+    const int64_t r0 = (int64_t)blockIdx.x * 64, mp = (o.count + 63) & ~(int64_t)63;
+    if (r0 >= o.count || (!o.write_rows && !o.trans)) return;
+    const T *source = static_cast<const T *>(o.source);
+    const int here = (int)min((int64_t)64, o.count - r0);
+    for (int i = tid; i < 64 * a.C; i += 256) {
+        const int r = i / a.C, c = i - r * a.C;
+        tile[r][c] = r < here ? source[(r0 + r) * a.C + c] : from_float<T>(0.0f);
+    }
+    __syncthreads();
+    if (o.write_rows) {
+        E *rows = reinterpret_cast<E *>(o.rows);
+        for (int i = tid; i < here * a.Cp; i += 256) {
+            const int r = i / a.Cp, c = i - r * a.Cp;
+            E p[PL];
+            pieces_of<E, PL>(c < a.C ? tile[r][c] : from_float<T>(0.0f), p);
+#pragma unroll
+            for (int q = 0; q < PL; ++q) rows[((r0 + r) * PL + q) * a.Cp + c] = p[q];
+        }
+    }
+    if (o.trans) {
+        E *trans = reinterpret_cast<E *>(o.trans);
+        const int place = tid & 63, r = (place & 32) + ((place >> 3) & 3) * 4 + (place & 3) + ((place & 4) << 2);
+        // (ignored rows of x as zeros, whatever they hold)
+        const bool keep = r < here && (blockIdx.y || ce_kept(a.target[r0 + r], a.ignore));
+        for (int c = tid >> 6; c < a.C; c += 4) {
+            E p[PL];
+            pieces_of<E, PL>(keep ? tile[r][c] : from_float<T>(0.0f), p);
+#pragma unroll
+            for (int q = 0; q < PL; ++q) trans[((int64_t)c * PL + q) * mp + r0 + place] = p[q];
+        }
+    }
+}
+
+// both gradients from the parts' sums: workgroups of dx, then of dW
+template <typename T>
+__global__ __launch_bounds__(256) void narrow_finish_kernel(NarrowArgs a, int64_t groups_x) {
+    const int64_t id = blockIdx.x;
+    if (id < groups_x)
+        ce_finish<T, true>(a.sums_x, a.parts_x, a.x.count, a.C, a.ld_sums, a.factors, a.factor, static_cast<T *>(a.grad_x), id);
+    else
+        ce_finish<T, false>(a.sums_w, a.parts_w, a.w.count, a.C, a.ld_sums, a.factors + 2 * a.x.count, a.factor, static_cast<T *>(a.grad_w), id - groups_x);
+}
+
+template <typename T, typename E, int PL>
+static void narrow_prepare(const NarrowArgs &a, bool backward, hipStream_t st) {
+    const int64_t most = a.x.count > a.w.count ? a.x.count : a.w.count;
+    hipLaunchKernelGGL((narrow_prepare_kernel<T, E, PL>), dim3((unsigned)ceil_div(most, 64), backward ? 3 : 2), dim3(256), 0, st, a);
+}
+
+template <typename X>
+static void narrow_stats(const NarrowArgs &a, hipStream_t st) {
+    hipLaunchKernelGGL((narrow_stats_kernel<X>), dim3((unsigned)ceil_div(a.x.count, kNarrowRows), (unsigned)a.parts_x), dim3(256), 0, st, a);
+}
+template <typename X>
+static void narrow_grads(const NarrowArgs &a, float unit, hipStream_t st) {
+    const int64_t bx = ceil_div(a.x.count, kNarrowRows), bw = ceil_div(a.w.count, kNarrowRows);
+    const int64_t gx = a.sums_x ? bx * a.parts_x : 0, gw = a.sums_w ? bw * a.parts_w : 0;
+    hipLaunchKernelGGL((narrow_grad_kernel<X>), dim3((unsigned)(gx + gw)), dim3(256), 0, st, a, bx, gx, bw, unit);
+}
+
+// f(X()) for the planes and the 32-element steps of a row
+template <typename E, int PL, typename F>
+static void narrow_steps(int ks, F f) {
+    if (ks == 1) f(Narrow<E, PL, 1>());
+    else if (ks == 2) f(Narrow<E, PL, 2>());
+    else if constexpr (PL == 1) {
+        if (ks == 3) f(Narrow<E, PL, 3>());
+        else f(Narrow<E, PL, 4>());
+    }
+}
+
+int ce_narrow_forward(int dtype, const NarrowArgs &a, hipStream_t st) {
+    const int ks = a.Cp / 32;
+    auto stats = [&](auto x) { narrow_stats<decltype(x)>(a, st); };
+    const bool prepare = a.x.write_rows || a.w.write_rows;
+    if (dtype == MVS_DTYPE_F32) {
+        narrow_prepare<float, bf16_t, 3>(a, false, st);
+        narrow_steps<bf16_t, 3>(ks, stats);
+    } else if (dtype == MVS_DTYPE_BF16) {
+        if (prepare) narrow_prepare<bf16_t, bf16_t, 1>(a, false, st);
+        narrow_steps<bf16_t, 1>(ks, stats);
+    } else {
+        if (prepare) narrow_prepare<f16_t, f16_t, 1>(a, false, st);
+        narrow_steps<f16_t, 1>(ks, stats);
+    }
     return check_launch("mvs_linear_ce_fwd");
 }
-int ce_narrow_grad(int dtype, int row_bytes, bool of_table, const NarrowArgs &a, int parts, hipStream_t st) {
-    MVS_DTYPE_DISPATCH(dtype, T, {
-        if (row_bytes == 128) narrow_launch_grad<T, 128>(of_table, a, parts, st);
-        else narrow_launch_grad<T, 256>(of_table, a, parts, st);
-    });
+
+int ce_narrow_backward(int dtype, const NarrowArgs &a, hipStream_t st) {
+    const int ks = a.Cp / 32;
+    const int64_t quads = a.ld_sums / 4, fx = a.sums_x ? ceil_div(a.x.count * quads, 256) : 0, fw = a.sums_w ? ceil_div(a.w.count * quads, 256) : 0;
+    const dim3 finish((unsigned)(fx + fw));
+    if (dtype == MVS_DTYPE_F32) {
+        narrow_prepare<float, bf16_t, 3>(a, true, st);
+        narrow_steps<bf16_t, 3>(ks, [&](auto x) { narrow_grads<decltype(x)>(a, GradUnit<float>::value, st); });
+        hipLaunchKernelGGL((narrow_finish_kernel<float>), finish, dim3(256), 0, st, a, fx);
+    } else if (dtype == MVS_DTYPE_BF16) {
+        narrow_prepare<bf16_t, bf16_t, 1>(a, true, st);
+        narrow_steps<bf16_t, 1>(ks, [&](auto x) { narrow_grads<decltype(x)>(a, GradUnit<bf16_t>::value, st); });
+        hipLaunchKernelGGL((narrow_finish_kernel<bf16_t>), finish, dim3(256), 0, st, a, fx);
+    } else {
+        narrow_prepare<f16_t, f16_t, 1>(a, true, st);
+        narrow_steps<f16_t, 1>(ks, [&](auto x) { narrow_grads<decltype(x)>(a, GradUnit<f16_t>::value, st); });
+        hipLaunchKernelGGL((narrow_finish_kernel<f16_t>), finish, dim3(256), 0, st, a, fx);
+    }
     return check_launch("mvs_linear_ce_bwd");
 }
 

@@ -12,8 +12,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import (DTYPES, MVS_LAYOUT_C4, MVS_LAYOUT_C8, MVS_LAYOUT_C16, MVS_LAYOUT_NCHW, MVS_LAYOUT_NHWC, MvsHipError, any_ptr, check,
-                   ptr, stream)
+from ._lib import (DTYPES, MVS_LAYOUT_C4, MVS_LAYOUT_C8, MVS_LAYOUT_C16, MVS_LAYOUT_NCHW, MVS_LAYOUT_NHWC, MvsHipError, check, ptr,
+                   stream)
 
 _I = ctypes.c_int
 
@@ -1720,6 +1720,29 @@ def _aligned16(t):
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _here(who, *tensors):
+    """The raw stream that `who` launches on, after the check that ptr() makes of every tensor, made once for all of them: on the
+    GPU, and on the current device.  (The training operators pass data_ptr() numbers: a check per pointer was a third of a small
+    call's time on the host.)"""
+    dev = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if not t.is_cuda:
+            raise MvsHipError(f"{who}: mvs_amd ops need device (HIP) tensors; got a CPU tensor")
+        if t.get_device() != dev:
+            raise MvsHipError(f"{who}: tensor on cuda:{t.get_device()} but the current device is cuda:{dev}: wrap the call in torch.cuda.device(...)")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _first_order(backward):
+    """A backward pass that is not differentiable again: refused by autograd where a second derivative is asked for
+    (once_differentiable, whose wrapping is skipped where no graph of the backward pass is being made)."""
+    once = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
+
+
 def _dtype_code(t, who):
     code = DTYPES.get(t.dtype)
     if code is None:
@@ -1752,9 +1775,10 @@ def act8_quantize(x):
     round-to-nearest-even(x / 2^k), off by at most half a step.  A block that holds an Inf or NaN reads back as NaN: a poisoned
     activation stays one.  No gradient passes through (what a backward pass reads is a constant to it)."""
     code = _dtype_code(x, "act8_quantize")
+    st = _here("act8_quantize", x)
     x = x.detach().contiguous()
     held = Act8.empty_for(x)
-    check(_lib.load().mvs_act8_quantize(any_ptr(x), code, x.numel(), any_ptr(held.codes), any_ptr(held.scales), stream()), "mvs_act8_quantize")
+    check(_lib.load().mvs_act8_quantize(x.data_ptr(), code, x.numel(), held.codes.data_ptr(), held.scales.data_ptr(), st), "mvs_act8_quantize")
     return held
 
 
@@ -1763,8 +1787,8 @@ def act8_dequantize(held, dtype=None):
     exact in float32 and bfloat16, at most the type's largest finite number."""
     out = torch.empty(held.shape, device=held.codes.device, dtype=held.dtype if dtype is None else dtype)
     code = _dtype_code(out, "act8_dequantize")
-    check(_lib.load().mvs_act8_dequantize(any_ptr(held.codes), any_ptr(held.scales), out.numel(), code, any_ptr(out), stream()),
-          "mvs_act8_dequantize")
+    check(_lib.load().mvs_act8_dequantize(held.codes.data_ptr(), held.scales.data_ptr(), out.numel(), code, out.data_ptr(),
+                                          _here("act8_dequantize", held.codes)), "mvs_act8_dequantize")
     return out
 
 
@@ -1821,15 +1845,18 @@ class _BnReluAct8CL(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, skip, running_mean, running_var, nbt, momentum, eps, relu, groups):
+        st = _here("bn_relu_cl", *[t for t in (x, weight, bias, skip, running_mean, running_var, nbt) if t is not None])
         x = _aligned16(_f32c(x))
         C = x.shape[-1]
         if x.shape[0] % groups:
             raise MvsHipError(f"bn_relu_cl: leading dimension {x.shape[0]} is not a multiple of groups={groups}")
+        if skip is not None and skip.shape != x.shape:
+            raise MvsHipError(f"bn_relu_cl: skip {tuple(skip.shape)} does not fit x {tuple(x.shape)}")
         N = x.numel() // C // groups
         lib = _lib.load()
-        nbytes = int(lib.mvs_bn_train_workspace_bytes(C))
-        if nbytes == 0:
-            raise MvsHipError(f"bn_relu_cl: C={C} not supported")
+        nbytes = lib.mvs_bn_train_workspace_bytes(C)
+        if nbytes == 0 or weight.numel() != C:
+            raise MvsHipError(f"bn_relu_cl: C={C} not supported by a BatchNorm of {weight.numel()} channels")
         ws = torch.empty((nbytes // 4,), device=x.device, dtype=torch.float32)
         w, b = _aligned16(_f32c(weight.detach())), _aligned16(_f32c(bias.detach()))
         sk = _aligned16(_f32c(skip)) if skip is not None else None
@@ -1838,30 +1865,31 @@ class _BnReluAct8CL(torch.autograd.Function):
         y = torch.empty_like(x)
         held = Act8.empty_for(x)
         mask = torch.empty(held.scales.shape, device=x.device, dtype=torch.int32) if relu else None
-        check(lib.mvs_bn_train_fwd_act8_f32(ptr(x), ptr(w), ptr(b), ptr(sk), int(groups), N, C, float(eps), float(momentum), int(relu),
-                                            ptr(running_mean), ptr(running_var), any_ptr(nbt), ptr(mean), ptr(invstd), ptr(y),
-                                            any_ptr(held.codes), any_ptr(held.scales), any_ptr(mask), ptr(ws), nbytes, stream()),
-              "mvs_bn_train_fwd_act8_f32")
+        at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        check(lib.mvs_bn_train_fwd_act8_f32(at(x), at(w), at(b), at(sk), int(groups), N, C, float(eps), float(momentum), int(relu),
+                                            ptr(running_mean), ptr(running_var), at(nbt), at(mean), at(invstd), at(y), at(held.codes),
+                                            at(held.scales), at(mask), at(ws), nbytes, st), "mvs_bn_train_fwd_act8_f32")
         ctx.save_for_backward(held.codes, held.scales, mask, w, mean, invstd)
         ctx.has_skip, ctx.groups = skip is not None, int(groups)
         ctx.mark_non_differentiable(*[t for t in (running_mean, running_var, nbt) if t is not None])
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gy):
         codes, scales, mask, w, mean, invstd = ctx.saved_tensors
+        st = _here("bn_relu_cl", gy, codes)
         gy = _aligned16(_f32c(gy))
         C = gy.shape[-1]
         N = gy.numel() // C // ctx.groups
         lib = _lib.load()
-        nbytes = int(lib.mvs_bn_train_workspace_bytes(C))
+        nbytes = lib.mvs_bn_train_workspace_bytes(C)
         ws = torch.empty((nbytes // 4,), device=gy.device, dtype=torch.float32)
         gx = torch.empty_like(gy)
         gw, gb = torch.empty_like(w), torch.empty_like(w)
-        check(lib.mvs_bn_train_bwd_act8_f32(ptr(gy), any_ptr(codes), any_ptr(scales), any_ptr(mask), ptr(w), ptr(mean), ptr(invstd),
-                                            ctx.groups, N, C, ptr(gx), ptr(gw), ptr(gb), ptr(ws), nbytes, stream()),
-              "mvs_bn_train_bwd_act8_f32")
+        check(lib.mvs_bn_train_bwd_act8_f32(gy.data_ptr(), codes.data_ptr(), scales.data_ptr(), None if mask is None else mask.data_ptr(), w.data_ptr(),
+                                            mean.data_ptr(), invstd.data_ptr(), ctx.groups, N, C, gx.data_ptr(), gw.data_ptr(), gb.data_ptr(),
+                                            ws.data_ptr(), nbytes, st), "mvs_bn_train_bwd_act8_f32")
         return gx, gw, gb, (gy if ctx.has_skip else None), None, None, None, None, None, None, None
 
 
@@ -2075,27 +2103,29 @@ class _LookupRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, index, scale):
         rows, C = table.shape
+        st = _here("lookup_rows", table, index)
         t = table.detach().contiguous()
         out = torch.empty((*index.shape, C), device=t.device, dtype=t.dtype)
-        check(_lib.load().mvs_lookup_rows_fwd(any_ptr(t), DTYPES[t.dtype], rows, C, any_ptr(index), index.numel(), scale, any_ptr(out), stream()),
+        check(_lib.load().mvs_lookup_rows_fwd(t.data_ptr(), DTYPES[t.dtype], rows, C, index.data_ptr(), index.numel(), scale, out.data_ptr(), st),
               "mvs_lookup_rows_fwd")
         ctx.save_for_backward(index)
         ctx.cfg = (rows, C, scale)
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         index, = ctx.saved_tensors
         rows, C, scale = ctx.cfg
+        st = _here("lookup_rows", g, index)
         g = g.contiguous()
         n = index.numel()
         lib = _lib.load()
-        nbytes = int(lib.mvs_lookup_rows_workspace_bytes(rows, C, n))
+        nbytes = lib.mvs_lookup_rows_workspace_bytes(rows, C, n)
         ws = torch.empty((nbytes,), device=g.device, dtype=torch.uint8)
         grad = torch.empty((rows, C), device=g.device, dtype=g.dtype)
-        check(lib.mvs_lookup_rows_bwd(any_ptr(g), DTYPES[g.dtype], any_ptr(index), n, rows, C, scale, any_ptr(grad), any_ptr(ws), nbytes,
-                                      stream()), "mvs_lookup_rows_bwd")
+        check(lib.mvs_lookup_rows_bwd(g.data_ptr(), DTYPES[g.dtype], index.data_ptr(), n, rows, C, scale, grad.data_ptr(), ws.data_ptr(), nbytes,
+                                      st), "mvs_lookup_rows_bwd")
         return grad, None, None
 
 
@@ -2122,36 +2152,40 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, x, weight, target, scale, ignore_index, reduction):
         n, C = x.shape
         V = weight.shape[0]
+        st = _here("linear_cross_entropy", x, weight, target)
         xd, wd = _aligned16(x.detach().contiguous()), _aligned16(weight.detach().contiguous())
         code = DTYPES[xd.dtype]
         lib = _lib.load()
-        nbytes = int(lib.mvs_linear_ce_workspace_bytes(n, V, C, code, 0, 0, 0))
+        nbytes = lib.mvs_linear_ce_workspace_bytes(n, V, C, code, 0, 0, 0)
         ws = torch.empty((nbytes,), device=xd.device, dtype=torch.uint8)
         loss = torch.empty((n,) if reduction == 0 else (), device=xd.device, dtype=torch.float32)
         state = torch.empty((n + 1,), device=xd.device, dtype=torch.float32)      # the rows' lse, and how many rows were kept
-        check(lib.mvs_linear_ce_fwd(any_ptr(xd), any_ptr(wd), code, any_ptr(target), n, V, C, scale, ignore_index, reduction, any_ptr(loss),
-                                    any_ptr(state[:n]), any_ptr(state[n:]), any_ptr(ws), nbytes, stream()), "mvs_linear_ce_fwd")
+        at = state.data_ptr()
+        check(lib.mvs_linear_ce_fwd(xd.data_ptr(), wd.data_ptr(), code, target.data_ptr(), n, V, C, scale, ignore_index, reduction, loss.data_ptr(),
+                                    at, at + 4 * n, ws.data_ptr(), nbytes, st), "mvs_linear_ce_fwd")
         ctx.save_for_backward(xd, wd, target, state)
         ctx.cfg = (scale, ignore_index, reduction)
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         x, w, target, state = ctx.saved_tensors
         scale, ignore_index, reduction = ctx.cfg
         n, C = x.shape
         V = w.shape[0]
+        st = _here("linear_cross_entropy", g, x)
         need_x, need_w = ctx.needs_input_grad[:2]
         lib = _lib.load()
         g = _f32c(g)
         code = DTYPES[x.dtype]
-        nbytes = int(lib.mvs_linear_ce_workspace_bytes(n, V, C, code, 1, int(need_x), int(need_w)))
+        nbytes = lib.mvs_linear_ce_workspace_bytes(n, V, C, code, 1, int(need_x), int(need_w))
         ws = torch.empty((nbytes,), device=x.device, dtype=torch.uint8)
         gx = torch.empty_like(x) if need_x else None
         gw = torch.empty_like(w) if need_w else None
-        check(lib.mvs_linear_ce_bwd(any_ptr(x), any_ptr(w), code, any_ptr(target), any_ptr(state[:n]), any_ptr(state[n:]), ptr(g), n, V, C,
-                                    scale, ignore_index, reduction, any_ptr(gx), any_ptr(gw), any_ptr(ws), nbytes, stream()),
+        at = state.data_ptr()
+        check(lib.mvs_linear_ce_bwd(x.data_ptr(), w.data_ptr(), code, target.data_ptr(), at, at + 4 * n, g.data_ptr(), n, V, C, scale, ignore_index,
+                                    reduction, gx.data_ptr() if need_x else None, gw.data_ptr() if need_w else None, ws.data_ptr(), nbytes, st),
               "mvs_linear_ce_bwd")
         return gx, gw, None, None, None, None
 
