@@ -23,14 +23,16 @@
 
 namespace mvs {
 
-template <int BM_, int BN_, int WM_, int WN_>
+// AHEAD: a wave reads its fragments half a step ahead.  One workgroup of 8 waves per CU needs it; two of 4 waves hide each other's
+// reads and are slower with it (8192 x 128000 x 2048 bfloat16 forward: 256 x 256 tiles 3.63 -> 3.52 ms, 128 x 128 4.26 -> 4.70 ms).
+template <int BM_, int BN_, int WM_, int WN_, bool AHEAD_>
 struct Tile {
+    static constexpr bool AHEAD = AHEAD_;
     static constexpr int BM = BM_, BN = BN_, WAVES_M = WM_, WAVES_N = WN_, WAVES = WM_ * WN_, THREADS = 64 * WAVES;
     static constexpr int TM = BM / WAVES_M / 16, TN = BN / WAVES_N / 16;
     static constexpr int STAGE = (BM + BN) * kRowBytes;
     static constexpr int COPIES = (BM + BN) / 8;                 // wave-wide copies of 8 rows
     static constexpr int PER_WAVE = (COPIES + WAVES - 1) / WAVES;
-    static_assert(COPIES % WAVES == 0 || COPIES < WAVES || PER_WAVE > 0, "");
 };
 
 // acc[tm][tn] += the tile (m0, n0) of A B^T over `steps` 128-byte steps of k
@@ -64,24 +66,52 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
     const int frow = lane & 15, fk = lane >> 4;
     const int swz0 = (fk ^ (frow & 7)) * 16, swz1 = ((4 + fk) ^ (frow & 7)) * 16;
     const int a_row = (wm * (X::BM / X::WAVES_M) + frow) * kRowBytes, b_row = (X::BM + wn * (X::BN / X::WAVES_N) + frow) * kRowBytes;
+    auto read = [&](int stage, int swz, u32x4_t (&fa)[X::TM], u32x4_t (&fb)[X::TN]) {
+        const char *at = lds + stage * X::STAGE + swz;
+#pragma unroll
+        for (int i = 0; i < X::TM; ++i) fa[i] = *reinterpret_cast<const u32x4_t *>(at + a_row + i * 16 * kRowBytes);
+#pragma unroll
+        for (int j = 0; j < X::TN; ++j) fb[j] = *reinterpret_cast<const u32x4_t *>(at + b_row + j * 16 * kRowBytes);
+    };
+    auto multiply = [&](const u32x4_t (&fa)[X::TM], const u32x4_t (&fb)[X::TN]) {
+#pragma unroll
+        for (int i = 0; i < X::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < X::TN; ++j) mma16(acc[i][j], fa[i], fb[j], T());
+    };
     copy(0);
-    for (int s = 0; s < steps; ++s) {
+    if constexpr (X::AHEAD) {
+        // The fragments of a half step are read while the matrix cores work on the half before it, across the stages' border too:
+        //     read second half of s | first half's products | stage s + 1 has landed, s is read out | copy s + 2 into its place,
+        //     read first half of s + 1 | second half's products
+        u32x4_t a0[X::TM], b0[X::TN], a1[X::TM], b1[X::TN];
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                         // stage s has landed for everybody, and nobody reads the other one any more
-        if (s + 1 < steps) copy((s + 1) & 1);
-        const char *stage = lds + (s & 1) * X::STAGE;
+        __syncthreads();
+        if (steps > 1) copy(1);
+        read(0, swz0, a0, b0);
+        for (int s = 0; s < steps; ++s) {
+            const int stage = s & 1;
+            read(stage, swz1, a1, b1);
+            multiply(a0, b0);
+            if (s + 1 < steps) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();      // (waits for this wave's reads too: the stage may be overwritten)
+                if (s + 2 < steps) copy(stage);
+                read(stage ^ 1, swz0, a0, b0);
+            }
+            multiply(a1, b1);
+        }
+    } else {
+        for (int s = 0; s < steps; ++s) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();                         // stage s has landed for everybody, and nobody reads the other one any more
+            if (s + 1 < steps) copy((s + 1) & 1);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int swz = half ? swz1 : swz0;
-            u32x4_t fa[X::TM], fb[X::TN];
-#pragma unroll
-            for (int i = 0; i < X::TM; ++i) fa[i] = *reinterpret_cast<const u32x4_t *>(stage + a_row + i * 16 * kRowBytes + swz);
-#pragma unroll
-            for (int j = 0; j < X::TN; ++j) fb[j] = *reinterpret_cast<const u32x4_t *>(stage + b_row + j * 16 * kRowBytes + swz);
-#pragma unroll
-            for (int i = 0; i < X::TM; ++i)
-#pragma unroll
-                for (int j = 0; j < X::TN; ++j) mma16(acc[i][j], fa[i], fb[j], T());
+            for (int half = 0; half < 2; ++half) {
+                u32x4_t fa[X::TM], fb[X::TN];
+                read(s & 1, half ? swz1 : swz0, fa, fb);
+                multiply(fa, fb);
+            }
         }
     }
 }
@@ -369,7 +399,20 @@ struct CePlan {
     size_t total;
 };
 
-using TileBig = Tile<128, 128, 2, 2>;
+// 128 x 128: 64 KiB of stages, two workgroups per CU.  256 x 256: 128 KiB, one workgroup of 8 waves (16 bits only: the float32
+// transpose of such a tile does not fit LDS) -- half the LDS and L2 traffic per operation.
+using Tile128 = Tile<128, 128, 2, 2, false>;
+using Tile256 = Tile<256, 256, 2, 4, true>;
+
+// Whether the [m][n] tiles of a 16-bit product are 256 x 256.  Both sizes' time goes as the area they cover in whole rounds of the
+// chip (256 CUs; two of the small workgroups per CU), and the larger one is 1.2 times as fast per area: 8192 x 128000 x 2048
+// forward 3.52 ms against 4.26, 4096 x 32000 x 1024 0.256 against 0.287; but 777 x 49999 x 768, 24 % of whose 256-row tiles is
+// empty, 0.115 against 0.097.
+static bool ce_big(int64_t m, int64_t n, int es) {
+    if (es != 2) return false;
+    const int64_t big = ceil_div(ceil_div(m, 256) * ceil_div(n, 256), 256) * 256, small = ceil_div(ceil_div(m, 128) * ceil_div(n, 128), 512) * 512;
+    return big * 4 * 5 < small * 6;
+}
 
 static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, bool need_x, bool need_w) {
     CePlan p = {};
@@ -398,7 +441,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
         split(V, n, p.per_w, p.parts_w);
     }
     if (!backward) {
-        p.tiles = p.narrow ? p.parts_x : ceil_div(V, TileBig::BM);
+        p.tiles = p.narrow ? p.parts_x : ceil_div(V, ce_big(V, n, p.es) ? 256 : 128);
         p.part = take((size_t)p.tiles * n * sizeof(float2));
         p.own = take((size_t)n * 4);
         p.rows = take((size_t)n * 4);
@@ -422,9 +465,9 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
         if (need_x) {
             p.dl = take((size_t)n * p.piece * p.es);
             p.wt = take((size_t)C * p.piece * p.es);
-            const int64_t tiles = ceil_div(C, TileBig::BM) * ceil_div(n, TileBig::BN), steps = round_up(V < p.piece ? V : p.piece, step) / step;
+            const int64_t side = ce_big(C, n, p.es) ? 256 : 128, tiles = ceil_div(C, side) * ceil_div(n, side), steps = round_up(V < p.piece ? V : p.piece, step) / step;
             // parts of k: enough workgroups for the chip's 256 CUs twice over, at least 8 steps each
-            int64_t parts = ceil_div(512, tiles > 0 ? tiles : 1);
+            int64_t parts = side == 256 ? 1 : ceil_div(512, tiles > 0 ? tiles : 1);
             if (parts > steps / 8) parts = steps / 8;
             if (parts < 1) parts = 1;
             p.parts = (int)ceil_div(steps, ceil_div(steps, parts));      // (as many as get work; a smaller last piece then has no more)
@@ -472,16 +515,6 @@ static int ce_check(const char *who, const void *x, const void *w, int dtype, co
     return MVS_OK;
 }
 
-// LDS of a kernel: the two stages, or what its epilogue lays there
-template <typename X>
-static unsigned ce_lds(size_t epilogue) { return (unsigned)(epilogue > 2 * (size_t)X::STAGE ? epilogue : 2 * (size_t)X::STAGE); }
-
-// (more than 64 KiB of dynamic LDS has to be asked for, once per kernel and device)
-template <typename F>
-static bool ce_allow_lds(F kernel, unsigned bytes) {
-    return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
-}
-
 template <typename T>
 static void ce_pad(const void *in, int64_t R, int C, char *out, int Cp, hipStream_t st) {
     if (R > 0)
@@ -489,7 +522,26 @@ static void ce_pad(const void *in, int64_t R, int C, char *out, int Cp, hipStrea
                            reinterpret_cast<T *>(out), Cp);
 }
 
-template <typename T, typename X>
+// a kernel on the tiles of its [m][n]: f(X()) sets the grid and launches
+template <typename T, typename F>
+static void ce_tiles(int64_t m, int64_t n, F f) {
+    if constexpr (sizeof(T) == 2) {
+        if (ce_big(m, n, 2)) { f(Tile256()); return; }
+    }
+    f(Tile128());
+}
+
+// two stages of LDS, or what the epilogue lays there if that is more (an error stands for check_launch)
+template <typename X, typename F, typename A>
+static void ce_launch(F kernel, const A &a, unsigned parts, size_t epilogue, hipStream_t st) {
+    const size_t stages = 2 * (size_t)X::STAGE;
+    const unsigned bytes = (unsigned)(epilogue > stages ? epilogue : stages);
+    // (more than 64 KiB of dynamic LDS has to be asked for)
+    if (bytes > 65536 && hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess) return;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tiles_m * a.tiles_n), parts), dim3(X::THREADS), bytes, st, a);
+}
+
+template <typename T>
 static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, char *ws, hipStream_t st) {
     CeArgs a = {};
     a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
@@ -502,14 +554,15 @@ static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const in
     }
     a.steps = p.Cp * p.es / kRowBytes;
     a.n = n; a.v_total = V; a.v_count = V;
-    a.tiles_m = p.tiles; a.tiles_n = ceil_div(n, X::BN);
     a.scale2 = scale * kLog2e;
     a.target = target;
     a.part = reinterpret_cast<float2 *>(ws + p.part);
     a.own = reinterpret_cast<float *>(ws + p.own);
-    const unsigned bytes = ce_lds<X>((size_t)X::WAVES_M * X::BN * sizeof(float2));
-    if (!ce_allow_lds(ce_stats_kernel<T, X>, bytes)) return check_launch("mvs_linear_ce_fwd");
-    hipLaunchKernelGGL((ce_stats_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), bytes, st, a);
+    ce_tiles<T>(V, n, [&](auto x) {
+        using X = decltype(x);
+        a.tiles_m = ceil_div(V, X::BM); a.tiles_n = ceil_div(n, X::BN);
+        ce_launch<X>(ce_stats_kernel<T, X>, a, 1, (size_t)X::WAVES_M * X::BN * sizeof(float2), st);
+    });
     return check_launch("mvs_linear_ce_fwd");
 }
 
@@ -526,7 +579,7 @@ static int ce_forward(int dtype, const void *x, const void *w, const int64_t *ta
             a.part = part; a.own = own;
             rc = ce_narrow_forward(dtype, a, st);
         } else {
-            MVS_DTYPE_DISPATCH(dtype, T, rc = (ce_wide_stats<T, TileBig>(p, x, w, target, n, V, C, scale, ws, st)));
+            MVS_DTYPE_DISPATCH(dtype, T, rc = (ce_wide_stats<T>(p, x, w, target, n, V, C, scale, ws, st)));
         }
         if (rc != MVS_OK) return rc;
         hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(256), 0, st, part, p.tiles, n, V, target, ignore, own, lse, rows);
@@ -535,7 +588,7 @@ static int ce_forward(int dtype, const void *x, const void *w, const int64_t *ta
     return check_launch("mvs_linear_ce_fwd");
 }
 
-template <typename T, typename X>
+template <typename T>
 static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const int64_t *target, const float *lse, const float *kept, const float *grad_loss,
                        int64_t n, int64_t V, int C, float scale, int64_t ignore, int reduction, void *grad_x, void *grad_w, char *ws, hipStream_t st) {
     const int step = kRowBytes / p.es;
@@ -554,24 +607,31 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
     const char *w_rows = a.w.p;
     a.steps = p.Cp * p.es / kRowBytes;
     a.n = n; a.v_total = V; a.ignore = ignore;
-    a.tiles_n = ceil_div(n, X::BN);
     a.scale2 = scale * kLog2e;
     a.target = target; a.lse2 = lse; a.ratio = factors + n;
     a.dl = grad_x ? ws + p.dl : nullptr;
     a.dlt = grad_w ? ws + p.dlt : nullptr;
     a.ld_dlt = p.np;
-    const unsigned grad_lds = ce_lds<X>((size_t)X::BM * (X::BN * sizeof(T) + 16)), product_lds = ce_lds<X>(0);
-    if (!ce_allow_lds(ce_grad_kernel<T, X>, grad_lds) || !ce_allow_lds(ce_product_kernel<T, X>, product_lds)) return check_launch("mvs_linear_ce_bwd");
     if (grad_w)      // x^T once; ignored rows as zeros, whatever they hold
         hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(p.np, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
                            reinterpret_cast<const T *>(a.x.p), n, C, (int64_t)p.Cp, target, ignore, reinterpret_cast<T *>(ws + p.xt), p.np);
+    auto product = [&](CeProduct &d) {
+        ce_tiles<T>(d.m, d.n, [&](auto x) {
+            using X = decltype(x);
+            d.tiles_m = ceil_div(d.m, X::BM); d.tiles_n = ceil_div(d.n, X::BN);
+            ce_launch<X>(ce_product_kernel<T, X>, d, (unsigned)ceil_div(d.steps, d.steps_per_part), 0, st);
+        });
+    };
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
         const int64_t count = V - v0 < p.piece ? V - v0 : p.piece, k = round_up(count, step);
         a.w.p = w_rows + v0 * p.Cp * p.es;
         a.w.rows = count;
         a.v0 = v0; a.v_count = count; a.ld_dl = k;
-        a.tiles_m = ceil_div(count, X::BM);
-        hipLaunchKernelGGL((ce_grad_kernel<T, X>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(X::THREADS), grad_lds, st, a);
+        ce_tiles<T>(count, n, [&](auto x) {
+            using X = decltype(x);
+            a.tiles_m = ceil_div(count, X::BM); a.tiles_n = ceil_div(n, X::BN);
+            ce_launch<X>(ce_grad_kernel<T, X>, a, 1, (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
+        });
         if (grad_x) {
             hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(k, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
                                reinterpret_cast<const T *>(a.w.p), count, C, (int64_t)p.Cp, (const int64_t *)nullptr, ignore,
@@ -581,12 +641,11 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             d.b = Operand{ws + p.dl, k * p.es, n};
             d.steps = (int)(k / step);
             d.steps_per_part = (int)ceil_div(d.steps, p.parts);
-            d.m = C; d.n = n; d.tiles_m = ceil_div(C, X::BM); d.tiles_n = ceil_div(n, X::BN);
+            d.m = C; d.n = n;
             d.sums = reinterpret_cast<float *>(ws + p.sums); d.ld_sums = p.c4;
             d.add = v0 > 0;
             // (a smaller last piece may have fewer parts of k: the sums of the others stay as they are)
-            hipLaunchKernelGGL((ce_product_kernel<T, X>), dim3((unsigned)(d.tiles_m * d.tiles_n), (unsigned)ceil_div(d.steps, d.steps_per_part)),
-                               dim3(X::THREADS), product_lds, st, d);
+            product(d);
         }
         if (grad_w) {
             CeProduct d = {};
@@ -594,10 +653,10 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             d.b = Operand{ws + p.dlt, p.np * p.es, count};
             d.steps = (int)(p.np / step);
             d.steps_per_part = d.steps;
-            d.m = C; d.n = count; d.tiles_m = ceil_div(C, X::BM); d.tiles_n = ceil_div(count, X::BN);
+            d.m = C; d.n = count;
             d.out = static_cast<T *>(grad_w) + v0 * C;
             d.top = factors + 2 * n; d.factor = factor;
-            hipLaunchKernelGGL((ce_product_kernel<T, X>), dim3((unsigned)(d.tiles_m * d.tiles_n)), dim3(X::THREADS), product_lds, st, d);
+            product(d);
         }
     }
     if (grad_x)
@@ -662,7 +721,7 @@ extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, c
         return ce_narrow_backward(dtype, a, as_stream(stream));
     }
     MVS_DTYPE_DISPATCH(dtype, T, {
-        return (ce_wide_backward<T, TileBig>(p, x, weight, target, lse, kept, grad_loss, n, V, C, scale, ignore_index, reduction, grad_x, grad_weight, ws,
+        return (ce_wide_backward<T>(p, x, weight, target, lse, kept, grad_loss, n, V, C, scale, ignore_index, reduction, grad_x, grad_weight, ws,
                                              as_stream(stream)));
     });
 }
