@@ -40,47 +40,74 @@ __device__ __forceinline__ bool ce_kept(int64_t target, int64_t ignore) { return
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
-// By one workgroup: a row's factor g_n (0 for an ignored one), and its ratio to the largest magnitude; factors[2 n] = that magnitude.
-// `tops`: a word of LDS per wave.
-__device__ __forceinline__ void ce_factors(const float *__restrict__ grad_loss, const float *__restrict__ kept, const int64_t *__restrict__ target, int64_t n,
-                                           int64_t ignore, int reduction, float *__restrict__ factors, float *tops) {
-    float common = reduction == 0 ? 0.0f : grad_loss[0];
-    if (reduction == 1) common = common / *kept;
-    auto factor = [&](int64_t i) { return !ce_kept(target[i], ignore) ? 0.0f : reduction == 0 ? grad_loss[i] : common; };
+// The rows that are kept, moved together (more than kTogether of them: fewer fill one tile anyway): kept row i is row map[i] of the
+// caller's, row r of the caller's is kept row place[r], -1 for an ignored one.  Everything between works on the kept rows: tiles and
+// steps beyond *count are not begun, and what an ignored row holds is never read.  map == NULL: all rows as they are, in which case
+// the kernels look at the targets.
+constexpr int kTogether = 128;
+struct CeRows {
+    const int *map, *place, *count;
+    const int64_t *target;            // of the kept rows
+    int64_t n;                        // rows of the caller's
+    int64_t ignore;
+};
+__device__ __forceinline__ int64_t ce_count(const CeRows &r) { return r.count ? *r.count : r.n; }
+__device__ __forceinline__ int64_t ce_original(const CeRows &r, int64_t i) { return r.map ? r.map[i] : i; }
+
+// g of the rows `first`, `first` + `step`, ... and their ratios to the largest magnitude: factors[i], factors[n + i], factors[2 n].
+// With one factor for all rows the ratio is 1; else one workgroup looks for the largest first.  `tops`: a word of LDS per wave.
+__device__ __forceinline__ void ce_factors(const CeRows &rows, const float *__restrict__ grad_loss, const float *__restrict__ kept, int reduction,
+                                           float *__restrict__ factors, int64_t first, int64_t step, float *tops) {
+    const int64_t count = ce_count(rows);
     float top = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) top = fmaxf(top, __builtin_fabsf(factor(i)));
+    if (reduction != 0) {
+        const float common = reduction == 2 ? grad_loss[0] : *kept > 0.0f ? grad_loss[0] / *kept : 0.0f;
+        for (int64_t i = first; i < count; i += step) {
+            const bool here = ce_kept(rows.target[i], rows.ignore) && common != 0.0f;
+            factors[i] = here ? common : 0.0f;
+            factors[rows.n + i] = here ? common / __builtin_fabsf(common) : 0.0f;
+        }
+        top = __builtin_fabsf(common);
+    } else {
+        auto factor = [&](int64_t i) { return ce_kept(rows.target[i], rows.ignore) ? grad_loss[ce_original(rows, i)] : 0.0f; };
+        for (int64_t i = first; i < count; i += step) top = fmaxf(top, __builtin_fabsf(factor(i)));
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (int w = 0; w < (int)blockDim.x / 64; ++w) top = fmaxf(top, tops[w]);
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const float g = factor(i);
-        factors[i] = g;
-        factors[n + i] = g == 0.0f ? 0.0f : g / top;
+        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        __syncthreads();
+        for (int w = 0; w < (int)blockDim.x / 64; ++w) top = fmaxf(top, tops[w]);
+        for (int64_t i = first; i < count; i += step) {
+            const float g = factor(i);
+            factors[i] = g;
+            factors[rows.n + i] = g == 0.0f ? 0.0f : g / top;
+        }
     }
-    if (threadIdx.x == 0) factors[2 * n] = top;
+    if (first == 0) factors[2 * rows.n] = top;
 }
 
-// out[row][c] = f * factor * the parts' sums, in order; f = g[row] (dx: 0 for an ignored row, whose sums may be anything) or g[0] (dW)
+// out[row][c] = f * factor * the parts' sums, in order.  PER_ROW (dx): f = g[i] of kept row i = place[row]; rows that are ignored
+// or have f = 0 are zeros, whatever their sums are.  Else (dW): f = g[0].
 template <typename T, bool PER_ROW>
-__device__ __forceinline__ void ce_finish(const float *__restrict__ sums, int parts, int64_t rows, int C, int64_t ld, const float *__restrict__ g, float factor,
-                                          T *__restrict__ out, int64_t block) {
-    const int64_t quads = ld >> 2, i = block * 256 + threadIdx.x, row = i / quads, c = (i - row * quads) * 4;
+__device__ __forceinline__ void ce_finish(const float *__restrict__ sums, int parts, int64_t rows, const int *__restrict__ place, int C, int64_t ld,
+                                          const float *__restrict__ g, float factor, T *__restrict__ out, int64_t block) {
+    const int64_t quads = ld >> 2, i = block * 256 + threadIdx.x, row = i / quads, quad = i - row * quads, c = quad * 4;
     if (row >= rows) return;
-    const f32x4_t *from = reinterpret_cast<const f32x4_t *>(sums) + i;
-    const int64_t step = rows * quads;
-    f32x4_t s = from[0];
-    int p = 1;
-    for (; p + 8 <= parts; p += 8) {
-        f32x4_t v[8];
+    const int64_t at = PER_ROW && place ? place[row] : row, step = rows * quads;
+    const float f = !PER_ROW ? g[0] : at >= 0 ? g[at] : 0.0f;
+    f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!PER_ROW || f != 0.0f) {
+        const f32x4_t *from = reinterpret_cast<const f32x4_t *>(sums) + at * quads + quad;
+        s = from[0];
+        int p = 1;
+        for (; p + 8 <= parts; p += 8) {
+            f32x4_t v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = from[(p + j) * step];
+            for (int j = 0; j < 8; ++j) v[j] = from[(p + j) * step];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[j];
+            for (int j = 0; j < 8; ++j) s += v[j];
+        }
+        for (; p < parts; ++p) s += from[p * step];
     }
-    for (; p < parts; ++p) s += from[p * step];
-    const float f = PER_ROW ? g[row] : g[0];
     Pack<T, 4> o;
 #pragma unroll
     for (int r = 0; r < 4; ++r) o.v[r] = from_float<T>(PER_ROW && f == 0.0f ? 0.0f : s[r] * f * factor);
@@ -100,18 +127,18 @@ inline bool ce_narrow(int C, int dtype) { return C <= (dtype == MVS_DTYPE_F32 ? 
 struct NarrowOperand {
     const void *source;               // [count][C] as the caller has it
     char *rows;                       // [count][planes][Cp] 16-bit pieces (one plane and C == Cp: `source`)
-    char *trans;                      // [C][planes][Mp], Mp = count rounded up to 64, in the order the lanes hold (NULL: not needed)
-    int64_t count;
+    char *trans;                      // [C][planes][pitch], pitch = count rounded up to 64, in the order the lanes hold (NULL: not needed)
+    int64_t count;                    // (x: of the caller's; the kernels take the kept ones')
+    int64_t pitch;
     bool write_rows;
 };
 struct NarrowArgs {
     NarrowOperand x, w;
     int C, Cp, planes;
-    int64_t per_x, per_w;             // table rows per part (the rows of x are fixed), rows of x per part (the table's are)
-    int parts_x, parts_w;
+    int64_t per_x;                    // table rows per part where the rows of x are fixed
+    int parts_x, parts_w;             // parts of the table; of the kept rows of x where the table's are fixed
     float scale2;                     // scale * log2 e
-    const int64_t *target;
-    int64_t ignore;
+    CeRows kept_rows;
     // forward
     float2 *part;                     // [part][n]
     float *own;

@@ -43,6 +43,7 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
     const int wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
     const unsigned lds_base = (unsigned)(uintptr_t)lds;
     // copy c moves the tile rows 8 c .. 8 c + 7 (A's, then B's): lane i = row 8 c + i / 8, LDS chunk i % 8
+    if (steps <= 0) return;
     const int r8 = lane >> 3, chunk = (lane & 7) ^ r8;
     const char *from[X::PER_WAVE];
 #pragma unroll
@@ -118,21 +119,24 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
 
 // Which tile a workgroup owns: the XCDs take consecutive runs of the list (each has its own L2), and the list walks 8 m-tiles wide
 // columns of the grid, so that the tiles an XCD works on share rows of both operands.
-__device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn) {
+// False for a workgroup that none is left for (fewer tiles than the host could tell).
+__device__ __forceinline__ bool tile_of(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn) {
+    if (id >= tiles_m * tiles_n) return false;
     const int64_t total = tiles_m * tiles_n, per = total >> 3, extra = total & 7, xcd = id & 7;
     const int64_t at = xcd * per + (xcd < extra ? xcd : extra) + (id >> 3);
     const int64_t band = at / (8 * tiles_n), wide = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8, in = at - band * 8 * tiles_n;
     tm = band * 8 + in % wide;
     tn = in / wide;
+    return true;
 }
 
 struct CeArgs {
     Operand w, x;                       // table piece and rows, padded along k
     int steps;                          // 128-byte steps of k
-    int64_t n, v_total, v0, v_count;    // rows; table; this piece
-    int64_t tiles_m, tiles_n, ignore;
+    int64_t v_total, v0, v_count;       // table; this piece
+    int64_t tiles_m, tiles_n;           // (of all rows; the kernels take the kept ones')
     float scale2;                       // scale * log2 e
-    const int64_t *target;
+    CeRows rows;
     // forward
     float2 *part;                       // [tile_m][n]: max, sum
     float *own;                         // [n]: the target's logit (base 2)
@@ -145,18 +149,21 @@ struct CeArgs {
 template <typename T, typename X>
 __global__ __launch_bounds__(X::THREADS) void ce_stats_kernel(CeArgs a) {
     extern __shared__ __align__(1024) char lds[];
+    const int64_t rows = ce_count(a.rows);
     int64_t tm, tn;
-    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    if (!tile_of(blockIdx.x, a.tiles_m, (rows + X::BN - 1) / X::BN, tm, tn)) return;
+    Operand x = a.x;
+    x.rows = rows;
     const int64_t m0 = tm * X::BM, n0 = tn * X::BN;
     f32x4_t acc[X::TM][X::TN] = {};
-    tile_product<T, X>(a.w, a.x, m0, n0, 0, a.steps, lds, acc);
+    tile_product<T, X>(a.w, x, m0, n0, 0, a.steps, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
     const int64_t v_lane = m0 + wm * (X::BM / X::WAVES_M) + (lane >> 4) * 4;
     float2 stat[X::TN];
 #pragma unroll
     for (int j = 0; j < X::TN; ++j) {
         const int64_t n = n0 + wn * (X::BN / X::WAVES_N) + j * 16 + (lane & 15);
-        const int64_t t = n < a.n ? a.target[n] : -1;
+        const int64_t t = n < rows ? a.rows.target[n] : -1;
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < X::TM; ++i)
@@ -188,7 +195,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_stats_kernel(CeArgs a) {
         for (int j = 0; j < X::TN; ++j) s[wm * X::BN + wn * (X::BN / X::WAVES_N) + j * 16 + lane] = stat[j];
     __syncthreads();
     for (int c = threadIdx.x; c < X::BN; c += X::THREADS) {
-        if (n0 + c >= a.n) continue;
+        if (n0 + c >= rows) continue;
         float2 r = s[c];
 #pragma unroll
         for (int w = 1; w < X::WAVES_M; ++w) {
@@ -196,14 +203,14 @@ __global__ __launch_bounds__(X::THREADS) void ce_stats_kernel(CeArgs a) {
             const float top = fmaxf(r.x, o.x), base = top == -INFINITY ? 0.0f : top;
             r = make_float2(top, r.y * __builtin_amdgcn_exp2f(r.x - base) + o.y * __builtin_amdgcn_exp2f(o.x - base));
         }
-        a.part[tm * a.n + n0 + c] = r;
+        a.part[tm * a.rows.n + n0 + c] = r;
     }
 }
 
 // Joins a row's tiles: 16 rows x 16 tiles at a time per workgroup.
-__global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__ part, int64_t tiles, int64_t n, int64_t v_total,
-                                                      const int64_t *__restrict__ target, int64_t ignore, const float *__restrict__ own,
-                                                      float *__restrict__ lse2, float *__restrict__ loss) {
+__global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__ part, int64_t tiles, int64_t v_total, CeRows rows,
+                                                      const float *__restrict__ own, float *__restrict__ lse2, float *__restrict__ loss) {
+    const int64_t n = ce_count(rows);
     __shared__ float2 s[256];
     const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
     float2 r = make_float2(-INFINITY, 0.0f);
@@ -212,16 +219,16 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__
         return make_float2(top, p.y * __builtin_amdgcn_exp2f(p.x - base) + q.y * __builtin_amdgcn_exp2f(q.x - base));
     };
     if (row < n)
-        for (int64_t t = threadIdx.x >> 4; t < tiles; t += 16) r = join(r, part[t * n + row]);
+        for (int64_t t = threadIdx.x >> 4; t < tiles; t += 16) r = join(r, part[t * rows.n + row]);
     s[threadIdx.x] = r;
     __syncthreads();
     if (threadIdx.x < 16 && row < n) {
         for (int t = 1; t < 16; ++t) r = join(r, s[t * 16 + threadIdx.x]);
-        const int64_t t = target[row];
-        const bool kept = ce_kept(t, ignore), named = t >= 0 && t < v_total;
+        const int64_t t = rows.target[row];
+        const bool kept = ce_kept(t, rows.ignore), named = t >= 0 && t < v_total;
         const float l = r.x + __builtin_amdgcn_logf(r.y);      // (base 2)
         lse2[row] = kept && !named ? __uint_as_float(0x7fc00000u) : l;
-        loss[row] = !kept ? 0.0f : !named ? __uint_as_float(0x7fc00000u) : (l - own[row]) * kLn2;
+        loss[ce_original(rows, row)] = !kept ? 0.0f : !named ? __uint_as_float(0x7fc00000u) : (l - own[row]) * kLn2;
     }
 }
 
@@ -247,20 +254,22 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(const float *__restrict_
 }
 
 // ---- backward
-__global__ __launch_bounds__(1024) void ce_factors_kernel(const float *grad_loss, const float *kept, const int64_t *target, int64_t n, int64_t ignore,
-                                                          int reduction, float *factors) {
+__global__ __launch_bounds__(1024) void ce_factors_kernel(CeRows rows, const float *grad_loss, const float *kept, int reduction, float *factors) {
     __shared__ float tops[16];
-    ce_factors(grad_loss, kept, target, n, ignore, reduction, factors, tops);
+    ce_factors(rows, grad_loss, kept, reduction, factors, (int64_t)blockIdx.x * 1024 + threadIdx.x, (int64_t)gridDim.x * 1024, tops);
 }
 
 template <typename T, typename X>
 __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
     extern __shared__ __align__(1024) char lds[];
+    const int64_t rows = ce_count(a.rows);
     int64_t tm, tn;
-    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    if (!tile_of(blockIdx.x, a.tiles_m, (rows + X::BN - 1) / X::BN, tm, tn)) return;
+    Operand x = a.x;
+    x.rows = rows;
     const int64_t m0 = tm * X::BM, n0 = tn * X::BN;      // (m0 within the piece)
     f32x4_t acc[X::TM][X::TN] = {};
-    tile_product<T, X>(a.w, a.x, m0, n0, 0, a.steps, lds, acc);
+    tile_product<T, X>(a.w, x, m0, n0, 0, a.steps, lds, acc);
     constexpr float unit = GradUnit<T>::value;
     constexpr int PITCH = X::BN * (int)sizeof(T) + 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
@@ -270,8 +279,8 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
     for (int j = 0; j < X::TN; ++j) {
         const int nl = wn * (X::BN / X::WAVES_N) + j * 16 + (lane & 15);
         const int64_t n = n0 + nl;
-        const int64_t t = n < a.n ? a.target[n] : a.ignore;
-        const bool kept = n < a.n && ce_kept(t, a.ignore);
+        const int64_t t = n < rows ? a.rows.target[n] : 0;
+        const bool kept = n < rows && ce_kept(t, a.rows.ignore);
         const float lse2 = kept ? a.lse2[n] : 0.0f, ratio = kept ? a.ratio[n] : 0.0f;
 #pragma unroll
         for (int i = 0; i < X::TM; ++i) {
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
                 if (a.dlt) *reinterpret_cast<T *>(lds + ml * PITCH + nl * (int)sizeof(T)) = from_float<T>(real ? d * ratio : 0.0f);
             }
             const int64_t m = m0 + m_lane + i * 16;
-            if (a.dl && n < a.n && m < a.ld_dl) *reinterpret_cast<Pack<T, 4> *>(static_cast<T *>(a.dl) + n * a.ld_dl + m) = out;
+            if (a.dl && n < rows && m < a.ld_dl) *reinterpret_cast<Pack<T, 4> *>(static_cast<T *>(a.dl) + n * a.ld_dl + m) = out;
         }
     }
     if (!a.dlt) return;
@@ -306,18 +315,27 @@ struct CeProduct {
     int steps, steps_per_part;
     int64_t m, n, tiles_m, tiles_n;
     float *sums;            // float32 sums [part][n][ld_sums] (added to if `add`), or NULL: `out` is written
-    int64_t ld_sums;
+    int64_t ld_sums, sum_rows;
     int add;
     void *out;              // [n][m] of T
     const float *top;       // `out` = sum * *top * factor
     float factor;
+    const int *count;       // kept rows: n (sums) or the extent of k (out) is at most that; NULL: as given
 };
 
 template <typename T, typename X>
 __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
     extern __shared__ __align__(1024) char lds[];
+    if (a.count) {
+        if (a.sums) {
+            a.n = a.b.rows = *a.count;
+            a.tiles_n = (a.n + X::BN - 1) / X::BN;
+        } else {
+            a.steps = a.steps_per_part = (int)((*a.count * (int64_t)sizeof(T) + kRowBytes - 1) / kRowBytes);
+        }
+    }
     int64_t tm, tn;
-    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    if (!tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn)) return;
     const int64_t m0 = tm * X::BM, n0 = tn * X::BN;
     const int first = blockIdx.y * a.steps_per_part, steps = min(a.steps_per_part, a.steps - first);
     f32x4_t acc[X::TM][X::TN] = {};
@@ -333,7 +351,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
             const int64_t m = m0 + wm * (X::BM / X::WAVES_M) + i * 16 + (lane >> 4) * 4;
             if (m >= a.m) continue;
             if (a.sums) {      // (rows of ld_sums floats, a multiple of 4: the padding behind m may be written)
-                f32x4_t *to = reinterpret_cast<f32x4_t *>(a.sums + ((int64_t)blockIdx.y * a.n + n) * a.ld_sums + m);
+                f32x4_t *to = reinterpret_cast<f32x4_t *>(a.sums + (blockIdx.y * a.sum_rows + n) * a.ld_sums + m);
                 *to = a.add ? *to + acc[i][j] : acc[i][j];
             } else {
                 T *to = static_cast<T *>(a.out) + n * a.m + m;
@@ -349,35 +367,95 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void ce_finish_kernel(const float *sums, int parts, int64_t rows, int C, int64_t ld, const float *g, float factor, T *out) {
-    ce_finish<T, true>(sums, parts, rows, C, ld, g, factor, out, blockIdx.x);
+__global__ __launch_bounds__(256) void ce_finish_kernel(const float *sums, int parts, CeRows rows, int C, int64_t ld, const float *g, float factor, T *out) {
+    ce_finish<T, true>(sums, parts, rows.n, rows.place, C, ld, g, factor, out, blockIdx.x);
 }
 
-// out[c][r] = in[r][c] for c < C, zero for r in [R, ld_out) and where the row's target is `ignore` (targets == NULL: nowhere).
-template <typename T>
-__global__ __launch_bounds__(256) void ce_transpose_kernel(const T *__restrict__ in, int64_t R, int C, int64_t ld_in, const int64_t *__restrict__ target,
-                                                           int64_t ignore, T *__restrict__ out, int64_t ld_out) {
-    __shared__ T tile[64][64 + 4 / sizeof(T)];
-    const int64_t r0 = (int64_t)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    for (int r = ty; r < 64; r += 4) {
+// Moves the kept rows together (CeRows), by one workgroup: 16 waves count their sixteenth of the targets, then number its kept rows.
+// `loss` (forward): the ignored rows' losses, 0.
+__global__ __launch_bounds__(1024) void ce_together_kernel(const int64_t *__restrict__ target, int64_t n, int64_t ignore, int *__restrict__ map, int *__restrict__ place,
+                                                           int64_t *__restrict__ kept_target, int *__restrict__ count, float *__restrict__ loss) {
+    __shared__ int counts[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t per = (n + 1023) / 1024 * 64, begin = wave * per, end = min(n, begin + per);
+    int mine = 0;
+#pragma unroll 8
+    for (int64_t i = begin + lane; i < end; i += 64) mine += ce_kept(target[i], ignore) ? 1 : 0;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
+    if (lane == 0) counts[wave] = mine;
+    __syncthreads();
+    int at = 0, all = 0;
+    for (int w = 0; w < 16; ++w) { at += w < wave ? counts[w] : 0; all += counts[w]; }
+    if (threadIdx.x == 0) *count = all;
+    for (int64_t i0 = begin; i0 < end; i0 += 256) {
+        int64_t t[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) t[u] = i0 + u * 64 + lane < end ? target[i0 + u * 64 + lane] : ignore;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = i0 + u * 64 + lane;
+            const bool kept = ce_kept(t[u], ignore);
+            const unsigned long long all_kept = __ballot(kept);
+            if (kept) {
+                const int to = at + __popcll(all_kept & ((1ull << lane) - 1));
+                map[to] = (int)i;
+                place[i] = to;
+                kept_target[to] = t[u];
+            } else if (i < end) {
+                place[i] = -1;
+                if (loss) loss[i] = 0.0f;
+            }
+            at += __popcll(all_kept);
+        }
+    }
+}
+
+// out[i][0 .. Cp) = in[map[i]][0 .. C), zeros, for the kept rows (all `n` where there is no map); VEC elements per access
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void ce_rows_kernel(const T *__restrict__ in, CeRows rows, int C, T *__restrict__ out, int Cp) {
+    const int vecs = Cp / VEC;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / vecs;
+    if (row >= ce_count(rows)) return;
+    const int c = (int)(i - row * vecs) * VEC;
+    Pack<T, VEC> v;
+    if (c < C) v = *reinterpret_cast<const Pack<T, VEC> *>(in + ce_original(rows, row) * C + c);
+    else
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v.v[j] = from_float<T>(0.0f);
+    reinterpret_cast<Pack<T, VEC> *>(out)[i] = v;
+}
+
+// out[c][r] = in[r][c] for c < C and r < rows, zero for the other r < ld_out and for ignored rows.  64 x 64 tiles through LDS, moved
+// VEC elements at a time on both sides (VEC > 1: ld_in, and C or its padding, reach whole vectors).
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void ce_transpose_kernel(const T *__restrict__ in, CeRows rows, bool look, int C, int64_t ld_in, T *__restrict__ out,
+                                                           int64_t ld_out) {
+    constexpr int PITCH = 64 + 4 / (int)sizeof(T), PER = 64 / VEC;
+    __shared__ T tile[64][PITCH];
+    const int64_t r0 = (int64_t)blockIdx.x * 64, R = ce_count(rows);
+    if (r0 >= R + 63) return;      // (nobody reads that far)
+    const int c0 = blockIdx.y * 64;
+    for (int i = threadIdx.x; i < 64 * PER; i += 256) {
+        const int r = i / PER, c = i % PER * VEC;
         const int64_t row = r0 + r;
-        const bool here = row < R && c0 + tx < C && (!target || ce_kept(target[row], ignore));
-        tile[r][tx] = here ? in[row * ld_in + c0 + tx] : from_float<T>(0.0f);
+        Pack<T, VEC> v;
+        if (row < R && c0 + c < ld_in && (!look || ce_kept(rows.target[row], rows.ignore))) v = *reinterpret_cast<const Pack<T, VEC> *>(in + row * ld_in + c0 + c);
+        else
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v.v[j] = from_float<T>(0.0f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) tile[r][c + j] = v.v[j];
     }
     __syncthreads();
-    for (int c = ty; c < 64; c += 4)
-        if (c0 + c < C && r0 + tx < ld_out) out[(int64_t)(c0 + c) * ld_out + r0 + tx] = tile[tx][c];
-}
-
-// out[r][0 .. Cp) = in[r][0 .. C), zeros
-template <typename T>
-__global__ __launch_bounds__(256) void ce_pad_kernel(const T *__restrict__ in, int64_t R, int C, T *__restrict__ out, int Cp) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= R * Cp) return;
-    const int64_t r = i / Cp;
-    const int c = (int)(i - r * Cp);
-    out[i] = c < C ? in[r * C + c] : from_float<T>(0.0f);
+    for (int i = threadIdx.x; i < 64 * PER; i += 256) {
+        const int c = i / PER, r = i % PER * VEC;
+        if (c0 + c >= C || r0 + r >= ld_out) continue;
+        Pack<T, VEC> v;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v.v[j] = tile[r + j][c];
+        *reinterpret_cast<Pack<T, VEC> *>(out + (int64_t)(c0 + c) * ld_out + r0 + r) = v;
+    }
 }
 
 // ---- host side
@@ -387,13 +465,16 @@ struct CePlan {
     int Cp;                          // C padded to whole 128-byte steps (narrow: to 32 elements)
     bool pad;                        // the operands are copied to rows of Cp (narrow: and into pieces)
     int64_t c4;                      // C rounded up to 4
+    bool together;                   // the kept rows are moved together
+    bool copy_x;                     // (wide) x is copied: padded, or moved together
     size_t xp, wp;                   // byte offsets: those copies
+    size_t map, place, targets, count;
     size_t part, own, rows;          // forward
     int64_t tiles;                   // statistics per row
     // backward
     int64_t piece, np;               // table rows per piece; n padded to 128 bytes of dl^T
     int parts;                       // of k in dx's product
-    int64_t per_x, per_w;            // narrow: rows of the table / of x per part
+    int64_t per_x;                   // narrow: rows of the table per part
     int parts_x, parts_w;
     size_t factors, dl, dlt, wt, xt, sums, sums_w;
     size_t total;
@@ -424,11 +505,17 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
     p.pad = p.Cp != C || (p.narrow && planes > 1);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
-    if (p.pad) {
-        const size_t row = (size_t)p.Cp * (p.narrow ? 2 * planes : p.es);
-        p.xp = take((size_t)n * row);
-        p.wp = take((size_t)V * row);
+    p.together = n > kTogether;
+    p.copy_x = p.pad || p.together;
+    if (p.together) {
+        p.map = take((size_t)n * 4);
+        p.place = take((size_t)n * 4);
+        p.targets = take((size_t)n * 8);
+        p.count = take(4);
     }
+    const size_t row = (size_t)p.Cp * (p.narrow ? 2 * planes : p.es);
+    if (p.copy_x) p.xp = take((size_t)n * row);
+    if (p.pad) p.wp = take((size_t)V * row);
     if (p.narrow && n > 0) {
         // parts of the rows that are walked: enough workgroups for the chip's 256 CUs four times over, at least 256 rows each
         auto split = [](int64_t fixed, int64_t moving, int64_t &per, int &parts) {
@@ -437,8 +524,9 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
             if (per < 256) per = 256;
             parts = (int)ceil_div(moving, per);
         };
+        int64_t per_w;
         split(n, V, p.per_x, p.parts_x);
-        split(V, n, p.per_w, p.parts_w);
+        split(V, n, per_w, p.parts_w);
     }
     if (!backward) {
         p.tiles = p.narrow ? p.parts_x : ceil_div(V, ce_big(V, n, p.es) ? 256 : 128);
@@ -482,15 +570,25 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
     return p;
 }
 
+static CeRows ce_rows(const CePlan &p, const int64_t *target, int64_t n, int64_t ignore, float *loss, char *ws, hipStream_t st) {
+    CeRows r = {};
+    r.target = target; r.n = n; r.ignore = ignore;
+    if (!p.together) return r;
+    int *map = reinterpret_cast<int *>(ws + p.map), *place = reinterpret_cast<int *>(ws + p.place), *count = reinterpret_cast<int *>(ws + p.count);
+    int64_t *targets = reinterpret_cast<int64_t *>(ws + p.targets);
+    hipLaunchKernelGGL(ce_together_kernel, dim3(1), dim3(1024), 0, st, target, n, ignore, map, place, targets, count, loss);
+    r.map = map; r.place = place; r.count = count; r.target = targets;
+    return r;
+}
+
 // the arguments of the narrow kernels that both passes share
-static NarrowArgs ce_narrow_args(const CePlan &p, int dtype, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale,
-                                 int64_t ignore, char *ws) {
+static NarrowArgs ce_narrow_args(const CePlan &p, int dtype, const void *x, const void *w, const CeRows &rows, int64_t V, int C, float scale, char *ws) {
     NarrowArgs a = {};
-    a.x = NarrowOperand{x, p.pad ? ws + p.xp : const_cast<char *>(static_cast<const char *>(x)), nullptr, n, p.pad};
-    a.w = NarrowOperand{w, p.pad ? ws + p.wp : const_cast<char *>(static_cast<const char *>(w)), nullptr, V, p.pad};
+    a.x = NarrowOperand{x, p.copy_x ? ws + p.xp : const_cast<char *>(static_cast<const char *>(x)), nullptr, rows.n, round_up(rows.n, 64), p.copy_x};
+    a.w = NarrowOperand{w, p.pad ? ws + p.wp : const_cast<char *>(static_cast<const char *>(w)), nullptr, V, round_up(V, 64), p.pad};
     a.C = C; a.Cp = p.Cp; a.planes = ce_planes(dtype);
-    a.per_x = p.per_x; a.per_w = p.per_w; a.parts_x = p.parts_x; a.parts_w = p.parts_w;
-    a.scale2 = scale * kLog2e; a.target = target; a.ignore = ignore; a.ld_sums = p.c4;
+    a.per_x = p.per_x; a.parts_x = p.parts_x; a.parts_w = p.parts_w;
+    a.scale2 = scale * kLog2e; a.kept_rows = rows; a.ld_sums = p.c4;
     return a;
 }
 
@@ -515,11 +613,40 @@ static int ce_check(const char *who, const void *x, const void *w, int dtype, co
     return MVS_OK;
 }
 
+// the operands as the tiles read them: x copied (the kept rows, padded) and the table padded where the plan says so
 template <typename T>
-static void ce_pad(const void *in, int64_t R, int C, char *out, int Cp, hipStream_t st) {
-    if (R > 0)
-        hipLaunchKernelGGL((ce_pad_kernel<T>), dim3((unsigned)ceil_div(R * Cp, 256)), dim3(256), 0, st, static_cast<const T *>(in), R, C,
-                           reinterpret_cast<T *>(out), Cp);
+static void ce_operands(const CePlan &p, const void *x, const void *w, const CeRows &rows, int64_t V, int C, char *ws, hipStream_t st, CeArgs &a) {
+    auto copy = [&](const void *in, const CeRows &r, char *out) {
+        constexpr int VEC = 16 / sizeof(T);
+        if (C % VEC == 0)
+            hipLaunchKernelGGL((ce_rows_kernel<T, VEC>), dim3((unsigned)ceil_div(r.n * (p.Cp / VEC), 256)), dim3(256), 0, st, static_cast<const T *>(in), r, C,
+                               reinterpret_cast<T *>(out), p.Cp);
+        else
+            hipLaunchKernelGGL((ce_rows_kernel<T, 1>), dim3((unsigned)ceil_div(r.n * p.Cp, 256)), dim3(256), 0, st, static_cast<const T *>(in), r, C,
+                               reinterpret_cast<T *>(out), p.Cp);
+    };
+    a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
+    a.x = Operand{static_cast<const char *>(x), (int64_t)p.Cp * p.es, rows.n};
+    if (p.copy_x) {
+        copy(x, rows, ws + p.xp);
+        a.x.p = ws + p.xp;
+    }
+    if (p.pad) {
+        CeRows table = {};
+        table.n = V;
+        copy(w, table, ws + p.wp);
+        a.w.p = ws + p.wp;
+    }
+    a.steps = p.Cp * p.es / kRowBytes;
+    a.v_total = V;
+    a.rows = rows;
+}
+
+template <typename T>
+static void ce_transpose(const char *in, const CeRows &rows, bool look, int C, int64_t ld_in, char *out, int64_t ld_out, hipStream_t st) {
+    constexpr int VEC = 16 / sizeof(T);      // (ld_in and ld_out are whole 128-byte steps)
+    hipLaunchKernelGGL((ce_transpose_kernel<T, VEC>), dim3((unsigned)ceil_div(ld_out, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
+                       reinterpret_cast<const T *>(in), rows, look, C, ld_in, reinterpret_cast<T *>(out), ld_out);
 }
 
 // a kernel on the tiles of its [m][n]: f(X()) sets the grid and launches
@@ -542,25 +669,16 @@ static void ce_launch(F kernel, const A &a, unsigned parts, size_t epilogue, hip
 }
 
 template <typename T>
-static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, char *ws, hipStream_t st) {
+static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const CeRows &rows, int64_t V, int C, float scale, char *ws, hipStream_t st) {
     CeArgs a = {};
-    a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
-    a.x = Operand{static_cast<const char *>(x), (int64_t)p.Cp * p.es, n};
-    if (p.pad) {
-        ce_pad<T>(x, n, C, ws + p.xp, p.Cp, st);
-        ce_pad<T>(w, V, C, ws + p.wp, p.Cp, st);
-        a.x.p = ws + p.xp;
-        a.w.p = ws + p.wp;
-    }
-    a.steps = p.Cp * p.es / kRowBytes;
-    a.n = n; a.v_total = V; a.v_count = V;
+    ce_operands<T>(p, x, w, rows, V, C, ws, st, a);
+    a.v_count = V;
     a.scale2 = scale * kLog2e;
-    a.target = target;
     a.part = reinterpret_cast<float2 *>(ws + p.part);
     a.own = reinterpret_cast<float *>(ws + p.own);
-    ce_tiles<T>(V, n, [&](auto x) {
+    ce_tiles<T>(V, rows.n, [&](auto x) {
         using X = decltype(x);
-        a.tiles_m = ceil_div(V, X::BM); a.tiles_n = ceil_div(n, X::BN);
+        a.tiles_m = ceil_div(V, X::BM); a.tiles_n = ceil_div(rows.n, X::BN);
         ce_launch<X>(ce_stats_kernel<T, X>, a, 1, (size_t)X::WAVES_M * X::BN * sizeof(float2), st);
     });
     return check_launch("mvs_linear_ce_fwd");
@@ -569,52 +687,44 @@ static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const in
 static int ce_forward(int dtype, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, int64_t ignore,
                       int reduction, float *loss, float *lse, float *kept, char *ws, hipStream_t st) {
     const CePlan p = ce_plan(n, V, C, dtype, false, false, false);
-    float *rows = reduction == 0 ? loss : reinterpret_cast<float *>(ws + p.rows);
+    float *losses = reduction == 0 ? loss : reinterpret_cast<float *>(ws + p.rows);
     if (n > 0) {
         float2 *part = reinterpret_cast<float2 *>(ws + p.part);
         float *own = reinterpret_cast<float *>(ws + p.own);
+        const CeRows rows = ce_rows(p, target, n, ignore, losses, ws, st);
         int rc = MVS_OK;
         if (p.narrow) {
-            NarrowArgs a = ce_narrow_args(p, dtype, x, w, target, n, V, C, scale, ignore, ws);
+            NarrowArgs a = ce_narrow_args(p, dtype, x, w, rows, V, C, scale, ws);
             a.part = part; a.own = own;
             rc = ce_narrow_forward(dtype, a, st);
         } else {
-            MVS_DTYPE_DISPATCH(dtype, T, rc = (ce_wide_stats<T>(p, x, w, target, n, V, C, scale, ws, st)));
+            MVS_DTYPE_DISPATCH(dtype, T, rc = (ce_wide_stats<T>(p, x, w, rows, V, C, scale, ws, st)));
         }
         if (rc != MVS_OK) return rc;
-        hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(256), 0, st, part, p.tiles, n, V, target, ignore, own, lse, rows);
+        hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(256), 0, st, part, p.tiles, V, rows, own, lse, losses);
     }
-    hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, rows, target, n, ignore, reduction, loss, kept);
+    hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, losses, target, n, ignore, reduction, loss, kept);
     return check_launch("mvs_linear_ce_fwd");
 }
 
 template <typename T>
-static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const int64_t *target, const float *lse, const float *kept, const float *grad_loss,
-                       int64_t n, int64_t V, int C, float scale, int64_t ignore, int reduction, void *grad_x, void *grad_w, char *ws, hipStream_t st) {
+static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const CeRows &rows, const float *lse, const float *kept, const float *grad_loss,
+                            int64_t V, int C, float scale, int reduction, void *grad_x, void *grad_w, char *ws, hipStream_t st) {
     const int step = kRowBytes / p.es;
+    const int64_t n = rows.n;
     float *factors = reinterpret_cast<float *>(ws + p.factors);
-    hipLaunchKernelGGL(ce_factors_kernel, dim3(1), dim3(1024), 0, st, grad_loss, kept, target, n, ignore, reduction, factors);
+    hipLaunchKernelGGL(ce_factors_kernel, dim3(reduction == 0 ? 1 : (unsigned)ceil_div(n, 1024)), dim3(1024), 0, st, rows, grad_loss, kept, reduction, factors);
     CeArgs a = {};
-    a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
-    a.x = Operand{static_cast<const char *>(x), (int64_t)p.Cp * p.es, n};
-    if (p.pad) {
-        ce_pad<T>(x, n, C, ws + p.xp, p.Cp, st);
-        ce_pad<T>(w, V, C, ws + p.wp, p.Cp, st);
-        a.x.p = ws + p.xp;
-        a.w.p = ws + p.wp;
-    }
+    ce_operands<T>(p, x, w, rows, V, C, ws, st, a);
     const float factor = scale / GradUnit<T>::value;
     const char *w_rows = a.w.p;
-    a.steps = p.Cp * p.es / kRowBytes;
-    a.n = n; a.v_total = V; a.ignore = ignore;
     a.scale2 = scale * kLog2e;
-    a.target = target; a.lse2 = lse; a.ratio = factors + n;
+    a.lse2 = lse; a.ratio = factors + n;
     a.dl = grad_x ? ws + p.dl : nullptr;
     a.dlt = grad_w ? ws + p.dlt : nullptr;
     a.ld_dlt = p.np;
-    if (grad_w)      // x^T once; ignored rows as zeros, whatever they hold
-        hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(p.np, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
-                           reinterpret_cast<const T *>(a.x.p), n, C, (int64_t)p.Cp, target, ignore, reinterpret_cast<T *>(ws + p.xt), p.np);
+    // x^T once; ignored rows as zeros, whatever they hold
+    if (grad_w) ce_transpose<T>(a.x.p, rows, !p.together, C, p.Cp, ws + p.xt, p.np, st);
     auto product = [&](CeProduct &d) {
         ce_tiles<T>(d.m, d.n, [&](auto x) {
             using X = decltype(x);
@@ -633,16 +743,16 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             ce_launch<X>(ce_grad_kernel<T, X>, a, 1, (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
         });
         if (grad_x) {
-            hipLaunchKernelGGL((ce_transpose_kernel<T>), dim3((unsigned)ceil_div(k, 64), (unsigned)ceil_div(C, 64)), dim3(256), 0, st,
-                               reinterpret_cast<const T *>(a.w.p), count, C, (int64_t)p.Cp, (const int64_t *)nullptr, ignore,
-                               reinterpret_cast<T *>(ws + p.wt), k);
+            CeRows table = {};
+            table.n = count;
+            ce_transpose<T>(a.w.p, table, false, C, p.Cp, ws + p.wt, k, st);
             CeProduct d = {};
             d.a = Operand{ws + p.wt, k * p.es, C};
             d.b = Operand{ws + p.dl, k * p.es, n};
             d.steps = (int)(k / step);
             d.steps_per_part = (int)ceil_div(d.steps, p.parts);
             d.m = C; d.n = n;
-            d.sums = reinterpret_cast<float *>(ws + p.sums); d.ld_sums = p.c4;
+            d.sums = reinterpret_cast<float *>(ws + p.sums); d.ld_sums = p.c4; d.sum_rows = n; d.count = rows.count;
             d.add = v0 > 0;
             // (a smaller last piece may have fewer parts of k: the sums of the others stay as they are)
             product(d);
@@ -655,13 +765,13 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             d.steps_per_part = d.steps;
             d.m = C; d.n = count;
             d.out = static_cast<T *>(grad_w) + v0 * C;
-            d.top = factors + 2 * n; d.factor = factor;
+            d.top = factors + 2 * n; d.factor = factor; d.count = rows.count;
             product(d);
         }
     }
     if (grad_x)
         hipLaunchKernelGGL((ce_finish_kernel<T>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
-                           p.parts, n, C, p.c4, factors, factor, static_cast<T *>(grad_x));
+                           p.parts, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));
     return check_launch("mvs_linear_ce_bwd");
 }
 
@@ -710,8 +820,9 @@ extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, c
     }
     const CePlan p = ce_plan(n, V, C, dtype, true, grad_x != nullptr, grad_weight != nullptr);
     char *ws = static_cast<char *>(workspace);
+    const CeRows rows = ce_rows(p, target, n, ignore_index, nullptr, ws, as_stream(stream));
     if (p.narrow) {
-        NarrowArgs a = ce_narrow_args(p, dtype, x, weight, target, n, V, C, scale, ignore_index, ws);
+        NarrowArgs a = ce_narrow_args(p, dtype, x, weight, rows, V, C, scale, ws);
         a.lse2 = lse; a.grad_loss = grad_loss; a.kept = kept; a.reduction = reduction;
         a.factors = reinterpret_cast<float *>(ws + p.factors);
         if (grad_x) { a.w.trans = ws + p.wt; a.sums_x = reinterpret_cast<float *>(ws + p.sums); }
@@ -721,7 +832,6 @@ extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, c
         return ce_narrow_backward(dtype, a, as_stream(stream));
     }
     MVS_DTYPE_DISPATCH(dtype, T, {
-        return (ce_wide_backward<T>(p, x, weight, target, lse, kept, grad_loss, n, V, C, scale, ignore_index, reduction, grad_x, grad_weight, ws,
-                                             as_stream(stream)));
+        return (ce_wide_backward<T>(p, x, weight, rows, lse, kept, grad_loss, V, C, scale, reduction, grad_x, grad_weight, ws, as_stream(stream)));
     });
 }

@@ -80,7 +80,7 @@ __device__ __forceinline__ void narrow_copy_rows(const NarrowOperand &o, int Cp,
 template <typename X>
 __device__ __forceinline__ void narrow_copy_trans(const NarrowOperand &o, int C, int64_t m0, unsigned to) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t mp = (o.count + 63) & ~(int64_t)63;
+    const int64_t mp = o.pitch;
 #pragma unroll
     for (int i = 0; i < (X::TRANS_COPIES + 3) / 4; ++i) {
         const int c = wave + i * 4;
@@ -139,6 +139,10 @@ __global__ __launch_bounds__(256) void narrow_stats_kernel(NarrowArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, lane_at = narrow_lane();
     const int64_t n0 = (int64_t)blockIdx.x * kNarrowRows + wave * 32, m_begin = (int64_t)blockIdx.y * a.per_x;
     const int rows = (int)min(a.per_x, a.w.count - m_begin);
+    NarrowOperand x = a.x;
+    x.count = ce_count(a.kept_rows);
+    if ((int64_t)blockIdx.x * kNarrowRows >= x.count) return;
+    const int64_t *targets = a.kept_rows.target;
     const unsigned base_lds = (unsigned)(uintptr_t)&lds[0][0];
     narrow_copy_rows<X>(a.w, a.Cp, m_begin, base_lds);
     // a negative scale is taken as its magnitude and negated rows: the largest logit is then that of the largest product
@@ -149,13 +153,13 @@ __global__ __launch_bounds__(256) void narrow_stats_kernel(NarrowArgs a) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int64_t n = n0 + j * 16 + ln;
-        narrow_fixed<X>(a.x, a.Cp, n, true, fixed[j]);
+        narrow_fixed<X>(x, a.Cp, n, true, fixed[j]);
         if (a.scale2 < 0.0f)
 #pragma unroll
             for (int k = 0; k < X::KS; ++k)
 #pragma unroll
                 for (int q = 0; q < X::PL; ++q) fixed[j][k][q] ^= 0x80008000u;
-        const int64_t t = (n < a.x.count ? a.target[n] : -1) - m_begin;
+        const int64_t t = (n < x.count ? targets[n] : -1) - m_begin;
         target[j] = t >= 0 && t < rows ? (int)t : -1;
         base[j] = -INFINITY;
         sum[j] = 0.0f;
@@ -207,7 +211,7 @@ __global__ __launch_bounds__(256) void narrow_stats_kernel(NarrowArgs a) {
         r += __shfl_xor(r, 16);
         r += __shfl_xor(r, 32);
         const int64_t n = n0 + j * 16 + ln;
-        if (lane < 16 && n < a.x.count) a.part[(int64_t)blockIdx.y * a.x.count + n] = make_float2(t, r);
+        if (lane < 16 && n < x.count) a.part[(int64_t)blockIdx.y * a.x.count + n] = make_float2(t, r);
     }
 }
 
@@ -222,33 +226,36 @@ template <typename X, bool OF_TABLE>
 __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOperand &fix, const NarrowOperand &mov, int64_t block, int64_t part, float unit,
                                             char *lds, NarrowRows &row_stats) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, group = lane >> 4, lane_at = narrow_lane();
-    const int64_t per = OF_TABLE ? a.per_w : a.per_x, n0 = block * kNarrowRows + wave * 32, m_begin = part * per;
-    const int rows = (int)min(per, mov.count - m_begin);
+    // (the kept rows are split evenly over the parts, in whole stages; a part may get none and then writes zeros)
+    const int64_t per = OF_TABLE ? (mov.count + a.parts_w * 64 - 1) / (a.parts_w * 64) * 64 : a.per_x;
+    const int64_t n0 = block * kNarrowRows + wave * 32, m_begin = part * per;
+    const int rows = (int)max((int64_t)0, min(per, mov.count - m_begin));
+    const int64_t *targets = a.kept_rows.target, ignore = a.kept_rows.ignore;
     const unsigned base_lds = (unsigned)(uintptr_t)lds;
     auto copy = [&](int m, int stage) {
         const unsigned to = base_lds + (unsigned)(stage * (X::ROWS_B + X::TRANS_B));
         narrow_copy_rows<X>(mov, a.Cp, m_begin + m, to);
         narrow_copy_trans<X>(mov, a.C, m_begin + m, to + (unsigned)X::ROWS_B);
     };
-    const float *ratios = a.factors + a.x.count;
+    const float *ratios = a.factors + a.kept_rows.n;
     float lse_next = 0.0f, ratio_next = 0.0f;
     int target_next = -1;
     auto stats = [&](int m) {      // thread t < MR's row of the stage, loaded a stage ahead
         const int64_t row = m_begin + m + threadIdx.x;
-        const bool kept = threadIdx.x < X::MR && m + (int)threadIdx.x < rows && ce_kept(a.target[row], a.ignore);
+        const bool kept = threadIdx.x < X::MR && m + (int)threadIdx.x < rows && ce_kept(targets[row], ignore);
         lse_next = kept ? a.lse2[row] : 0.0f;
         ratio_next = kept ? ratios[row] * unit : 0.0f;
-        target_next = kept ? (int)(a.target[row] >= 0 && a.target[row] < fix.count ? a.target[row] : -1) : -1;
+        target_next = kept ? (int)(targets[row] >= 0 && targets[row] < fix.count ? targets[row] : -1) : -1;
     };
-    copy(0, 0);
+    if (rows > 0) copy(0, 0);
     if (OF_TABLE) stats(0);
     u32x4_t fixed[2][X::KS][X::PL];
     int target[2];
     float lse[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const int64_t n = n0 + j * 16 + ln, t = !OF_TABLE && n < fix.count ? a.target[n] : a.ignore;
-        const bool kept = OF_TABLE || ce_kept(t, a.ignore);
+        const int64_t n = n0 + j * 16 + ln, t = !OF_TABLE && n < fix.count ? targets[n] : 0;
+        const bool kept = OF_TABLE || (n < fix.count && ce_kept(t, ignore));
         // (whatever an ignored row holds, its S are 0 and its exponentials those of -Inf)
         narrow_fixed<X>(fix, a.Cp, n, kept, fixed[j]);
         lse[j] = OF_TABLE ? 0.0f : kept ? a.lse2[n] : INFINITY;
@@ -332,6 +339,7 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
         }
     }
     float *sums = OF_TABLE ? a.sums_w : a.sums_x;
+    const int64_t sum_rows = OF_TABLE ? a.w.count : a.kept_rows.n;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int64_t n = n0 + j * 16 + ln;
@@ -339,7 +347,7 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
 #pragma unroll
         for (int c = 0; c < X::CT; ++c) {
             const int col = c * 16 + group * 4;
-            if (col < a.C) *reinterpret_cast<f32x4_t *>(sums + (part * fix.count + n) * a.ld_sums + col) = out[c][j];
+            if (col < a.C) *reinterpret_cast<f32x4_t *>(sums + (part * sum_rows + n) * a.ld_sums + col) = out[c][j];
         }
     }
 }
@@ -350,8 +358,13 @@ __global__ __launch_bounds__(256, 2) void narrow_grad_kernel(NarrowArgs a, int64
     __shared__ __align__(1024) char lds[2 * (X::ROWS_B + X::TRANS_B)];
     __shared__ NarrowRows row_stats;
     const int64_t id = blockIdx.x;
-    if (id < groups_x) narrow_grad<X, false>(a, a.x, a.w, id % blocks_x, id / blocks_x, unit, lds, row_stats);
-    else narrow_grad<X, true>(a, a.w, a.x, (id - groups_x) % blocks_w, (id - groups_x) / blocks_w, unit, lds, row_stats);
+    NarrowOperand x = a.x;
+    x.count = ce_count(a.kept_rows);
+    if (id < groups_x) {
+        if (id % blocks_x * kNarrowRows < x.count) narrow_grad<X, false>(a, x, a.w, id % blocks_x, id / blocks_x, unit, lds, row_stats);
+    } else {
+        narrow_grad<X, true>(a, a.w, x, (id - groups_x) % blocks_w, (id - groups_x) / blocks_w, unit, lds, row_stats);
+    }
 }
 
 // a value's pieces: 8 bits each, the first one cut instead of rounded where rounding would overflow
@@ -379,17 +392,18 @@ __global__ __launch_bounds__(256) void narrow_prepare_kernel(NarrowArgs a) {
     __shared__ float tops[4];
     const int tid = threadIdx.x;
     if (blockIdx.y == 2) {
-        if (blockIdx.x == 0) ce_factors(a.grad_loss, a.kept, a.target, a.x.count, a.ignore, a.reduction, a.factors, tops);
+        if (a.reduction != 0) ce_factors(a.kept_rows, a.grad_loss, a.kept, a.reduction, a.factors, (int64_t)blockIdx.x * 256 + tid, (int64_t)gridDim.x * 256, tops);
+        else if (blockIdx.x == 0) ce_factors(a.kept_rows, a.grad_loss, a.kept, a.reduction, a.factors, tid, 256, tops);
         return;
     }
     const NarrowOperand &o = blockIdx.y ? a.w : a.x;
-    const int64_t r0 = (int64_t)blockIdx.x * 64, mp = (o.count + 63) & ~(int64_t)63;
-    if (r0 >= o.count || (!o.write_rows && !o.trans)) return;
+    const int64_t r0 = (int64_t)blockIdx.x * 64, mp = o.pitch, count = blockIdx.y ? o.count : ce_count(a.kept_rows);
+    if (r0 >= count || (!o.write_rows && !o.trans)) return;
     const T *source = static_cast<const T *>(o.source);
-    const int here = (int)min((int64_t)64, o.count - r0);
+    const int here = (int)min((int64_t)64, count - r0);
     for (int i = tid; i < 64 * a.C; i += 256) {
         const int r = i / a.C, c = i - r * a.C;
-        tile[r][c] = r < here ? source[(r0 + r) * a.C + c] : from_float<T>(0.0f);
+        tile[r][c] = r < here ? source[(blockIdx.y ? r0 + r : ce_original(a.kept_rows, r0 + r)) * a.C + c] : from_float<T>(0.0f);
     }
     __syncthreads();
     if (o.write_rows) {
@@ -406,7 +420,7 @@ __global__ __launch_bounds__(256) void narrow_prepare_kernel(NarrowArgs a) {
         E *trans = reinterpret_cast<E *>(o.trans);
         const int place = tid & 63, r = (place & 32) + ((place >> 3) & 3) * 4 + (place & 3) + ((place & 4) << 2);
         // (ignored rows of x as zeros, whatever they hold)
-        const bool keep = r < here && (blockIdx.y || ce_kept(a.target[r0 + r], a.ignore));
+        const bool keep = r < here && (blockIdx.y || ce_kept(a.kept_rows.target[r0 + r], a.kept_rows.ignore));
         for (int c = tid >> 6; c < a.C; c += 4) {
             E p[PL];
             pieces_of<E, PL>(keep ? tile[r][c] : from_float<T>(0.0f), p);
@@ -421,9 +435,9 @@ template <typename T>
 __global__ __launch_bounds__(256) void narrow_finish_kernel(NarrowArgs a, int64_t groups_x) {
     const int64_t id = blockIdx.x;
     if (id < groups_x)
-        ce_finish<T, true>(a.sums_x, a.parts_x, a.x.count, a.C, a.ld_sums, a.factors, a.factor, static_cast<T *>(a.grad_x), id);
+        ce_finish<T, true>(a.sums_x, a.parts_x, a.x.count, a.kept_rows.place, a.C, a.ld_sums, a.factors, a.factor, static_cast<T *>(a.grad_x), id);
     else
-        ce_finish<T, false>(a.sums_w, a.parts_w, a.w.count, a.C, a.ld_sums, a.factors + 2 * a.x.count, a.factor, static_cast<T *>(a.grad_w), id - groups_x);
+        ce_finish<T, false>(a.sums_w, a.parts_w, a.w.count, (const int *)nullptr, a.C, a.ld_sums, a.factors + 2 * a.x.count, a.factor, static_cast<T *>(a.grad_w), id - groups_x);
 }
 
 template <typename T, typename E, int PL>

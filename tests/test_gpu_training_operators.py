@@ -494,3 +494,18 @@ def test_double_backward_is_refused():
     g, = torch.autograd.grad(ops.linear_cross_entropy(leaf, w, t), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), leaf)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,C", [(1000, 300, 32), (1000, 300, 200), (5000, 100, 16), (129, 50, 160), (300, 70000, 40)])
+@pytest.mark.parametrize("kept", ["first", "last", "one", "half", "none", "all"])
+def test_linear_cross_entropy_kept_rows_anywhere(n, V, C, dtype, kept):
+    """More than a tile of rows: the kept ones are moved together, wherever they are and however few."""
+    x, w, t, _ = ce_case(n, V, C, dtype, ignored=0.0, seed=12)
+    keep = torch.zeros(n, dtype=torch.bool, device="cuda")
+    {"first": lambda: keep[:70].fill_(True), "last": lambda: keep[-70:].fill_(True), "one": lambda: keep[n // 2:n // 2 + 1].fill_(True),
+     "half": lambda: keep[::2].fill_(True), "none": lambda: None, "all": lambda: keep.fill_(True)}[kept]()
+    t = torch.where(keep, t, -100)
+    x[~keep] = float("nan")
+    ce_check(x, w, t, 1.5, reduction="mean")
+    ce_check(x, w, t, 1.5, reduction="none")
