@@ -10,12 +10,32 @@ namespace mvs {
 
 constexpr int kUnroll = 4;
 
-// One 16-byte vector of the tensor per lane and step; n_vec of them, the rest (n - n_vec * VEC < 32 values) by the last workgroup.
+// Any alignment, and the ragged block behind the whole ones: 8 blocks from `block0` on, 32 lanes each, one value a lane.
 template <typename T>
-__global__ __launch_bounds__(256) void act8_quantize_kernel(const T *__restrict__ x, int64_t n, signed char *__restrict__ codes,
+__device__ __forceinline__ void act8_quantize_lanes(const T *__restrict__ x, int64_t n, int64_t block0, signed char *__restrict__ codes,
+                                                    unsigned char *__restrict__ scales) {
+    const int64_t b = block0 + threadIdx.x / 32, i = b * kAct8Block + threadIdx.x % 32;
+    const float f = i < n ? to_float(x[i]) : 0.0f;
+    unsigned amax = __float_as_uint(f) & 0x7fffffffu;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) amax = umax_xor(amax, o);
+    const unsigned byte = act8_scale_byte(amax);
+    if (i >= n) return;
+    codes[i] = byte == kAct8Nan ? (signed char)0 : (signed char)act8_code(f, act8_inverse(byte));
+    if (threadIdx.x % 32 == 0) scales[b] = (unsigned char)byte;
+}
+
+// One 16-byte vector of the tensor per lane and step over the `whole` blocks that are moved so (0: off alignment); the workgroups behind
+// theirs take the other blocks value by value.
+template <typename T>
+__global__ __launch_bounds__(256) void act8_quantize_kernel(const T *__restrict__ x, int64_t n, int64_t whole, int64_t groups, signed char *__restrict__ codes,
                                                             unsigned char *__restrict__ scales) {
+    if (blockIdx.x >= groups) {
+        act8_quantize_lanes(x, n, whole + (blockIdx.x - groups) * 8, codes, scales);
+        return;
+    }
     constexpr int VEC = 16 / sizeof(T), LANES = kAct8Block / VEC;
-    const int64_t n_vec = n / kAct8Block * LANES;      // vectors of whole blocks
+    const int64_t n_vec = whole * LANES;
     const int64_t first = (int64_t)blockIdx.x * 256 * kUnroll + threadIdx.x;
     Pack<T, VEC> v[kUnroll];
 #pragma unroll
@@ -48,21 +68,6 @@ __global__ __launch_bounds__(256) void act8_quantize_kernel(const T *__restrict_
     }
 }
 
-// Any alignment, and the ragged block behind the whole ones: 32 lanes per block of values, one value each.  Blocks from `block0` on.
-template <typename T>
-__global__ __launch_bounds__(256) void act8_quantize_lanes_kernel(const T *__restrict__ x, int64_t n, int64_t block0,
-                                                                  signed char *__restrict__ codes, unsigned char *__restrict__ scales) {
-    const int64_t b = block0 + (int64_t)blockIdx.x * 8 + threadIdx.x / 32, i = b * kAct8Block + threadIdx.x % 32;
-    const float f = i < n ? to_float(x[i]) : 0.0f;
-    unsigned amax = __float_as_uint(f) & 0x7fffffffu;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) amax = umax_xor(amax, o);
-    const unsigned byte = act8_scale_byte(amax);
-    if (i >= n) return;
-    codes[i] = byte == kAct8Nan ? (signed char)0 : (signed char)act8_code(f, act8_inverse(byte));
-    if (threadIdx.x % 32 == 0) scales[b] = (unsigned char)byte;
-}
-
 template <typename T>
 __device__ __forceinline__ T act8_back(float v) {
     constexpr float most = DtypeMax<T>::value;
@@ -71,9 +76,14 @@ __device__ __forceinline__ T act8_back(float v) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void act8_dequantize_kernel(const signed char *__restrict__ codes, const unsigned char *__restrict__ scales,
-                                                              int64_t n, T *__restrict__ out) {
+                                                              int64_t n, int64_t whole, int64_t groups, T *__restrict__ out) {
+    if (blockIdx.x >= groups) {
+        const int64_t i = whole * kAct8Block + (blockIdx.x - groups) * 256 + threadIdx.x;
+        if (i < n) out[i] = act8_back<T>((float)codes[i] * act8_step(scales[i / kAct8Block]));
+        return;
+    }
     constexpr int VEC = 16 / sizeof(T), LANES = kAct8Block / VEC;
-    const int64_t n_vec = n / kAct8Block * LANES;
+    const int64_t n_vec = whole * LANES;
     const int64_t first = (int64_t)blockIdx.x * 256 * kUnroll + threadIdx.x;
     Pack<unsigned, VEC / 4> q[kUnroll];
     unsigned byte[kUnroll];
@@ -95,13 +105,6 @@ __global__ __launch_bounds__(256) void act8_dequantize_kernel(const signed char 
         for (int j = 0; j < VEC; ++j) o.v[j] = act8_back<T>(act8_value(q[u].v[j / 4], j % 4, step));
         reinterpret_cast<Pack<T, VEC> *>(out)[i] = o;
     }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void act8_dequantize_lanes_kernel(const signed char *__restrict__ codes, const unsigned char *__restrict__ scales,
-                                                                    int64_t n, int64_t first, T *__restrict__ out) {
-    const int64_t i = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) out[i] = act8_back<T>((float)codes[i] * act8_step(scales[i / kAct8Block]));
 }
 
 static int act8_check(const char *who, const void *wide, int dtype, int64_t n, const void *codes, const void *scales) {
@@ -132,12 +135,8 @@ extern "C" int mvs_act8_quantize(const void *x, int dtype, int64_t n, signed cha
     hipStream_t st = as_stream(stream);
     const int64_t whole = act8_wide(x, codes) ? n / kAct8Block : 0, blocks = (n + kAct8Block - 1) / kAct8Block;
     MVS_DTYPE_DISPATCH(dtype, T, {
-        const T *p = static_cast<const T *>(x);
-        const int64_t vecs = whole * (kAct8Block * sizeof(T) / 16);
-        if (vecs)
-            hipLaunchKernelGGL((act8_quantize_kernel<T>), dim3((unsigned)((vecs + 256 * kUnroll - 1) / (256 * kUnroll))), dim3(256), 0, st, p, n, codes, scales);
-        if (blocks > whole)
-            hipLaunchKernelGGL((act8_quantize_lanes_kernel<T>), dim3((unsigned)((blocks - whole + 7) / 8)), dim3(256), 0, st, p, n, whole, codes, scales);
+        const int64_t groups = (whole * (kAct8Block * (int)sizeof(T) / 16) + 256 * kUnroll - 1) / (256 * kUnroll), rest = (blocks - whole + 7) / 8;
+        hipLaunchKernelGGL((act8_quantize_kernel<T>), dim3((unsigned)(groups + rest)), dim3(256), 0, st, static_cast<const T *>(x), n, whole, groups, codes, scales);
     });
     return check_launch("mvs_act8_quantize");
 }
@@ -148,12 +147,8 @@ extern "C" int mvs_act8_dequantize(const signed char *codes, const unsigned char
     hipStream_t st = as_stream(stream);
     const int64_t whole = act8_wide(out, codes) ? n / kAct8Block : 0;
     MVS_DTYPE_DISPATCH(dtype, T, {
-        T *p = static_cast<T *>(out);
-        const int64_t vecs = whole * (kAct8Block * sizeof(T) / 16), first = whole * kAct8Block;
-        if (vecs)
-            hipLaunchKernelGGL((act8_dequantize_kernel<T>), dim3((unsigned)((vecs + 256 * kUnroll - 1) / (256 * kUnroll))), dim3(256), 0, st, codes, scales, n, p);
-        if (n > first)
-            hipLaunchKernelGGL((act8_dequantize_lanes_kernel<T>), dim3((unsigned)((n - first + 255) / 256)), dim3(256), 0, st, codes, scales, n, first, p);
+        const int64_t groups = (whole * (kAct8Block * (int)sizeof(T) / 16) + 256 * kUnroll - 1) / (256 * kUnroll), rest = (n - whole * kAct8Block + 255) / 256;
+        hipLaunchKernelGGL((act8_dequantize_kernel<T>), dim3((unsigned)(groups + rest)), dim3(256), 0, st, codes, scales, n, whole, groups, static_cast<T *>(out));
     });
     return check_launch("mvs_act8_dequantize");
 }

@@ -426,6 +426,139 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const T *__restrict__ in, 
     reinterpret_cast<Pack<T, VEC> *>(out)[i] = v;
 }
 
+// ---- few rows (at most kFew): both gradients in one pass over the table
+// With so few rows a product tile is mostly empty and W^T costs more than the products: bound by reading W and writing dW, once each.
+// A thread owns VEC columns, keeps x (times the row's ratio) and dx of NR rows there in registers and walks 64 table rows:
+//     dx[n] += dl[n][v] W[v],  dW[v] = sum_n dl[n][v] ratio_n x[n]
+constexpr int kFew = 16, kFewTable = 64;
+struct CeFew {
+    const void *w, *x, *dl;
+    int64_t count, ld_dl;               // table rows of the piece; elements per row of dl
+    int n, C, Cp, threads;              // threads per table row, a power of two
+    const float *ratio, *top;
+    float factor;
+    void *grad_w;                       // [count][C] or NULL
+    float *sums;                        // [part][n][c4] or NULL
+    int64_t c4;
+    int add;
+};
+
+template <typename T, int NR, int VEC>
+__global__ __launch_bounds__(256) void ce_few_kernel(CeFew a) {
+    __shared__ float d[kFewTable][NR];
+    __shared__ float joined[256][VEC];
+    const int tid = threadIdx.x, col = (blockIdx.y * a.threads + (tid & (a.threads - 1))) * VEC, sub = tid / a.threads, subs = 256 / a.threads;
+    const int64_t v0 = (int64_t)blockIdx.x * kFewTable;
+    const int rows = (int)min((int64_t)kFewTable, a.count - v0);
+    const bool here = col < a.Cp;
+    for (int i = tid; i < kFewTable * NR; i += 256) {
+        const int v = i / NR, r = i % NR;
+        d[v][r] = v < rows && r < a.n ? to_float(static_cast<const T *>(a.dl)[r * a.ld_dl + v0 + v]) : 0.0f;
+    }
+    float x[NR][VEC], dx[NR][VEC];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        Pack<T, VEC> p;
+        const float ratio = r < a.n ? a.ratio[r] : 0.0f;
+        if (here && ratio != 0.0f) p = *reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.x) + (int64_t)r * a.Cp + col);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            x[r][j] = here && ratio != 0.0f ? to_float(p.v[j]) * ratio : 0.0f;      // (an ignored row's values are not looked at)
+            dx[r][j] = 0.0f;
+        }
+    }
+    __syncthreads();
+    const float f = a.grad_w ? *a.top * a.factor : 0.0f;
+    const Pack<T, VEC> *w = reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.w) + v0 * a.Cp + col);
+    const int stride = a.Cp / VEC;
+    if (here)
+        for (int v = sub; v < rows; v += 4 * subs) {
+            Pack<T, VEC> p[4];
+            if (a.sums)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (v + u * subs < rows) p[u] = w[(int64_t)(v + u * subs) * stride];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int row = v + u * subs;
+                if (row >= rows) break;
+                float out[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) out[j] = 0.0f;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const float g = d[row][r];
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        if (a.sums) dx[r][j] = __builtin_fmaf(g, to_float(p[u].v[j]), dx[r][j]);
+                        out[j] = __builtin_fmaf(g, x[r][j], out[j]);
+                    }
+                }
+                if (a.grad_w && col < a.C) {      // (the padding's columns are nobody's)
+                    T *to = static_cast<T *>(a.grad_w) + (v0 + row) * a.C + col;
+                    Pack<T, VEC> o;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(out[j] * f);
+                    if (a.C % VEC == 0) *reinterpret_cast<Pack<T, VEC> *>(to) = o;
+                    else
+                        for (int j = 0; j < VEC; ++j) if (col + j < a.C) to[j] = o.v[j];
+                }
+            }
+        }
+    if (!a.sums) return;
+    for (int r = 0; r < a.n; ++r) {      // the threads of a column, in order
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < NR; ++q)
+            if (q == r)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) joined[tid][j] = dx[q][j];
+        __syncthreads();
+        if (sub == 0 && col < a.c4) {
+            float s[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s[j] = 0.0f;
+            for (int q = 0; q < subs; ++q)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s[j] += joined[q * a.threads + tid][j];
+            float *to = a.sums + ((int64_t)blockIdx.x * a.n + r) * a.c4 + col;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (col + j < a.c4) to[j] = a.add ? to[j] + s[j] : s[j];
+        }
+    }
+}
+
+// dx from many parts of few rows: 16 quads of columns x 16 shares of the parts per workgroup, the shares joined in order
+template <typename T>
+__global__ __launch_bounds__(256) void ce_few_finish_kernel(const float *__restrict__ sums, int parts, int n, int C, int64_t c4, const float *__restrict__ g,
+                                                            float factor, T *__restrict__ out) {
+    __shared__ f32x4_t shares[16][16];
+    const int64_t quads = c4 / 4, i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15), row = i / quads, step = n * quads;
+    const int share = threadIdx.x >> 4;
+    const f32x4_t *from = reinterpret_cast<const f32x4_t *>(sums) + i;
+    f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row < n)
+        for (int p = share; p < parts; p += 128) {
+            f32x4_t v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (p + j * 16 < parts) v[j] = from[(p + j * 16) * step];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (p + j * 16 < parts) s += v[j];
+        }
+    shares[share][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (share != 0 || row >= n) return;
+    for (int q = 1; q < 16; ++q) s += shares[q][threadIdx.x];
+    const float f = g[row];
+    const int64_t c = (i - row * quads) * 4;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (c + r < C) out[row * C + c + r] = from_float<T>(f == 0.0f ? 0.0f : s[r] * f * factor);
+}
+
 // out[c][r] = in[r][c] for c < C and r < rows, zero for the other r < ld_out and for ignored rows.  64 x 64 tiles through LDS, moved
 // VEC elements at a time on both sides (VEC > 1: ld_in, and C or its padding, reach whole vectors).
 template <typename T, int VEC>
@@ -465,6 +598,7 @@ struct CePlan {
     int Cp;                          // C padded to whole 128-byte steps (narrow: to 32 elements)
     bool pad;                        // the operands are copied to rows of Cp (narrow: and into pieces)
     int64_t c4;                      // C rounded up to 4
+    bool few;                        // wide rows, at most kFew of them
     bool together;                   // the kept rows are moved together
     bool copy_x;                     // (wide) x is copied: padded, or moved together
     size_t xp, wp;                   // byte offsets: those copies
@@ -499,6 +633,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
     CePlan p = {};
     p.es = (int)dtype_size(dtype);
     p.narrow = ce_narrow(C, dtype);
+    p.few = !p.narrow && n <= kFew;
     p.c4 = round_up(C, 4);
     const int step = kRowBytes / p.es, planes = ce_planes(dtype);
     p.Cp = (int)round_up(C, p.narrow ? 32 : step);
@@ -550,7 +685,11 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
         if (p.piece > round_up(V, 256)) p.piece = round_up(V, 256);
         p.np = round_up(n, step);
         p.factors = take((size_t)(2 * n + 1) * 4);
-        if (need_x) {
+        if (p.few) {
+            p.dl = take((size_t)n * p.piece * p.es);
+            p.parts = (int)ceil_div(V < p.piece ? V : p.piece, kFewTable);
+            if (need_x) p.sums = take((size_t)p.parts * n * p.c4 * 4);
+        } else if (need_x) {
             p.dl = take((size_t)n * p.piece * p.es);
             p.wt = take((size_t)C * p.piece * p.es);
             const int64_t side = ce_big(C, n, p.es) ? 256 : 128, tiles = ceil_div(C, side) * ceil_div(n, side), steps = round_up(V < p.piece ? V : p.piece, step) / step;
@@ -561,7 +700,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
             p.parts = (int)ceil_div(steps, ceil_div(steps, parts));      // (as many as get work; a smaller last piece then has no more)
             p.sums = take((size_t)p.parts * n * p.c4 * 4);
         }
-        if (need_w) {
+        if (need_w && !p.few) {
             p.dlt = take((size_t)p.piece * p.np * p.es);
             p.xt = take((size_t)C * p.np * p.es);
         }
@@ -669,6 +808,21 @@ static void ce_launch(F kernel, const A &a, unsigned parts, size_t epilogue, hip
 }
 
 template <typename T>
+static void ce_few(CeFew d, hipStream_t st) {
+    auto launch = [&](auto kernel, int vec) {
+        d.threads = 1;
+        while (d.threads < 256 && d.threads * vec < d.Cp) d.threads *= 2;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(d.count, kFewTable), (unsigned)ceil_div(d.Cp, d.threads * vec)), dim3(256), 0, st, d);
+    };
+    // 16-byte accesses while x and dx of NR rows at that many columns fit the registers, 8-byte ones for more
+    constexpr int VEC = 16 / sizeof(T), HALF = VEC / 2, EIGHT = sizeof(T) == 2 ? HALF : VEC;
+    if (d.n == 1) launch(ce_few_kernel<T, 1, VEC>, VEC);
+    else if (d.n <= 4) launch(ce_few_kernel<T, 4, VEC>, VEC);
+    else if (d.n <= 8) launch(ce_few_kernel<T, 8, EIGHT>, EIGHT);
+    else launch(ce_few_kernel<T, 16, HALF>, HALF);
+}
+
+template <typename T>
 static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const CeRows &rows, int64_t V, int C, float scale, char *ws, hipStream_t st) {
     CeArgs a = {};
     ce_operands<T>(p, x, w, rows, V, C, ws, st, a);
@@ -720,11 +874,11 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
     const char *w_rows = a.w.p;
     a.scale2 = scale * kLog2e;
     a.lse2 = lse; a.ratio = factors + n;
-    a.dl = grad_x ? ws + p.dl : nullptr;
-    a.dlt = grad_w ? ws + p.dlt : nullptr;
+    a.dl = grad_x || p.few ? ws + p.dl : nullptr;
+    a.dlt = grad_w && !p.few ? ws + p.dlt : nullptr;
     a.ld_dlt = p.np;
     // x^T once; ignored rows as zeros, whatever they hold
-    if (grad_w) ce_transpose<T>(a.x.p, rows, !p.together, C, p.Cp, ws + p.xt, p.np, st);
+    if (a.dlt) ce_transpose<T>(a.x.p, rows, !p.together, C, p.Cp, ws + p.xt, p.np, st);
     auto product = [&](CeProduct &d) {
         ce_tiles<T>(d.m, d.n, [&](auto x) {
             using X = decltype(x);
@@ -742,6 +896,17 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             a.tiles_m = ceil_div(count, X::BM); a.tiles_n = ceil_div(n, X::BN);
             ce_launch<X>(ce_grad_kernel<T, X>, a, 1, (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
         });
+        if (p.few) {
+            CeFew d = {};
+            d.w = a.w.p; d.x = a.x.p; d.dl = a.dl; d.count = count; d.ld_dl = k;
+            d.n = (int)n; d.C = C; d.Cp = p.Cp;
+            d.ratio = factors + n; d.top = factors + 2 * n; d.factor = factor;
+            d.grad_w = grad_w ? static_cast<T *>(grad_w) + v0 * C : nullptr;
+            d.sums = grad_x ? reinterpret_cast<float *>(ws + p.sums) : nullptr;
+            d.c4 = p.c4; d.add = v0 > 0;
+            ce_few<T>(d, st);
+            continue;
+        }
         if (grad_x) {
             CeRows table = {};
             table.n = count;
@@ -769,7 +934,10 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             product(d);
         }
     }
-    if (grad_x)
+    if (grad_x && p.few)
+        hipLaunchKernelGGL((ce_few_finish_kernel<T>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 16)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
+                           p.parts, (int)n, C, p.c4, factors, factor, static_cast<T *>(grad_x));
+    else if (grad_x)
         hipLaunchKernelGGL((ce_finish_kernel<T>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
                            p.parts, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));
     return check_launch("mvs_linear_ce_bwd");

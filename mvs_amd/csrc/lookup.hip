@@ -7,14 +7,15 @@
 // Backward: every row of the dense gradient is written once, most of them as zeros, and every row of g is read once.  Who adds to a
 // row is known only after the indices are sorted.  The sort is stable, so a row's terms come in the order of i and equal calls
 // give equal bits; floating-point atomics on the rows would need neither sort nor order, but sum in another order every time.
-//   sort   up to kRankMax indices: a term's place is the number of smaller keys, plus that of equal keys in front of it -- one
-//          launch, n^2 / 2^14 cycles on the chip; more: least-significant-digit radix sort of (key, i), digits of up to 10 bits,
-//          three launches each (count per tile, one workgroup's scan, place).
+//   sort   up to kRankMax indices: the place of term i is the number of (key, i) below its own -- one launch, n^2 comparisons of two
+//          instructions; more: least-significant-digit radix sort, digits of up to 10 bits, three launches each (count per tile, one
+//          workgroup's scan, place).
 //   rows   the sorted terms are cut into pieces of kPiece; a piece's lanes walk it with the loads of 8 terms in flight and write
 //          the sum of each run of equal keys that lies within the piece.  A run that leaves the piece (a frequent index) leaves
 //          float32 partial sums, at most two per piece.  The same launch writes the zero rows (found by binary search, 64 table
 //          rows per wave's worth of lanes).
-//   join   the pieces of a long run, in order, four spans of them at a time.
+//   join   the partial sums of the runs that leave their piece, in order: short runs a wave each, long ones four spans of pieces at
+//          a time.  A run's end is found 64 pieces per look.
 #include <utility>
 
 #include "dtype.h"
@@ -23,12 +24,13 @@ namespace mvs {
 
 constexpr int kRankMax = 8192;
 constexpr int kPiece = 16;         // sorted terms per piece
-constexpr int kTile = 4096;        // keys per workgroup of a radix pass
+constexpr int kJoin = 16;          // pieces that a workgroup of the join looks at
 constexpr int kMaxDigit = 10;
 
 struct LookupPlan {
     int64_t n, rows;
     int key_bits, passes, digit_bits;
+    int tile;                     // keys per workgroup of a radix pass: small while that fills the chip, large before the scan of the counts is long
     int64_t tiles, pieces;
     size_t keys0, vals0, keys1, vals1, hist, part, total;      // byte offsets into the workspace
 };
@@ -39,7 +41,8 @@ static LookupPlan lookup_plan(int64_t rows, int C, int64_t n) {
     while (p.key_bits < 32 && ((int64_t)1 << p.key_bits) <= rows) ++p.key_bits;      // keys 0 .. rows (rows: names no row)
     p.passes = n <= kRankMax ? 0 : (p.key_bits + kMaxDigit - 1) / kMaxDigit;
     p.digit_bits = p.passes ? (p.key_bits + p.passes - 1) / p.passes : 0;
-    p.tiles = (n + kTile - 1) / kTile;
+    p.tile = n <= 131072 ? 1024 : 4096;
+    p.tiles = (n + p.tile - 1) / p.tile;
     p.pieces = (n + kPiece - 1) / kPiece;
     auto align = [](size_t b) { return (b + 255) & ~(size_t)255; };
     size_t at = 0;
@@ -67,47 +70,50 @@ __global__ __launch_bounds__(256) void lookup_fwd_kernel(const T *__restrict__ t
     const bool named = row >= 0 && row < rows;
     const Pack<T, VEC> *from = reinterpret_cast<const Pack<T, VEC> *>(table + (named ? row : 0) * C);
     Pack<T, VEC> *to = reinterpret_cast<Pack<T, VEC> *>(out + i * C);
-    for (int c = lane; c < vecs; c += lanes) {
-        Pack<T, VEC> v;
-        if (named) v = from[c];
+    for (int c0 = lane; c0 < vecs; c0 += 4 * lanes) {
+        Pack<T, VEC> v[4];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v.v[j] = from_float<T>(named ? to_float(v.v[j]) * scale : 0.0f);
-        to[c] = v;
+        for (int u = 0; u < 4; ++u)
+            if (named && c0 + u * lanes < vecs) v[u] = from[c0 + u * lanes];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (c0 + u * lanes >= vecs) break;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[u].v[j] = from_float<T>(named ? to_float(v[u].v[j]) * scale : 0.0f);
+            to[c0 + u * lanes] = v[u];
+        }
     }
 }
 
 // ---- sort
-// 64 terms per workgroup, four waves each against a quarter of the keys; the keys pass through LDS 1024 at a time.
-__global__ __launch_bounds__(256) void lookup_rank_kernel(const int64_t *__restrict__ index, int n, int64_t rows, unsigned *__restrict__ keys,
-                                                          unsigned *__restrict__ vals) {
-    __shared__ unsigned tile[1024];
-    __shared__ int ranks[256];
-    const int tid = threadIdx.x, i = blockIdx.x * 64 + (tid & 63), quarter = tid >> 6;
-    const unsigned mine = i < n ? lookup_key(index[i], rows) : 0u;
+// 64 terms per workgroup, each of 16 waves against a sixteenth of the keys; the keys pass through LDS 2048 at a time.
+__global__ __launch_bounds__(1024) void lookup_rank_kernel(const int64_t *__restrict__ index, int n, int64_t rows, unsigned *__restrict__ keys,
+                                                           unsigned *__restrict__ vals) {
+    __shared__ unsigned long long tile[2048];
+    __shared__ int ranks[1024];
+    const int tid = threadIdx.x, i = blockIdx.x * 64 + (tid & 63), wave = tid >> 6;
+    auto key_of = [&](int j) { return j < n ? (unsigned long long)lookup_key(index[j], rows) << 32 | (unsigned)j : ~0ull; };
+    const unsigned long long mine = key_of(i);
     int rank = 0;
-    for (int base = 0; base < n; base += 1024) {
+    for (int base = 0; base < n; base += 2048) {
         __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int j = base + u * 256 + tid;
-            tile[u * 256 + tid] = j < n ? lookup_key(index[j], rows) : 0xffffffffu;
-        }
+        tile[tid] = key_of(base + tid);
+        tile[tid + 1024] = key_of(base + tid + 1024);
         __syncthreads();
-        const uint4 *t4 = reinterpret_cast<const uint4 *>(tile + quarter * 256);
-        const int j0 = base + quarter * 256;
-#pragma unroll 8
+        const ulonglong2 *t2 = reinterpret_cast<const ulonglong2 *>(tile + wave * 128);
+#pragma unroll 16
         for (int j = 0; j < 64; ++j) {
-            const uint4 k = t4[j];      // (one address for the wave)
-            const int jj = j0 + j * 4;
-            rank += (k.x < mine || (k.x == mine && jj < i)) + (k.y < mine || (k.y == mine && jj + 1 < i)) +
-                    (k.z < mine || (k.z == mine && jj + 2 < i)) + (k.w < mine || (k.w == mine && jj + 3 < i));
+            const ulonglong2 k = t2[j];      // (one address for the wave)
+            rank += (k.x < mine) + (k.y < mine);
         }
     }
     ranks[tid] = rank;
     __syncthreads();
-    if (quarter == 0 && i < n) {
-        const int r = ranks[tid] + ranks[tid + 64] + ranks[tid + 128] + ranks[tid + 192];
-        keys[r] = mine;
+    if (wave == 0 && i < n) {
+        int r = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) r += ranks[w * 64 + tid];
+        keys[r] = (unsigned)(mine >> 32);
         vals[r] = (unsigned)i;
     }
 }
@@ -115,14 +121,14 @@ __global__ __launch_bounds__(256) void lookup_rank_kernel(const int64_t *__restr
 // counts per (digit, tile), digit-major: their exclusive scan is where a tile's keys of a digit go
 template <bool FIRST>
 __global__ __launch_bounds__(256) void lookup_count_kernel(const int64_t *__restrict__ index, const unsigned *__restrict__ keys, int64_t n,
-                                                           int64_t rows, int shift, int bits, int64_t tiles, unsigned *__restrict__ hist) {
+                                                           int64_t rows, int shift, int bits, int64_t tiles, int tile, unsigned *__restrict__ hist) {
     __shared__ unsigned count[1 << kMaxDigit];
     const int digits = 1 << bits;
     for (int d = threadIdx.x; d < digits; d += 256) count[d] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * kTile;
+    const int64_t base = (int64_t)blockIdx.x * tile;
 #pragma unroll 4
-    for (int u = 0; u < kTile / 256; ++u) {
+    for (int u = 0; u < tile / 256; ++u) {
         const int64_t i = base + u * 256 + threadIdx.x;
         if (i < n) {
             const unsigned key = FIRST ? lookup_key(index[i], rows) : keys[i];
@@ -133,33 +139,44 @@ __global__ __launch_bounds__(256) void lookup_count_kernel(const int64_t *__rest
     for (int d = threadIdx.x; d < digits; d += 256) hist[(int64_t)d * tiles + blockIdx.x] = count[d];
 }
 
-// exclusive scan of `m` counts in place, by one workgroup
+// exclusive scan of `m` counts in place, by one workgroup: a wave takes 1024 consecutive ones, 256 at a time.  (The last access of
+// four may reach behind m, not behind the 256 bytes its region is rounded up to.)
 __global__ __launch_bounds__(1024) void lookup_scan_kernel(unsigned *__restrict__ hist, int64_t m) {
     __shared__ unsigned sums[16];
     unsigned carry = 0;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t base = 0; base < m; base += 8192) {
-        const int64_t at = base + (int64_t)threadIdx.x * 8;
-        unsigned v[8], sum = 0;
+    for (int64_t base = 0; base < m; base += 16384) {
+        uint4 v[4];
+        unsigned before[4], all = 0;      // of the wave's range: what lies before this lane's four, and its sum
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { v[j] = at + j < m ? hist[at + j] : 0u; }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { const unsigned t = v[j]; v[j] = sum; sum += t; }
-        unsigned incl = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned t = (unsigned)__shfl_up((int)incl, o);
-            if (lane >= o) incl += t;
+        for (int r = 0; r < 4; ++r) {
+            const int64_t at = base + wave * 1024 + r * 256 + lane * 4;
+            v[r] = at < m ? *reinterpret_cast<const uint4 *>(hist + at) : make_uint4(0, 0, 0, 0);
         }
-        if (lane == 63) sums[wave] = incl;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const unsigned sum = v[r].x + v[r].y + v[r].z + v[r].w;
+            unsigned incl = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const unsigned t = (unsigned)__shfl_up((int)incl, o);
+                if (lane >= o) incl += t;
+            }
+            before[r] = all + incl - sum;
+            all += (unsigned)__shfl((int)incl, 63);
+        }
+        if (lane == 0) sums[wave] = all;
         __syncthreads();
-        unsigned before = carry, all = 0;
+        unsigned ahead = carry, total = 0;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) { if (w < wave) before += sums[w]; all += sums[w]; }
-        before += incl - sum;
+        for (int w = 0; w < 16; ++w) { if (w < wave) ahead += sums[w]; total += sums[w]; }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (at + j < m) hist[at + j] = before + v[j];
-        carry += all;
+        for (int r = 0; r < 4; ++r) {
+            const int64_t at = base + wave * 1024 + r * 256 + lane * 4;
+            const unsigned x = ahead + before[r], y = x + v[r].x, z = y + v[r].y, w = z + v[r].z;
+            if (at < m) *reinterpret_cast<uint4 *>(hist + at) = make_uint4(x, y, z, w);
+        }
+        carry += total;
         __syncthreads();
     }
 }
@@ -169,9 +186,9 @@ __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// Places a tile's keys: 4 waves, each 1024 consecutive keys in 16 rounds of 64.  A key's place is the tile's start of its digit,
+// Places a tile's keys: 4 waves, each a quarter of them in ROUNDS rounds of 64.  A key's place is the tile's start of its digit,
 // plus the earlier waves' count of it, plus the wave's own earlier ones, plus the lanes in front of it that hold the same digit.
-template <bool FIRST>
+template <bool FIRST, int ROUNDS>
 __global__ __launch_bounds__(256) void lookup_place_kernel(const int64_t *__restrict__ index, const unsigned *__restrict__ keys_in,
                                                            const unsigned *__restrict__ vals_in, int64_t n, int64_t rows, int shift, int bits,
                                                            int64_t tiles, const unsigned *__restrict__ hist, unsigned *__restrict__ keys_out,
@@ -183,10 +200,10 @@ __global__ __launch_bounds__(256) void lookup_place_kernel(const int64_t *__rest
         for (int w = 0; w < 4; ++w) count[w][d] = 0;
     }
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * kTile + wave * 1024;
-    unsigned key[16];
+    const int64_t base = ((int64_t)blockIdx.x * 4 + wave) * (ROUNDS * 64);
+    unsigned key[ROUNDS];
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
+    for (int u = 0; u < ROUNDS; ++u) {
         const int64_t i = base + u * 64 + lane;
         key[u] = 0;
         if (i < n) {
@@ -202,7 +219,7 @@ __global__ __launch_bounds__(256) void lookup_place_kernel(const int64_t *__rest
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
+    for (int u = 0; u < ROUNDS; ++u) {
         const int64_t i = base + u * 64 + lane;
         const bool here = i < n;
         const unsigned digit = key[u] >> shift & (digits - 1);
@@ -332,39 +349,96 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(LookupRows a) {
     }
 }
 
-// A run that begins in piece p and goes on: its partials are p's second one and the first ones of the pieces behind it that begin
-// with its key.  256 threads = 4 spans x 64 columns; 16 pieces are looked at per workgroup.
-template <typename T>
+// The partial sums of a run that begins in piece p and goes on: p's second one, and the first ones of the pieces behind it that begin
+// with its key.  A workgroup looks at kJoin pieces and owns 64 * VEC columns.
+template <typename T, int VEC>
 __global__ __launch_bounds__(256) void lookup_join_kernel(LookupRows a) {
-    __shared__ float spans[4][64];
-    const int col = blockIdx.y * 64 + (threadIdx.x & 63), span = threadIdx.x >> 6;
-    for (int64_t piece = (int64_t)blockIdx.x * 16; piece < min(a.pieces - 1, (int64_t)blockIdx.x * 16 + 16); ++piece) {
-        const int64_t p0 = piece * kPiece, end = p0 + kPiece;      // (not the last piece: it is full)
-        const unsigned key = a.keys[end - 1];
-        if (key == (unsigned)a.rows || a.keys[end] != key) continue;
-        if (a.keys[p0] == key && p0 > 0 && a.keys[p0 - 1] == key) continue;      // (begins further ahead)
-        const int64_t stop = lookup_lower(a.keys + end, a.n - end, key + 1) + end;      // first term behind the run
-        const int64_t more = (stop - end + kPiece - 1) / kPiece, each = (more + 3) / 4;
-        float sum = 0.0f;
+    __shared__ Pack<float, VEC> spans[4][64];
+    constexpr int LONG = 16;      // pieces from which the four waves share a run
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = (blockIdx.y * 64 + lane) * VEC;
+    const int64_t p0 = (int64_t)blockIdx.x * kJoin, mine = p0 + lane;
+    bool owner = lane < kJoin && mine < a.pieces - 1, longer = false;      // (the last piece goes on nowhere; the others are full)
+    unsigned my_key = 0;
+    if (owner) {
+        const int64_t first = mine * kPiece, end = first + kPiece, probe = end + (LONG - 1) * kPiece;
+        my_key = a.keys[end - 1];
+        const unsigned next = a.keys[end], head = a.keys[first], before = first > 0 ? a.keys[first - 1] : ~0u, far = probe < a.n ? a.keys[probe] : ~0u;
+        owner = my_key != (unsigned)a.rows && next == my_key && !(head == my_key && before == my_key);
+        longer = owner && far == my_key;
+    }
+    const unsigned long long owners = __ballot(owner && !longer);      // (the same in all four waves)
+    unsigned long long long_ones = __ballot(longer);
+    auto length = [&](int64_t piece, unsigned key) {          // pieces behind `piece` that begin with its last key
+        int64_t more = 0;
+        while (true) {
+            const int64_t q = piece + 1 + more + lane;
+            const unsigned long long same = __ballot(q < a.pieces && a.keys[q * kPiece] == key);
+            if (same != ~0ull) return more + __builtin_ctzll(~same);
+            more += 64;
+        }
+    };
+    auto add = [&](float (&sum)[VEC], int64_t from, int64_t to) {      // first partials of pieces [from, to)
+        for (int64_t q = from; q < to; q += 8) {
+            Pack<float, VEC> v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (q + j < to) v[j] = *reinterpret_cast<const Pack<float, VEC> *>(a.part + (q + j) * 2 * a.C + col);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (q + j < to)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) sum[e] += v[j].v[e];
+        }
+    };
+    auto write = [&](const float (&sum)[VEC], unsigned key) {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.v[e] = from_float<T>(sum[e] * a.scale);
+        *reinterpret_cast<Pack<T, VEC> *>(static_cast<T *>(a.out) + (int64_t)key * a.C + col) = o;
+    };
+    auto begin = [&](float (&sum)[VEC], int64_t piece) {
+        const Pack<float, VEC> v = *reinterpret_cast<const Pack<float, VEC> *>(a.part + (piece * 2 + 1) * a.C + col);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] = v.v[e];
+    };
+    // short runs: every fourth one a wave's
+    int turn = 0;
+    for (unsigned long long left = owners; left; left &= left - 1, ++turn) {
+        if ((turn & 3) != wave) continue;
+        const int at = __builtin_ctzll(left);
+        const int64_t piece = p0 + at;
+        const unsigned key = (unsigned)__shfl((int)my_key, at);
+        const int64_t more = length(piece, key);
         if (col < a.C) {
-            if (span == 0) sum = a.part[(piece * 2 + 1) * a.C + col];
-            const int64_t from = piece + 1 + span * each, to = min(piece + 1 + more, from + each);
-            int64_t q = from;
-            for (; q + 8 <= to; q += 8) {
-                float v[8];
+            float sum[VEC];
+            begin(sum, piece);
+            add(sum, piece + 1, piece + 1 + more);
+            write(sum, key);
+        }
+    }
+    for (; long_ones; long_ones &= long_ones - 1) {
+        const int at = __builtin_ctzll(long_ones);
+        const int64_t piece = p0 + at;
+        const unsigned key = (unsigned)__shfl((int)my_key, at);
+        const int64_t more = length(piece, key), each = (more + 3) / 4;
+        float sum[VEC];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = a.part[(q + j) * 2 * a.C + col];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum += v[j];
-            }
-            for (; q < to; ++q) sum += a.part[q * 2 * a.C + col];
+        for (int e = 0; e < VEC; ++e) sum[e] = 0.0f;
+        if (col < a.C) {
+            if (wave == 0) begin(sum, piece);
+            const int64_t from = piece + 1 + wave * each;
+            add(sum, from, min(piece + 1 + more, from + each));
         }
         __syncthreads();
-        spans[span][threadIdx.x & 63] = sum;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) spans[wave][lane].v[e] = sum[e];
         __syncthreads();
-        if (span == 0 && col < a.C) {
-            const int t = threadIdx.x;
-            static_cast<T *>(a.out)[(int64_t)key * a.C + col] = from_float<T>((((spans[0][t] + spans[1][t]) + spans[2][t]) + spans[3][t]) * a.scale);
+        if (wave == 0 && col < a.C) {
+#pragma unroll
+            for (int w = 1; w < 4; ++w)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sum[e] += spans[w][lane].v[e];
+            write(sum, key);
         }
     }
 }
@@ -391,7 +465,7 @@ static bool lookup_wide(const void *a, const void *b, int dtype, int C) { return
 
 template <typename T, int VEC>
 static void lookup_launch_fwd(const void *table, int64_t rows, int C, const int64_t *index, int64_t n, float scale, void *out, hipStream_t st) {
-    const int lanes = lookup_lanes(C / VEC);
+    const int lanes = min(64, lookup_lanes(C / VEC));      // (four accesses of a long row in flight per lane)
     hipLaunchKernelGGL((lookup_fwd_kernel<T, VEC>), dim3((unsigned)((n * lanes + 255) / 256)), dim3(256), 0, st, static_cast<const T *>(table), rows, C, index,
                        n, scale, static_cast<T *>(out), lanes);
 }
@@ -402,8 +476,10 @@ static void lookup_launch_rows(LookupRows a, hipStream_t st) {
     a.sum_groups = (a.pieces * a.lanes + 255) / 256;
     const int64_t zero_groups = (a.rows + 63) / 64;
     hipLaunchKernelGGL((lookup_rows_kernel<T, VEC>), dim3((unsigned)(a.sum_groups + zero_groups)), dim3(256), 0, st, a);
-    if (a.pieces > 1)
-        hipLaunchKernelGGL((lookup_join_kernel<T>), dim3((unsigned)((a.pieces + 15) / 16), (unsigned)((a.C + 63) / 64)), dim3(256), 0, st, a);
+    if (a.pieces > 1) {
+        constexpr int JOIN = VEC == 1 ? 1 : 4;      // (rows of whole 16 bytes are whole float4 of sums)
+        hipLaunchKernelGGL((lookup_join_kernel<T, JOIN>), dim3((unsigned)((a.pieces + kJoin - 1) / kJoin), (unsigned)((a.C + 64 * JOIN - 1) / (64 * JOIN))), dim3(256), 0, st, a);
+    }
 }
 
 }  // namespace mvs
@@ -442,22 +518,28 @@ extern "C" int mvs_lookup_rows_bwd(const void *grad_out, int dtype, const int64_
     char *ws = static_cast<char *>(workspace);
     unsigned *keys = reinterpret_cast<unsigned *>(ws + p.keys0), *vals = reinterpret_cast<unsigned *>(ws + p.vals0);
     if (n > 0 && p.passes == 0) {
-        hipLaunchKernelGGL(lookup_rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, index, (int)n, rows, keys, vals);
+        hipLaunchKernelGGL(lookup_rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st, index, (int)n, rows, keys, vals);
     } else if (n > 0) {
         unsigned *keys_to = reinterpret_cast<unsigned *>(ws + p.keys1), *vals_to = reinterpret_cast<unsigned *>(ws + p.vals1);
         unsigned *hist = reinterpret_cast<unsigned *>(ws + p.hist);
+        auto count = [&](auto kernel, int shift, int bits) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)p.tiles), dim3(256), 0, st, index, keys, n, rows, shift, bits, p.tiles, p.tile, hist);
+            hipLaunchKernelGGL(lookup_scan_kernel, dim3(1), dim3(1024), 0, st, hist, p.tiles << bits);
+        };
+        auto place = [&](auto kernel, int shift, int bits) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)p.tiles), dim3(256), 0, st, index, keys, vals, n, rows, shift, bits, p.tiles, hist, keys_to, vals_to);
+        };
         for (int pass = 0; pass < p.passes; ++pass) {
             const int shift = pass * p.digit_bits, bits = min(p.digit_bits, p.key_bits - shift);
-            const dim3 grid((unsigned)p.tiles), block(256);
-            const int64_t m = p.tiles << bits;
+            const bool small = p.tile == 1024;
             if (pass == 0) {
-                hipLaunchKernelGGL((lookup_count_kernel<true>), grid, block, 0, st, index, keys, n, rows, shift, bits, p.tiles, hist);
-                hipLaunchKernelGGL(lookup_scan_kernel, dim3(1), dim3(1024), 0, st, hist, m);
-                hipLaunchKernelGGL((lookup_place_kernel<true>), grid, block, 0, st, index, keys, vals, n, rows, shift, bits, p.tiles, hist, keys_to, vals_to);
+                count(lookup_count_kernel<true>, shift, bits);
+                if (small) place(lookup_place_kernel<true, 4>, shift, bits);
+                else place(lookup_place_kernel<true, 16>, shift, bits);
             } else {
-                hipLaunchKernelGGL((lookup_count_kernel<false>), grid, block, 0, st, index, keys, n, rows, shift, bits, p.tiles, hist);
-                hipLaunchKernelGGL(lookup_scan_kernel, dim3(1), dim3(1024), 0, st, hist, m);
-                hipLaunchKernelGGL((lookup_place_kernel<false>), grid, block, 0, st, index, keys, vals, n, rows, shift, bits, p.tiles, hist, keys_to, vals_to);
+                count(lookup_count_kernel<false>, shift, bits);
+                if (small) place(lookup_place_kernel<false, 4>, shift, bits);
+                else place(lookup_place_kernel<false, 16>, shift, bits);
             }
             std::swap(keys, keys_to);
             std::swap(vals, vals_to);

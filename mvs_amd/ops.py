@@ -1857,39 +1857,48 @@ class _BnReluAct8CL(torch.autograd.Function):
         nbytes = lib.mvs_bn_train_workspace_bytes(C)
         if nbytes == 0 or weight.numel() != C:
             raise MvsHipError(f"bn_relu_cl: C={C} not supported by a BatchNorm of {weight.numel()} channels")
-        ws = torch.empty((nbytes // 4,), device=x.device, dtype=torch.float32)
+        ws = torch.empty((nbytes,), device=x.device, dtype=torch.uint8)
         w, b = _aligned16(_f32c(weight.detach())), _aligned16(_f32c(bias.detach()))
         sk = _aligned16(_f32c(skip)) if skip is not None else None
-        mean = torch.empty((groups, C), device=x.device, dtype=torch.float32)
-        invstd = torch.empty_like(mean)
+        stats = torch.empty((2, groups, C), device=x.device, dtype=torch.float32)      # mean, 1 / standard deviation
         y = torch.empty_like(x)
-        held = Act8.empty_for(x)
-        mask = torch.empty(held.scales.shape, device=x.device, dtype=torch.int32) if relu else None
-        at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        # codes, scales and mask in one tensor (a small layer's call is as long as its allocations)
+        scales_at, mask_at, size = _BnReluAct8CL._layout(x.numel(), relu)
+        held = torch.empty((size,), device=x.device, dtype=torch.uint8)
+        at, hp, sp = lambda t: None if t is None else t.data_ptr(), held.data_ptr(), stats.data_ptr()  # noqa: E731
         check(lib.mvs_bn_train_fwd_act8_f32(at(x), at(w), at(b), at(sk), int(groups), N, C, float(eps), float(momentum), int(relu),
-                                            ptr(running_mean), ptr(running_var), at(nbt), at(mean), at(invstd), at(y), at(held.codes),
-                                            at(held.scales), at(mask), at(ws), nbytes, st), "mvs_bn_train_fwd_act8_f32")
-        ctx.save_for_backward(held.codes, held.scales, mask, w, mean, invstd)
-        ctx.has_skip, ctx.groups = skip is not None, int(groups)
+                                            ptr(running_mean), ptr(running_var), at(nbt), sp, sp + 4 * groups * C, at(y), hp, hp + scales_at,
+                                            hp + mask_at if relu else None, at(ws), nbytes, st), "mvs_bn_train_fwd_act8_f32")
+        ctx.save_for_backward(held, w, stats)
+        ctx.has_skip, ctx.groups, ctx.relu = skip is not None, int(groups), bool(relu)
         ctx.mark_non_differentiable(*[t for t in (running_mean, running_var, nbt) if t is not None])
         return y
 
     @staticmethod
+    def _layout(n, relu):
+        """Byte offsets of the scales and the mask behind the n codes, and the size of all."""
+        up = lambda v: (v + 15) & ~15  # noqa: E731
+        blocks = (n + ACT8_BLOCK - 1) // ACT8_BLOCK
+        return up(n), up(n) + up(blocks), up(n) + up(blocks) + (4 * blocks if relu else 0)
+
+    @staticmethod
     @_first_order
     def backward(ctx, gy):
-        codes, scales, mask, w, mean, invstd = ctx.saved_tensors
-        st = _here("bn_relu_cl", gy, codes)
+        held, w, stats = ctx.saved_tensors
+        st = _here("bn_relu_cl", gy, held)
         gy = _aligned16(_f32c(gy))
         C = gy.shape[-1]
         N = gy.numel() // C // ctx.groups
         lib = _lib.load()
         nbytes = lib.mvs_bn_train_workspace_bytes(C)
-        ws = torch.empty((nbytes // 4,), device=gy.device, dtype=torch.float32)
+        ws = torch.empty((nbytes,), device=gy.device, dtype=torch.uint8)
         gx = torch.empty_like(gy)
         gw, gb = torch.empty_like(w), torch.empty_like(w)
-        check(lib.mvs_bn_train_bwd_act8_f32(gy.data_ptr(), codes.data_ptr(), scales.data_ptr(), None if mask is None else mask.data_ptr(), w.data_ptr(),
-                                            mean.data_ptr(), invstd.data_ptr(), ctx.groups, N, C, gx.data_ptr(), gw.data_ptr(), gb.data_ptr(),
-                                            ws.data_ptr(), nbytes, st), "mvs_bn_train_bwd_act8_f32")
+        scales_at, mask_at, _ = _BnReluAct8CL._layout(gy.numel(), ctx.relu)
+        hp, sp = held.data_ptr(), stats.data_ptr()
+        check(lib.mvs_bn_train_bwd_act8_f32(gy.data_ptr(), hp, hp + scales_at, hp + mask_at if ctx.relu else None, w.data_ptr(), sp, sp + 4 * ctx.groups * C,
+                                            ctx.groups, N, C, gx.data_ptr(), gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), nbytes, st),
+              "mvs_bn_train_bwd_act8_f32")
         return gx, gw, gb, (gy if ctx.has_skip else None), None, None, None, None, None, None, None
 
 

@@ -509,3 +509,14 @@ def test_linear_cross_entropy_kept_rows_anywhere(n, V, C, dtype, kept):
     x[~keep] = float("nan")
     ce_check(x, w, t, 1.5, reduction="mean")
     ce_check(x, w, t, 1.5, reduction="none")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,C", [(1, 40, 129), (2, 63, 257), (3, 64, 512), (4, 65, 1000), (5, 700, 130), (8, 1000, 2048), (9, 129, 2056), (15, 3000, 300),
+                                   (16, 200, 4100), (17, 200, 300), (1, 20000, 1024)])
+def test_linear_cross_entropy_few_rows(n, V, C, dtype):
+    """One row to a few (and one more): both gradients in one pass over the table."""
+    x, w, t, _ = ce_case(n, V, C, dtype, ignored=0.3 if n > 1 else 0.0, seed=13)
+    x[t == -100] = float("nan")
+    ce_check(x, w, t, 1.0)
+    ce_check(x, w, t, 1.0, reduction="none")
