@@ -23,6 +23,20 @@ __device__ __forceinline__ bf16_t from_float<bf16_t>(float x) {
 template <>
 __device__ __forceinline__ f16_t from_float<f16_t>(float x) { return f16_t{(_Float16)x}; }
 
+// two values as one 32-bit word of two 16-bit elements (one instruction), and back
+__device__ __forceinline__ unsigned pack2(float a, float b, bf16_t) {
+    typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+    const pair_t p = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(unsigned, p);
+}
+__device__ __forceinline__ unsigned pack2(float a, float b, f16_t) {
+    typedef _Float16 pair_t __attribute__((ext_vector_type(2)));
+    const pair_t p = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(unsigned, p);
+}
+__device__ __forceinline__ float low_of(unsigned p, bf16_t) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float high_of(unsigned p, bf16_t) { return __uint_as_float(p & 0xffff0000u); }
+
 // largest finite value of a type
 template <typename T> struct DtypeMax;
 template <> struct DtypeMax<float> { static constexpr float value = 3.4028234663852886e38f; };

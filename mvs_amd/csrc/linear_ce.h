@@ -26,8 +26,8 @@ __device__ __forceinline__ void mma16(f32x4_t &c, u32x4_t a, u32x4_t b, f16_t) {
 }
 
 // dl is carried times this
-template <typename T> struct GradUnit { static constexpr float value = 1.0f; };
-template <> struct GradUnit<f16_t> { static constexpr float value = 16384.0f; };
+template <typename T> struct GradUnit { static constexpr float value = 1.0f, log2 = 0.0f; };
+template <> struct GradUnit<f16_t> { static constexpr float value = 16384.0f, log2 = 14.0f; };
 
 // One operand of a product: rows of `ld` bytes, the last of them `rows - 1` (a tile's rows beyond it read that one again)
 struct Operand {
@@ -54,8 +54,9 @@ struct CeRows {
 __device__ __forceinline__ int64_t ce_count(const CeRows &r) { return r.count ? *r.count : r.n; }
 __device__ __forceinline__ int64_t ce_original(const CeRows &r, int64_t i) { return r.map ? r.map[i] : i; }
 
-// g of the rows `first`, `first` + `step`, ... and their ratios to the largest magnitude: factors[i], factors[n + i], factors[2 n].
-// With one factor for all rows the ratio is 1; else one workgroup looks for the largest first.  `tops`: a word of LDS per wave.
+// g of the rows `first`, `first` + `step`, ... and their ratios to one number, which is the last: factors[i], factors[n + i],
+// factors[2 n].  One factor for all rows is that number, the ratios are 1; else it is the largest magnitude, which one workgroup
+// looks for first.  `tops`: a word of LDS per wave.
 __device__ __forceinline__ void ce_factors(const CeRows &rows, const float *__restrict__ grad_loss, const float *__restrict__ kept, int reduction,
                                            float *__restrict__ factors, int64_t first, int64_t step, float *tops) {
     const int64_t count = ce_count(rows);
@@ -65,9 +66,9 @@ __device__ __forceinline__ void ce_factors(const CeRows &rows, const float *__re
         for (int64_t i = first; i < count; i += step) {
             const bool here = ce_kept(rows.target[i], rows.ignore) && common != 0.0f;
             factors[i] = here ? common : 0.0f;
-            factors[rows.n + i] = here ? common / __builtin_fabsf(common) : 0.0f;
+            factors[rows.n + i] = here ? common / common : 0.0f;      // (1; NaN where it is not a number to divide by)
         }
-        top = __builtin_fabsf(common);
+        top = common;
     } else {
         auto factor = [&](int64_t i) { return ce_kept(rows.target[i], rows.ignore) ? grad_loss[ce_original(rows, i)] : 0.0f; };
         for (int64_t i = first; i < count; i += step) top = fmaxf(top, __builtin_fabsf(factor(i)));
@@ -88,17 +89,17 @@ __device__ __forceinline__ void ce_factors(const CeRows &rows, const float *__re
 // out[row][c] = f * factor * the parts' sums, in order.  PER_ROW (dx): f = g[i] of kept row i = place[row]; rows that are ignored
 // or have f = 0 are zeros, whatever their sums are.  Else (dW): f = g[0].
 template <typename T, bool PER_ROW>
-__device__ __forceinline__ void ce_finish(const float *__restrict__ sums, int parts, int64_t rows, const int *__restrict__ place, int C, int64_t ld,
+__device__ __forceinline__ void ce_finish(const float *__restrict__ sums, int64_t parts, int64_t rows, int64_t sum_rows, const int *__restrict__ place, int C, int64_t ld,
                                           const float *__restrict__ g, float factor, T *__restrict__ out, int64_t block) {
     const int64_t quads = ld >> 2, i = block * 256 + threadIdx.x, row = i / quads, quad = i - row * quads, c = quad * 4;
     if (row >= rows) return;
-    const int64_t at = PER_ROW && place ? place[row] : row, step = rows * quads;
+    const int64_t at = PER_ROW && place ? place[row] : row, step = sum_rows * quads;
     const float f = !PER_ROW ? g[0] : at >= 0 ? g[at] : 0.0f;
     f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
     if (!PER_ROW || f != 0.0f) {
         const f32x4_t *from = reinterpret_cast<const f32x4_t *>(sums) + at * quads + quad;
         s = from[0];
-        int p = 1;
+        int64_t p = 1;
         for (; p + 8 <= parts; p += 8) {
             f32x4_t v[8];
 #pragma unroll
@@ -124,6 +125,36 @@ inline int ce_planes(int dtype) { return dtype == MVS_DTYPE_F32 ? 3 : 1; }
 // whether rows of C elements are narrow
 inline bool ce_narrow(int C, int dtype) { return C <= (dtype == MVS_DTYPE_F32 ? 64 : 128); }
 
+// How the work is cut: a workgroup owns kNarrowRows fixed rows and a part of the moving ones, in stages of 64.  `slots` is a number of
+// workgroups that fills whole rounds of the chip (256 CUs x 3); every workgroup gets the same number of stages, four at least, so
+// that they need at most `slots` (and one more per block of fixed rows).  Worked out alike on the host, which does not know how many
+// rows are kept, and on the device.
+struct NarrowSplit {
+    int64_t blocks_x, blocks_w;       // blocks of fixed rows of x (the table moves), of the table (x moves); 0: not wanted
+    int64_t parts_x, parts_w;
+    int64_t per_x, per_w;             // moving rows per part
+};
+constexpr int64_t kNarrowStatsSlots = 2 * 768, kNarrowGradSlots = 4 * 768;
+__host__ __device__ inline NarrowSplit narrow_split(int64_t count, int64_t V, int64_t slots, bool of_x, bool of_table) {
+    NarrowSplit s = {};
+    const int64_t stages_v = (V + 63) / 64, stages_n = (count + 63) / 64;
+    s.blocks_x = of_x ? (count + kNarrowRows - 1) / kNarrowRows : 0;
+    s.blocks_w = of_table ? (V + kNarrowRows - 1) / kNarrowRows : 0;
+    const int64_t share = (s.blocks_x * stages_v + s.blocks_w * stages_n + slots - 1) / slots, least = share > 4 ? share : 4;
+    const int64_t x = stages_v / least > 1 ? (stages_v + stages_v / least - 1) / (stages_v / least) : stages_v;      // stages per part
+    const int64_t w = stages_n / least > 1 ? (stages_n + stages_n / least - 1) / (stages_n / least) : stages_n;
+    s.per_x = x * 64;
+    s.per_w = w * 64;
+    s.parts_x = (stages_v + x - 1) / x;
+    s.parts_w = w > 0 ? (stages_n + w - 1) / w : 1;
+    return s;
+}
+// workgroups, or parts times blocks, that any number of kept rows up to n can come to
+inline int64_t narrow_most(int64_t blocks, int64_t moving, int64_t slots) {
+    const int64_t stages = (moving + 63) / 64, whole = blocks * (stages / 4 > 1 ? stages / 4 : 1);
+    return whole < slots + blocks ? whole : slots + blocks;
+}
+
 struct NarrowOperand {
     const void *source;               // [count][C] as the caller has it
     char *rows;                       // [count][planes][Cp] 16-bit pieces (one plane and C == Cp: `source`)
@@ -135,19 +166,17 @@ struct NarrowOperand {
 struct NarrowArgs {
     NarrowOperand x, w;
     int C, Cp, planes;
-    int64_t per_x;                    // table rows per part where the rows of x are fixed
-    int parts_x, parts_w;             // parts of the table; of the kept rows of x where the table's are fixed
     float scale2;                     // scale * log2 e
     CeRows kept_rows;
     // forward
-    float2 *part;                     // [part][n]
+    float2 *part;                     // [part][kept row]
     float *own;
     // backward
     const float *lse2;
     const float *grad_loss, *kept;
     int reduction;
-    float *factors;                   // [n] g, [n] g / max|g|, [1] max|g|
-    float *sums_x, *sums_w;           // [part][rows][ld_sums]; NULL: that gradient is not wanted
+    float *factors;                   // ce_factors
+    float *sums_x, *sums_w;           // [part][kept row / table row][ld_sums]; NULL: that gradient is not wanted
     int64_t ld_sums;
     float factor;                     // scale over the unit that dl is carried in
     void *grad_x, *grad_w;

@@ -207,10 +207,11 @@ __global__ __launch_bounds__(X::THREADS) void ce_stats_kernel(CeArgs a) {
     }
 }
 
-// Joins a row's tiles: 16 rows x 16 tiles at a time per workgroup.
+// Joins a row's tiles (`tiles` == 0: the narrow kernels' parts): 16 rows x 16 tiles at a time per workgroup.
 __global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__ part, int64_t tiles, int64_t v_total, CeRows rows,
                                                       const float *__restrict__ own, float *__restrict__ lse2, float *__restrict__ loss) {
-    const int64_t n = ce_count(rows);
+    const int64_t n = ce_count(rows), ld = tiles ? rows.n : n;
+    if (!tiles) tiles = narrow_split(n, v_total, kNarrowStatsSlots, true, false).parts_x;
     __shared__ float2 s[256];
     const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
     float2 r = make_float2(-INFINITY, 0.0f);
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__
         return make_float2(top, p.y * __builtin_amdgcn_exp2f(p.x - base) + q.y * __builtin_amdgcn_exp2f(q.x - base));
     };
     if (row < n)
-        for (int64_t t = threadIdx.x >> 4; t < tiles; t += 16) r = join(r, part[t * rows.n + row]);
+        for (int64_t t = threadIdx.x >> 4; t < tiles; t += 16) r = join(r, part[t * ld + row]);
     s[threadIdx.x] = r;
     __syncthreads();
     if (threadIdx.x < 16 && row < n) {
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void ce_finish_kernel(const float *sums, int parts, CeRows rows, int C, int64_t ld, const float *g, float factor, T *out) {
-    ce_finish<T, true>(sums, parts, rows.n, rows.place, C, ld, g, factor, out, blockIdx.x);
+    ce_finish<T, true>(sums, parts, rows.n, rows.n, rows.place, C, ld, g, factor, out, blockIdx.x);
 }
 
 // Moves the kept rows together (CeRows), by one workgroup: 16 waves count their sixteenth of the targets, then number its kept rows.
@@ -604,12 +605,10 @@ struct CePlan {
     size_t xp, wp;                   // byte offsets: those copies
     size_t map, place, targets, count;
     size_t part, own, rows;          // forward
-    int64_t tiles;                   // statistics per row
+    int64_t tiles;                   // (wide) statistics per row
     // backward
     int64_t piece, np;               // table rows per piece; n padded to 128 bytes of dl^T
     int parts;                       // of k in dx's product
-    int64_t per_x;                   // narrow: rows of the table per part
-    int parts_x, parts_w;
     size_t factors, dl, dlt, wt, xt, sums, sums_w;
     size_t total;
 };
@@ -651,32 +650,21 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
     const size_t row = (size_t)p.Cp * (p.narrow ? 2 * planes : p.es);
     if (p.copy_x) p.xp = take((size_t)n * row);
     if (p.pad) p.wp = take((size_t)V * row);
-    if (p.narrow && n > 0) {
-        // parts of the rows that are walked: enough workgroups for the chip's 256 CUs four times over, at least 256 rows each
-        auto split = [](int64_t fixed, int64_t moving, int64_t &per, int &parts) {
-            const int64_t want = ceil_div(1024, ceil_div(fixed, kNarrowRows));
-            per = round_up(ceil_div(moving, want), 64);
-            if (per < 256) per = 256;
-            parts = (int)ceil_div(moving, per);
-        };
-        int64_t per_w;
-        split(n, V, p.per_x, p.parts_x);
-        split(V, n, per_w, p.parts_w);
-    }
+    const int64_t blocks_x = ceil_div(n, kNarrowRows), blocks_w = ceil_div(V, kNarrowRows);
     if (!backward) {
-        p.tiles = p.narrow ? p.parts_x : ceil_div(V, ce_big(V, n, p.es) ? 256 : 128);
-        p.part = take((size_t)p.tiles * n * sizeof(float2));
+        p.tiles = p.narrow ? 0 : ceil_div(V, ce_big(V, n, p.es) ? 256 : 128);
+        p.part = take((p.narrow ? (size_t)narrow_most(blocks_x, V, kNarrowStatsSlots) * kNarrowRows : (size_t)p.tiles * n) * sizeof(float2));
         p.own = take((size_t)n * 4);
         p.rows = take((size_t)n * 4);
     } else if (p.narrow) {
         p.factors = take((size_t)(2 * n + 1) * 4);
         if (need_x) {
             p.wt = take((size_t)C * planes * round_up(V, 64) * 2);
-            p.sums = take((size_t)p.parts_x * n * p.c4 * 4);
+            p.sums = take((size_t)narrow_most(blocks_x, V, kNarrowGradSlots) * kNarrowRows * p.c4 * 4);
         }
         if (need_w) {
             p.xt = take((size_t)C * planes * round_up(n, 64) * 2);
-            p.sums_w = take((size_t)p.parts_w * V * p.c4 * 4);
+            p.sums_w = take((size_t)narrow_most(blocks_w, n, kNarrowGradSlots) * kNarrowRows * p.c4 * 4);
         }
     } else {
         // the piece: dl of at most 2^26 values, whole tiles
@@ -726,7 +714,6 @@ static NarrowArgs ce_narrow_args(const CePlan &p, int dtype, const void *x, cons
     a.x = NarrowOperand{x, p.copy_x ? ws + p.xp : const_cast<char *>(static_cast<const char *>(x)), nullptr, rows.n, round_up(rows.n, 64), p.copy_x};
     a.w = NarrowOperand{w, p.pad ? ws + p.wp : const_cast<char *>(static_cast<const char *>(w)), nullptr, V, round_up(V, 64), p.pad};
     a.C = C; a.Cp = p.Cp; a.planes = ce_planes(dtype);
-    a.per_x = p.per_x; a.parts_x = p.parts_x; a.parts_w = p.parts_w;
     a.scale2 = scale * kLog2e; a.kept_rows = rows; a.ld_sums = p.c4;
     return a;
 }

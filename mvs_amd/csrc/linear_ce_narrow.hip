@@ -124,11 +124,14 @@ __device__ __forceinline__ void narrow_pieces(const f32x4_t &lo, const f32x4_t &
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         float v0 = w < 2 ? lo[w * 2] : hi[w * 2 - 4], v1 = w < 2 ? lo[w * 2 + 1] : hi[w * 2 - 3];
-#pragma unroll
-        for (int q = 0; q < PL; ++q) {
-            const Pack<E, 2> p{{from_float<E>(v0), from_float<E>(v1)}};
-            d[q][w] = __builtin_bit_cast(unsigned, p);
-            if (q + 1 < PL) { v0 -= to_float(p.v[0]); v1 -= to_float(p.v[1]); }
+        d[0][w] = pack2(v0, v1, E());
+        if constexpr (PL == 3) {
+            v0 -= low_of(d[0][w], E());
+            v1 -= high_of(d[0][w], E());
+            d[1][w] = pack2(v0, v1, E());
+            v0 -= low_of(d[1][w], E());
+            v1 -= high_of(d[1][w], E());
+            d[2][w] = pack2(v0, v1, E());
         }
     }
 }
@@ -137,11 +140,13 @@ template <typename X>
 __global__ __launch_bounds__(256) void narrow_stats_kernel(NarrowArgs a) {
     __shared__ __align__(1024) char lds[2][X::ROWS_B];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, lane_at = narrow_lane();
-    const int64_t n0 = (int64_t)blockIdx.x * kNarrowRows + wave * 32, m_begin = (int64_t)blockIdx.y * a.per_x;
-    const int rows = (int)min(a.per_x, a.w.count - m_begin);
     NarrowOperand x = a.x;
     x.count = ce_count(a.kept_rows);
-    if ((int64_t)blockIdx.x * kNarrowRows >= x.count) return;
+    const NarrowSplit split = narrow_split(x.count, a.w.count, kNarrowStatsSlots, true, false);
+    if (blockIdx.x >= split.blocks_x * split.parts_x) return;
+    const int64_t block = blockIdx.x % split.blocks_x, part = blockIdx.x / split.blocks_x;
+    const int64_t n0 = block * kNarrowRows + wave * 32, m_begin = part * split.per_x;
+    const int rows = (int)min(split.per_x, a.w.count - m_begin);
     const int64_t *targets = a.kept_rows.target;
     const unsigned base_lds = (unsigned)(uintptr_t)&lds[0][0];
     narrow_copy_rows<X>(a.w, a.Cp, m_begin, base_lds);
@@ -211,25 +216,23 @@ __global__ __launch_bounds__(256) void narrow_stats_kernel(NarrowArgs a) {
         r += __shfl_xor(r, 16);
         r += __shfl_xor(r, 32);
         const int64_t n = n0 + j * 16 + ln;
-        if (lane < 16 && n < x.count) a.part[(int64_t)blockIdx.y * a.x.count + n] = make_float2(t, r);
+        if (lane < 16 && n < x.count) a.part[part * x.count + n] = make_float2(t, r);
     }
 }
 
 // statistics of a stage's moving rows (of_table), in LDS
 struct NarrowRows {
-    float lse[2][64], ratio[2][64];
+    float lse[2][64], ratio[2][64];      // (lse: less the logarithm of the unit that dl is carried in)
     int target[2][64];
 };
 
 // OF_TABLE: fixed = table rows, moving = rows of x (statistics along m); else fixed = rows of x, moving = table rows
 template <typename X, bool OF_TABLE>
-__device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOperand &fix, const NarrowOperand &mov, int64_t block, int64_t part, float unit,
+__device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOperand &fix, const NarrowOperand &mov, int64_t block, int64_t part, int64_t per, float unit, float log_unit,
                                             char *lds, NarrowRows &row_stats) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, group = lane >> 4, lane_at = narrow_lane();
-    // (the kept rows are split evenly over the parts, in whole stages; a part may get none and then writes zeros)
-    const int64_t per = OF_TABLE ? (mov.count + a.parts_w * 64 - 1) / (a.parts_w * 64) * 64 : a.per_x;
     const int64_t n0 = block * kNarrowRows + wave * 32, m_begin = part * per;
-    const int rows = (int)max((int64_t)0, min(per, mov.count - m_begin));
+    const int rows = (int)min(per, mov.count - m_begin);      // (0: no row is kept; dW's sums are then zeros)
     const int64_t *targets = a.kept_rows.target, ignore = a.kept_rows.ignore;
     const unsigned base_lds = (unsigned)(uintptr_t)lds;
     auto copy = [&](int m, int stage) {
@@ -243,8 +246,8 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
     auto stats = [&](int m) {      // thread t < MR's row of the stage, loaded a stage ahead
         const int64_t row = m_begin + m + threadIdx.x;
         const bool kept = threadIdx.x < X::MR && m + (int)threadIdx.x < rows && ce_kept(targets[row], ignore);
-        lse_next = kept ? a.lse2[row] : 0.0f;
-        ratio_next = kept ? ratios[row] * unit : 0.0f;
+        lse_next = kept ? a.lse2[row] - log_unit : 0.0f;
+        ratio_next = kept ? ratios[row] : 0.0f;
         target_next = kept ? (int)(targets[row] >= 0 && targets[row] < fix.count ? targets[row] : -1) : -1;
     };
     if (rows > 0) copy(0, 0);
@@ -258,7 +261,7 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
         const bool kept = OF_TABLE || (n < fix.count && ce_kept(t, ignore));
         // (whatever an ignored row holds, its S are 0 and its exponentials those of -Inf)
         narrow_fixed<X>(fix, a.Cp, n, kept, fixed[j]);
-        lse[j] = OF_TABLE ? 0.0f : kept ? a.lse2[n] : INFINITY;
+        lse[j] = OF_TABLE ? 0.0f : kept ? a.lse2[n] - log_unit : INFINITY;
         target[j] = OF_TABLE ? (int)n : kept && t >= m_begin && t - m_begin < rows ? (int)(t - m_begin) : -1;
     }
     f32x4_t out[X::CT][2] = {};
@@ -283,20 +286,34 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
             f32x4_t s[2][2] = {};
             narrow_first<X>(tile, half * 2, lane_at, fixed, s);
             if (OF_TABLE) {
+                // what the 32 rows need beyond the exponential: nothing (factor 1 each, no target among this wave's columns), or all of it
+                const int mine = half * 32 + (lane & 31);
+                const float my_ratio = row_stats.ratio[stage][mine];
+                const bool plain = !__ballot(my_ratio != 1.0f || (unsigned)(row_stats.target[stage][mine] - (int)n0) < 32u);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int at = half * 32 + i * 16 + group * 4;
-                    const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(&row_stats.lse[stage][at]), r4 = *reinterpret_cast<const f32x4_t *>(&row_stats.ratio[stage][at]);
-                    const u32x4_t t4 = *reinterpret_cast<const u32x4_t *>(&row_stats.target[stage][at]);
+                    const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(&row_stats.lse[stage][at]);
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][r], a.scale2, -l4[r]));
-                            if ((int)t4[r] == target[j]) d -= 1.0f;
-                            s[i][j][r] = r4[r] == 0.0f ? 0.0f : d * r4[r];      // (an ignored row's S may be anything)
-                        }
+                        for (int r = 0; r < 4; ++r) s[i][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][r], a.scale2, -l4[r]));
                 }
+                if (!plain)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int at = half * 32 + i * 16 + group * 4;
+                        const f32x4_t r4 = *reinterpret_cast<const f32x4_t *>(&row_stats.ratio[stage][at]);
+                        const u32x4_t t4 = *reinterpret_cast<const u32x4_t *>(&row_stats.target[stage][at]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                float d = s[i][j][r];
+                                if ((int)t4[r] == target[j]) d -= unit;
+                                s[i][j][r] = r4[r] == 0.0f ? 0.0f : d * r4[r];      // (an ignored row's S may be anything)
+                            }
+                    }
             } else {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -309,13 +326,8 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) if (d == i * 16 + group * 4 + r) s[i][j][r] -= 1.0f;
+                            for (int r = 0; r < 4; ++r) if (d == i * 16 + group * 4 + r) s[i][j][r] -= unit;
                     }
-                    if (unit != 1.0f)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) s[i][j][r] *= unit;
                 }
                 if (mh + 32 > rows) {
 #pragma unroll
@@ -339,7 +351,6 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
         }
     }
     float *sums = OF_TABLE ? a.sums_w : a.sums_x;
-    const int64_t sum_rows = OF_TABLE ? a.w.count : a.kept_rows.n;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int64_t n = n0 + j * 16 + ln;
@@ -347,24 +358,24 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
 #pragma unroll
         for (int c = 0; c < X::CT; ++c) {
             const int col = c * 16 + group * 4;
-            if (col < a.C) *reinterpret_cast<f32x4_t *>(sums + (part * sum_rows + n) * a.ld_sums + col) = out[c][j];
+            if (col < a.C) *reinterpret_cast<f32x4_t *>(sums + (part * fix.count + n) * a.ld_sums + col) = out[c][j];
         }
     }
 }
 
 // One launch for both gradients: the workgroups of dx, then those of dW.
 template <typename X>
-__global__ __launch_bounds__(256, 2) void narrow_grad_kernel(NarrowArgs a, int64_t blocks_x, int64_t groups_x, int64_t blocks_w, float unit) {
+__global__ __launch_bounds__(256, 2) void narrow_grad_kernel(NarrowArgs a, float unit, float log_unit) {
     __shared__ __align__(1024) char lds[2 * (X::ROWS_B + X::TRANS_B)];
     __shared__ NarrowRows row_stats;
-    const int64_t id = blockIdx.x;
     NarrowOperand x = a.x;
     x.count = ce_count(a.kept_rows);
-    if (id < groups_x) {
-        if (id % blocks_x * kNarrowRows < x.count) narrow_grad<X, false>(a, x, a.w, id % blocks_x, id / blocks_x, unit, lds, row_stats);
-    } else {
-        narrow_grad<X, true>(a, a.w, x, (id - groups_x) % blocks_w, (id - groups_x) / blocks_w, unit, lds, row_stats);
-    }
+    const NarrowSplit split = narrow_split(x.count, a.w.count, kNarrowGradSlots, a.sums_x != nullptr, a.sums_w != nullptr);
+    const int64_t id = blockIdx.x, groups_x = split.blocks_x * split.parts_x, of_table = id - groups_x;
+    if (of_table < 0)
+        narrow_grad<X, false>(a, x, a.w, id % split.blocks_x, id / split.blocks_x, split.per_x, unit, log_unit, lds, row_stats);
+    else if (of_table < split.blocks_w * split.parts_w)
+        narrow_grad<X, true>(a, a.w, x, of_table % split.blocks_w, of_table / split.blocks_w, split.per_w, unit, log_unit, lds, row_stats);
 }
 
 // a value's pieces: 8 bits each, the first one cut instead of rounded where rounding would overflow
@@ -401,20 +412,27 @@ __global__ __launch_bounds__(256) void narrow_prepare_kernel(NarrowArgs a) {
     if (r0 >= count || (!o.write_rows && !o.trans)) return;
     const T *source = static_cast<const T *>(o.source);
     const int here = (int)min((int64_t)64, count - r0);
-    for (int i = tid; i < 64 * a.C; i += 256) {
-        const int r = i / a.C, c = i - r * a.C;
-        tile[r][c] = r < here ? source[(blockIdx.y ? r0 + r : ce_original(a.kept_rows, r0 + r)) * a.C + c] : from_float<T>(0.0f);
+    const int lane = tid & 31, row = tid >> 5;      // 32 columns x 8 rows at a time
+    for (int c = lane; c < a.C; c += 32) {
+        T v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int r = row + u * 8;
+            if (r < here) v[u] = source[(blockIdx.y ? r0 + r : ce_original(a.kept_rows, r0 + r)) * a.C + c];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) tile[row + u * 8][c] = row + u * 8 < here ? v[u] : from_float<T>(0.0f);
     }
     __syncthreads();
     if (o.write_rows) {
         E *rows = reinterpret_cast<E *>(o.rows);
-        for (int i = tid; i < here * a.Cp; i += 256) {
-            const int r = i / a.Cp, c = i - r * a.Cp;
-            E p[PL];
-            pieces_of<E, PL>(c < a.C ? tile[r][c] : from_float<T>(0.0f), p);
+        for (int c = lane; c < a.Cp; c += 32)
+            for (int r = row; r < here; r += 8) {
+                E p[PL];
+                pieces_of<E, PL>(c < a.C ? tile[r][c] : from_float<T>(0.0f), p);
 #pragma unroll
-            for (int q = 0; q < PL; ++q) rows[((r0 + r) * PL + q) * a.Cp + c] = p[q];
-        }
+                for (int q = 0; q < PL; ++q) rows[((r0 + r) * PL + q) * a.Cp + c] = p[q];
+            }
     }
     if (o.trans) {
         E *trans = reinterpret_cast<E *>(o.trans);
@@ -433,11 +451,13 @@ __global__ __launch_bounds__(256) void narrow_prepare_kernel(NarrowArgs a) {
 // both gradients from the parts' sums: workgroups of dx, then of dW
 template <typename T>
 __global__ __launch_bounds__(256) void narrow_finish_kernel(NarrowArgs a, int64_t groups_x) {
-    const int64_t id = blockIdx.x;
+    const int64_t id = blockIdx.x, count = ce_count(a.kept_rows);
+    const NarrowSplit split = narrow_split(count, a.w.count, kNarrowGradSlots, a.sums_x != nullptr, a.sums_w != nullptr);
     if (id < groups_x)
-        ce_finish<T, true>(a.sums_x, a.parts_x, a.x.count, a.kept_rows.place, a.C, a.ld_sums, a.factors, a.factor, static_cast<T *>(a.grad_x), id);
+        ce_finish<T, true>(a.sums_x, split.parts_x, a.x.count, count, a.kept_rows.place, a.C, a.ld_sums, a.factors, a.factor, static_cast<T *>(a.grad_x), id);
     else
-        ce_finish<T, false>(a.sums_w, a.parts_w, a.w.count, (const int *)nullptr, a.C, a.ld_sums, a.factors + 2 * a.x.count, a.factor, static_cast<T *>(a.grad_w), id - groups_x);
+        ce_finish<T, false>(a.sums_w, split.parts_w, a.w.count, a.w.count, (const int *)nullptr, a.C, a.ld_sums, a.factors + 2 * a.x.count, a.factor,
+                            static_cast<T *>(a.grad_w), id - groups_x);
 }
 
 template <typename T, typename E, int PL>
@@ -448,13 +468,14 @@ static void narrow_prepare(const NarrowArgs &a, bool backward, hipStream_t st) {
 
 template <typename X>
 static void narrow_stats(const NarrowArgs &a, hipStream_t st) {
-    hipLaunchKernelGGL((narrow_stats_kernel<X>), dim3((unsigned)ceil_div(a.x.count, kNarrowRows), (unsigned)a.parts_x), dim3(256), 0, st, a);
+    const int64_t groups = narrow_most(ceil_div(a.x.count, kNarrowRows), a.w.count, kNarrowStatsSlots);
+    hipLaunchKernelGGL((narrow_stats_kernel<X>), dim3((unsigned)groups), dim3(256), 0, st, a);
 }
-template <typename X>
-static void narrow_grads(const NarrowArgs &a, float unit, hipStream_t st) {
-    const int64_t bx = ceil_div(a.x.count, kNarrowRows), bw = ceil_div(a.w.count, kNarrowRows);
-    const int64_t gx = a.sums_x ? bx * a.parts_x : 0, gw = a.sums_w ? bw * a.parts_w : 0;
-    hipLaunchKernelGGL((narrow_grad_kernel<X>), dim3((unsigned)(gx + gw)), dim3(256), 0, st, a, bx, gx, bw, unit);
+template <typename X, typename T>
+static void narrow_grads(const NarrowArgs &a, hipStream_t st) {
+    const int64_t bx = a.sums_x ? ceil_div(a.x.count, kNarrowRows) : 0, bw = a.sums_w ? ceil_div(a.w.count, kNarrowRows) : 0;
+    const int64_t groups = narrow_most(bx, a.w.count, kNarrowGradSlots) + narrow_most(bw, a.x.count, kNarrowGradSlots);
+    hipLaunchKernelGGL((narrow_grad_kernel<X>), dim3((unsigned)groups), dim3(256), 0, st, a, GradUnit<T>::value, GradUnit<T>::log2);
 }
 
 // f(X()) for the planes and the 32-element steps of a row
@@ -491,15 +512,15 @@ int ce_narrow_backward(int dtype, const NarrowArgs &a, hipStream_t st) {
     const dim3 finish((unsigned)(fx + fw));
     if (dtype == MVS_DTYPE_F32) {
         narrow_prepare<float, bf16_t, 3>(a, true, st);
-        narrow_steps<bf16_t, 3>(ks, [&](auto x) { narrow_grads<decltype(x)>(a, GradUnit<float>::value, st); });
+        narrow_steps<bf16_t, 3>(ks, [&](auto x) { narrow_grads<decltype(x), float>(a, st); });
         hipLaunchKernelGGL((narrow_finish_kernel<float>), finish, dim3(256), 0, st, a, fx);
     } else if (dtype == MVS_DTYPE_BF16) {
         narrow_prepare<bf16_t, bf16_t, 1>(a, true, st);
-        narrow_steps<bf16_t, 1>(ks, [&](auto x) { narrow_grads<decltype(x)>(a, GradUnit<bf16_t>::value, st); });
+        narrow_steps<bf16_t, 1>(ks, [&](auto x) { narrow_grads<decltype(x), bf16_t>(a, st); });
         hipLaunchKernelGGL((narrow_finish_kernel<bf16_t>), finish, dim3(256), 0, st, a, fx);
     } else {
         narrow_prepare<f16_t, f16_t, 1>(a, true, st);
-        narrow_steps<f16_t, 1>(ks, [&](auto x) { narrow_grads<decltype(x)>(a, GradUnit<f16_t>::value, st); });
+        narrow_steps<f16_t, 1>(ks, [&](auto x) { narrow_grads<decltype(x), f16_t>(a, st); });
         hipLaunchKernelGGL((narrow_finish_kernel<f16_t>), finish, dim3(256), 0, st, a, fx);
     }
     return check_launch("mvs_linear_ce_bwd");

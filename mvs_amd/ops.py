@@ -1724,12 +1724,14 @@ def _here(who, *tensors):
     """The raw stream that `who` launches on, after the check that ptr() makes of every tensor, made once for all of them: on the
     GPU, and on the current device.  (The training operators pass data_ptr() numbers: a check per pointer was a third of a small
     call's time on the host.)"""
-    dev = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    dev = tensors[0].get_device()
     for t in tensors:
         if not t.is_cuda:
             raise MvsHipError(f"{who}: mvs_amd ops need device (HIP) tensors; got a CPU tensor")
         if t.get_device() != dev:
-            raise MvsHipError(f"{who}: tensor on cuda:{t.get_device()} but the current device is cuda:{dev}: wrap the call in torch.cuda.device(...)")
+            raise MvsHipError(f"{who}: tensors on cuda:{dev} and cuda:{t.get_device()}")
+    if dev != torch._C._cuda_getDevice():
+        raise MvsHipError(f"{who}: tensor on cuda:{dev} but the current device is cuda:{torch.cuda.current_device()}: wrap the call in torch.cuda.device(...)")
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
@@ -1850,6 +1852,9 @@ class _BnReluAct8CL(torch.autograd.Function):
         C = x.shape[-1]
         if x.shape[0] % groups:
             raise MvsHipError(f"bn_relu_cl: leading dimension {x.shape[0]} is not a multiple of groups={groups}")
+        for t in (running_mean, running_var):
+            if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
+                raise MvsHipError("bn_relu_cl: the running statistics are contiguous float32")
         if skip is not None and skip.shape != x.shape:
             raise MvsHipError(f"bn_relu_cl: skip {tuple(skip.shape)} does not fit x {tuple(x.shape)}")
         N = x.numel() // C // groups
@@ -1857,17 +1862,17 @@ class _BnReluAct8CL(torch.autograd.Function):
         nbytes = lib.mvs_bn_train_workspace_bytes(C)
         if nbytes == 0 or weight.numel() != C:
             raise MvsHipError(f"bn_relu_cl: C={C} not supported by a BatchNorm of {weight.numel()} channels")
-        ws = torch.empty((nbytes,), device=x.device, dtype=torch.uint8)
-        w, b = _aligned16(_f32c(weight.detach())), _aligned16(_f32c(bias.detach()))
+        ws = x.new_empty((nbytes >> 2,))
+        w, b = _aligned16(_f32c(weight)), _aligned16(_f32c(bias))
         sk = _aligned16(_f32c(skip)) if skip is not None else None
-        stats = torch.empty((2, groups, C), device=x.device, dtype=torch.float32)      # mean, 1 / standard deviation
+        stats = x.new_empty((2, groups, C))      # mean, 1 / standard deviation
         y = torch.empty_like(x)
         # codes, scales and mask in one tensor (a small layer's call is as long as its allocations)
         scales_at, mask_at, size = _BnReluAct8CL._layout(x.numel(), relu)
-        held = torch.empty((size,), device=x.device, dtype=torch.uint8)
+        held = x.new_empty((size,), dtype=torch.uint8)
         at, hp, sp = lambda t: None if t is None else t.data_ptr(), held.data_ptr(), stats.data_ptr()  # noqa: E731
         check(lib.mvs_bn_train_fwd_act8_f32(at(x), at(w), at(b), at(sk), int(groups), N, C, float(eps), float(momentum), int(relu),
-                                            ptr(running_mean), ptr(running_var), at(nbt), sp, sp + 4 * groups * C, at(y), hp, hp + scales_at,
+                                            at(running_mean), at(running_var), at(nbt), sp, sp + 4 * groups * C, at(y), hp, hp + scales_at,
                                             hp + mask_at if relu else None, at(ws), nbytes, st), "mvs_bn_train_fwd_act8_f32")
         ctx.save_for_backward(held, w, stats)
         ctx.has_skip, ctx.groups, ctx.relu = skip is not None, int(groups), bool(relu)
@@ -1891,7 +1896,7 @@ class _BnReluAct8CL(torch.autograd.Function):
         N = gy.numel() // C // ctx.groups
         lib = _lib.load()
         nbytes = lib.mvs_bn_train_workspace_bytes(C)
-        ws = torch.empty((nbytes,), device=gy.device, dtype=torch.uint8)
+        ws = gy.new_empty((nbytes >> 2,))
         gx = torch.empty_like(gy)
         gw, gb = torch.empty_like(w), torch.empty_like(w)
         scales_at, mask_at, _ = _BnReluAct8CL._layout(gy.numel(), ctx.relu)
@@ -2113,8 +2118,8 @@ class _LookupRows(torch.autograd.Function):
     def forward(ctx, table, index, scale):
         rows, C = table.shape
         st = _here("lookup_rows", table, index)
-        t = table.detach().contiguous()
-        out = torch.empty((*index.shape, C), device=t.device, dtype=t.dtype)
+        t = table.contiguous()
+        out = t.new_empty((*index.shape, C))
         check(_lib.load().mvs_lookup_rows_fwd(t.data_ptr(), DTYPES[t.dtype], rows, C, index.data_ptr(), index.numel(), scale, out.data_ptr(), st),
               "mvs_lookup_rows_fwd")
         ctx.save_for_backward(index)
@@ -2131,8 +2136,8 @@ class _LookupRows(torch.autograd.Function):
         n = index.numel()
         lib = _lib.load()
         nbytes = lib.mvs_lookup_rows_workspace_bytes(rows, C, n)
-        ws = torch.empty((nbytes,), device=g.device, dtype=torch.uint8)
-        grad = torch.empty((rows, C), device=g.device, dtype=g.dtype)
+        ws = index.new_empty((nbytes + 7 >> 3,))
+        grad = g.new_empty((rows, C))
         check(lib.mvs_lookup_rows_bwd(g.data_ptr(), DTYPES[g.dtype], index.data_ptr(), n, rows, C, scale, grad.data_ptr(), ws.data_ptr(), nbytes,
                                       st), "mvs_lookup_rows_bwd")
         return grad, None, None
@@ -2148,9 +2153,9 @@ def lookup_rows(table, index, scale=1.0):
         raise MvsHipError(f"lookup_rows: the table is [rows, C], got {tuple(table.shape)}")
     if index.dtype not in (torch.int64, torch.int32):
         raise MvsHipError(f"lookup_rows: the index holds int64 or int32, got {index.dtype}")
-    if index.device != table.device:
-        raise MvsHipError(f"lookup_rows: index on {index.device}, table on {table.device}")
-    return _LookupRows.apply(table, index.to(torch.int64).contiguous(), float(scale))
+    if index.dtype is not torch.int64 or not index.is_contiguous():
+        index = index.to(torch.int64).contiguous()
+    return _LookupRows.apply(table, index, float(scale))
 
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -2162,13 +2167,13 @@ class _LinearCrossEntropy(torch.autograd.Function):
         n, C = x.shape
         V = weight.shape[0]
         st = _here("linear_cross_entropy", x, weight, target)
-        xd, wd = _aligned16(x.detach().contiguous()), _aligned16(weight.detach().contiguous())
+        xd, wd = _aligned16(x.contiguous()), _aligned16(weight.contiguous())
         code = DTYPES[xd.dtype]
         lib = _lib.load()
         nbytes = lib.mvs_linear_ce_workspace_bytes(n, V, C, code, 0, 0, 0)
-        ws = torch.empty((nbytes,), device=xd.device, dtype=torch.uint8)
-        loss = torch.empty((n,) if reduction == 0 else (), device=xd.device, dtype=torch.float32)
-        state = torch.empty((n + 1,), device=xd.device, dtype=torch.float32)      # the rows' lse, and how many rows were kept
+        ws = target.new_empty((nbytes + 7 >> 3,))
+        loss = xd.new_empty((n,) if reduction == 0 else (), dtype=torch.float32)
+        state = xd.new_empty((n + 1,), dtype=torch.float32)      # the rows' lse, and how many rows were kept
         at = state.data_ptr()
         check(lib.mvs_linear_ce_fwd(xd.data_ptr(), wd.data_ptr(), code, target.data_ptr(), n, V, C, scale, ignore_index, reduction, loss.data_ptr(),
                                     at, at + 4 * n, ws.data_ptr(), nbytes, st), "mvs_linear_ce_fwd")
@@ -2189,7 +2194,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         g = _f32c(g)
         code = DTYPES[x.dtype]
         nbytes = lib.mvs_linear_ce_workspace_bytes(n, V, C, code, 1, int(need_x), int(need_w))
-        ws = torch.empty((nbytes,), device=x.device, dtype=torch.uint8)
+        ws = target.new_empty((nbytes + 7 >> 3,))
         gx = torch.empty_like(x) if need_x else None
         gw = torch.empty_like(w) if need_w else None
         at = state.data_ptr()
@@ -2213,14 +2218,14 @@ def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduct
         raise MvsHipError(f"linear_cross_entropy: x is {x.dtype}, weight {weight.dtype}")
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise MvsHipError(f"linear_cross_entropy: x is [..., C] and weight [V, C], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    if tuple(target.shape) != tuple(x.shape[:-1]):
+    if target.shape != x.shape[:-1]:
         raise MvsHipError(f"linear_cross_entropy: target {tuple(target.shape)} does not fit x {tuple(x.shape)}")
     if target.dtype not in (torch.int64, torch.int32):
         raise MvsHipError(f"linear_cross_entropy: the target holds int64 or int32, got {target.dtype}")
-    if not (x.device == weight.device == target.device):
-        raise MvsHipError(f"linear_cross_entropy: x on {x.device}, weight on {weight.device}, target on {target.device}")
     if reduction not in _REDUCTIONS:
         raise MvsHipError(f"linear_cross_entropy: reduction is 'none', 'mean' or 'sum', got {reduction!r}")
-    loss = _LinearCrossEntropy.apply(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1).to(torch.int64).contiguous(), float(scale),
-                                     int(ignore_index), _REDUCTIONS[reduction])
-    return loss.reshape(target.shape) if reduction == "none" else loss
+    rows, shape = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), target.shape
+    if target.dtype is not torch.int64 or target.dim() != 1 or not target.is_contiguous():
+        target = target.reshape(-1).to(torch.int64).contiguous()
+    loss = _LinearCrossEntropy.apply(rows, weight, target, float(scale), int(ignore_index), _REDUCTIONS[reduction])
+    return loss.reshape(shape) if reduction == "none" else loss
