@@ -724,7 +724,7 @@ int mvs_bn_train_bwd_act8_f32(const float *grad_y, const signed char *codes, con
 /* Rows of a table by index, times `scale`: out[i] = scale * table[index[i]], computed in float32 and rounded once.  table
  * [rows, C], out [n, C] contiguous, of one type; index int64.  An index outside [0, rows) names no row: out[i] = 0 and no
  * gradient.  The gradient (grad_table overwritten) is summed in float32 in the order of i -- the indices are sorted, stably, in
- * the workspace; no atomics, so equal calls give equal bits. */
+ * the workspace; no floating-point atomics, so equal calls give equal bits.  C at most 2^20. */
 int mvs_lookup_rows_fwd(const void *table, int dtype, int64_t rows, int C, const int64_t *index, int64_t n, float scale, void *out,
                         void *stream);
 size_t mvs_lookup_rows_workspace_bytes(int64_t rows, int C, int64_t n);
@@ -734,12 +734,14 @@ int mvs_lookup_rows_bwd(const void *grad_out, int dtype, const int64_t *index, i
 /* Softmax cross entropy of n rows against a table of V rows without the logits: l[i][v] = scale * <x[i], weight[v]>,
  * loss_i = logsumexp_v l[i][v] - l[i][target[i]].  x [n, C], weight [V, C] contiguous, of one type, 16-byte aligned; target int64.
  * A row whose target is ignore_index has loss 0 and no gradient, whatever x holds there; a target outside [0, V) otherwise makes
- * the row's loss NaN.  Products are summed in float32 (float32 operands: on the float32 matrix pipe), losses are float32.
+ * the row's loss NaN.  Products are summed in float32, losses are float32; float32 operands run on the float32 matrix pipe, rows of
+ * at most 64 of them as three bfloat16 pieces (24 bits; an Inf among them counts as a NaN).
  * reduction: 0 none (loss [n]), 1 mean over the rows kept (0 / 0 = NaN if there are none; gradients are then zero), 2 sum.
- * lse [n] and kept [1] (the number of rows kept, as a float) are for the backward pass.
+ * lse [n] (of the kept rows, in the backward pass's order) and kept [1] (their number, as a float) are for the backward pass.
  * Backward: grad_loss [n] (reduction 0) or [1]; grad_x [n, C] and grad_weight [V, C] in the operands' type, either may be NULL.
  * The logits are formed again, a piece of the table at a time; the workspace (mvs_linear_ce_workspace_bytes; backward != 0 for
- * the backward pass, with need_x / need_w for the gradients asked for) holds a piece's gradient and no more. */
+ * the backward pass, with need_x / need_w for the gradients asked for) holds a piece's gradient, transposes of the operands' size
+ * and partial sums.  No atomics: equal calls give equal bits. */
 size_t mvs_linear_ce_workspace_bytes(int64_t n, int64_t V, int C, int dtype, int backward, int need_x, int need_w);
 int mvs_linear_ce_fwd(const void *x, const void *weight, int dtype, const int64_t *target, int64_t n, int64_t V, int C, float scale,
                       int64_t ignore_index, int reduction, float *loss, float *lse, float *kept, void *workspace,

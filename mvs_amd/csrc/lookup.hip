@@ -448,8 +448,8 @@ static int lookup_check(const char *who, const void *table, const void *wide, in
         set_error("%s: invalid argument (rows=%lld, C=%d, n=%lld, dtype=%d)", who, (long long)rows, C, (long long)n, dtype);
         return MVS_EINVAL;
     }
-    if (rows > 0x7ffffffe || n > 0x7ffffffe) {
-        set_error("%s: rows=%lld, n=%lld (at most 2^31 - 2 each)", who, (long long)rows, (long long)n);
+    if (rows > 0x7ffffffe || n > 0x7ffffffe || C > (1 << 20)) {
+        set_error("%s: rows=%lld, n=%lld (at most 2^31 - 2 each), C=%d (at most 2^20)", who, (long long)rows, (long long)n, C);
         return MVS_EUNSUPPORTED;
     }
     return MVS_OK;
@@ -500,7 +500,7 @@ extern "C" int mvs_lookup_rows_fwd(const void *table, int dtype, int64_t rows, i
 }
 
 extern "C" size_t mvs_lookup_rows_workspace_bytes(int64_t rows, int C, int64_t n) {
-    if (rows < 1 || C < 1 || n < 0 || rows > 0x7ffffffe || n > 0x7ffffffe) return 0;
+    if (rows < 1 || C < 1 || n < 0 || rows > 0x7ffffffe || n > 0x7ffffffe || C > (1 << 20)) return 0;
     return lookup_plan(rows, C, n).total + 256;
 }
 

@@ -1787,10 +1787,14 @@ def act8_quantize(x):
 def act8_dequantize(held, dtype=None):
     """The values that an Act8 stands for, in the type it was made from (or `dtype`): codes times their block's power of two,
     exact in float32 and bfloat16, at most the type's largest finite number."""
-    out = torch.empty(held.shape, device=held.codes.device, dtype=held.dtype if dtype is None else dtype)
-    code = _dtype_code(out, "act8_dequantize")
-    check(_lib.load().mvs_act8_dequantize(held.codes.data_ptr(), held.scales.data_ptr(), out.numel(), code, out.data_ptr(),
-                                          _here("act8_dequantize", held.codes)), "mvs_act8_dequantize")
+    codes, scales = held.codes, held.scales
+    st = _here("act8_dequantize", codes, scales)
+    out = torch.empty(held.shape, device=codes.device, dtype=held.dtype if dtype is None else dtype)
+    code, n = _dtype_code(out, "act8_dequantize"), out.numel()
+    if codes.dtype != torch.int8 or scales.dtype != torch.uint8 or codes.numel() != n or scales.numel() != (n + ACT8_BLOCK - 1) // ACT8_BLOCK or \
+            not (codes.is_contiguous() and scales.is_contiguous()):
+        raise MvsHipError(f"act8_dequantize: {codes.numel()} {codes.dtype} codes and {scales.numel()} {scales.dtype} scales do not hold a tensor {held.shape}")
+    check(_lib.load().mvs_act8_dequantize(codes.data_ptr(), scales.data_ptr(), n, code, out.data_ptr(), st), "mvs_act8_dequantize")
     return out
 
 
@@ -1853,14 +1857,14 @@ class _BnReluAct8CL(torch.autograd.Function):
         if x.shape[0] % groups:
             raise MvsHipError(f"bn_relu_cl: leading dimension {x.shape[0]} is not a multiple of groups={groups}")
         for t in (running_mean, running_var):
-            if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
-                raise MvsHipError("bn_relu_cl: the running statistics are contiguous float32")
+            if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != C):
+                raise MvsHipError(f"bn_relu_cl: the running statistics are {C} contiguous float32 numbers")
         if skip is not None and skip.shape != x.shape:
             raise MvsHipError(f"bn_relu_cl: skip {tuple(skip.shape)} does not fit x {tuple(x.shape)}")
         N = x.numel() // C // groups
         lib = _lib.load()
         nbytes = lib.mvs_bn_train_workspace_bytes(C)
-        if nbytes == 0 or weight.numel() != C:
+        if nbytes == 0 or weight.numel() != C or bias.numel() != C:
             raise MvsHipError(f"bn_relu_cl: C={C} not supported by a BatchNorm of {weight.numel()} channels")
         ws = x.new_empty((nbytes >> 2,))
         w, b = _aligned16(_f32c(weight)), _aligned16(_f32c(bias))
@@ -2149,8 +2153,8 @@ def lookup_rows(table, index, scale=1.0):
     no gradient.  The table's gradient is dense, summed in float32 in the order of the indices (sorted, stably; no atomics): equal
     calls give equal bits however often an index repeats."""
     _dtype_code(table, "lookup_rows")
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
-        raise MvsHipError(f"lookup_rows: the table is [rows, C], got {tuple(table.shape)}")
+    if table.dim() != 2 or table.shape[0] < 1 or not 0 < table.shape[1] <= 1 << 20:
+        raise MvsHipError(f"lookup_rows: the table is [rows, C] with C at most 2^20, got {tuple(table.shape)}")
     if index.dtype not in (torch.int64, torch.int32):
         raise MvsHipError(f"lookup_rows: the index holds int64 or int32, got {index.dtype}")
     if index.dtype is not torch.int64 or not index.is_contiguous():
@@ -2212,11 +2216,13 @@ def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduct
     A row with target == ignore_index has loss 0 and leaves no trace in a gradient, whatever x holds there (the mean over no row at
     all is 0 / 0 = NaN, its gradients zero); any other target outside [0, V) makes its row's loss and the gradients NaN.
     Products are summed in float32.  For 16-bit operands the backward pass rounds each logit's gradient to that type before its two
-    products (half a unit in the last place of each term, of either sign); float32 stays float32 throughout."""
+    products (half a unit in the last place of each term, of either sign); float32 operands keep 24 bits throughout (rows of at most
+    64 go through the matrix cores as three bfloat16 pieces: the sums are as exact, an Inf among them counts as a NaN).  Equal calls
+    give equal bits."""
     _dtype_code(x, "linear_cross_entropy")
     if weight.dtype != x.dtype:
         raise MvsHipError(f"linear_cross_entropy: x is {x.dtype}, weight {weight.dtype}")
-    if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+    if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1 or not 0 < weight.shape[1] <= 1 << 20:
         raise MvsHipError(f"linear_cross_entropy: x is [..., C] and weight [V, C], got {tuple(x.shape)} and {tuple(weight.shape)}")
     if target.shape != x.shape[:-1]:
         raise MvsHipError(f"linear_cross_entropy: target {tuple(target.shape)} does not fit x {tuple(x.shape)}")

@@ -520,3 +520,121 @@ def test_linear_cross_entropy_few_rows(n, V, C, dtype):
     x[t == -100] = float("nan")
     ce_check(x, w, t, 1.0)
     ce_check(x, w, t, 1.0, reduction="none")
+
+
+# ------------------------------------------------------------------ offsets beyond 32 bits
+def test_act8_beyond_2_to_31_values():
+    n = (1 << 31) + 100
+    x = torch.empty(n, device="cuda", dtype=torch.bfloat16)
+    x[:100], x[100:-200], x[-200:] = randn(100, seed=1), 0.0, randn(200, seed=2)
+    held = ops.act8_quantize(x)
+    back = ops.act8_dequantize(held)
+    small = torch.cat([x[:128], x[-228:]])      # whole blocks of the head; the last blocks (2^31 is a multiple of 32: -228 begins one)
+    want = ops.act8_dequantize(ops.act8_quantize(small))
+    assert torch.equal(back[:128], want[:128]) and torch.equal(back[-228:], want[128:])
+    assert int(torch.count_nonzero(back[128:-228])) == 0
+
+
+def test_lookup_rows_in_a_table_beyond_2_to_31_elements():
+    rows, C, n = 1_100_000, 2048, 300
+    table = torch.zeros(rows, C, device="cuda", dtype=torch.bfloat16)
+    index = torch.randint(rows, (n,), generator=gen(1), device="cuda")
+    index[:3] = rows - 1
+    table[index] = randn(n, C, seed=2).to(table.dtype)
+    leaf = table.requires_grad_()
+    out = ops.lookup_rows(leaf, index)
+    assert torch.equal(out, table.detach()[index])
+    g = randn(n, C, seed=3).to(table.dtype)
+    grad, = torch.autograd.grad(out, leaf, g)
+    for row in (int(index[0]), int(index[10])):
+        want = g[index == row].double().sum(0)
+        assert ((grad[row].double() - want).abs() <= 4 * half_ulp(table.dtype) * g[index == row].double().abs().sum(0)).all()
+    untouched = torch.ones(rows, dtype=torch.bool, device="cuda")
+    untouched[index] = False
+    assert int(torch.count_nonzero(grad.view(torch.int16).amax(1)[untouched])) == 0
+
+
+@pytest.mark.parametrize("n", [3, 70])
+def test_linear_cross_entropy_with_a_table_beyond_2_to_31_elements(n):
+    V, C = 1_100_000, 2048
+    w = torch.empty(V, C, device="cuda", dtype=torch.bfloat16)
+    for v in range(0, V, 100_000):
+        w[v:v + 100_000] = randn(min(100_000, V - v), C, seed=v) / math.sqrt(C)
+    t = torch.randint(V, (n,), generator=gen(1), device="cuda")
+    t[0], t[1] = V - 1, V - 2
+    x = (randn(n, C, seed=2) + 4 * w[t].float()).to(torch.bfloat16)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    loss = ops.linear_cross_entropy(*leaves, t)
+    gx, gw = torch.autograd.grad(loss, leaves)
+    logits = torch.cat([x.detach().double() @ w.detach()[v:v + 100_000].double().t() for v in range(0, V, 100_000)], 1)
+    lse = torch.logsumexp(logits, 1)
+    want = (lse - logits.gather(1, t.unsqueeze(1)).squeeze(1)).mean()
+    assert abs(float(loss.detach()) - float(want)) < 1e-4
+    p = torch.exp(logits - lse.unsqueeze(1)) / n
+    p[torch.arange(n, device="cuda"), t] -= 1 / n
+    want_x = sum(p[:, v:v + 100_000] @ w.detach()[v:v + 100_000].double() for v in range(0, V, 100_000))
+    assert float((gx.double() - want_x).norm() / want_x.norm()) < 2 * half_ulp(torch.bfloat16)
+    for v in (0, V // 2, V - 100):      # dW = p^T x: h for dl, h for the result, relative to the terms
+        mine, want_w = gw[v:v + 100].double(), p[:, v:v + 100].t() @ x.detach().double()
+        mag = p[:, v:v + 100].abs().t() @ x.detach().double().abs()
+        assert ((mine - want_w).abs() <= 3 * half_ulp(torch.bfloat16) * mag).all()
+
+
+def test_linear_cross_entropy_few_rows_in_pieces():
+    """16 rows against a table of more than 2^26 / 16 rows: the one-pass kernel adds the second piece's sums to the first's."""
+    n, V, C = 16, (1 << 22) + 777, 136
+    w = randn(V, C, seed=1).to(torch.float16) * 0.1
+    t = torch.randint(V, (n,), generator=gen(1), device="cuda")
+    t[0], t[1] = V - 1, -100
+    x = (randn(n, C, seed=2) + 8 * w[t.clamp(min=0)].float()).to(torch.float16)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    loss = ops.linear_cross_entropy(*leaves, t)
+    gx, gw = torch.autograd.grad(loss, leaves)
+    keep = t >= 0
+    logits = x.detach()[keep].double() @ w.detach().double().t()
+    lse = torch.logsumexp(logits, 1)
+    k = int(keep.sum())
+    assert abs(float(loss.detach()) - float((lse - logits.gather(1, t[keep].unsqueeze(1)).squeeze(1)).mean())) < 1e-4
+    p = torch.exp(logits - lse.unsqueeze(1)) / k
+    p[torch.arange(k, device="cuda"), t[keep]] -= 1 / k
+    want = p @ w.detach().double()
+    assert float((gx[keep].double() - want).norm() / want.norm()) < 2 * half_ulp(torch.float16) and (gx[~keep] == 0).all()
+    for rows in (slice(0, 100), slice(V - 800, V)):
+        want = p[:, rows].t() @ x.detach()[keep].double()
+        mag = p[:, rows].abs().t() @ x.detach()[keep].double().abs()
+        assert ((gw[rows].double() - want).abs() <= 3 * half_ulp(torch.float16) * mag + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,C", [(300, 200), (5, 200)])
+def test_linear_cross_entropy_wide_rows_captured_and_replayed(n, C, dtype):
+    x, w, t, _ = ce_case(n, 900, C, dtype, seed=20)
+    leaves = [x.detach().requires_grad_(), w.detach().requires_grad_()]
+
+    def step(a, b, target):
+        loss = ops.linear_cross_entropy(a, b, target)
+        return [loss, *torch.autograd.grad(loss, (a, b))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves, t)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*leaves, t)
+    for seed in (21, 22, 23):      # another number of kept rows each time
+        x2, w2, t2, _ = ce_case(n, 900, C, dtype, ignored=0.1 * (seed - 20), seed=seed)
+        with torch.no_grad():
+            leaves[0].copy_(x2), leaves[1].copy_(w2), t.copy_(t2)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step(x2.requires_grad_(), w2.requires_grad_(), t2)):
+            assert torch.equal(a, b), seed
+
+
+def test_act8_dequantize_refuses_what_does_not_fit():
+    held = ops.act8_quantize(randn(100, seed=1))
+    for bad in (ops.Act8(held.codes, held.scales, (101,), torch.float32), ops.Act8(held.codes, held.scales[:3], (100,), torch.float32),
+                ops.Act8(held.codes.float(), held.scales, (100,), torch.float32), ops.Act8(held.codes[::2], held.scales, (50,), torch.float32)):
+        with pytest.raises(ops.MvsHipError, match="act8_dequantize"):
+            ops.act8_dequantize(bad)

@@ -109,6 +109,8 @@ def test_lookup_entry_points_refuse_bad_arguments():
         assert lib.mvs_lookup_rows_fwd(table, dtype, rows, C, index, n, 1.0, out, None) == EINVAL
         assert lib.mvs_lookup_rows_bwd(out, dtype, index, n, rows, C, 1.0, table, FAKE, 1 << 30, None) == EINVAL
     assert lib.mvs_lookup_rows_fwd(FAKE, 0, 1 << 31, 8, FAKE, 5, 1.0, FAKE, None) == EUNSUPPORTED
+    assert lib.mvs_lookup_rows_fwd(FAKE, 0, 10, (1 << 20) + 1, FAKE, 5, 1.0, FAKE, None) == EUNSUPPORTED
+    assert lib.mvs_lookup_rows_workspace_bytes(10, (1 << 20) + 1, 5) == 0
     assert lib.mvs_lookup_rows_bwd(FAKE, 0, FAKE, 1 << 31, 10, 8, 1.0, FAKE, FAKE, 1 << 30, None) == EUNSUPPORTED
     for ws, nbytes in ((None, 1 << 30), (FAKE, need - 1), (ODD, 1 << 30)):
         assert lib.mvs_lookup_rows_bwd(FAKE, 0, FAKE, 5, 10, 8, 1.0, FAKE, ws, nbytes, None) == EWORKSPACE
