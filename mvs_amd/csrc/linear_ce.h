@@ -127,20 +127,23 @@ inline bool ce_narrow(int C, int dtype) { return C <= (dtype == MVS_DTYPE_F32 ? 
 
 // How the work is cut: a workgroup owns kNarrowRows fixed rows and a part of the moving ones, in stages of 64.  `slots` is a number of
 // workgroups that fills whole rounds of the chip (256 CUs x 3); every workgroup gets the same number of stages, four at least, so
-// that they need at most `slots` (and one more per block of fixed rows).  Worked out alike on the host, which does not know how many
-// rows are kept, and on the device.
+// that they need at most `slots` (and one more per block of fixed rows).  Little work is one round: a workgroup's start and the sums
+// it leaves then count for more than what the shares' rounding leaves idle.  Worked out alike on the host, which does not know how
+// many rows are kept, and on the device.
 struct NarrowSplit {
     int64_t blocks_x, blocks_w;       // blocks of fixed rows of x (the table moves), of the table (x moves); 0: not wanted
     int64_t parts_x, parts_w;
     int64_t per_x, per_w;             // moving rows per part
 };
-constexpr int64_t kNarrowStatsSlots = 2 * 768, kNarrowGradSlots = 4 * 768;
+constexpr int64_t kNarrowRound = 768, kNarrowStatsSlots = 2 * kNarrowRound, kNarrowGradSlots = 4 * kNarrowRound;
 __host__ __device__ inline NarrowSplit narrow_split(int64_t count, int64_t V, int64_t slots, bool of_x, bool of_table) {
     NarrowSplit s = {};
     const int64_t stages_v = (V + 63) / 64, stages_n = (count + 63) / 64;
     s.blocks_x = of_x ? (count + kNarrowRows - 1) / kNarrowRows : 0;
     s.blocks_w = of_table ? (V + kNarrowRows - 1) / kNarrowRows : 0;
-    const int64_t share = (s.blocks_x * stages_v + s.blocks_w * stages_n + slots - 1) / slots, least = share > 4 ? share : 4;
+    const int64_t stages = s.blocks_x * stages_v + s.blocks_w * stages_n;
+    if (stages <= 16 * kNarrowRound) slots = kNarrowRound;
+    const int64_t share = (stages + slots - 1) / slots, least = share > 4 ? share : 4;
     const int64_t x = stages_v / least > 1 ? (stages_v + stages_v / least - 1) / (stages_v / least) : stages_v;      // stages per part
     const int64_t w = stages_n / least > 1 ? (stages_n + stages_n / least - 1) / (stages_n / least) : stages_n;
     s.per_x = x * 64;

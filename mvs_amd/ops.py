@@ -1603,6 +1603,7 @@ class _VarianceConv0(torch.autograd.Function):
                     gw = conv3d_wgrad_c8_f16(var, var_absmax, g, g_absmax)
                 if gw is None:
                     gw = conv3d_wgrad_c8(var, g)
+                var = None        # (read back from 8 bits: its memory is the input gradient's next)
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
             wt = w.flip(2, 3, 4).permute(1, 0, 2, 3, 4).contiguous()      # (32, 8, k) as a conv weight
             pk = pack_conv3d_weight(wt, False, 1, split=True)
