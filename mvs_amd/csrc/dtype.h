@@ -47,6 +47,18 @@ template <> struct DtypeMax<f16_t> { static constexpr float value = 65504.0f; };
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
 
+// A Pack written as one access.  (Assigned as a struct beside a branch that writes its elements one by one, the compiler shares the
+// elements' stores between the two: three narrow stores in place of a wide one.)
+template <typename T, int VEC>
+__device__ __forceinline__ void put(void *to, const Pack<T, VEC> &p) {
+    if constexpr (sizeof(p) % 8 == 0) {
+        typedef unsigned words_t __attribute__((ext_vector_type(sizeof(p) / 4)));
+        *static_cast<words_t *>(to) = __builtin_bit_cast(words_t, p);
+    } else {
+        *static_cast<Pack<T, VEC> *>(to) = p;
+    }
+}
+
 inline size_t dtype_size(int dtype) { return dtype == MVS_DTYPE_F32 ? 4 : (dtype == MVS_DTYPE_BF16 || dtype == MVS_DTYPE_F16) ? 2 : 0; }
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

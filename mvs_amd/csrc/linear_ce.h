@@ -113,7 +113,7 @@ __device__ __forceinline__ void ce_finish(const float *__restrict__ sums, int64_
 #pragma unroll
     for (int r = 0; r < 4; ++r) o.v[r] = from_float<T>(PER_ROW && f == 0.0f ? 0.0f : s[r] * f * factor);
     T *to = out + row * C + c;
-    if ((C & 3) == 0) *reinterpret_cast<Pack<T, 4> *>(to) = o;
+    if ((C & 3) == 0) put(to, o);
     else
         for (int r = 0; r < 4; ++r) if (c + r < C) to[r] = o.v[r];
 }

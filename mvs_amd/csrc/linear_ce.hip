@@ -359,7 +359,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
                 Pack<T, 4> o;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o.v[r] = from_float<T>(acc[i][j][r] * f);
-                if ((a.m & 3) == 0) *reinterpret_cast<Pack<T, 4> *>(to) = o;
+                if ((a.m & 3) == 0) put(to, o);
                 else
                     for (int r = 0; r < 4; ++r) if (m + r < a.m) to[r] = o.v[r];
             }
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeFew a) {
                     Pack<T, VEC> o;
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(out[j] * f);
-                    if (a.C % VEC == 0) *reinterpret_cast<Pack<T, VEC> *>(to) = o;
+                    if (a.C % VEC == 0) put(to, o);
                     else
                         for (int j = 0; j < VEC; ++j) if (col + j < a.C) to[j] = o.v[j];
                 }

@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(LookupRows a) {
                     Pack<T, VEC> o;
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(sum[j] * a.scale);
-                    reinterpret_cast<Pack<T, VEC> *>(out + (int64_t)key[k] * a.C)[c] = o;
+                    put(reinterpret_cast<Pack<T, VEC> *>(out + (int64_t)key[k] * a.C) + c, o);
                 }
                 from_before = false;
 #pragma unroll
