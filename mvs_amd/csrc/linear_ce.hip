@@ -19,6 +19,8 @@
 // one in both passes, so a row's p sum to one).  16-bit dl: float16 carries it times 2^14 (|p - 1| <= 1: no overflow, and p down to
 // 4e-9 keeps a normal number's precision), the row's gradient factor is applied after the product in float32 (dx) or, relative to
 // the largest one, before the rounding (dW) -- 1 / N of a mean never reaches a 16-bit number.
+#include <type_traits>
+
 #include "linear_ce.h"
 
 namespace mvs {
@@ -146,6 +148,15 @@ struct CeArgs {
     int64_t ld_dl, ld_dlt;
 };
 
+// How far row t of the table lies beyond a lane's first, v_lane, where it is within the wave's rows (16 i + r: the lane's own are
+// r = 0 .. 3), -1 elsewhere.  Few tiles hold a given row's target: the epilogues ask the whole wave once and compare element by
+// element only there.
+template <typename X>
+__device__ __forceinline__ int target_ahead(int64_t t, int64_t v_lane) {
+    const int64_t d = t - v_lane;
+    return d >= 0 && d < X::TM * 16 && (d & 15) < 4 ? (int)d : -1;
+}
+
 template <typename T, typename X>
 __global__ __launch_bounds__(X::THREADS) void ce_stats_kernel(CeArgs a) {
     extern __shared__ __align__(1024) char lds[];
@@ -159,30 +170,49 @@ __global__ __launch_bounds__(X::THREADS) void ce_stats_kernel(CeArgs a) {
     tile_product<T, X>(a.w, x, m0, n0, 0, a.steps, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
     const int64_t v_lane = m0 + wm * (X::BM / X::WAVES_M) + (lane >> 4) * 4;
+    // rows of the table from a lane's first to the table's end: all of a tile's but where the table ends in it
+    const int there = (int)min(a.v_total - v_lane, (int64_t)X::BM);
+    const bool ends = m0 + X::BM > a.v_total;
     float2 stat[X::TN];
 #pragma unroll
     for (int j = 0; j < X::TN; ++j) {
         const int64_t n = n0 + wn * (X::BN / X::WAVES_N) + j * 16 + (lane & 15);
         const int64_t t = n < rows ? a.rows.target[n] : -1;
-        float top = -INFINITY;
+        const int ahead = target_ahead<X>(t, v_lane);
+        if (__any(ahead >= 0 && t < a.v_total)) {
 #pragma unroll
-        for (int i = 0; i < X::TM; ++i)
+            for (int i = 0; i < X::TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t v = v_lane + i * 16 + r;
-                const float l = v < a.v_total ? acc[i][j][r] * a.scale2 : -INFINITY;
-                acc[i][j][r] = l;
-                top = fmaxf(top, l);
-                if (v == t && v < a.v_total) a.own[n] = l;
-            }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float base = top == -INFINITY ? 0.0f : top;      // (a tile of -Inf alone sums to 0; Inf - Inf and NaN make the sum NaN)
-        float sum = 0.0f;
+                for (int r = 0; r < 4; ++r)
+                    if (ahead == i * 16 + r && t < a.v_total) a.own[n] = acc[i][j][r] * a.scale2;
+        }
+        // (a lane's rows behind the table's end, and tiles of -Inf alone, sum to 0; Inf - Inf and NaN make the sum NaN)
+        float top = -INFINITY, sum = 0.0f;
+        auto statistics = [&](auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
+            float high = -INFINITY, low = INFINITY;      // (the scale may be negative)
 #pragma unroll
-        for (int i = 0; i < X::TM; ++i)
+            for (int i = 0; i < X::TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(acc[i][j][r] - base);
+                for (int r = 0; r < 4; ++r)
+                    if (WHOLE || i * 16 + r < there) {
+                        high = fmaxf(high, acc[i][j][r]);
+                        low = fminf(low, acc[i][j][r]);
+                    }
+            if (WHOLE || there > 0) top = fmaxf(high * a.scale2, low * a.scale2);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int i = 0; i < X::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], a.scale2, -base));
+                    sum += WHOLE || i * 16 + r < there ? e : 0.0f;
+                }
+        };
+        if (ends) statistics(std::false_type());
+        else statistics(std::true_type());
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         stat[j] = make_float2(top, sum);
@@ -275,6 +305,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
     constexpr int PITCH = X::BN * (int)sizeof(T) + 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
     const int m_lane = wm * (X::BM / X::WAVES_M) + (lane >> 4) * 4;
+    const bool ends = m0 + X::BM > a.v_count;      // the piece ends in this tile
     __syncthreads();      // the stages have been read: LDS holds the transpose from here on
 #pragma unroll
     for (int j = 0; j < X::TN; ++j) {
@@ -282,18 +313,34 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
         const int64_t n = n0 + nl;
         const int64_t t = n < rows ? a.rows.target[n] : 0;
         const bool kept = n < rows && ce_kept(t, a.rows.ignore);
-        const float lse2 = kept ? a.lse2[n] : 0.0f, ratio = kept ? a.ratio[n] : 0.0f;
+        const float lse2 = kept ? a.lse2[n] - GradUnit<T>::log2 : 0.0f, ratio = kept ? a.ratio[n] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < X::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], a.scale2, -lse2));      // unit * p
+        const int ahead = target_ahead<X>(t, a.v0 + m0 + m_lane);
+        if (__any(ahead >= 0)) {
+#pragma unroll
+            for (int i = 0; i < X::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (ahead == i * 16 + r) acc[i][j][r] -= unit;
+        }
+        if (ends) {
+#pragma unroll
+            for (int i = 0; i < X::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (m0 + m_lane + i * 16 + r >= a.v_count) acc[i][j][r] = 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < X::TM; ++i) {
             Pack<T, 4> out;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int ml = m_lane + i * 16 + r;
-                const bool real = kept && m0 + ml < a.v_count;
-                const float p = __builtin_amdgcn_exp2f(acc[i][j][r] * a.scale2 - lse2);
-                const float d = real ? (a.v0 + m0 + ml == t ? p - 1.0f : p) * unit : 0.0f;
+                const float d = kept ? acc[i][j][r] : 0.0f;
                 out.v[r] = from_float<T>(d);
-                if (a.dlt) *reinterpret_cast<T *>(lds + ml * PITCH + nl * (int)sizeof(T)) = from_float<T>(real ? d * ratio : 0.0f);
+                if (a.dlt) *reinterpret_cast<T *>(lds + (m_lane + i * 16 + r) * PITCH + nl * (int)sizeof(T)) = from_float<T>(kept ? d * ratio : 0.0f);
             }
             const int64_t m = m0 + m_lane + i * 16;
             if (a.dl && n < rows && m < a.ld_dl) *reinterpret_cast<Pack<T, 4> *>(static_cast<T *>(a.dl) + n * a.ld_dl + m) = out;
