@@ -27,9 +27,10 @@ namespace mvs {
 
 // AHEAD: a wave reads its fragments half a step ahead.  One workgroup of 8 waves per CU needs it; two of 4 waves hide each other's
 // reads and are slower with it (8192 x 128000 x 2048 bfloat16 forward: 256 x 256 tiles 3.63 -> 3.52 ms, 128 x 128 4.26 -> 4.70 ms).
-template <int BM_, int BN_, int WM_, int WN_, bool AHEAD_>
+// LATE: the copies of a later stage are issued behind the products that follow the barrier, not before them.
+template <int BM_, int BN_, int WM_, int WN_, bool AHEAD_, bool LATE_ = false>
 struct Tile {
-    static constexpr bool AHEAD = AHEAD_;
+    static constexpr bool AHEAD = AHEAD_, LATE = LATE_;
     static constexpr int BM = BM_, BN = BN_, WAVES_M = WM_, WAVES_N = WN_, WAVES = WM_ * WN_, THREADS = 64 * WAVES;
     static constexpr int TM = BM / WAVES_M / 16, TN = BN / WAVES_N / 16;
     static constexpr int STAGE = (BM + BN) * kRowBytes;
@@ -56,13 +57,13 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
         const Operand &o = of_a ? a : b;
         from[i] = o.p + (row < o.rows ? row : o.rows - 1) * o.ld + k_byte0 + chunk * 16;
     }
-    auto copy = [&](int stage) {
+    auto copy = [&](int stage, int advance = kRowBytes) {
 #pragma unroll
         for (int i = 0; i < X::PER_WAVE; ++i) {
             const int c = wave + i * X::WAVES;
             if (X::COPIES % X::WAVES == 0 || c < X::COPIES) {
                 glds16(from[i], lds_base + (unsigned)(stage * X::STAGE + c * 1024));
-                from[i] += kRowBytes;
+                from[i] += advance;
             }
         }
     };
@@ -76,34 +77,61 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
 #pragma unroll
         for (int j = 0; j < X::TN; ++j) fb[j] = *reinterpret_cast<const u32x4_t *>(at + b_row + j * 16 * kRowBytes);
     };
-    auto multiply = [&](const u32x4_t (&fa)[X::TM], const u32x4_t (&fb)[X::TN]) {
+    auto multiply = [&](const u32x4_t (&fa)[X::TM], const u32x4_t (&fb)[X::TN], int first, int last) {
 #pragma unroll
         for (int i = 0; i < X::TM; ++i)
+            if (i >= first && i < last)
 #pragma unroll
-            for (int j = 0; j < X::TN; ++j) mma16(acc[i][j], fa[i], fb[j], T());
+                for (int j = 0; j < X::TN; ++j) mma16(acc[i][j], fa[i], fb[j], T());
     };
     copy(0);
     if constexpr (X::AHEAD) {
         // The fragments of a half step are read while the matrix cores work on the half before it, across the stages' border too:
-        //     read second half of s | first half's products | stage s + 1 has landed, s is read out | copy s + 2 into its place,
-        //     read first half of s + 1 | second half's products
+        //     read second half of s | first half's products, half of them | stage s + 1 has landed, s is read out | copy s + 2 into
+        //     its place | the other half of them | read first half of s + 1 | second half's products
+        // The waves of a SIMD meet at the barrier with products left, so that its matrix cores go on.  No branch in the loop: around
+        // the reads it would have the compiler wait for them at once.  So the last two steps' copies read the last step's bytes
+        // again, into a stage that is not read any more, and the last step's products stand behind the loop.
+        constexpr int HALF = X::TM / 2;
+        auto pace = [] {      // one read behind each of the first products
+#pragma unroll
+            for (int i = 0; i < X::TM + X::TN; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // matrix instructions
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // LDS reads
+            }
+        };
         u32x4_t a0[X::TM], b0[X::TN], a1[X::TM], b1[X::TN];
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (steps > 1) copy(1);
+        if (steps > 1) copy(1, steps > 2 ? kRowBytes : 0);
         read(0, swz0, a0, b0);
-        for (int s = 0; s < steps; ++s) {
-            const int stage = s & 1;
+        int stage = 0;
+        for (int s = 0; s + 1 < steps; ++s, stage ^= 1) {
             read(stage, swz1, a1, b1);
-            multiply(a0, b0);
-            if (s + 1 < steps) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();      // (waits for this wave's reads too: the stage may be overwritten)
-                if (s + 2 < steps) copy(stage);
-                read(stage ^ 1, swz0, a0, b0);
+            multiply(a0, b0, 0, HALF);
+            pace();
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();      // (waits for this wave's reads too: the stage may be overwritten)
+            const int advance = s + 3 < steps ? kRowBytes : 0;
+            if constexpr (X::LATE) {
+                multiply(a0, b0, HALF, X::TM);
+                __builtin_amdgcn_sched_barrier(0);
+                copy(stage, advance);
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                copy(stage, advance);
+                multiply(a0, b0, HALF, X::TM);
             }
-            multiply(a1, b1);
+            read(stage ^ 1, swz0, a0, b0);
+            multiply(a1, b1, 0, X::TM);
+            pace();
+            if constexpr (X::LATE) __builtin_amdgcn_sched_barrier(0);
         }
+        read(stage, swz1, a1, b1);
+        multiply(a0, b0, 0, X::TM);
+        multiply(a1, b1, 0, X::TM);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the copies of the last steps, before LDS is used for something else
     } else {
         for (int s = 0; s < steps; ++s) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -113,7 +141,7 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
             for (int half = 0; half < 2; ++half) {
                 u32x4_t fa[X::TM], fb[X::TN];
                 read(s & 1, half ? swz1 : swz0, fa, fb);
-                multiply(fa, fb);
+                multiply(fa, fb, 0, X::TM);
             }
         }
     }
@@ -664,6 +692,9 @@ struct CePlan {
 // transpose of such a tile does not fit LDS) -- half the LDS and L2 traffic per operation.
 using Tile128 = Tile<128, 128, 2, 2, false>;
 using Tile256 = Tile<256, 256, 2, 4, true>;
+// The statistics read the whole table once, from memory, and take the copies late better (8192 x 64000 x 2048: 1.60 ms against 1.70);
+// the backward pass' products read a piece that the caches hold, and take them early (dx's 1.80 ms against 1.96).
+using Tile256Late = Tile<256, 256, 2, 4, true, true>;
 
 // Whether the [m][n] tiles of a 16-bit product are 256 x 256.  Both sizes' time goes as the area they cover in whole rounds of the
 // chip (256 CUs; two of the small workgroups per CU), and the larger one is 1.2 times as fast per area: 8192 x 128000 x 2048
@@ -728,8 +759,8 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
             p.dl = take((size_t)n * p.piece * p.es);
             p.wt = take((size_t)C * p.piece * p.es);
             const int64_t side = ce_big(C, n, p.es) ? 256 : 128, tiles = ceil_div(C, side) * ceil_div(n, side), steps = round_up(V < p.piece ? V : p.piece, step) / step;
-            // parts of k: enough workgroups for the chip's 256 CUs twice over, at least 8 steps each
-            int64_t parts = side == 256 ? 1 : ceil_div(512, tiles > 0 ? tiles : 1);
+            // parts of k: as many workgroups as one round of the chip takes (two per CU), at least 8 steps each
+            int64_t parts = side == 256 || tiles == 0 ? 1 : 512 / tiles;
             if (parts > steps / 8) parts = steps / 8;
             if (parts < 1) parts = 1;
             p.parts = (int)ceil_div(steps, ceil_div(steps, parts));      // (as many as get work; a smaller last piece then has no more)
@@ -865,7 +896,7 @@ static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const Ce
     a.part = reinterpret_cast<float2 *>(ws + p.part);
     a.own = reinterpret_cast<float *>(ws + p.own);
     ce_tiles<T>(V, rows.n, [&](auto x) {
-        using X = decltype(x);
+        using X = std::conditional_t<std::is_same_v<decltype(x), Tile256>, Tile256Late, decltype(x)>;
         a.tiles_m = ceil_div(V, X::BM); a.tiles_n = ceil_div(rows.n, X::BN);
         ce_launch<X>(ce_stats_kernel<T, X>, a, 1, (size_t)X::WAVES_M * X::BN * sizeof(float2), st);
     });
