@@ -278,7 +278,13 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__
         return make_float2(top, p.y * __builtin_amdgcn_exp2f(p.x - base) + q.y * __builtin_amdgcn_exp2f(q.x - base));
     };
     if (row < n)
-        for (int64_t t = threadIdx.x >> 4; t < tiles; t += 16) r = join(r, part[t * ld + row]);
+        for (int64_t t = threadIdx.x >> 4; t < tiles; t += 64) {      // (four loads under way)
+            float2 p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = t + 16 * u < tiles ? part[(t + 16 * u) * ld + row] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) r = join(r, p[u]);
+        }
     s[threadIdx.x] = r;
     __syncthreads();
     if (threadIdx.x < 16 && row < n) {
