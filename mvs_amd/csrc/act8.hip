@@ -30,13 +30,14 @@ __device__ __forceinline__ void act8_quantize_lanes(const T *__restrict__ x, int
 template <typename T>
 __global__ __launch_bounds__(256) void act8_quantize_kernel(const T *__restrict__ x, int64_t n, int64_t whole, int64_t groups, signed char *__restrict__ codes,
                                                             unsigned char *__restrict__ scales) {
-    if (blockIdx.x >= groups) {
-        act8_quantize_lanes(x, n, whole + (blockIdx.x - groups) * 8, codes, scales);
+    const int64_t group = group_of();
+    if (group >= groups) {
+        act8_quantize_lanes(x, n, whole + (group - groups) * 8, codes, scales);
         return;
     }
     constexpr int VEC = 16 / sizeof(T), LANES = kAct8Block / VEC;
     const int64_t n_vec = whole * LANES;
-    const int64_t first = (int64_t)blockIdx.x * 256 * kUnroll + threadIdx.x;
+    const int64_t first = group * 256 * kUnroll + threadIdx.x;
     Pack<T, VEC> v[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -77,14 +78,15 @@ __device__ __forceinline__ T act8_back(float v) {
 template <typename T>
 __global__ __launch_bounds__(256) void act8_dequantize_kernel(const signed char *__restrict__ codes, const unsigned char *__restrict__ scales,
                                                               int64_t n, int64_t whole, int64_t groups, T *__restrict__ out) {
-    if (blockIdx.x >= groups) {
-        const int64_t i = whole * kAct8Block + (blockIdx.x - groups) * 256 + threadIdx.x;
+    const int64_t group = group_of();
+    if (group >= groups) {
+        const int64_t i = whole * kAct8Block + (group - groups) * 256 + threadIdx.x;
         if (i < n) out[i] = act8_back<T>((float)codes[i] * act8_step(scales[i / kAct8Block]));
         return;
     }
     constexpr int VEC = 16 / sizeof(T), LANES = kAct8Block / VEC;
     const int64_t n_vec = whole * LANES;
-    const int64_t first = (int64_t)blockIdx.x * 256 * kUnroll + threadIdx.x;
+    const int64_t first = group * 256 * kUnroll + threadIdx.x;
     Pack<unsigned, VEC / 4> q[kUnroll];
     unsigned byte[kUnroll];
 #pragma unroll
@@ -116,7 +118,7 @@ static int act8_check(const char *who, const void *wide, int dtype, int64_t n, c
         set_error("%s: the tensor is not aligned to its element size", who);
         return MVS_EINVAL;
     }
-    if (n > (int64_t)1 << 38) {      // (a grid has at most 2^31 - 1 workgroups)
+    if (n > (int64_t)1 << 38) {
         set_error("%s: n=%lld is beyond 2^38", who, (long long)n);
         return MVS_EUNSUPPORTED;
     }
@@ -136,7 +138,7 @@ extern "C" int mvs_act8_quantize(const void *x, int dtype, int64_t n, signed cha
     const int64_t whole = act8_wide(x, codes) ? n / kAct8Block : 0, blocks = (n + kAct8Block - 1) / kAct8Block;
     MVS_DTYPE_DISPATCH(dtype, T, {
         const int64_t groups = (whole * (kAct8Block * (int)sizeof(T) / 16) + 256 * kUnroll - 1) / (256 * kUnroll), rest = (blocks - whole + 7) / 8;
-        hipLaunchKernelGGL((act8_quantize_kernel<T>), dim3((unsigned)(groups + rest)), dim3(256), 0, st, static_cast<const T *>(x), n, whole, groups, codes, scales);
+        hipLaunchKernelGGL((act8_quantize_kernel<T>), grid_of(groups + rest), dim3(256), 0, st, static_cast<const T *>(x), n, whole, groups, codes, scales);
     });
     return check_launch("mvs_act8_quantize");
 }
@@ -148,7 +150,7 @@ extern "C" int mvs_act8_dequantize(const signed char *codes, const unsigned char
     const int64_t whole = act8_wide(out, codes) ? n / kAct8Block : 0;
     MVS_DTYPE_DISPATCH(dtype, T, {
         const int64_t groups = (whole * (kAct8Block * (int)sizeof(T) / 16) + 256 * kUnroll - 1) / (256 * kUnroll), rest = (n - whole * kAct8Block + 255) / 256;
-        hipLaunchKernelGGL((act8_dequantize_kernel<T>), dim3((unsigned)(groups + rest)), dim3(256), 0, st, codes, scales, n, whole, groups, static_cast<T *>(out));
+        hipLaunchKernelGGL((act8_dequantize_kernel<T>), grid_of(groups + rest), dim3(256), 0, st, codes, scales, n, whole, groups, static_cast<T *>(out));
     });
     return check_launch("mvs_act8_dequantize");
 }

@@ -59,6 +59,14 @@ __device__ __forceinline__ void put(void *to, const Pack<T, VEC> &p) {
     }
 }
 
+// A launch counts the threads of a dimension in 32 bits: more than kGridRow workgroups (of at most 1024) are rows of that many, and
+// those behind the last one find nothing to do.
+constexpr int64_t kGridRow = (int64_t)1 << 21;
+inline dim3 grid_of(int64_t groups) {
+    return groups <= kGridRow ? dim3((unsigned)groups) : dim3((unsigned)kGridRow, (unsigned)((groups + kGridRow - 1) / kGridRow));
+}
+__device__ __forceinline__ int64_t group_of() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 inline size_t dtype_size(int dtype) { return dtype == MVS_DTYPE_F32 ? 4 : (dtype == MVS_DTYPE_BF16 || dtype == MVS_DTYPE_F16) ? 2 : 0; }
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

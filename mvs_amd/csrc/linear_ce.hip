@@ -190,7 +190,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_stats_kernel(CeArgs a) {
     extern __shared__ __align__(1024) char lds[];
     const int64_t rows = ce_count(a.rows);
     int64_t tm, tn;
-    if (!tile_of(blockIdx.x, a.tiles_m, (rows + X::BN - 1) / X::BN, tm, tn)) return;
+    if (!tile_of(group_of(), a.tiles_m, (rows + X::BN - 1) / X::BN, tm, tn)) return;
     Operand x = a.x;
     x.rows = rows;
     const int64_t m0 = tm * X::BM, n0 = tn * X::BN;
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__
     const int64_t n = ce_count(rows), ld = tiles ? rows.n : n;
     if (!tiles) tiles = narrow_split(n, v_total, kNarrowStatsSlots, true, false).parts_x;
     __shared__ float2 s[256];
-    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+    const int64_t row = group_of() * 16 + (threadIdx.x & 15);
     float2 r = make_float2(-INFINITY, 0.0f);
     auto join = [](float2 p, float2 q) {
         const float top = fmaxf(p.x, q.x), base = top == -INFINITY ? 0.0f : top;
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void ce_finish_kernel(const float *sums, int parts, CeRows rows, int C, int64_t ld, const float *g, float factor, T *out) {
-    ce_finish<T, true>(sums, parts, rows.n, rows.n, rows.place, C, ld, g, factor, out, blockIdx.x);
+    ce_finish<T, true>(sums, parts, rows.n, rows.n, rows.place, C, ld, g, factor, out, group_of());
 }
 
 // Moves the kept rows together (CeRows), by one workgroup: 16 waves count their sixteenth of the targets, then number its kept rows.
@@ -497,7 +497,7 @@ __global__ __launch_bounds__(1024) void ce_together_kernel(const int64_t *__rest
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void ce_rows_kernel(const T *__restrict__ in, CeRows rows, int C, T *__restrict__ out, int Cp) {
     const int vecs = Cp / VEC;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / vecs;
+    const int64_t i = group_of() * 256 + threadIdx.x, row = i / vecs;
     if (row >= ce_count(rows)) return;
     const int c = (int)(i - row * vecs) * VEC;
     Pack<T, VEC> v;
@@ -703,13 +703,13 @@ using Tile256 = Tile<256, 256, 2, 4, true>;
 using Tile256Late = Tile<256, 256, 2, 4, true, true>;
 
 // Whether the [m][n] tiles of a 16-bit product are 256 x 256.  Both sizes' time goes as the area they cover in whole rounds of the
-// chip (256 CUs; two of the small workgroups per CU), and the larger one is 1.2 times as fast per area: 8192 x 128000 x 2048
-// forward 3.52 ms against 4.26, 4096 x 32000 x 1024 0.256 against 0.287; but 777 x 49999 x 768, 24 % of whose 256-row tiles is
-// empty, 0.115 against 0.097.
+// chip (256 CUs; two of the small workgroups per CU), and the larger one is 4 / 3 as fast per area: statistics of 8192 x 64000 x 2048
+// 1.60 ms against 2.13, of 5120 x 8192 x 2048 (a round of them is not full) 0.162 against 0.187; but the softmax gradient of
+// 777 x 49999 x 768, 24 % of whose 256-row tiles is empty, 0.128 against 0.113.
 static bool ce_big(int64_t m, int64_t n, int es) {
     if (es != 2) return false;
     const int64_t big = ceil_div(ceil_div(m, 256) * ceil_div(n, 256), 256) * 256, small = ceil_div(ceil_div(m, 128) * ceil_div(n, 128), 512) * 512;
-    return big * 4 * 5 < small * 6;
+    return big * 3 < small;
 }
 
 static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, bool need_x, bool need_w) {
@@ -812,8 +812,8 @@ static int ce_check(const char *who, const void *x, const void *w, int dtype, co
         set_error("%s: x, weight and the workspace are to be aligned to 16 bytes", who);
         return MVS_EINVAL;
     }
-    if (n > ((int64_t)1 << 30) || V > ((int64_t)1 << 30) || C > (1 << 20) || ceil_div(n, 64) * ceil_div(V, 64) > 0x7fffffff) {
-        set_error("%s: n=%lld, V=%lld (at most 2^30 each, n V / 4096 below 2^31), C=%d (at most 2^20)", who, (long long)n, (long long)V, C);
+    if (n > ((int64_t)1 << 29) || V > ((int64_t)1 << 29) || C > (1 << 20) || ceil_div(n, 64) * ceil_div(V, 64) > 0x7fffffff) {
+        set_error("%s: n=%lld, V=%lld (at most 2^29 each, n V / 4096 below 2^31), C=%d (at most 2^20)", who, (long long)n, (long long)V, C);
         return MVS_EUNSUPPORTED;
     }
     if (workspace_bytes < need) {
@@ -829,10 +829,10 @@ static void ce_operands(const CePlan &p, const void *x, const void *w, const CeR
     auto copy = [&](const void *in, const CeRows &r, char *out) {
         constexpr int VEC = 16 / sizeof(T);
         if (C % VEC == 0)
-            hipLaunchKernelGGL((ce_rows_kernel<T, VEC>), dim3((unsigned)ceil_div(r.n * (p.Cp / VEC), 256)), dim3(256), 0, st, static_cast<const T *>(in), r, C,
+            hipLaunchKernelGGL((ce_rows_kernel<T, VEC>), grid_of(ceil_div(r.n * (p.Cp / VEC), 256)), dim3(256), 0, st, static_cast<const T *>(in), r, C,
                                reinterpret_cast<T *>(out), p.Cp);
         else
-            hipLaunchKernelGGL((ce_rows_kernel<T, 1>), dim3((unsigned)ceil_div(r.n * p.Cp, 256)), dim3(256), 0, st, static_cast<const T *>(in), r, C,
+            hipLaunchKernelGGL((ce_rows_kernel<T, 1>), grid_of(ceil_div(r.n * p.Cp, 256)), dim3(256), 0, st, static_cast<const T *>(in), r, C,
                                reinterpret_cast<T *>(out), p.Cp);
     };
     a.w = Operand{static_cast<const char *>(w), (int64_t)p.Cp * p.es, V};
@@ -870,12 +870,12 @@ static void ce_tiles(int64_t m, int64_t n, F f) {
 
 // two stages of LDS, or what the epilogue lays there if that is more (an error stands for check_launch)
 template <typename X, typename F, typename A>
-static void ce_launch(F kernel, const A &a, unsigned parts, size_t epilogue, hipStream_t st) {
+static void ce_launch(F kernel, const A &a, dim3 grid, size_t epilogue, hipStream_t st) {
     const size_t stages = 2 * (size_t)X::STAGE;
     const unsigned bytes = (unsigned)(epilogue > stages ? epilogue : stages);
     // (more than 64 KiB of dynamic LDS has to be asked for)
     if (bytes > 65536 && hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess) return;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tiles_m * a.tiles_n), parts), dim3(X::THREADS), bytes, st, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(X::THREADS), bytes, st, a);
 }
 
 template <typename T>
@@ -904,7 +904,7 @@ static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const Ce
     ce_tiles<T>(V, rows.n, [&](auto x) {
         using X = std::conditional_t<std::is_same_v<decltype(x), Tile256>, Tile256Late, decltype(x)>;
         a.tiles_m = ceil_div(V, X::BM); a.tiles_n = ceil_div(rows.n, X::BN);
-        ce_launch<X>(ce_stats_kernel<T, X>, a, 1, (size_t)X::WAVES_M * X::BN * sizeof(float2), st);
+        ce_launch<X>(ce_stats_kernel<T, X>, a, grid_of(a.tiles_m * a.tiles_n), (size_t)X::WAVES_M * X::BN * sizeof(float2), st);
     });
     return check_launch("mvs_linear_ce_fwd");
 }
@@ -926,7 +926,7 @@ static int ce_forward(int dtype, const void *x, const void *w, const int64_t *ta
             MVS_DTYPE_DISPATCH(dtype, T, rc = (ce_wide_stats<T>(p, x, w, rows, V, C, scale, ws, st)));
         }
         if (rc != MVS_OK) return rc;
-        hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(256), 0, st, part, p.tiles, V, rows, own, lse, losses);
+        hipLaunchKernelGGL(ce_join_kernel, grid_of(ceil_div(n, 16)), dim3(256), 0, st, part, p.tiles, V, rows, own, lse, losses);
     }
     hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, losses, target, n, ignore, reduction, loss, kept);
     return check_launch("mvs_linear_ce_fwd");
@@ -954,7 +954,7 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
         ce_tiles<T>(d.m, d.n, [&](auto x) {
             using X = decltype(x);
             d.tiles_m = ceil_div(d.m, X::BM); d.tiles_n = ceil_div(d.n, X::BN);
-            ce_launch<X>(ce_product_kernel<T, X>, d, (unsigned)ceil_div(d.steps, d.steps_per_part), 0, st);
+            ce_launch<X>(ce_product_kernel<T, X>, d, dim3((unsigned)(d.tiles_m * d.tiles_n), (unsigned)ceil_div(d.steps, d.steps_per_part)), 0, st);
         });
     };
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
@@ -965,7 +965,7 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
         ce_tiles<T>(count, n, [&](auto x) {
             using X = decltype(x);
             a.tiles_m = ceil_div(count, X::BM); a.tiles_n = ceil_div(n, X::BN);
-            ce_launch<X>(ce_grad_kernel<T, X>, a, 1, (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
+            ce_launch<X>(ce_grad_kernel<T, X>, a, dim3((unsigned)(a.tiles_m * a.tiles_n)), (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
         });
         if (p.few) {
             CeFew d = {};
@@ -1009,7 +1009,7 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
         hipLaunchKernelGGL((ce_few_finish_kernel<T>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 16)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
                            p.parts, (int)n, C, p.c4, factors, factor, static_cast<T *>(grad_x));
     else if (grad_x)
-        hipLaunchKernelGGL((ce_finish_kernel<T>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
+        hipLaunchKernelGGL((ce_finish_kernel<T>), grid_of(ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
                            p.parts, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));
     return check_launch("mvs_linear_ce_bwd");
 }

@@ -451,7 +451,7 @@ __global__ __launch_bounds__(256) void narrow_prepare_kernel(NarrowArgs a) {
 // both gradients from the parts' sums: workgroups of dx, then of dW
 template <typename T>
 __global__ __launch_bounds__(256) void narrow_finish_kernel(NarrowArgs a, int64_t groups_x) {
-    const int64_t id = blockIdx.x, count = ce_count(a.kept_rows);
+    const int64_t id = group_of(), count = ce_count(a.kept_rows);
     const NarrowSplit split = narrow_split(count, a.w.count, kNarrowGradSlots, a.sums_x != nullptr, a.sums_w != nullptr);
     if (id < groups_x)
         ce_finish<T, true>(a.sums_x, split.parts_x, a.x.count, count, a.kept_rows.place, a.C, a.ld_sums, a.factors, a.factor, static_cast<T *>(a.grad_x), id);
@@ -509,7 +509,7 @@ int ce_narrow_forward(int dtype, const NarrowArgs &a, hipStream_t st) {
 int ce_narrow_backward(int dtype, const NarrowArgs &a, hipStream_t st) {
     const int ks = a.Cp / 32;
     const int64_t quads = a.ld_sums / 4, fx = a.sums_x ? ceil_div(a.x.count * quads, 256) : 0, fw = a.sums_w ? ceil_div(a.w.count * quads, 256) : 0;
-    const dim3 finish((unsigned)(fx + fw));
+    const dim3 finish = grid_of(fx + fw);
     if (dtype == MVS_DTYPE_F32) {
         narrow_prepare<float, bf16_t, 3>(a, true, st);
         narrow_steps<bf16_t, 3>(ks, [&](auto x) { narrow_grads<decltype(x), float>(a, st); });

@@ -64,7 +64,7 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void lookup_fwd_kernel(const T *__restrict__ table, int64_t rows, int C, const int64_t *__restrict__ index,
                                                          int64_t n, float scale, T *__restrict__ out, int lanes) {
     const int lane = threadIdx.x & (lanes - 1), vecs = C / VEC;
-    const int64_t i = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    const int64_t i = group_of() * (256 / lanes) + threadIdx.x / lanes;
     if (i >= n) return;
     const int64_t row = index[i];
     const bool named = row >= 0 && row < rows;
@@ -270,9 +270,10 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void lookup_rows_kernel(LookupRows a) {
     const int tid = threadIdx.x, lane = tid & (a.lanes - 1), vecs = a.C / VEC;
     T *out = static_cast<T *>(a.out);
-    if (blockIdx.x >= a.sum_groups) {
+    const int64_t group = group_of();
+    if (group >= a.sum_groups) {
         __shared__ unsigned long long empty_rows;
-        const int64_t v0 = (blockIdx.x - a.sum_groups) * 64;
+        const int64_t v0 = (group - a.sum_groups) * 64;
         if (tid < 64) {
             const int64_t v = v0 + tid;
             bool empty = v < a.rows;
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(LookupRows a) {
         }
         return;
     }
-    const int64_t piece = (int64_t)blockIdx.x * (256 / a.lanes) + tid / a.lanes;
+    const int64_t piece = group * (256 / a.lanes) + tid / a.lanes;
     if (piece >= a.pieces) return;
     const int64_t p0 = piece * kPiece;
     const int count = (int)(a.n - p0 < kPiece ? a.n - p0 : kPiece);
@@ -466,7 +467,7 @@ static bool lookup_wide(const void *a, const void *b, int dtype, int C) { return
 template <typename T, int VEC>
 static void lookup_launch_fwd(const void *table, int64_t rows, int C, const int64_t *index, int64_t n, float scale, void *out, hipStream_t st) {
     const int lanes = min(64, lookup_lanes(C / VEC));      // (four accesses of a long row in flight per lane)
-    hipLaunchKernelGGL((lookup_fwd_kernel<T, VEC>), dim3((unsigned)((n * lanes + 255) / 256)), dim3(256), 0, st, static_cast<const T *>(table), rows, C, index,
+    hipLaunchKernelGGL((lookup_fwd_kernel<T, VEC>), grid_of((n * lanes + 255) / 256), dim3(256), 0, st, static_cast<const T *>(table), rows, C, index,
                        n, scale, static_cast<T *>(out), lanes);
 }
 
@@ -475,7 +476,7 @@ static void lookup_launch_rows(LookupRows a, hipStream_t st) {
     a.lanes = lookup_lanes(a.C / VEC);
     a.sum_groups = (a.pieces * a.lanes + 255) / 256;
     const int64_t zero_groups = (a.rows + 63) / 64;
-    hipLaunchKernelGGL((lookup_rows_kernel<T, VEC>), dim3((unsigned)(a.sum_groups + zero_groups)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((lookup_rows_kernel<T, VEC>), grid_of(a.sum_groups + zero_groups), dim3(256), 0, st, a);
     if (a.pieces > 1) {
         constexpr int JOIN = VEC == 1 ? 1 : 4;      // (rows of whole 16 bytes are whole float4 of sums)
         hipLaunchKernelGGL((lookup_join_kernel<T, JOIN>), dim3((unsigned)((a.pieces + kJoin - 1) / kJoin), (unsigned)((a.C + 64 * JOIN - 1) / (64 * JOIN))), dim3(256), 0, st, a);

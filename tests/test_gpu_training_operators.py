@@ -580,6 +580,53 @@ def test_linear_cross_entropy_with_a_table_beyond_2_to_31_elements(n):
         assert ((mine - want_w).abs() <= 3 * half_ulp(torch.bfloat16) * mag).all()
 
 
+def test_act8_off_alignment_beyond_2_to_32_values():
+    n = (1 << 32) + 100      # one lane a value: more threads than a grid's row has
+    x = torch.zeros(n + 1, device="cuda")[1:]
+    x[:100], x[-200:] = randn(100, seed=1), randn(200, seed=2)
+    held = ops.act8_quantize(x)
+    small = ops.act8_quantize(torch.cat([x[:128], x[-228:]]))
+    assert torch.equal(held.codes[:128], small.codes[:128]) and torch.equal(held.codes[-228:], small.codes[128:])
+    assert int(torch.count_nonzero(held.codes[128:-228])) == 0
+    del x
+    back = ops.act8_dequantize(held)
+    want = ops.act8_dequantize(small)
+    assert torch.equal(back[:128], want[:128]) and torch.equal(back[-228:], want[128:])
+
+
+def test_lookup_rows_of_more_than_2_to_32_threads():
+    rows, C, n = 11, 129, (1 << 26) + 5      # 64 lanes a row of odd length
+    table = randn(rows, C, seed=1).to(torch.float16)
+    index = torch.arange(n, device="cuda") % (rows + 1)      # (every twelfth names no row)
+    out = ops.lookup_rows(table, index)
+    padded = torch.cat([table, torch.zeros(1, C, device="cuda", dtype=table.dtype)])
+    for at in (0, n // 2, n - 4096):
+        assert torch.equal(out[at:at + 4096], padded[index[at:at + 4096]])
+
+
+def test_lookup_rows_gradient_of_more_than_2_to_30_rows():
+    rows, n = (1 << 30) + 77, 50
+    leaf = torch.zeros(rows, 1, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    index = torch.randint(rows, (n,), generator=gen(1), device="cuda")
+    index[0], index[1] = rows - 1, 0
+    g = randn(n, 1, seed=2).to(torch.bfloat16)
+    grad, = torch.autograd.grad(ops.lookup_rows(leaf, index), leaf, g)
+    assert torch.equal(grad[index], g)
+    grad[index] = 0
+    assert int(torch.count_nonzero(grad)) == 0
+
+
+def test_linear_cross_entropy_of_more_than_2_to_32_threads():
+    """Half a million rows against a million: a forward pass of 2^23 tiles of 512 threads."""
+    n, V, C = (1 << 19) + 3, (1 << 20) + 5, 136
+    x, w = randn(n, C, seed=1).to(torch.bfloat16), (randn(V, C, seed=2) * 0.1).to(torch.bfloat16)
+    t = torch.randint(V, (n,), generator=gen(3), device="cuda")
+    loss = ops.linear_cross_entropy(x, w, t, reduction="none")
+    for at in (0, n // 2, n - 40):
+        logits = x[at:at + 40].double() @ w.double().t()
+        want = torch.logsumexp(logits, 1) - logits.gather(1, t[at:at + 40].unsqueeze(1)).squeeze(1)
+        assert float((loss[at:at + 40].double() - want).abs().max()) < 1e-4
+
 def test_linear_cross_entropy_few_rows_in_pieces():
     """16 rows against a table of more than 2^26 / 16 rows: the one-pass kernel adds the second piece's sums to the first's."""
     n, V, C = 16, (1 << 22) + 777, 136
