@@ -88,8 +88,9 @@ def matching_cells(depth, src_proj, ref_proj, mask=None):
 
 def feature_matching_loss(ref_fea, src_fea, ref_cells, src_cells, temperature=1.0):
     """Cross entropy of finding a point's cell in the source view by its feature in the reference view: over the pairs (point) of
-    ref_cells, src_cells [B,P] (cell numbers y * w + x; -1 on either side: no such pair), the softmax of <ref feature, source
-    feature> / temperature over ALL cells of the source map, averaged over the pairs there are (NaN if there is none).
+    ref_cells, src_cells [B,P] (cell numbers y * w + x; -1 on either side: no such pair; a number beyond its map: NaN), the softmax of
+    <ref feature, source feature> / temperature over ALL cells of the source map, averaged over the pairs there are (NaN if there is
+    none).
     ref_fea, src_fea [B,C,h,w]; differentiable in both.  The [P, h*w] scores are never stored (ops.linear_cross_entropy), several
     points may share a cell (ops.lookup_rows)."""
     B, C, h, w = src_fea.shape
@@ -97,7 +98,7 @@ def feature_matching_loss(ref_fea, src_fea, ref_cells, src_cells, temperature=1.
     for b in range(B):
         rows = [f[b].permute(1, 2, 0).reshape(-1, C) for f in (ref_fea, src_fea)]
         paired = (ref_cells[b] >= 0) & (src_cells[b] >= 0)
-        target = torch.where(paired, src_cells[b], torch.full_like(src_cells[b], -100))
+        target = torch.where(paired, src_cells[b].masked_fill(ref_cells[b] >= rows[0].shape[0], h * w), -100)
         total = total + ops.linear_cross_entropy(ops.lookup_rows(rows[0], ref_cells[b]), rows[1], target, scale=1.0 / temperature,
                                                  reduction="sum")
     return total / ((ref_cells >= 0) & (src_cells >= 0)).sum()

@@ -560,13 +560,18 @@ class MVSNet(nn.Module):
     def matching_loss(self, imgs, proj_matrices, depth, mask=None, temperature=0.1):
         """Supervision of FeatureNet alone, from the depth the reference view is trained on: every reference cell with a depth has to
         find its cell in each source view among all of them (feature_matching_loss over matching_cells), averaged over the source
-        views.  imgs [B,V,3,H,W], proj_matrices [B,V,4,4], depth and mask [B,H/4,W/4].  Add it to mvsnet_loss, or train on it first;
-        training mode, FeatureNet's HIP layers (each view with its own batch statistics, as in forward())."""
+        views.  imgs [B,V,3,H,W], proj_matrices [B,V,4,4], depth and mask [B,H/4,W/4].  Train on it first, or add it to mvsnet_loss (a
+        second pass of FeatureNet, which counts as one more update of its running statistics); training mode, FeatureNet's HIP
+        layers (each view with its own batch statistics, as in forward())."""
         if not (self.training and self.feature.hip_supported()):
             raise ops.MvsHipError("matching_loss: a training step on FeatureNet's HIP layers (model.train())")
         if imgs.shape[1] != proj_matrices.shape[1] or imgs.shape[1] < 2:
             raise ops.MvsHipError(f"matching_loss: {imgs.shape[1]} images and {proj_matrices.shape[1]} projection matrices, two views at least")
         B, V = imgs.shape[:2]
+        want = (B, (imgs.shape[3] + 3) // 4, (imgs.shape[4] + 3) // 4)
+        for name, t in (("depth", depth), ("mask", mask)):
+            if t is not None and tuple(t.shape) != want:
+                raise ops.MvsHipError(f"matching_loss: {name} is {tuple(t.shape)}, the feature maps {want}")
         fea = self.feature.forward_train_hip(imgs.transpose(0, 1).reshape(V * B, *imgs.shape[2:]), groups=V, act8=self.train_act8)
         fea = fea.reshape(V, B, *fea.shape[1:]).permute(0, 1, 4, 2, 3)             # [V,B,C,h,w] views of channels-last maps
         here = torch.arange(fea.shape[3] * fea.shape[4], device=fea.device).expand(B, -1)

@@ -163,3 +163,22 @@ def test_model_matching_loss_trains_featurenet_only():
     assert res[0] == res[1] and math.isfinite(res[0])
     with pytest.raises(ops.MvsHipError, match="matching_loss"):
         model.eval().matching_loss(imgs, proj, gt)
+
+
+def test_matching_loss_refuses_another_grid_and_shows_cells_beyond_a_map():
+    model = MVSNet(refine=False).cuda().train()
+    imgs, proj, _, gt = _scene()
+    mask = torch.ones_like(gt)
+    before = model.feature.conv0.bn.running_mean.clone()
+    with pytest.raises(ops.MvsHipError, match="depth"):
+        model.matching_loss(imgs, proj, gt[:, :-1])
+    with pytest.raises(ops.MvsHipError, match="mask"):
+        model.matching_loss(imgs, proj, gt, mask[:, :, :-1])
+    assert torch.equal(model.feature.conv0.bn.running_mean, before)
+    fea = torch.randn(1, 32, 6, 7, device="cuda")
+    cells = torch.arange(5, device="cuda").unsqueeze(0)
+    assert math.isfinite(float(feature_matching_loss(fea, fea, cells, cells)))
+    for r, c in ((42, 3), (3, 42)):
+        ref, src = cells.clone(), cells.clone()
+        ref[0, 2], src[0, 2] = r, c
+        assert math.isnan(float(feature_matching_loss(fea, fea, ref, src)))
