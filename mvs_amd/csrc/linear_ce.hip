@@ -3,17 +3,23 @@
 //   forward    a tile of logits lives in the matrix cores' accumulators and leaves as one (max, sum of exponentials) per row and
 //              tile; a second launch joins a row's tiles.  2 N V C operations, (N + V) C elements read.
 //   backward   dl = (p - 1[t]) g needs the logits again: a piece of the table at a time (N * piece <= 2^26, so that what it writes
-//              stays in the last-level cache), one launch forms the tile's logits once more and writes dl and its transpose,
-//              rounded to the operands' type; two products follow, dx += dl W and dW = dl^T x.  6 N V C operations: 8 in all, of
-//              which 6 are the definition's and 2 buy the N V logits not being kept.
+//              stays in the last-level cache), one launch forms the tile's logits once more and writes dl, rounded to the operands'
+//              type; two products follow, dx += dl W and dW = dl^T x.  6 N V C operations: 8 in all, of which 6 are the
+//              definition's and 2 buy the N V logits not being kept.
 //
-// All four products are one kernel shape: C[m][n] = sum_k A[m][k] B[n][k] with both operands contiguous along k -- x, W, dl and dl^T
-// are so by themselves, W^T and x^T are written by a transposing pass (W piece by piece).  A workgroup owns a BM x BN tile and
-// walks k in 128-byte steps: rows of both operands go from memory to LDS by DMA, two stages, the 16-byte chunks of a row exchanged by
-// its low three bits (chunk ^ row & 7) so that the fragment reads of 16 rows spread over the banks; a lane's 16-byte chunk is one
-// 16x16x32 fragment (16 bits) or four 16x16x4 ones (float32: lane group g holds k = 4 g + j for the j-th, on both sides).
+// All four products are one kernel shape, C[m][n] = sum_k A[m][k] B[n][k].  A workgroup owns a BM x BN tile and walks k in 128-byte
+// steps: both operands go from memory to LDS by DMA, two stages, the 16-byte chunks of a row exchanged by a few bits of its number so
+// that what a wave reads spreads over the banks.  An operand whose rows run along k lies there as BM rows of 128 bytes, a lane's 16
+// bytes are one 16x16x32 fragment (16 bits) or four 16x16x4 ones (float32: lane group g holds k = 4 g + j for the j-th, on both
+// sides).  Of 16 bits, an operand whose rows run along the tile -- W in dx, x and dl in dW -- lies there as 64 rows of k and is read
+// by columns (ds_read_b64_tr_b16), so nothing is transposed in memory: against a pass that transposed W and x and a dl^T beside dl,
+// the backward pass of 583 x 49999 x 768 float16 takes 229 instead of 297 us, of 8192 x 64000 x 2048 bfloat16 5.30 instead of 5.64 ms.
+// float32, rows with factors of their own (reduction 'none') and few rows have those transposes.
 // m runs over table rows or channels, n over the rows of x or of W: a lane of the accumulator then holds four consecutive m of one
 // n, so a row's softmax statistics reduce within the lane first, and results leave as vectors.
+//
+// Bound by the matrix cores: 256 x 256 tiles reach 1340 TFLOP/s in the statistics of 8192 x 64000 x 2048 bfloat16 and 1250 in its
+// products (a library product of those operands 1400), half of what the cores could issue at 2.4 GHz.
 //
 // Numbers: sums, statistics and exponentials in float32, exponents in base 2 (one rounding of scale * log2 e per logit, the same
 // one in both passes, so a row's p sum to one).  16-bit dl: float16 carries it times 2^14 (|p - 1| <= 1: no overflow, and p down to
@@ -38,44 +44,112 @@ struct Tile {
     static constexpr int PER_WAVE = (COPIES + WAVES - 1) / WAVES;
 };
 
-// acc[tm][tn] += the tile (m0, n0) of A B^T over `steps` 128-byte steps of k
-template <typename T, typename X>
-__device__ __forceinline__ void tile_product(const Operand &a, const Operand &b, int64_t m0, int64_t n0, int64_t k_byte0, int steps, char *lds,
+// A lane's 16 bytes at base + offset -> LDS byte address `to` + 16 * lane (the copy of glds16 with a wave's base in scalar registers,
+// which the vector unit may have written just before: five instructions' wait).
+__device__ __forceinline__ void copy16(const char *base, unsigned offset, unsigned to) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\t"
+                 "global_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(offset), "s"(base), "s"(to)
+                 : "memory");
+}
+
+// Four rows of 16 elements, 16 bits each: lane 4 r + q of a group of 16 points at elements 4 q .. 4 q + 3 of row r, lane i gets the
+// column i.
+__device__ __forceinline__ uint2 read_columns(const char *at) {
+    typedef short four_t __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) four_t *)(uintptr_t)(unsigned)(uintptr_t)at));
+}
+
+// One operand in LDS: `SIDE` tile rows of 128 bytes of k -- or, ALONG (16 bits), 64 rows of k of SIDE elements, as a matrix has them whose
+// rows run along the tile: its fragments are read as columns.  The 16-byte chunks of a row are exchanged by a few bits of its number,
+// so that what a wave reads at once lies in different banks.
+template <int SIDE, bool ALONG>
+struct Stage {
+    static constexpr bool COLUMNS = ALONG;
+    static constexpr int ROW = ALONG ? 2 * SIDE : kRowBytes, CHUNKS = ROW / 16, ROWS = 64 / CHUNKS;      // (ROWS: of one copy of 1 KiB)
+    static __device__ __forceinline__ int exchange(int row) { return ALONG ? ((row & 3) | (row >> 1 & 4)) * 2 : row & 7; }
+    static __device__ __forceinline__ int row_of(int copy, int lane) { return copy * ROWS + lane / CHUNKS; }
+    // byte offset, from the tile's corner, of what lane `lane` of copy `copy` moves; beyond the matrix' last tile row or column: that again
+    static __device__ __forceinline__ unsigned offset(const Operand &o, int64_t tile0, int copy, int lane) {
+        const int row = row_of(copy, lane), chunk = (lane % CHUNKS) ^ exchange(row);
+        if (ALONG) return (unsigned)row * (unsigned)o.ld + (unsigned)min((int64_t)chunk * 16, o.ld - 16 - tile0 * 2);
+        return (unsigned)min((int64_t)row, o.rows - 1 - tile0) * (unsigned)o.ld + chunk * 16;
+    }
+};
+
+// acc[tm][tn] += the tile (m0, n0) of A B^T over the 128-byte steps first .. first + steps - 1 of k (16 bits: 64 elements).  A_ALONG,
+// B_ALONG: that operand is given with k along its rows, [k][m] or [k][n].  The steps are walked backward: the one that may end behind
+// the last row of k is then the first, and the only copy that has to look.
+template <typename T, typename X, bool A_ALONG = false, bool B_ALONG = false>
+__device__ __forceinline__ void tile_product(const Operand &a, const Operand &b, int64_t m0, int64_t n0, int first, int steps, char *lds,
                                              f32x4_t (&acc)[X::TM][X::TN]) {
+    static_assert((!A_ALONG && !B_ALONG) || sizeof(T) == 2, "columns are read of 16-bit elements");
+    using SA = Stage<X::BM, A_ALONG>;
+    using SB = Stage<X::BN, B_ALONG>;
+    if (steps <= 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
     const unsigned lds_base = (unsigned)(uintptr_t)lds;
-    // copy c moves the tile rows 8 c .. 8 c + 7 (A's, then B's): lane i = row 8 c + i / 8, LDS chunk i % 8
-    if (steps <= 0) return;
-    const int r8 = lane >> 3, chunk = (lane & 7) ^ r8;
-    const char *from[X::PER_WAVE];
+    // copy c moves 1 KiB of the stage, A's and then B's
+    constexpr int COPIES_A = X::BM / 8, PER_A = COPIES_A / X::WAVES;
+    static_assert(COPIES_A % X::WAVES == 0 && X::COPIES % X::WAVES == 0, "whole copies per wave, of one operand each");
+    const int64_t last = first + steps - 1;
+    const char *base_a = a.p + (A_ALONG ? last * 64 * a.ld + m0 * 2 : m0 * a.ld + last * kRowBytes);
+    const char *base_b = b.p + (B_ALONG ? last * 64 * b.ld + n0 * 2 : n0 * b.ld + last * kRowBytes);
+    unsigned offset[X::PER_WAVE];
 #pragma unroll
     for (int i = 0; i < X::PER_WAVE; ++i) {
         const int c = wave + i * X::WAVES;
-        const bool of_a = c < X::BM / 8;
-        const int64_t row = of_a ? m0 + c * 8 + r8 : n0 + (c - X::BM / 8) * 8 + r8;
-        const Operand &o = of_a ? a : b;
-        from[i] = o.p + (row < o.rows ? row : o.rows - 1) * o.ld + k_byte0 + chunk * 16;
+        offset[i] = i < PER_A ? SA::offset(a, m0, c, lane) : SB::offset(b, n0, c - COPIES_A, lane);
     }
-    auto copy = [&](int stage, int advance = kRowBytes) {
+    auto issue = [&](int stage, int i, unsigned from) {
+        copy16(i < PER_A ? base_a : base_b, from, lds_base + (unsigned)(stage * X::STAGE + (wave + i * X::WAVES) * 1024));
+    };
+    auto retreat = [&](bool really) {
+        base_a -= really ? (A_ALONG ? 64 * a.ld : kRowBytes) : 0;
+        base_b -= really ? (B_ALONG ? 64 * b.ld : kRowBytes) : 0;
+    };
+    auto copy = [&](int stage, bool more = true) {
+#pragma unroll
+        for (int i = 0; i < X::PER_WAVE; ++i) issue(stage, i, offset[i]);
+        retreat(more);
+    };
+    auto copy_first = [&] {
 #pragma unroll
         for (int i = 0; i < X::PER_WAVE; ++i) {
             const int c = wave + i * X::WAVES;
-            if (X::COPIES % X::WAVES == 0 || c < X::COPIES) {
-                glds16(from[i], lds_base + (unsigned)(stage * X::STAGE + c * 1024));
-                from[i] += advance;
+            const bool of_a = i < PER_A;
+            unsigned from = offset[i];
+            if (of_a ? A_ALONG : B_ALONG) {
+                const Operand &o = of_a ? a : b;
+                const int64_t behind = last * 64 + (of_a ? SA::row_of(c, lane) : SB::row_of(c - COPIES_A, lane)) - (o.rows - 1);
+                if (behind > 0) from -= (unsigned)behind * (unsigned)o.ld;
             }
+            issue(0, i, from);
         }
+        retreat(steps > 1);
     };
     const int frow = lane & 15, fk = lane >> 4;
-    const int swz0 = (fk ^ (frow & 7)) * 16, swz1 = ((4 + fk) ^ (frow & 7)) * 16;
-    const int a_row = (wm * (X::BM / X::WAVES_M) + frow) * kRowBytes, b_row = (X::BM + wn * (X::BN / X::WAVES_N) + frow) * kRowBytes;
-    auto read = [&](int stage, int swz, u32x4_t (&fa)[X::TM], u32x4_t (&fb)[X::TN]) {
-        const char *at = lds + stage * X::STAGE + swz;
+    // a fragment: 16 tile rows x 64 bytes of k (half a step); a lane's 16 bytes are 8 k of one tile row, or four of each of its two reads
+    const int col_row = 8 * fk + (frow >> 2), col_swz = Stage<X::BM, true>::exchange(col_row);
+    auto fragment = [&](auto side, const char *at, int tile_row, int half) {
+        using S = decltype(side);
+        if constexpr (!S::COLUMNS) {
+            return *reinterpret_cast<const u32x4_t *>(at + (tile_row + frow) * S::ROW + (((4 * half + fk) ^ (frow & 7)) * 16));
+        } else {
+            const char *from = at + (half * 32 + col_row) * S::ROW + (((tile_row / 8) ^ col_swz) * 16) + (frow & 3) * 8;
+            const uint2 low = read_columns(from), high = read_columns(from + 4 * S::ROW);
+            return u32x4_t{low.x, low.y, high.x, high.y};
+        }
+    };
+    auto read = [&](int stage, int half, u32x4_t (&fa)[X::TM], u32x4_t (&fb)[X::TN]) {
+        const char *at = lds + stage * X::STAGE;
 #pragma unroll
-        for (int i = 0; i < X::TM; ++i) fa[i] = *reinterpret_cast<const u32x4_t *>(at + a_row + i * 16 * kRowBytes);
+        for (int i = 0; i < X::TM; ++i) fa[i] = fragment(SA(), at, wm * (X::BM / X::WAVES_M) + i * 16, half);
 #pragma unroll
-        for (int j = 0; j < X::TN; ++j) fb[j] = *reinterpret_cast<const u32x4_t *>(at + b_row + j * 16 * kRowBytes);
+        for (int j = 0; j < X::TN; ++j) fb[j] = fragment(SB(), at + X::BM * kRowBytes, wn * (X::BN / X::WAVES_N) + j * 16, half);
     };
     auto multiply = [&](const u32x4_t (&fa)[X::TM], const u32x4_t (&fb)[X::TN], int first, int last) {
 #pragma unroll
@@ -84,7 +158,7 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
 #pragma unroll
                 for (int j = 0; j < X::TN; ++j) mma16(acc[i][j], fa[i], fb[j], T());
     };
-    copy(0);
+    copy_first();
     if constexpr (X::AHEAD) {
         // The fragments of a half step are read while the matrix cores work on the half before it, across the stages' border too:
         //     read second half of s | first half's products, half of them | stage s + 1 has landed, s is read out | copy s + 2 into
@@ -93,42 +167,47 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
         // the reads it would have the compiler wait for them at once.  So the last two steps' copies read the last step's bytes
         // again, into a stage that is not read any more, and the last step's products stand behind the loop.
         constexpr int HALF = X::TM / 2;
-        auto pace = [] {      // one read behind each of the first products
+        auto pace = [] {      // a fragment's read behind each of the first products (masks: matrix instructions, LDS reads)
 #pragma unroll
-            for (int i = 0; i < X::TM + X::TN; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // matrix instructions
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // LDS reads
+            for (int i = 0; i < X::TM; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, A_ALONG ? 2 : 1, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < X::TN; ++j) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, B_ALONG ? 2 : 1, 0);
             }
         };
         u32x4_t a0[X::TM], b0[X::TN], a1[X::TM], b1[X::TN];
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (steps > 1) copy(1, steps > 2 ? kRowBytes : 0);
-        read(0, swz0, a0, b0);
+        if (steps > 1) copy(1, steps > 2);
+        read(0, 0, a0, b0);
         int stage = 0;
         for (int s = 0; s + 1 < steps; ++s, stage ^= 1) {
-            read(stage, swz1, a1, b1);
+            read(stage, 1, a1, b1);
             multiply(a0, b0, 0, HALF);
             pace();
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();      // (waits for this wave's reads too: the stage may be overwritten)
-            const int advance = s + 3 < steps ? kRowBytes : 0;
+            const bool more = s + 3 < steps;
             if constexpr (X::LATE) {
                 multiply(a0, b0, HALF, X::TM);
                 __builtin_amdgcn_sched_barrier(0);
-                copy(stage, advance);
+                copy(stage, more);
                 __builtin_amdgcn_sched_barrier(0);
             } else {
-                copy(stage, advance);
+                copy(stage, more);
                 multiply(a0, b0, HALF, X::TM);
             }
-            read(stage ^ 1, swz0, a0, b0);
+            read(stage ^ 1, 0, a0, b0);
             multiply(a1, b1, 0, X::TM);
             pace();
             if constexpr (X::LATE) __builtin_amdgcn_sched_barrier(0);
         }
-        read(stage, swz1, a1, b1);
+        read(stage, 1, a1, b1);
         multiply(a0, b0, 0, X::TM);
         multiply(a1, b1, 0, X::TM);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the copies of the last steps, before LDS is used for something else
@@ -140,7 +219,7 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 u32x4_t fa[X::TM], fb[X::TN];
-                read(s & 1, half ? swz1 : swz0, fa, fb);
+                read(s & 1, half, fa, fb);
                 multiply(fa, fb, 0, X::TM);
             }
         }
@@ -174,6 +253,7 @@ struct CeArgs {
     const float *lse2, *ratio;
     void *dl, *dlt;                     // [n][ld_dl], [v][ld_dlt]; either may be NULL
     int64_t ld_dl, ld_dlt;
+    int dl_step;                        // dl has rows of zeros behind the last kept one, up to a multiple of this
 };
 
 // How far row t of the table lies beyond a lane's first, v_lane, where it is within the wave's rows (16 i + r: the lane's own are
@@ -340,6 +420,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
     const int m_lane = wm * (X::BM / X::WAVES_M) + (lane >> 4) * 4;
     const bool ends = m0 + X::BM > a.v_count;      // the piece ends in this tile
+    const int64_t dl_rows = (rows + a.dl_step - 1) / a.dl_step * a.dl_step;
     __syncthreads();      // the stages have been read: LDS holds the transpose from here on
 #pragma unroll
     for (int j = 0; j < X::TN; ++j) {
@@ -377,7 +458,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
                 if (a.dlt) *reinterpret_cast<T *>(lds + (m_lane + i * 16 + r) * PITCH + nl * (int)sizeof(T)) = from_float<T>(kept ? d * ratio : 0.0f);
             }
             const int64_t m = m0 + m_lane + i * 16;
-            if (a.dl && n < rows && m < a.ld_dl) *reinterpret_cast<Pack<T, 4> *>(static_cast<T *>(a.dl) + n * a.ld_dl + m) = out;
+            if (a.dl && n < dl_rows && m < a.ld_dl) *reinterpret_cast<Pack<T, 4> *>(static_cast<T *>(a.dl) + n * a.ld_dl + m) = out;
         }
     }
     if (!a.dlt) return;
@@ -405,7 +486,7 @@ struct CeProduct {
     const int *count;       // kept rows: n (sums) or the extent of k (out) is at most that; NULL: as given
 };
 
-template <typename T, typename X>
+template <typename T, typename X, bool A_ALONG, bool B_ALONG>
 __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
     extern __shared__ __align__(1024) char lds[];
     if (a.count) {
@@ -413,6 +494,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
             a.n = a.b.rows = *a.count;
             a.tiles_n = (a.n + X::BN - 1) / X::BN;
         } else {
+            if (A_ALONG) a.a.rows = *a.count;      // (dl has rows of zeros behind the last kept one)
             a.steps = a.steps_per_part = (int)((*a.count * (int64_t)sizeof(T) + kRowBytes - 1) / kRowBytes);
         }
     }
@@ -421,7 +503,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
     const int64_t m0 = tm * X::BM, n0 = tn * X::BN;
     const int first = blockIdx.y * a.steps_per_part, steps = min(a.steps_per_part, a.steps - first);
     f32x4_t acc[X::TM][X::TN] = {};
-    tile_product<T, X>(a.a, a.b, m0, n0, (int64_t)first * kRowBytes, steps, lds, acc);
+    tile_product<T, X, A_ALONG, B_ALONG>(a.a, a.b, m0, n0, first, steps, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
     const float f = a.sums ? 1.0f : *a.top * a.factor;
 #pragma unroll
@@ -701,7 +783,7 @@ struct CePlan {
 // transpose of such a tile does not fit LDS) -- half the LDS and L2 traffic per operation.
 using Tile128 = Tile<128, 128, 2, 2, false>;
 using Tile256 = Tile<256, 256, 2, 4, true>;
-// The statistics read the whole table once, from memory, and take the copies late better (8192 x 64000 x 2048: 1.60 ms against 1.70);
+// The statistics read the whole table once, from memory, and take the copies late better (8192 x 64000 x 2048: 1.58 ms against 1.70);
 // the backward pass' products read a piece that the caches hold, and take them early (dx's 1.80 ms against 1.96).
 using Tile256Late = Tile<256, 256, 2, 4, true, true>;
 
@@ -764,9 +846,11 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
             p.dl = take((size_t)n * p.piece * p.es);
             p.parts = (int)ceil_div(V < p.piece ? V : p.piece, kFewTable);
             if (need_x) p.sums = take((size_t)p.parts * n * p.c4 * 4);
-        } else if (need_x) {
-            p.dl = take((size_t)n * p.piece * p.es);
-            p.wt = take((size_t)C * p.piece * p.es);
+        } else {
+            if (need_x || p.es == 2) p.dl = take((size_t)p.np * p.piece * p.es);
+            if (need_x && p.es == 4) p.wt = take((size_t)C * p.piece * p.es);
+        }
+        if (need_x && !p.few) {
             const int64_t side = ce_big(C, n, p.es) ? 256 : 128, tiles = ceil_div(C, side) * ceil_div(n, side), steps = round_up(V < p.piece ? V : p.piece, step) / step;
             // parts of k: as many workgroups as one round of the chip takes (two per CU), at least 8 steps each
             int64_t parts = side == 256 || tiles == 0 ? 1 : 512 / tiles;
@@ -818,6 +902,10 @@ static int ce_check(const char *who, const void *x, const void *w, int dtype, co
     }
     if (n > ((int64_t)1 << 29) || V > ((int64_t)1 << 29) || C > (1 << 20) || ceil_div(n, 64) * ceil_div(V, 64) > 0x7fffffff) {
         set_error("%s: n=%lld, V=%lld (at most 2^29 each, n V / 4096 below 2^31), C=%d (at most 2^20)", who, (long long)n, (long long)V, C);
+        return MVS_EUNSUPPORTED;
+    }
+    if (n > ((int64_t)1 << 23) && !ce_narrow(C, dtype)) {      // (a tile's rows of dl^T are addressed in 32 bits)
+        set_error("%s: n=%lld rows of C=%d, at most 2^23 of that length at a time", who, (long long)n, C);
         return MVS_EUNSUPPORTED;
     }
     if (workspace_bytes < need) {
@@ -949,16 +1037,20 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
     const char *w_rows = a.w.p;
     a.scale2 = scale * kLog2e;
     a.lse2 = lse; a.ratio = factors + n;
-    a.dl = grad_x || p.few ? ws + p.dl : nullptr;
-    a.dlt = grad_w && !p.few ? ws + p.dlt : nullptr;
+    // dW's product takes dl and x as they are, k along their rows, where it can: 16 bits, no row in between that is ignored, one factor
+    // for all rows (else dl^T carries the rows' ratios).
+    const bool along = sizeof(T) == 2 && p.together && reduction != 0;
+    a.dl = grad_x || p.few || (along && grad_w) ? ws + p.dl : nullptr;
+    a.dlt = grad_w && !p.few && !along ? ws + p.dlt : nullptr;
     a.ld_dlt = p.np;
+    a.dl_step = along ? step : 1;      // (dW's product reads whole steps of rows; along: dl has p.np of them)
     // x^T once; ignored rows as zeros, whatever they hold
     if (a.dlt) ce_transpose<T>(a.x.p, rows, !p.together, C, p.Cp, ws + p.xt, p.np, st);
-    auto product = [&](CeProduct &d) {
+    auto product = [&](CeProduct &d, auto a_along, auto b_along) {
         ce_tiles<T>(d.m, d.n, [&](auto x) {
             using X = decltype(x);
             d.tiles_m = ceil_div(d.m, X::BM); d.tiles_n = ceil_div(d.n, X::BN);
-            ce_launch<X>(ce_product_kernel<T, X>, d, dim3((unsigned)(d.tiles_m * d.tiles_n), (unsigned)ceil_div(d.steps, d.steps_per_part)), 0, st);
+            ce_launch<X>(ce_product_kernel<T, X, decltype(a_along)::value, decltype(b_along)::value>, d, dim3((unsigned)(d.tiles_m * d.tiles_n), (unsigned)ceil_div(d.steps, d.steps_per_part)), 0, st);
         });
     };
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
@@ -983,11 +1075,15 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             continue;
         }
         if (grad_x) {
-            CeRows table = {};
-            table.n = count;
-            ce_transpose<T>(a.w.p, table, false, C, p.Cp, ws + p.wt, k, st);
             CeProduct d = {};
-            d.a = Operand{ws + p.wt, k * p.es, C};
+            if constexpr (sizeof(T) == 2) {
+                d.a = a.w;
+            } else {
+                CeRows table = {};
+                table.n = count;
+                ce_transpose<T>(a.w.p, table, false, C, p.Cp, ws + p.wt, k, st);
+                d.a = Operand{ws + p.wt, k * p.es, C};
+            }
             d.b = Operand{ws + p.dl, k * p.es, n};
             d.steps = (int)(k / step);
             d.steps_per_part = (int)ceil_div(d.steps, p.parts);
@@ -995,18 +1091,26 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             d.sums = reinterpret_cast<float *>(ws + p.sums); d.ld_sums = p.c4; d.sum_rows = n; d.count = rows.count;
             d.add = v0 > 0;
             // (a smaller last piece may have fewer parts of k: the sums of the others stay as they are)
-            product(d);
+            product(d, std::bool_constant<sizeof(T) == 2>(), std::false_type());
         }
         if (grad_w) {
             CeProduct d = {};
-            d.a = Operand{ws + p.xt, p.np * p.es, C};
-            d.b = Operand{ws + p.dlt, p.np * p.es, count};
             d.steps = (int)(p.np / step);
             d.steps_per_part = d.steps;
             d.m = C; d.n = count;
             d.out = static_cast<T *>(grad_w) + v0 * C;
             d.top = factors + 2 * n; d.factor = factor; d.count = rows.count;
-            product(d);
+            if constexpr (sizeof(T) == 2) {
+                if (along) {
+                    d.a = a.x;
+                    d.b = Operand{ws + p.dl, k * p.es, p.np};
+                    product(d, std::true_type(), std::true_type());
+                    continue;
+                }
+            }
+            d.a = Operand{ws + p.xt, p.np * p.es, C};
+            d.b = Operand{ws + p.dlt, p.np * p.es, count};
+            product(d, std::false_type(), std::false_type());
         }
     }
     if (grad_x && p.few)

@@ -135,7 +135,7 @@ def test_linear_ce_entry_points_refuse_bad_arguments(call):
                    dict(x=ODD), dict(w=ODD), dict(ws=ODD), dict(lse=None), dict(kept=None)):
         assert _ce(call, **change) == EINVAL, change
         assert f"mvs_linear_ce_{call}" in _text()
-    for change in (dict(n=1 << 31), dict(V=1 << 31), dict(C=1 << 21), dict(n=1 << 24, V=1 << 24)):
+    for change in (dict(n=1 << 31), dict(V=1 << 31), dict(C=1 << 21), dict(n=1 << 24, V=1 << 24), dict(n=(1 << 23) + 1, C=129)):
         assert _ce(call, nbytes=1 << 60, **change) == EUNSUPPORTED, change
     assert _ce(call, nbytes=64) == EWORKSPACE
     assert _ce("fwd", loss=None) == EINVAL
