@@ -724,7 +724,7 @@ int mvs_bn_train_bwd_act8_f32(const float *grad_y, const signed char *codes, con
 /* Rows of a table by index, times `scale`: out[i] = scale * table[index[i]], computed in float32 and rounded once.  table
  * [rows, C], out [n, C] contiguous, of one type; index int64.  An index outside [0, rows) names no row: out[i] = 0 and no
  * gradient.  The gradient (grad_table overwritten) is summed in float32 in the order of i -- the indices are sorted, stably, in
- * the workspace; no floating-point atomics, so equal calls give equal bits.  C at most 2^20. */
+ * the workspace; no floating-point atomics, so equal calls give equal bits.  C at most 2^20, rows and n below 2^31 - 1. */
 int mvs_lookup_rows_fwd(const void *table, int dtype, int64_t rows, int C, const int64_t *index, int64_t n, float scale, void *out,
                         void *stream);
 size_t mvs_lookup_rows_workspace_bytes(int64_t rows, int C, int64_t n);
@@ -741,7 +741,8 @@ int mvs_lookup_rows_bwd(const void *grad_out, int dtype, const int64_t *index, i
  * Backward: grad_loss [n] (reduction 0) or [1]; grad_x [n, C] and grad_weight [V, C] in the operands' type, either may be NULL.
  * The logits are formed again, a piece of the table at a time; the workspace (mvs_linear_ce_workspace_bytes; backward != 0 for
  * the backward pass, with need_x / need_w for the gradients asked for) holds a piece's gradient, transposes of the operands' size
- * and partial sums.  No atomics: equal calls give equal bits. */
+ * and partial sums.  No atomics: equal calls give equal bits.  At most 2^29 rows of either kind (2^23 rows of x where a row is
+ * longer than 64 float32 or 128 16-bit values), C at most 2^20. */
 size_t mvs_linear_ce_workspace_bytes(int64_t n, int64_t V, int C, int dtype, int backward, int need_x, int need_w);
 int mvs_linear_ce_fwd(const void *x, const void *weight, int dtype, const int64_t *target, int64_t n, int64_t V, int C, float scale,
                       int64_t ignore_index, int reduction, float *loss, float *lse, float *kept, void *workspace,

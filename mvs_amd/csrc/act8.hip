@@ -2,7 +2,8 @@
 //
 // Both directions are bound by the memory they move, n (e + 1 + 1/32) bytes for elements of e bytes.  A lane moves 16 bytes of
 // the wide side per access, so a block of 32 is 8 lanes (float32) or 4 (16 bits) and its maximum a few lane exchanges; kUnroll
-// accesses of a lane are issued together.  Measured figures: see kUnroll below.
+// accesses of a lane are issued together.  16.9 million bfloat16 values: to codes 12.4 us, back 9.4 us (4.1 and 5.5 TB/s; a copy of
+// memory of that size moves 5.1); 655360 float32 values, a feature map: 3.6 and 3.2 us, which is what an empty launch takes.
 #include "act8.h"
 #include "dtype.h"
 

@@ -17,7 +17,9 @@
 // products.  dl is split the same way in the registers.
 //
 // Operations: 10 N V C forward and backward (the logits three times) instead of 8, all on chip.  A 32 x 32 block of logits costs a
-// wave 24 + 24 matrix instructions of 16 cycles (float32, C = 32, a gradient) and about as many cycles of exponentials and splitting.
+// wave 24 + 24 matrix instructions of 16 cycles (float32, C = 32, a gradient) and about as many cycles of exponentials and splitting,
+// so the gradients are bound by both pipes at once: of 14336 x 20480 x 32 float32 they take 377 us, the matrix cores busy 54 % of it
+// and the vector unit 67 %; the statistics 118 us.  919 x 20480 x 32: gradients 36 us, statistics 14 us, the copies in pieces 7 us a pass.
 #include "linear_ce.h"
 
 namespace mvs {

@@ -2,7 +2,8 @@
 //
 //   out[i] = s T[index i]            grad T[v] = s sum over {i : index i = v}, in the order of i, of g[i]
 //
-// Forward: bound by the rows it reads and writes; 16 bytes per lane, a power-of-two number of lanes per row.
+// Forward: bound by the rows it reads and writes; 16 bytes per lane, a power-of-two number of lanes per row (65536 of 128000 rows of
+// 4 KiB, a few of them most of the batch: 91 us; 1021 rows of 128 bytes: 2.4 us).
 //
 // Backward: every row of the dense gradient is written once, most of them as zeros, and every row of g is read once.  Who adds to a
 // row is known only after the indices are sorted.  The sort is stable, so a row's terms come in the order of i and equal calls
@@ -16,6 +17,9 @@
 //          rows per wave's worth of lanes).
 //   join   the partial sums of the runs that leave their piece, in order: short runs a wave each, long ones four spans of pieces at
 //          a time.  A run's end is found 64 pieces per look.
+// Bound by memory for large ones: 65536 rows of 4 KiB into 128000 (268 MB read, 524 MB written) sort 32 us, rows 178 us (4.5 TB/s),
+// join 42 us; by latency for small ones: 1021 rows of 128 bytes into 20480 sort 5.8, rows 7.9, join 3.4 us.  The rank sort takes
+// 5.8 us for 1021 and 16.9 us for 8191 indices, where the radix sort's six launches take 32.
 #include <utility>
 
 #include "dtype.h"
