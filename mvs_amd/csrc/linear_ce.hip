@@ -226,17 +226,37 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
     }
 }
 
-// Which tile a workgroup owns: the XCDs take consecutive runs of the list (each has its own L2), and the list walks 8 m-tiles wide
-// columns of the grid, so that the tiles an XCD works on share rows of both operands.
-// False for a workgroup that none is left for (fewer tiles than the host could tell).
-__device__ __forceinline__ bool tile_of(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn) {
-    if (id >= tiles_m * tiles_n) return false;
-    const int64_t total = tiles_m * tiles_n, per = total >> 3, extra = total & 7, xcd = id & 7;
-    const int64_t at = xcd * per + (xcd < extra ? xcd : extra) + (id >> 3);
+// Which tile, and which of the parts that k is cut into, a workgroup owns.  The list is part by part, within it 8 m-tiles wide columns
+// of the grid; the XCDs take consecutive runs of it (each has its own L2), so that the tiles an XCD works on share rows of both
+// operands.  False for a workgroup that none is left for (fewer tiles than the host could tell).
+__device__ __forceinline__ bool tile_of(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t parts, int64_t &tm, int64_t &tn, int64_t &part) {
+    const int64_t tiles = tiles_m * tiles_n, total = tiles * parts;
+    if (id >= total) return false;
+    const int64_t per = total >> 3, extra = total & 7, xcd = id & 7;
+    int64_t at = xcd * per + (xcd < extra ? xcd : extra) + (id >> 3);
+    part = at / tiles;
+    at -= part * tiles;
     const int64_t band = at / (8 * tiles_n), wide = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8, in = at - band * 8 * tiles_n;
-    tm = band * 8 + in % wide;
-    tn = in / wide;
+    // (one number for the workgroup, in scalar registers, where the copies' bases come from it)
+    tm = __builtin_amdgcn_readfirstlane((int)(band * 8 + in % wide));
+    tn = __builtin_amdgcn_readfirstlane((int)(in / wide));
+    part = __builtin_amdgcn_readfirstlane((int)part);
     return true;
+}
+__device__ __forceinline__ bool tile_of(int64_t id, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn) {
+    int64_t part;
+    return tile_of(id, tiles_m, tiles_n, 1, tm, tn, part);
+}
+
+// How many parts dx's product cuts k into, of `steps` in the first piece of the table: as many workgroups as one round of the chip takes
+// (two of the small tiles per CU), at least 8 steps each.  Worked out alike on the device, which knows how many rows are kept.
+constexpr int64_t kRound = 512;
+__host__ __device__ inline int64_t ce_parts(int64_t count, int C, int64_t steps, bool big) {
+    const int64_t tiles = ((C + 127) / 128) * ((count + 127) / 128);
+    int64_t parts = big || tiles == 0 ? 1 : kRound / tiles;
+    if (parts > steps / 8) parts = steps / 8;
+    if (parts < 1) parts = 1;
+    return (steps + (steps + parts - 1) / parts - 1) / ((steps + parts - 1) / parts);      // (as many as get work)
 }
 
 struct CeArgs {
@@ -472,13 +492,13 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
     }
 }
 
-// out[n][m] (+)= factor * sum_k A[m][k] B[n][k]; blockIdx.y = part of k
+// out[n][m] (+)= factor * sum_k A[m][k] B[n][k]
 struct CeProduct {
     Operand a, b;
-    int steps, steps_per_part;
+    int steps, first_steps; // of k, of the first piece's k
     int64_t m, n, tiles_m, tiles_n;
-    float *sums;            // float32 sums [part][n][ld_sums] (added to if `add`), or NULL: `out` is written
-    int64_t ld_sums, sum_rows;
+    float *sums;            // float32 sums [part][n][ld_sums] (added to if `add`), or NULL: `out` is written, k is not cut
+    int64_t ld_sums;
     int add;
     void *out;              // [n][m] of T
     const float *top;       // `out` = sum * *top * factor
@@ -495,13 +515,14 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
             a.tiles_n = (a.n + X::BN - 1) / X::BN;
         } else {
             if (A_ALONG) a.a.rows = *a.count;      // (dl has rows of zeros behind the last kept one)
-            a.steps = a.steps_per_part = (int)((*a.count * (int64_t)sizeof(T) + kRowBytes - 1) / kRowBytes);
+            a.steps = (int)((*a.count * (int64_t)sizeof(T) + kRowBytes - 1) / kRowBytes);
         }
     }
-    int64_t tm, tn;
-    if (!tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn)) return;
+    const int64_t parts = a.sums ? ce_parts(a.n, (int)a.m, a.first_steps, X::BM == 256) : 1;
+    int64_t tm, tn, part;
+    if (!tile_of(blockIdx.x, a.tiles_m, a.tiles_n, parts, tm, tn, part)) return;
     const int64_t m0 = tm * X::BM, n0 = tn * X::BN;
-    const int first = blockIdx.y * a.steps_per_part, steps = min(a.steps_per_part, a.steps - first);
+    const int each = (int)((a.steps + parts - 1) / parts), first = (int)part * each, steps = min(each, a.steps - first);
     f32x4_t acc[X::TM][X::TN] = {};
     tile_product<T, X, A_ALONG, B_ALONG>(a.a, a.b, m0, n0, first, steps, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
@@ -515,7 +536,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
             const int64_t m = m0 + wm * (X::BM / X::WAVES_M) + i * 16 + (lane >> 4) * 4;
             if (m >= a.m) continue;
             if (a.sums) {      // (rows of ld_sums floats, a multiple of 4: the padding behind m may be written)
-                f32x4_t *to = reinterpret_cast<f32x4_t *>(a.sums + (blockIdx.y * a.sum_rows + n) * a.ld_sums + m);
+                f32x4_t *to = reinterpret_cast<f32x4_t *>(a.sums + (part * a.n + n) * a.ld_sums + m);
                 *to = a.add ? *to + acc[i][j] : acc[i][j];
             } else {
                 T *to = static_cast<T *>(a.out) + n * a.m + m;
@@ -531,8 +552,9 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void ce_finish_kernel(const float *sums, int parts, CeRows rows, int C, int64_t ld, const float *g, float factor, T *out) {
-    ce_finish<T, true>(sums, parts, rows.n, rows.n, rows.place, C, ld, g, factor, out, group_of());
+__global__ __launch_bounds__(256) void ce_finish_kernel(const float *sums, int64_t first_steps, bool big, CeRows rows, int C, int64_t ld, const float *g, float factor, T *out) {
+    const int64_t count = ce_count(rows);
+    ce_finish<T, true>(sums, ce_parts(count, C, first_steps, big), rows.n, count, rows.place, C, ld, g, factor, out, group_of());
 }
 
 // Moves the kept rows together (CeRows): a workgroup counts the kept rows before its `chunk`, its 16 waves those of their sixteenth,
@@ -775,7 +797,9 @@ struct CePlan {
     int64_t tiles;                   // (wide) statistics per row
     // backward
     int64_t piece, np;               // table rows per piece; n padded to 128 bytes of dl^T
-    int parts;                       // of k in dx's product
+    int parts;                       // (few rows) sums of dx
+    int64_t first_steps;             // (wide) of k in dx's product, the first piece
+    bool big;                        // dx's tiles are 256 x 256
     size_t factors, dl, dlt, wt, xt, sums, sums_w;
     size_t total;
 };
@@ -852,13 +876,12 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
             if (need_x && p.es == 4) p.wt = take((size_t)C * p.piece * p.es);
         }
         if (need_x && !p.few) {
-            const int64_t side = ce_big(C, n, p.es) ? 256 : 128, tiles = ceil_div(C, side) * ceil_div(n, side), steps = round_up(V < p.piece ? V : p.piece, step) / step;
-            // parts of k: as many workgroups as one round of the chip takes (two per CU), at least 8 steps each
-            int64_t parts = side == 256 || tiles == 0 ? 1 : 512 / tiles;
-            if (parts > steps / 8) parts = steps / 8;
-            if (parts < 1) parts = 1;
-            p.parts = (int)ceil_div(steps, ceil_div(steps, parts));      // (as many as get work; a smaller last piece then has no more)
-            p.sums = take((size_t)p.parts * n * p.c4 * 4);
+            p.first_steps = round_up(V < p.piece ? V : p.piece, step) / step;
+            p.big = ce_big(C, n, p.es);
+            // rows of all parts' sums, however many rows are kept: whole tiles of a round, or one part of n
+            const int64_t most = kRound / ceil_div(C, 128) * 128, even = ceil_div(p.first_steps, 8) * n;
+            const int64_t rows = p.big ? n : most < even ? most : even;
+            p.sums = take((size_t)(rows > n ? rows : n) * p.c4 * 4);
         }
         if (need_w && !p.few) {
             p.dlt = take((size_t)p.piece * p.np * p.es);
@@ -1051,7 +1074,8 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
         ce_tiles<T>(d.m, d.n, [&](auto x) {
             using X = decltype(x);
             d.tiles_m = ceil_div(d.m, X::BM); d.tiles_n = ceil_div(d.n, X::BN);
-            ce_launch<X>(ce_product_kernel<T, X, decltype(a_along)::value, decltype(b_along)::value>, d, dim3((unsigned)(d.tiles_m * d.tiles_n), (unsigned)ceil_div(d.steps, d.steps_per_part)), 0, st);
+            const int64_t tiles = d.tiles_m * d.tiles_n, groups = d.sums && X::BM == 128 && tiles < kRound ? kRound : tiles;
+            ce_launch<X>(ce_product_kernel<T, X, decltype(a_along)::value, decltype(b_along)::value>, d, dim3((unsigned)groups), 0, st);
         });
     };
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
@@ -1087,9 +1111,9 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             }
             d.b = Operand{ws + p.dl, k * p.es, n};
             d.steps = (int)(k / step);
-            d.steps_per_part = (int)ceil_div(d.steps, p.parts);
+            d.first_steps = (int)p.first_steps;
             d.m = C; d.n = n;
-            d.sums = reinterpret_cast<float *>(ws + p.sums); d.ld_sums = p.c4; d.sum_rows = n; d.count = rows.count;
+            d.sums = reinterpret_cast<float *>(ws + p.sums); d.ld_sums = p.c4; d.count = rows.count;
             d.add = v0 > 0;
             // (a smaller last piece may have fewer parts of k: the sums of the others stay as they are)
             product(d, std::bool_constant<sizeof(T) == 2>(), std::false_type());
@@ -1097,7 +1121,6 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
         if (grad_w) {
             CeProduct d = {};
             d.steps = (int)(p.np / step);
-            d.steps_per_part = d.steps;
             d.m = C; d.n = count;
             d.out = static_cast<T *>(grad_w) + v0 * C;
             d.top = factors + 2 * n; d.factor = factor; d.count = rows.count;
@@ -1119,7 +1142,7 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
                            p.parts, (int)n, C, p.c4, factors, factor, static_cast<T *>(grad_x));
     else if (grad_x)
         hipLaunchKernelGGL((ce_finish_kernel<T>), grid_of(ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
-                           p.parts, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));
+                           p.first_steps, p.big, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));
     return check_launch("mvs_linear_ce_bwd");
 }
 
