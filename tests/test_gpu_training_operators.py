@@ -399,6 +399,78 @@ def test_linear_cross_entropy_one_gradient_at_a_time_and_shapes():
     assert torch.equal(ops.linear_cross_entropy(x, w.t().contiguous().t(), t, reduction="none"), flat)
 
 
+# rows longer than the narrow kernels take: few of them, those of one tile, and those that are moved together
+WIDE = [10, 70, 200]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", WIDE)
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_linear_cross_entropy_wide_rows_reductions_and_scales(reduction, n, dtype):
+    x, w, t, _ = ce_case(n, 701, 200, dtype, seed=n)
+    for scale in (1.0, 4.0, 0.125, -2.0, 0.0):
+        ce_check(x, w, t, scale, reduction=reduction)
+    ce_check(x, w, t.clamp(min=3), 1.0, ignore=3, reduction=reduction)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", WIDE)
+def test_linear_cross_entropy_wide_rows_without_a_kept_one(n, dtype):
+    x, w, t, _ = ce_case(n, 150, 136, dtype, ignored=2.0)
+    for reduction in ("mean", "sum", "none"):
+        ce_check(x, w, t, 1.0, reduction=reduction)
+    t[n // 2] = 149      # ... and with one
+    for reduction in ("mean", "sum", "none"):
+        ce_check(x, w, t, 1.0, reduction=reduction)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", WIDE)
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_linear_cross_entropy_wide_rows_ignored_and_poisoned(reduction, n, dtype):
+    x, w, t, _ = ce_case(n, 333, 200, dtype, seed=7)
+    t[3], t[n - 1], t[1], t[n - 2] = -100, -100, 0, 332
+    clean = x.clone()
+    clean[[3, n - 1]] = 0
+    x[3], x[n - 1, 5] = float("nan"), float("inf")
+    res = []
+    for rows in (x, clean):
+        leaves = [rows.detach().requires_grad_(), w.detach().requires_grad_()]
+        loss = ops.linear_cross_entropy(*leaves, t, reduction=reduction)
+        res.append([loss.detach(), *torch.autograd.grad(loss.sum(), leaves)])
+    for a, b in zip(*res):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    # the last kept row holds a NaN, or names no class: it shows in its own gradient and in the table's, and nowhere else
+    for target in (332, 333):
+        bad = clean.clone()
+        t[n - 2] = target
+        if target == 332:
+            bad[n - 2, 9] = float("nan")
+        leaves = [bad.requires_grad_(), w.detach().requires_grad_()]
+        loss = ops.linear_cross_entropy(*leaves, t, reduction=reduction)
+        gx, gw = torch.autograd.grad(loss.sum(), leaves)
+        assert torch.isnan(gx[n - 2]).all() and torch.isfinite(gx[:n - 2]).all() and (gx[[3, n - 1]] == 0).all() and torch.isnan(gw).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", WIDE)
+def test_linear_cross_entropy_wide_rows_one_gradient_at_a_time(n, dtype):
+    x, w, t, _ = ce_case(n, 500, 140, dtype, seed=10)
+    both = torch.autograd.grad(ops.linear_cross_entropy(a := x.detach().requires_grad_(), b := w.detach().requires_grad_(), t), (a, b))
+    again = torch.autograd.grad(ops.linear_cross_entropy(a, b, t), (a, b))
+    gx, = torch.autograd.grad(ops.linear_cross_entropy(a := x.detach().requires_grad_(), w, t), (a,))
+    gw, = torch.autograd.grad(ops.linear_cross_entropy(x, b := w.detach().requires_grad_(), t), (b,))
+    assert torch.equal(gx, both[0]) and torch.equal(gw, both[1]) and torch.equal(again[0], gx) and torch.equal(again[1], gw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,V,C", [(600, 40001, 768), (9001, 700, 1000), (3000, 5000, 1096)])
+def test_linear_cross_entropy_on_large_tiles(n, V, C, dtype):
+    """Sizes at which the 256 x 256 tiles are taken, with ragged edges on every side: by dW's product, by dx's, by the logits'."""
+    x, w, t, _ = ce_case(n, V, C, dtype, seed=3)
+    ce_check(x, w, t, 1.0)
+
+
 def test_linear_cross_entropy_against_differences():
     x, w, t, _ = ce_case(12, 40, 8, torch.float32, seed=11)
     leaves = [x.detach().requires_grad_(), w.detach().requires_grad_()]
