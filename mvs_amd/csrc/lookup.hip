@@ -11,15 +11,15 @@
 //   sort   up to kRankMax indices: the place of term i is the number of (key, i) below its own -- one launch, n^2 comparisons of two
 //          instructions; more: least-significant-digit radix sort, digits of up to 10 bits, three launches each (count per tile, one
 //          workgroup's scan, place).
-//   rows   the sorted terms are cut into pieces of kPiece; a piece's lanes walk it with the loads of 8 terms in flight and write
+//   rows   the sorted terms are cut into pieces of 16 to 128; a piece's lanes walk it with the loads of 8 terms in flight and write
 //          the sum of each run of equal keys that lies within the piece.  A run that leaves the piece (a frequent index) leaves
 //          float32 partial sums, at most two per piece.  The same launch writes the zero rows (found by binary search, 64 table
 //          rows per wave's worth of lanes).
 //   join   the partial sums of the runs that leave their piece, in order: short runs a wave each, long ones four spans of pieces at
 //          a time.  A run's end is found 64 pieces per look.
-// Bound by memory for large ones: 65536 rows of 4 KiB into 128000 (268 MB read, 524 MB written) sort 32 us, rows 178 us (4.5 TB/s),
-// join 42 us; by latency for small ones: 1021 rows of 128 bytes into 20480 sort 5.8, rows 7.9, join 3.4 us.  The rank sort takes
-// 5.8 us for 1021 and 16.9 us for 8191 indices, where the radix sort's six launches take 32.
+// Bound by memory for large ones: 65536 rows of 4 KiB into 128000, a few of them most of the batch (268 MB read, 524 MB written): sort
+// 32 us, rows 170 us (4.7 TB/s), join 21 us; by latency for small ones: 1021 rows of 128 bytes into 20480 sort 5.8, rows 7, join
+// 3.4 us.  The rank sort takes 5.8 us for 1021 and 16.9 us for 8191 indices, where the radix sort's six launches take 32.
 #include <utility>
 
 #include "dtype.h"
@@ -27,7 +27,6 @@
 namespace mvs {
 
 constexpr int kRankMax = 8192;
-constexpr int kPiece = 16;         // sorted terms per piece
 constexpr int kJoin = 16;          // pieces that a workgroup of the join looks at
 constexpr int kMaxDigit = 10;
 
@@ -35,6 +34,7 @@ struct LookupPlan {
     int64_t n, rows;
     int key_bits, passes, digit_bits;
     int tile;                     // keys per workgroup of a radix pass: small while that fills the chip, large before the scan of the counts is long
+    int terms;                    // sorted terms per piece
     int64_t tiles, pieces;
     size_t keys0, vals0, keys1, vals1, hist, part, total;      // byte offsets into the workspace
 };
@@ -47,7 +47,11 @@ static LookupPlan lookup_plan(int64_t rows, int C, int64_t n) {
     p.digit_bits = p.passes ? (p.key_bits + p.passes - 1) / p.passes : 0;
     p.tile = n <= 131072 ? 1024 : 4096;
     p.tiles = (n + p.tile - 1) / p.tile;
-    p.pieces = (n + kPiece - 1) / kPiece;
+    // Short pieces fill the chip, long ones leave fewer partial sums: 65536 x 2048 bfloat16 into 128000 rows 227 / 217 / 245 us by pieces
+    // of 16 / 32 / 64 where the indices are spread evenly, 290 / 242 / 254 where a few are frequent; 10^6 x 64 float32 171 / 146 / 135
+    // and 440 / 276 / 205.
+    p.terms = n <= 1 << 14 ? 16 : n <= 1 << 18 ? 32 : n <= 1 << 22 ? 64 : 128;
+    p.pieces = (n + p.terms - 1) / p.terms;
     auto align = [](size_t b) { return (b + 255) & ~(size_t)255; };
     size_t at = 0;
     p.keys0 = at; at += align((size_t)n * 4);
@@ -265,7 +269,7 @@ struct LookupRows {
     void *out;
     float *part;           // [pieces][2][C]: the run that comes from the piece before, the run that goes on into the next
     int64_t n, rows, pieces, sum_groups;
-    int C, lanes;
+    int C, lanes, terms;
     float scale;
 };
 
@@ -302,39 +306,44 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(LookupRows a) {
     }
     const int64_t piece = group * (256 / a.lanes) + tid / a.lanes;
     if (piece >= a.pieces) return;
-    const int64_t p0 = piece * kPiece;
-    const int count = (int)(a.n - p0 < kPiece ? a.n - p0 : kPiece);
+    const int64_t p0 = piece * a.terms;
+    const int count = (int)(a.n - p0 < a.terms ? a.n - p0 : a.terms);
     const unsigned none = (unsigned)a.rows;
-    const unsigned before = p0 > 0 ? a.keys[p0 - 1] : 0xffffffffu, behind = p0 + count < a.n ? a.keys[p0 + count] : 0xffffffffu;
+    const unsigned before = p0 > 0 ? a.keys[p0 - 1] : 0xffffffffu;
     const T *grad = static_cast<const T *>(a.grad);
-    unsigned key[kPiece], val[kPiece];
+    // eight terms and the key behind them, read while the eight before them are summed
+    struct Terms { unsigned key[9], val[8]; };
+    auto terms_at = [&](int from) {
+        Terms t;
 #pragma unroll
-    for (int t = 0; t < kPiece; ++t) {
-        key[t] = t < count ? a.keys[p0 + t] : 0xffffffffu;
-        val[t] = t < count ? a.vals[p0 + t] : 0u;
-    }
+        for (int k = 0; k < 9; ++k) t.key[k] = from + k <= count && p0 + from + k < a.n ? a.keys[p0 + from + k] : 0xffffffffu;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t.val[k] = from + k < count ? a.vals[p0 + from + k] : 0u;
+        return t;
+    };
+    const Terms head = terms_at(0);
     for (int c = lane; c < vecs; c += a.lanes) {
         float sum[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
-        bool from_before = key[0] == before;
-#pragma unroll
-        for (int half = 0; half < kPiece; half += 8) {
+        bool from_before = head.key[0] == before;
+        Terms now = head;
+        for (int from = 0; from < count; from += 8) {
             Pack<T, VEC> g[8];
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
-                if (half + t < count && key[half + t] != none)
-                    g[t] = reinterpret_cast<const Pack<T, VEC> *>(grad + (int64_t)val[half + t] * a.C)[c];
+            for (int k = 0; k < 8; ++k)
+                if (from + k < count && now.key[k] != none)
+                    g[k] = reinterpret_cast<const Pack<T, VEC> *>(grad + (int64_t)now.val[k] * a.C)[c];
+            const Terms then = terms_at(from + 8);
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const int k = half + t;
-                if (k >= count || key[k] == none) continue;
+            for (int k = 0; k < 8; ++k) {
+                const unsigned key = now.key[k];
+                if (from + k >= count || key == none) continue;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) sum[j] += to_float(g[t].v[j]);
-                const bool last = k == count - 1;
-                const unsigned next = last ? behind : key[k + 1 < kPiece ? k + 1 : k];
-                if (!last && next == key[k]) continue;
-                const bool goes_on = last && behind == key[k];
+                for (int j = 0; j < VEC; ++j) sum[j] += to_float(g[k].v[j]);
+                const bool last = from + k == count - 1;
+                if (!last && now.key[k + 1] == key) continue;
+                const bool goes_on = last && now.key[k + 1] == key;
                 if (from_before || goes_on) {
                     // (a run that fills the piece and leaves it on both sides counts as coming from before)
                     float *to = a.part + (piece * 2 + (from_before ? 0 : 1)) * a.C + c * VEC;
@@ -344,12 +353,13 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(LookupRows a) {
                     Pack<T, VEC> o;
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(sum[j] * a.scale);
-                    put(reinterpret_cast<Pack<T, VEC> *>(out + (int64_t)key[k] * a.C) + c, o);
+                    put(reinterpret_cast<Pack<T, VEC> *>(out + (int64_t)key * a.C) + c, o);
                 }
                 from_before = false;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
             }
+            now = then;
         }
     }
 }
@@ -365,7 +375,7 @@ __global__ __launch_bounds__(256) void lookup_join_kernel(LookupRows a) {
     bool owner = lane < kJoin && mine < a.pieces - 1, longer = false;      // (the last piece goes on nowhere; the others are full)
     unsigned my_key = 0;
     if (owner) {
-        const int64_t first = mine * kPiece, end = first + kPiece, probe = end + (LONG - 1) * kPiece;
+        const int64_t first = mine * a.terms, end = first + a.terms, probe = end + (LONG - 1) * a.terms;
         my_key = a.keys[end - 1];
         const unsigned next = a.keys[end], head = a.keys[first], before = first > 0 ? a.keys[first - 1] : ~0u, far = probe < a.n ? a.keys[probe] : ~0u;
         owner = my_key != (unsigned)a.rows && next == my_key && !(head == my_key && before == my_key);
@@ -377,7 +387,7 @@ __global__ __launch_bounds__(256) void lookup_join_kernel(LookupRows a) {
         int64_t more = 0;
         while (true) {
             const int64_t q = piece + 1 + more + lane;
-            const unsigned long long same = __ballot(q < a.pieces && a.keys[q * kPiece] == key);
+            const unsigned long long same = __ballot(q < a.pieces && a.keys[q * a.terms] == key);
             if (same != ~0ull) return more + __builtin_ctzll(~same);
             more += 64;
         }
@@ -552,7 +562,7 @@ extern "C" int mvs_lookup_rows_bwd(const void *grad_out, int dtype, const int64_
     }
     LookupRows a = {};
     a.grad = grad_out; a.keys = keys; a.vals = vals; a.out = grad_table; a.part = reinterpret_cast<float *>(ws + p.part);
-    a.n = n; a.rows = rows; a.pieces = p.pieces; a.C = C; a.scale = scale;
+    a.n = n; a.rows = rows; a.pieces = p.pieces; a.terms = p.terms; a.C = C; a.scale = scale;
     const bool wide = lookup_wide(grad_out, grad_table, dtype, C);
     MVS_DTYPE_DISPATCH(dtype, T, {
         if (wide) lookup_launch_rows<T, 16 / sizeof(T)>(a, st);

@@ -238,6 +238,29 @@ def test_lookup_rows_shapes_strides_and_empty():
     assert (grad == 0).all()
 
 
+@pytest.mark.parametrize("n", [16384, 16385, 40000, (1 << 18) + 1, (1 << 22) + 3])
+@pytest.mark.parametrize("spread", ["flat", "steep", "one"])
+def test_lookup_rows_gradient_pieces_of_every_length(n, spread):
+    """Runs of equal indices that end on, before and behind the ends of the pieces that the sorted terms are cut into."""
+    rows, C = 1000, 8
+    if spread == "flat":
+        index = torch.randint(-1, rows + 1, (n,), generator=gen(1), device="cuda")
+    elif spread == "steep":
+        index = (rows * torch.rand(n, generator=gen(1), device="cuda", dtype=torch.float64) ** 8).long()
+    else:
+        index = torch.full((n,), 7, device="cuda")
+        index[::3001] = 11
+    g = randn(n, C, seed=2)
+    leaf = torch.zeros(rows, C, device="cuda").requires_grad_()
+    grad, = torch.autograd.grad(ops.lookup_rows(leaf, index, 0.5), leaf, g)
+    named = (index >= 0) & (index < rows)
+    at, terms = index[named].cpu(), g[named].double().cpu()      # (in order, on the CPU: a card's float64 atomics on one row queue for minutes)
+    zero = torch.zeros(rows, C, dtype=torch.float64)
+    want, mag = zero.index_add(0, at, terms) * 0.5, zero.index_add(0, at, terms.abs()) * 0.5
+    count = torch.bincount(at, minlength=rows).unsqueeze(1)
+    assert ((grad.cpu().double() - want).abs() <= (count + 2) * U * mag).all()
+    assert torch.equal(grad, torch.autograd.grad(ops.lookup_rows(leaf, index, 0.5), leaf, g)[0])
+
 # ------------------------------------------------------------------ cross entropy against a large table
 def ce_case(n, V, C, dtype, ignored=0.2, sharp=1.0, seed=0):
     w = randn(V, C, seed=seed + 1) / math.sqrt(C)
