@@ -619,7 +619,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const T *__restrict__ in, 
 // With so few rows a product tile is mostly empty and W^T costs more than the products: bound by reading W and writing dW, once each.
 // A thread owns VEC columns, keeps x (times the row's ratio) and dx of NR rows there in registers and walks 64 table rows:
 //     dx[n] += dl[n][v] W[v],  dW[v] = sum_n dl[n][v] ratio_n x[n]
-// One row against 32000 x 1024 bfloat16: 24 us for 131 MB (5.4 TB/s); the tiles that form the logits read the table at 4.1 TB/s.
+// Two rows against 32000 x 1024 bfloat16: 25 us for 131 MB; the tiles that form the logits before it read the table at 4.1 TB/s.
 constexpr int kFew = 16, kFewTable = 64;
 struct CeFew {
     const void *w, *x, *dl;
@@ -627,21 +627,120 @@ struct CeFew {
     int n, C, Cp, threads;              // threads per table row, a power of two
     const float *ratio, *top;
     float factor;
+    // (the logits formed here) what dl is made of
+    const float *lse2;
+    const int64_t *target;
+    int64_t ignore, v0;                 // v0: the piece's first table row
+    float scale2;
+    float2 *part;                       // (statistics) [part]
+    float *own;
     void *grad_w;                       // [count][C] or NULL
     float *sums;                        // [part][n][c4] or NULL
     int64_t c4;
     int add;
 };
 
-template <typename T, int NR, int VEC>
+// A single row against BATCH table rows per `threads` threads (their columns of them in p): <w, x> for all of them.  `shares`: of one
+// batch; two in turn, the barrier of the batch in between keeps them apart.
+template <typename T, int VEC, int BATCH>
+__device__ __forceinline__ void few_logits(const Pack<T, VEC> (&p)[BATCH], const float (&x)[VEC], int threads, float (&shares)[4][BATCH], float (&l)[BATCH]) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        l[u] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) l[u] = __builtin_fmaf(to_float(p[u].v[j]), x[j], l[u]);
+    }
+    for (int o = 1; o < threads && o < 64; o <<= 1)
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) l[u] += __shfl_xor(l[u], o);
+    if (threads <= 64) return;
+    const int wave = tid >> 6, waves = threads / 64, first = wave / waves * waves;      // (a row's threads are several waves)
+    if ((tid & 63) == 0)
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) shares[wave][u] = l[u];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        l[u] = shares[first][u];
+        for (int q = 1; q < waves; ++q) l[u] += shares[first + q][u];
+    }
+}
+
+// The statistics of a single float32 row whose columns a workgroup holds whole (32000 x 1024: forward 41 us, with tiles of which one
+// row in 128 is real 79; 16-bit tiles are bound by reading the table, and faster: 23 us against 33).
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void ce_one_stats_kernel(CeFew a) {
+    constexpr int BATCH = 8;
+    __shared__ float shares[2][4][BATCH], all[kFewTable];
+    const int tid = threadIdx.x, col = (tid & (a.threads - 1)) * VEC, sub = tid / a.threads, subs = 256 / a.threads;
+    const int64_t v0 = (int64_t)blockIdx.x * kFewTable;
+    const int rows = (int)min((int64_t)kFewTable, a.count - v0);
+    const bool here = col < a.Cp;
+    Pack<T, VEC> px;
+    float x[VEC];
+    if (here) px = *reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.x) + col);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = here ? to_float(px.v[j]) : 0.0f;
+    const Pack<T, VEC> *w = reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.w) + v0 * a.Cp + col);
+    const int stride = a.Cp / VEC;
+    for (int b = 0; b * BATCH * subs < rows; ++b) {
+        const int v = b * BATCH * subs + sub;
+        Pack<T, VEC> p[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            if (here && v + u * subs < rows) p[u] = w[(int64_t)(v + u * subs) * stride];
+            else
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) p[u].v[j] = from_float<T>(0.0f);
+        }
+        float l[BATCH];
+        few_logits<T, VEC, BATCH>(p, x, a.threads, shares[b & 1], l);
+        if ((tid & (a.threads - 1)) == 0)
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u)
+                if (v + u * subs < rows) all[v + u * subs] = l[u] * a.scale2;
+    }
+    __syncthreads();
+    if (tid >= 64) return;
+    const int64_t t = a.target[0];
+    const float l = tid < rows ? all[tid] : -INFINITY;
+    if (tid < rows && t == v0 + tid) *a.own = l;
+    float top = l;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    float sum = __builtin_amdgcn_exp2f(l - (top == -INFINITY ? 0.0f : top));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    if (tid == 0) a.part[blockIdx.x] = make_float2(top, sum);
+}
+
+// LOGITS: a single row whose columns a workgroup holds whole forms its logits here too, from the values that it has in registers for the
+// products -- one read of the table instead of two, and no launch for dl.  (32000 x 1024: bfloat16 48 -> 40 us, float32 122 -> 64; two
+// to four rows 54 -> 63 us, their sums across the lanes cost more than a tile's matrix instructions.)
+template <typename T, int NR, int VEC, bool LOGITS>
 __global__ __launch_bounds__(256) void ce_few_kernel(CeFew a) {
-    __shared__ float d[kFewTable][NR];
+    static_assert(!LOGITS || NR == 1, "a single row");
+    constexpr int BATCH = LOGITS ? 8 : 4;      // table rows of a thread under way
+    __shared__ float d[LOGITS ? 1 : kFewTable][NR];
+    __shared__ float shares[LOGITS ? 2 : 1][4][BATCH];
     __shared__ float joined[256][VEC];
     const int tid = threadIdx.x, col = (blockIdx.y * a.threads + (tid & (a.threads - 1))) * VEC, sub = tid / a.threads, subs = 256 / a.threads;
     const int64_t v0 = (int64_t)blockIdx.x * kFewTable;
     const int rows = (int)min((int64_t)kFewTable, a.count - v0);
     const bool here = col < a.Cp;
-    for (int i = tid; i < kFewTable * NR; i += 256) {
+    float lse2 = INFINITY, ratio_w = 0.0f;      // (an ignored row: logits of 0, exponentials of -Inf)
+    int target = -1;
+    bool kept = false;
+    if constexpr (LOGITS) {
+        const int64_t t = a.target[0];
+        kept = ce_kept(t, a.ignore);
+        if (kept) {
+            lse2 = a.lse2[0];
+            ratio_w = a.ratio[0];
+            target = t - a.v0 >= v0 && t - a.v0 < v0 + rows ? (int)(t - a.v0 - v0) : -1;
+        }
+    } else for (int i = tid; i < kFewTable * NR; i += 256) {
         const int v = i / NR, r = i % NR;
         d[v][r] = v < rows && r < a.n ? to_float(static_cast<const T *>(a.dl)[r * a.ld_dl + v0 + v]) : 0.0f;
     }
@@ -649,7 +748,7 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeFew a) {
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
         Pack<T, VEC> p;
-        const float ratio = r < a.n ? a.ratio[r] : 0.0f;
+        const float ratio = r >= a.n ? 0.0f : !LOGITS ? a.ratio[r] : kept ? 1.0f : 0.0f;      // (LOGITS: x itself)
         if (here && ratio != 0.0f) p = *reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.x) + (int64_t)r * a.Cp + col);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -661,40 +760,59 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeFew a) {
     const float f = a.grad_w ? *a.top * a.factor : 0.0f;
     const Pack<T, VEC> *w = reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.w) + v0 * a.Cp + col);
     const int stride = a.Cp / VEC;
-    if (here)
-        for (int v = sub; v < rows; v += 4 * subs) {
-            Pack<T, VEC> p[4];
-            if (a.sums)
+    for (int b = 0; b * BATCH * subs < rows; ++b) {
+        const int v = b * BATCH * subs + sub;
+        Pack<T, VEC> p[BATCH];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (v + u * subs < rows) p[u] = w[(int64_t)(v + u * subs) * stride];
+        for (int u = 0; u < BATCH; ++u) {
+            const int row = v + u * subs;
+            if (here && row < rows && (LOGITS || a.sums)) p[u] = w[(int64_t)row * stride];
+            else
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int row = v + u * subs;
-                if (row >= rows) break;
-                float out[VEC];
+                for (int j = 0; j < VEC; ++j) p[u].v[j] = from_float<T>(0.0f);
+        }
+        float g[BATCH][NR];
+        if constexpr (LOGITS) {
+            float l[BATCH];
+            few_logits<T, VEC, BATCH>(p, x[0], a.threads, shares[b & 1], l);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) out[j] = 0.0f;
+            for (int u = 0; u < BATCH; ++u) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(l[u], a.scale2, -lse2));
+                g[u][0] = v + u * subs == target ? e - 1.0f : e;
+            }
+        } else {
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const float g = d[row][r];
+            for (int u = 0; u < BATCH; ++u)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        if (a.sums) dx[r][j] = __builtin_fmaf(g, to_float(p[u].v[j]), dx[r][j]);
-                        out[j] = __builtin_fmaf(g, x[r][j], out[j]);
-                    }
-                }
-                if (a.grad_w && col < a.C) {      // (the padding's columns are nobody's)
-                    T *to = static_cast<T *>(a.grad_w) + (v0 + row) * a.C + col;
-                    Pack<T, VEC> o;
+                for (int r = 0; r < NR; ++r) g[u][r] = v + u * subs < rows ? d[v + u * subs][r] : 0.0f;
+        }
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(out[j] * f);
-                    if (a.C % VEC == 0) put(to, o);
-                    else
-                        for (int j = 0; j < VEC; ++j) if (col + j < a.C) to[j] = o.v[j];
+        for (int u = 0; u < BATCH; ++u) {
+            const int row = v + u * subs;
+            if (!here || row >= rows) break;
+            float out[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) out[j] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const float gw = LOGITS ? g[u][r] * ratio_w : g[u][r];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if (a.sums) dx[r][j] = __builtin_fmaf(g[u][r], to_float(p[u].v[j]), dx[r][j]);
+                    out[j] = __builtin_fmaf(gw, x[r][j], out[j]);
                 }
             }
+            if (a.grad_w && col < a.C) {      // (the padding's columns are nobody's)
+                T *to = static_cast<T *>(a.grad_w) + (v0 + row) * a.C + col;
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(out[j] * f);
+                if (a.C % VEC == 0) put(to, o);
+                else
+                    for (int j = 0; j < VEC; ++j) if (col + j < a.C) to[j] = o.v[j];
+            }
         }
+    }
     if (!a.sums) return;
     for (int r = 0; r < a.n; ++r) {      // the threads of a column, in order
         __syncthreads();
@@ -789,6 +907,7 @@ struct CePlan {
     bool pad;                        // the operands are copied to rows of Cp (narrow: and into pieces)
     int64_t c4;                      // C rounded up to 4
     bool few;                        // wide rows, at most kFew of them
+    bool one;                        // a single one, no longer than a workgroup of its kernels holds
     bool together;                   // the kept rows are moved together
     bool copy_x;                     // (wide) x is copied: padded, or moved together
     size_t xp, wp;                   // byte offsets: those copies
@@ -830,6 +949,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
     p.c4 = round_up(C, 4);
     const int step = kRowBytes / p.es, planes = ce_planes(dtype);
     p.Cp = (int)round_up(C, p.narrow ? 32 : step);
+    p.one = p.few && n == 1 && p.Cp <= 256 * 16 / p.es;
     p.pad = p.Cp != C || (p.narrow && planes > 1);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
@@ -846,7 +966,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
     if (p.pad) p.wp = take((size_t)V * row);
     const int64_t blocks_x = ceil_div(n, kNarrowRows), blocks_w = ceil_div(V, kNarrowRows);
     if (!backward) {
-        p.tiles = p.narrow ? 0 : ceil_div(V, ce_big(V, n, p.es) ? 256 : 128);
+        p.tiles = p.narrow ? 0 : ceil_div(V, p.one && p.es == 4 ? kFewTable : ce_big(V, n, p.es) ? 256 : 128);
         p.part = take((p.narrow ? (size_t)narrow_most(blocks_x, V, kNarrowStatsSlots) * kNarrowRows : (size_t)p.tiles * n) * sizeof(float2));
         p.own = take((size_t)n * 4);
         p.rows = take((size_t)n * 4);
@@ -1003,10 +1123,14 @@ static void ce_few(CeFew d, hipStream_t st) {
     };
     // 16-byte accesses while x and dx of NR rows at that many columns fit the registers, 8-byte ones for more
     constexpr int VEC = 16 / sizeof(T), HALF = VEC / 2, EIGHT = sizeof(T) == 2 ? HALF : VEC;
-    if (d.n == 1) launch(ce_few_kernel<T, 1, VEC>, VEC);
-    else if (d.n <= 4) launch(ce_few_kernel<T, 4, VEC>, VEC);
-    else if (d.n <= 8) launch(ce_few_kernel<T, 8, EIGHT>, EIGHT);
-    else launch(ce_few_kernel<T, 16, HALF>, HALF);
+    if constexpr (sizeof(T) == 4) {
+        if (d.part) { launch(ce_one_stats_kernel<T, VEC>, VEC); return; }
+    }
+    if (d.target) launch(ce_few_kernel<T, 1, VEC, true>, VEC);
+    else if (d.n == 1) launch(ce_few_kernel<T, 1, VEC, false>, VEC);
+    else if (d.n <= 4) launch(ce_few_kernel<T, 4, VEC, false>, VEC);
+    else if (d.n <= 8) launch(ce_few_kernel<T, 8, EIGHT, false>, EIGHT);
+    else launch(ce_few_kernel<T, 16, HALF, false>, HALF);
 }
 
 template <typename T>
@@ -1017,6 +1141,13 @@ static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const Ce
     a.scale2 = scale * kLog2e;
     a.part = reinterpret_cast<float2 *>(ws + p.part);
     a.own = reinterpret_cast<float *>(ws + p.own);
+    if (p.one && sizeof(T) == 4) {
+        CeFew d = {};
+        d.w = a.w.p; d.x = a.x.p; d.count = V; d.n = 1; d.C = C; d.Cp = p.Cp;
+        d.target = rows.target; d.scale2 = a.scale2; d.part = a.part; d.own = a.own;
+        ce_few<T>(d, st);
+        return check_launch("mvs_linear_ce_fwd");
+    }
     ce_tiles<T>(V, rows.n, [&](auto x) {
         using X = std::conditional_t<std::is_same_v<decltype(x), Tile256>, Tile256Late, decltype(x)>;
         a.tiles_m = ceil_div(V, X::BM); a.tiles_n = ceil_div(rows.n, X::BN);
@@ -1078,12 +1209,14 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             ce_launch<X>(ce_product_kernel<T, X, decltype(a_along)::value, decltype(b_along)::value>, d, dim3((unsigned)groups), 0, st);
         });
     };
+    const bool logits = p.one;
+    const float few_factor = logits ? scale : factor;      // (its dl is float32 throughout, not carried in a unit)
     for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
         const int64_t count = V - v0 < p.piece ? V - v0 : p.piece, k = round_up(count, step);
         a.w.p = w_rows + v0 * p.Cp * p.es;
         a.w.rows = count;
         a.v0 = v0; a.v_count = count; a.ld_dl = k;
-        ce_tiles<T>(count, n, [&](auto x) {
+        if (!logits) ce_tiles<T>(count, n, [&](auto x) {
             using X = decltype(x);
             a.tiles_m = ceil_div(count, X::BM); a.tiles_n = ceil_div(n, X::BN);
             ce_launch<X>(ce_grad_kernel<T, X>, a, dim3((unsigned)(a.tiles_m * a.tiles_n)), (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
@@ -1092,7 +1225,8 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             CeFew d = {};
             d.w = a.w.p; d.x = a.x.p; d.dl = a.dl; d.count = count; d.ld_dl = k;
             d.n = (int)n; d.C = C; d.Cp = p.Cp;
-            d.ratio = factors + n; d.top = factors + 2 * n; d.factor = factor;
+            d.ratio = factors + n; d.top = factors + 2 * n; d.factor = few_factor;
+            if (logits) { d.lse2 = lse; d.target = rows.target; d.ignore = rows.ignore; d.v0 = v0; d.scale2 = a.scale2; }
             d.grad_w = grad_w ? static_cast<T *>(grad_w) + v0 * C : nullptr;
             d.sums = grad_x ? reinterpret_cast<float *>(ws + p.sums) : nullptr;
             d.c4 = p.c4; d.add = v0 > 0;
@@ -1139,7 +1273,7 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
     }
     if (grad_x && p.few)
         hipLaunchKernelGGL((ce_few_finish_kernel<T>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 16)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
-                           p.parts, (int)n, C, p.c4, factors, factor, static_cast<T *>(grad_x));
+                           p.parts, (int)n, C, p.c4, factors, few_factor, static_cast<T *>(grad_x));
     else if (grad_x)
         hipLaunchKernelGGL((ce_finish_kernel<T>), grid_of(ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
                            p.first_steps, p.big, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));

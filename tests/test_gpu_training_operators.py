@@ -486,6 +486,29 @@ def test_linear_cross_entropy_wide_rows_one_gradient_at_a_time(n, dtype):
     assert torch.equal(gx, both[0]) and torch.equal(gw, both[1]) and torch.equal(again[0], gx) and torch.equal(again[1], gw)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [65, 129, 200, 500, 1000, 1024, 1025, 2048, 2050, 3000])
+def test_linear_cross_entropy_of_a_single_row(C, dtype):
+    """Rows that a workgroup holds whole, and longer ones; the target in the table's first, last and other rows, or ignored."""
+    V = 331
+    x, w, t, _ = ce_case(1, V, C, dtype, ignored=0.0, seed=C)
+    for target in (0, 63, 64, V - 1, -100):
+        t[0] = target
+        for scale in (1.0, -0.5, 0.0):
+            ce_check(x, w, t, scale, reduction="sum")
+    x[0, C - 1] = float("nan")
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    for target, wrong in ((-100, False), (5, True)):
+        t[0] = target
+        loss = ops.linear_cross_entropy(*leaves, t, reduction="sum")
+        gx, gw = torch.autograd.grad(loss, leaves)
+        assert math.isnan(float(loss.detach())) == wrong and bool(torch.isnan(gx).all()) == wrong and bool(torch.isnan(gw).all()) == wrong
+        assert wrong or ((gx == 0).all() and (gw == 0).all())
+    leaves[0] = torch.full_like(x, float("inf")).detach().requires_grad_()
+    t[0] = 5
+    gx, gw = torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, reduction="sum"), leaves)
+    assert not torch.isfinite(gx).any() and not torch.isfinite(gw).any()
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n,V,C", [(600, 40001, 768), (9001, 700, 1000), (3000, 5000, 1096)])
 def test_linear_cross_entropy_on_large_tiles(n, V, C, dtype):
