@@ -615,12 +615,15 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const T *__restrict__ in, 
     reinterpret_cast<Pack<T, VEC> *>(out)[i] = v;
 }
 
-// ---- few rows (at most kFew): both gradients in one pass over the table
-// With so few rows a product tile is mostly empty and W^T costs more than the products: bound by reading W and writing dW, once each.
+// ---- few rows (ce_few_rows): both gradients in one pass over the table
+// With so few rows a product tile is mostly empty: bound by reading W and writing dW, once each.
 // A thread owns VEC columns, keeps x (times the row's ratio) and dx of NR rows there in registers and walks 64 table rows:
 //     dx[n] += dl[n][v] W[v],  dW[v] = sum_n dl[n][v] ratio_n x[n]
 // Two rows against 32000 x 1024 bfloat16: 25 us for 131 MB; the tiles that form the logits before it read the table at 4.1 TB/s.
-constexpr int kFew = 16, kFewTable = 64;
+constexpr int kFewTable = 64;
+// How many rows are few.  16 bits, 32000 x 1024: two rows 55 us against the tiles' 66, four 57, eight 68 (sixteen 145); 100000 x 2048 four
+// 388 against 368.  float32, whose tiles need W^T: sixteen 172 against 242.
+static int ce_few_rows(int es) { return es == 2 ? 4 : 16; }
 struct CeFew {
     const void *w, *x, *dl;
     int64_t count, ld_dl;               // table rows of the piece; elements per row of dl
@@ -906,7 +909,7 @@ struct CePlan {
     int Cp;                          // C padded to whole 128-byte steps (narrow: to 32 elements)
     bool pad;                        // the operands are copied to rows of Cp (narrow: and into pieces)
     int64_t c4;                      // C rounded up to 4
-    bool few;                        // wide rows, at most kFew of them
+    bool few;                        // wide rows, few of them
     bool one;                        // a single one, no longer than a workgroup of its kernels holds
     bool together;                   // the kept rows are moved together
     bool copy_x;                     // (wide) x is copied: padded, or moved together
@@ -945,7 +948,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
     CePlan p = {};
     p.es = (int)dtype_size(dtype);
     p.narrow = ce_narrow(C, dtype);
-    p.few = !p.narrow && n <= kFew;
+    p.few = !p.narrow && n <= ce_few_rows(p.es);
     p.c4 = round_up(C, 4);
     const int step = kRowBytes / p.es, planes = ce_planes(dtype);
     p.Cp = (int)round_up(C, p.narrow ? 32 : step);
@@ -1122,15 +1125,16 @@ static void ce_few(CeFew d, hipStream_t st) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(d.count, kFewTable), (unsigned)ceil_div(d.Cp, d.threads * vec)), dim3(256), 0, st, d);
     };
     // 16-byte accesses while x and dx of NR rows at that many columns fit the registers, 8-byte ones for more
-    constexpr int VEC = 16 / sizeof(T), HALF = VEC / 2, EIGHT = sizeof(T) == 2 ? HALF : VEC;
+    constexpr int VEC = 16 / sizeof(T);
     if constexpr (sizeof(T) == 4) {
-        if (d.part) { launch(ce_one_stats_kernel<T, VEC>, VEC); return; }
+        if (d.part) launch(ce_one_stats_kernel<T, VEC>, VEC);
+        else if (d.n > 8) launch(ce_few_kernel<T, 16, VEC / 2, false>, VEC / 2);
+        else if (d.n > 4) launch(ce_few_kernel<T, 8, VEC, false>, VEC);
+        if (d.part || d.n > 4) return;
     }
     if (d.target) launch(ce_few_kernel<T, 1, VEC, true>, VEC);
     else if (d.n == 1) launch(ce_few_kernel<T, 1, VEC, false>, VEC);
-    else if (d.n <= 4) launch(ce_few_kernel<T, 4, VEC, false>, VEC);
-    else if (d.n <= 8) launch(ce_few_kernel<T, 8, EIGHT, false>, EIGHT);
-    else launch(ce_few_kernel<T, 16, HALF, false>, HALF);
+    else launch(ce_few_kernel<T, 4, VEC, false>, VEC);
 }
 
 template <typename T>

@@ -770,6 +770,30 @@ def test_linear_cross_entropy_few_rows_in_pieces():
         assert ((gw[rows].double() - want).abs() <= 3 * half_ulp(torch.float16) * mag + 2.0 ** -25).all()
 
 
+
+@pytest.mark.parametrize("n,V,C", [(16, (1 << 22) + 777, 66), (1, (1 << 26) + 77, 66)])
+def test_linear_cross_entropy_few_float32_rows_in_pieces(n, V, C):
+    w = randn(V, C, seed=1) * 0.1
+    t = torch.randint(V, (n,), generator=gen(1), device="cuda")
+    t[0] = V - 1
+    x = randn(n, C, seed=2)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    loss = ops.linear_cross_entropy(*leaves, t, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, leaves)
+    spans = [slice(v, min(v + (1 << 22), V)) for v in range(0, V, 1 << 22)]
+    logits = torch.cat([x.detach().double() @ w.detach()[s].double().t() for s in spans], 1)
+    lse = torch.logsumexp(logits, 1)
+    assert abs(float(loss.detach()) - float((lse - logits.gather(1, t.unsqueeze(1)).squeeze(1)).sum())) < 1e-4 * n
+    p = torch.exp(logits - lse.unsqueeze(1))
+    p[torch.arange(n, device="cuda"), t] -= 1
+    want = sum(p[:, s] @ w.detach()[s].double() for s in spans)
+    # p: a logit is off by at most (C + 4) u |x||w| < 1e-5, its exponential by that part of it; V terms of either sign in float32
+    assert float((gx.double() - want).norm() / want.norm()) < 1e-4
+    for rows in (slice(0, 100), slice(V - 800, V)):
+        want = p[:, rows].t() @ x.detach().double()
+        mag = p[:, rows].abs().t() @ x.detach().double().abs()
+        assert ((gw[rows].double() - want).abs() <= 4e-5 * mag).all()
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,C", [(300, 200), (5, 200)])
 def test_linear_cross_entropy_wide_rows_captured_and_replayed(n, C, dtype):
