@@ -33,6 +33,7 @@ template <> struct GradUnit<f16_t> { static constexpr float value = 16384.0f, lo
 struct Operand {
     const char *p;
     int64_t ld, rows;
+    int64_t plane;      // (float32 in pieces) bytes from a piece's plane to the next one's
 };
 
 __device__ __forceinline__ bool ce_kept(int64_t target, int64_t ignore) { return target != ignore; }
@@ -116,6 +117,23 @@ __device__ __forceinline__ void ce_finish(const float *__restrict__ sums, int64_
     if ((C & 3) == 0) put(to, o);
     else
         for (int r = 0; r < 4; ++r) if (c + r < C) to[r] = o.v[r];
+}
+
+// a value's pieces: 8 bits each, the first one cut instead of rounded where rounding would overflow
+template <typename E, int PL, typename T>
+__device__ __forceinline__ void pieces_of(T value, E (&p)[PL]) {
+    if constexpr (PL == 1) {
+        p[0] = value;
+    } else {
+        float v = value;
+        p[0] = from_float<E>(v);
+        if (__builtin_fabsf(v) > DtypeMax<E>::value && __builtin_fabsf(v) <= DtypeMax<float>::value) p[0].bits = (unsigned short)(__float_as_uint(v) >> 16);
+#pragma unroll
+        for (int q = 1; q < PL; ++q) {
+            v -= to_float(p[q - 1]);
+            p[q] = from_float<E>(v);
+        }
+    }
 }
 
 // ---- narrow rows: linear_ce_narrow.hip

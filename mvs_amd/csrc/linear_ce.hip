@@ -14,7 +14,9 @@
 // sides).  Of 16 bits, an operand whose rows run along the tile -- W in dx, x and dl in dW -- lies there as 64 rows of k and is read
 // by columns (ds_read_b64_tr_b16), so nothing is transposed in memory: against a pass that transposed W and x and a dl^T beside dl,
 // the backward pass of 583 x 49999 x 768 float16 takes 229 instead of 297 us, of 8192 x 64000 x 2048 bfloat16 5.30 instead of 5.64 ms.
-// float32, rows with factors of their own (reduction 'none') and few rows have those transposes.
+// float32, rows with factors of their own (reduction 'none') and rows that fill no more than one tile have those transposes.
+// More than 256 float32 rows are carried as three bfloat16 pieces each (pieces_t): the same tiles, over six times the steps of k, at
+// 205 to 217 TFLOP/s of float32 products where the float32 matrix instructions reach 85 to 135.
 // m runs over table rows or channels, n over the rows of x or of W: a lane of the accumulator then holds four consecutive m of one
 // n, so a row's softmax statistics reduce within the lane first, and results leave as vectors.
 //
@@ -30,6 +32,16 @@
 #include "linear_ce.h"
 
 namespace mvs {
+
+// An element of a float32 operand that is carried as three bfloat16 pieces, a plane each: the products are six of the nine piece
+// products (the others are below 2^-24 of it), one after the other along k, the smallest first.
+struct pieces_t { unsigned short bits; };
+template <typename T> constexpr bool kPieces = std::is_same_v<T, pieces_t>;
+template <typename T> struct Given { using type = T; };      // what the caller has
+template <> struct Given<pieces_t> { using type = float; };
+__device__ __forceinline__ void mma16(f32x4_t &c, u32x4_t a, u32x4_t b, pieces_t) { mma16(c, a, b, bf16_t()); }
+constexpr int kPairs = 6;
+constexpr unsigned kPieceOfA = 0x001012, kPieceOfB = 0x010210;      // of pair 0, 1, .. from the lowest four bits on
 
 // AHEAD: a wave reads its fragments half a step ahead.  One workgroup of 8 waves per CU needs it; two of 4 waves hide each other's
 // reads and are slower with it (8192 x 128000 x 2048 bfloat16 forward: 256 x 256 tiles 3.63 -> 3.52 ms, 128 x 128 4.26 -> 4.70 ms).
@@ -89,6 +101,7 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
     using SA = Stage<X::BM, A_ALONG>;
     using SB = Stage<X::BN, B_ALONG>;
     if (steps <= 0) return;
+    const int total = kPieces<T> ? kPairs * steps : steps;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / X::WAVES_N, wn = wave % X::WAVES_N;
     const unsigned lds_base = (unsigned)(uintptr_t)lds;
@@ -107,9 +120,24 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
     auto issue = [&](int stage, int i, unsigned from) {
         copy16(i < PER_A ? base_a : base_b, from, lds_base + (unsigned)(stage * X::STAGE + (wave + i * X::WAVES) * 1024));
     };
+    const char *const start_a = base_a, *const start_b = base_b;
+    int pair = 0, left = steps;
+    if constexpr (kPieces<T>) {
+        base_a += (kPieceOfA & 15) * a.plane;
+        base_b += (kPieceOfB & 15) * b.plane;
+    }
     auto retreat = [&](bool really) {
-        base_a -= really ? (A_ALONG ? 64 * a.ld : kRowBytes) : 0;
-        base_b -= really ? (B_ALONG ? 64 * b.ld : kRowBytes) : 0;
+        if constexpr (kPieces<T>) {
+            const bool over = really && left == 1;
+            left = over ? steps : left - (really ? 1 : 0);
+            pair += over ? 1 : 0;
+            const char *next_a = start_a + (kPieceOfA >> 4 * pair & 15) * a.plane, *next_b = start_b + (kPieceOfB >> 4 * pair & 15) * b.plane;
+            base_a = over ? next_a : base_a - (really ? (A_ALONG ? 64 * a.ld : kRowBytes) : 0);
+            base_b = over ? next_b : base_b - (really ? (B_ALONG ? 64 * b.ld : kRowBytes) : 0);
+        } else {
+            base_a -= really ? (A_ALONG ? 64 * a.ld : kRowBytes) : 0;
+            base_b -= really ? (B_ALONG ? 64 * b.ld : kRowBytes) : 0;
+        }
     };
     auto copy = [&](int stage, bool more = true) {
 #pragma unroll
@@ -122,14 +150,14 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
             const int c = wave + i * X::WAVES;
             const bool of_a = i < PER_A;
             unsigned from = offset[i];
-            if (of_a ? A_ALONG : B_ALONG) {
+            if (!kPieces<T> && (of_a ? A_ALONG : B_ALONG)) {      // (planes end in whole steps, rows of zeros)
                 const Operand &o = of_a ? a : b;
                 const int64_t behind = last * 64 + (of_a ? SA::row_of(c, lane) : SB::row_of(c - COPIES_A, lane)) - (o.rows - 1);
                 if (behind > 0) from -= (unsigned)behind * (unsigned)o.ld;
             }
             issue(0, i, from);
         }
-        retreat(steps > 1);
+        retreat(total > 1);
     };
     const int frow = lane & 15, fk = lane >> 4;
     // a fragment: 16 tile rows x 64 bytes of k (half a step); a lane's 16 bytes are 8 k of one tile row, or four of each of its two reads
@@ -182,17 +210,17 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
         u32x4_t a0[X::TM], b0[X::TN], a1[X::TM], b1[X::TN];
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (steps > 1) copy(1, steps > 2);
+        if (total > 1) copy(1, total > 2);
         read(0, 0, a0, b0);
         int stage = 0;
-        for (int s = 0; s + 1 < steps; ++s, stage ^= 1) {
+        for (int s = 0; s + 1 < total; ++s, stage ^= 1) {
             read(stage, 1, a1, b1);
             multiply(a0, b0, 0, HALF);
             pace();
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();      // (waits for this wave's reads too: the stage may be overwritten)
-            const bool more = s + 3 < steps;
+            const bool more = s + 3 < total;
             if constexpr (X::LATE) {
                 multiply(a0, b0, HALF, X::TM);
                 __builtin_amdgcn_sched_barrier(0);
@@ -212,10 +240,10 @@ __device__ __forceinline__ void tile_product(const Operand &a, const Operand &b,
         multiply(a1, b1, 0, X::TM);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the copies of the last steps, before LDS is used for something else
     } else {
-        for (int s = 0; s < steps; ++s) {
+        for (int s = 0; s < total; ++s) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();                         // stage s has landed for everybody, and nobody reads the other one any more
-            if (s + 1 < steps) copy((s + 1) & 1);
+            if (s + 1 < total) copy((s + 1) & 1);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 u32x4_t fa[X::TM], fb[X::TN];
@@ -273,6 +301,7 @@ struct CeArgs {
     const float *lse2, *ratio;
     void *dl, *dlt;                     // [n][ld_dl], [v][ld_dlt]; either may be NULL
     int64_t ld_dl, ld_dlt;
+    int64_t dl_plane;                   // (pieces) bytes from a plane of dl to the next
     int dl_step;                        // dl has rows of zeros behind the last kept one, up to a multiple of this
 };
 
@@ -470,18 +499,32 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < X::TM; ++i) {
-            Pack<T, 4> out;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float d = kept ? acc[i][j][r] : 0.0f;
-                out.v[r] = from_float<T>(d);
-                if (a.dlt) *reinterpret_cast<T *>(lds + (m_lane + i * 16 + r) * PITCH + nl * (int)sizeof(T)) = from_float<T>(kept ? d * ratio : 0.0f);
-            }
             const int64_t m = m0 + m_lane + i * 16;
-            if (a.dl && n < dl_rows && m < a.ld_dl) *reinterpret_cast<Pack<T, 4> *>(static_cast<T *>(a.dl) + n * a.ld_dl + m) = out;
+            if constexpr (kPieces<T>) {
+                Pack<bf16_t, 4> out[3];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    bf16_t p[3];
+                    pieces_of<bf16_t, 3>(kept ? acc[i][j][r] : 0.0f, p);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) out[q].v[r] = p[q];
+                }
+                if (n < dl_rows && m < a.ld_dl)
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) put(static_cast<char *>(a.dl) + q * a.dl_plane + (n * a.ld_dl + m) * 2, out[q]);
+            } else {
+                Pack<T, 4> out;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float d = kept ? acc[i][j][r] : 0.0f;
+                    out.v[r] = from_float<T>(d);
+                    if (a.dlt) *reinterpret_cast<T *>(lds + (m_lane + i * 16 + r) * PITCH + nl * (int)sizeof(T)) = from_float<T>(kept ? d * ratio : 0.0f);
+                }
+                if (a.dl && n < dl_rows && m < a.ld_dl) *reinterpret_cast<Pack<T, 4> *>(static_cast<T *>(a.dl) + n * a.ld_dl + m) = out;
+            }
         }
     }
-    if (!a.dlt) return;
+    if (kPieces<T> || !a.dlt) return;
     __syncthreads();
     constexpr int PER16 = 16 / (int)sizeof(T), CHUNKS = X::BN / PER16;
     for (int c = threadIdx.x; c < X::BM * CHUNKS; c += X::THREADS) {
@@ -514,7 +557,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
             a.n = a.b.rows = *a.count;
             a.tiles_n = (a.n + X::BN - 1) / X::BN;
         } else {
-            if (A_ALONG) a.a.rows = *a.count;      // (dl has rows of zeros behind the last kept one)
+            if (A_ALONG && !kPieces<T>) a.a.rows = *a.count;      // (dl, and x in pieces, have rows of zeros behind the last kept one)
             a.steps = (int)((*a.count * (int64_t)sizeof(T) + kRowBytes - 1) / kRowBytes);
         }
     }
@@ -539,10 +582,11 @@ __global__ __launch_bounds__(X::THREADS) void ce_product_kernel(CeProduct a) {
                 f32x4_t *to = reinterpret_cast<f32x4_t *>(a.sums + (part * a.n + n) * a.ld_sums + m);
                 *to = a.add ? *to + acc[i][j] : acc[i][j];
             } else {
-                T *to = static_cast<T *>(a.out) + n * a.m + m;
-                Pack<T, 4> o;
+                using O = typename Given<T>::type;
+                O *to = static_cast<O *>(a.out) + n * a.m + m;
+                Pack<O, 4> o;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o.v[r] = from_float<T>(acc[i][j][r] * f);
+                for (int r = 0; r < 4; ++r) o.v[r] = from_float<O>(acc[i][j][r] * f);
                 if ((a.m & 3) == 0) put(to, o);
                 else
                     for (int r = 0; r < 4; ++r) if (m + r < a.m) to[r] = o.v[r];
@@ -613,6 +657,37 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const T *__restrict__ in, 
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v.v[j] = from_float<T>(0.0f);
     reinterpret_cast<Pack<T, VEC> *>(out)[i] = v;
+}
+
+// float32 rows (the kept ones) as three planes of bfloat16 pieces, padded with zeros to rows of Cp and to whole steps of rows
+__global__ __launch_bounds__(256) void ce_pieces_kernel(const float *__restrict__ in, CeRows rows, int C, char *__restrict__ out, int Cp, int64_t plane) {
+    const int vecs = Cp / 8;
+    const int64_t i = group_of() * 256 + threadIdx.x, row = i / vecs, count = ce_count(rows);
+    if (row >= ((count + 63) & ~(int64_t)63)) return;
+    const int c = (int)(i - row * vecs) * 8;
+    const float *from = in + (row < count ? ce_original(rows, row) : 0) * C + c;
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 8; h += 4) {
+        if ((C & 3) == 0 && row < count && c + h < C) {
+            const f32x4_t four = *reinterpret_cast<const f32x4_t *>(from + h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[h + j] = four[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[h + j] = row < count && c + h + j < C ? from[h + j] : 0.0f;
+        }
+    }
+    Pack<bf16_t, 8> o[3];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        bf16_t p[3];
+        pieces_of<bf16_t, 3>(v[j], p);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) o[q].v[j] = p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) put(out + q * plane + i * 16, o[q]);
 }
 
 // ---- few rows (ce_few_rows): both gradients in one pass over the table
@@ -905,6 +980,7 @@ __global__ __launch_bounds__(256) void ce_transpose_kernel(const T *__restrict__
 // ---- host side
 struct CePlan {
     int es;                          // element size
+    bool pieces;                     // wide float32 rows in pieces (then 2)
     bool narrow;                     // linear_ce_narrow.hip
     int Cp;                          // C padded to whole 128-byte steps (narrow: to 32 elements)
     bool pad;                        // the operands are copied to rows of Cp (narrow: and into pieces)
@@ -944,16 +1020,22 @@ static bool ce_big(int64_t m, int64_t n, int es) {
     return big * 3 < small;
 }
 
-static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, bool need_x, bool need_w) {
+// Whether wide float32 rows go through the 16-bit matrix cores in pieces: six products at eight times the rate or more, for the
+// conversion of the table.  Forward / backward of 300 x 20000 x 256 51 / 127 us against 48 / 157, of 2000 x 32000 x 1024 0.64 / 2.27 ms
+// against 0.99 / 2.93, of 4096 x 65536 x 256 0.65 / 3.38 against 1.12 / 3.49.
+static bool ce_in_pieces(int64_t n, int C, int dtype) { return dtype == MVS_DTYPE_F32 && !ce_narrow(C, dtype) && n > 256; }
+
+static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool pieces, bool backward, bool need_x, bool need_w) {
     CePlan p = {};
-    p.es = (int)dtype_size(dtype);
+    p.pieces = pieces;
+    p.es = pieces ? 2 : (int)dtype_size(dtype);
     p.narrow = ce_narrow(C, dtype);
     p.few = !p.narrow && n <= ce_few_rows(p.es);
     p.c4 = round_up(C, 4);
     const int step = kRowBytes / p.es, planes = ce_planes(dtype);
     p.Cp = (int)round_up(C, p.narrow ? 32 : step);
     p.one = p.few && n == 1 && p.Cp <= 256 * 16 / p.es;
-    p.pad = p.Cp != C || (p.narrow && planes > 1);
+    p.pad = p.Cp != C || (p.narrow && planes > 1) || pieces;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
     p.together = n > kTogether;
@@ -965,8 +1047,8 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
         p.count = take(4);
     }
     const size_t row = (size_t)p.Cp * (p.narrow ? 2 * planes : p.es);
-    if (p.copy_x) p.xp = take((size_t)n * row);
-    if (p.pad) p.wp = take((size_t)V * row);
+    if (p.copy_x) p.xp = take(pieces ? (size_t)round_up(n, 64) * row * 3 : (size_t)n * row);
+    if (p.pad) p.wp = take(pieces ? (size_t)round_up(V, 64) * row * 3 : (size_t)V * row);
     const int64_t blocks_x = ceil_div(n, kNarrowRows), blocks_w = ceil_div(V, kNarrowRows);
     if (!backward) {
         p.tiles = p.narrow ? 0 : ceil_div(V, p.one && p.es == 4 ? kFewTable : ce_big(V, n, p.es) ? 256 : 128);
@@ -984,8 +1066,9 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
             p.sums_w = take((size_t)narrow_most(blocks_w, n, kNarrowGradSlots) * kNarrowRows * p.c4 * 4);
         }
     } else {
-        // the piece: dl of at most 2^26 values, whole tiles
-        p.piece = ((int64_t)1 << 26) / (n > 0 ? n : 1) / 256 * 256;
+        // the piece: dl of at most 2^26 values, whole tiles (float32 in pieces 2^27: the products then fill the chip, 8000 x 60000 x 768
+        // 15.2 / 14.0 / 13.4 ms by 2^25 / 2^26 / 2^27)
+        p.piece = ((int64_t)1 << (pieces ? 27 : 26)) / (n > 0 ? n : 1) / 256 * 256;
         if (p.piece < 256) p.piece = 256;
         if (p.piece > round_up(V, 256)) p.piece = round_up(V, 256);
         p.np = round_up(n, step);
@@ -995,7 +1078,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
             p.parts = (int)ceil_div(V < p.piece ? V : p.piece, kFewTable);
             if (need_x) p.sums = take((size_t)p.parts * n * p.c4 * 4);
         } else {
-            if (need_x || p.es == 2) p.dl = take((size_t)p.np * p.piece * p.es);
+            if (need_x || p.es == 2) p.dl = take((size_t)p.np * p.piece * p.es * (pieces ? 3 : 1));
             if (need_x && p.es == 4) p.wt = take((size_t)C * p.piece * p.es);
         }
         if (need_x && !p.few) {
@@ -1006,7 +1089,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool backward, boo
             const int64_t rows = p.big ? n : most < even ? most : even;
             p.sums = take((size_t)(rows > n ? rows : n) * p.c4 * 4);
         }
-        if (need_w && !p.few) {
+        if (need_w && !p.few && !pieces) {
             p.dlt = take((size_t)p.piece * p.np * p.es);
             p.xt = take((size_t)C * p.np * p.es);
         }
@@ -1065,6 +1148,21 @@ static int ce_check(const char *who, const void *x, const void *w, int dtype, co
 // the operands as the tiles read them: x copied (the kept rows, padded) and the table padded where the plan says so
 template <typename T>
 static void ce_operands(const CePlan &p, const void *x, const void *w, const CeRows &rows, int64_t V, int C, char *ws, hipStream_t st, CeArgs &a) {
+    a.steps = p.Cp * p.es / kRowBytes;
+    a.v_total = V;
+    a.rows = rows;
+    if constexpr (kPieces<T>) {
+        auto planes = [&](const void *in, const CeRows &r, char *out) {
+            const int64_t padded = round_up(r.n, 64), plane = padded * p.Cp * 2;
+            hipLaunchKernelGGL(ce_pieces_kernel, grid_of(ceil_div(padded * (p.Cp / 8), 256)), dim3(256), 0, st, static_cast<const float *>(in), r, C, out, p.Cp, plane);
+            return Operand{out, (int64_t)p.Cp * 2, r.n, plane};
+        };
+        CeRows table = {};
+        table.n = V;
+        a.x = planes(x, rows, ws + p.xp);
+        a.w = planes(w, table, ws + p.wp);
+        return;
+    } else {
     auto copy = [&](const void *in, const CeRows &r, char *out) {
         constexpr int VEC = 16 / sizeof(T);
         if (C % VEC == 0)
@@ -1086,9 +1184,7 @@ static void ce_operands(const CePlan &p, const void *x, const void *w, const CeR
         copy(w, table, ws + p.wp);
         a.w.p = ws + p.wp;
     }
-    a.steps = p.Cp * p.es / kRowBytes;
-    a.v_total = V;
-    a.rows = rows;
+    }
 }
 
 template <typename T>
@@ -1145,7 +1241,7 @@ static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const Ce
     a.scale2 = scale * kLog2e;
     a.part = reinterpret_cast<float2 *>(ws + p.part);
     a.own = reinterpret_cast<float *>(ws + p.own);
-    if (p.one && sizeof(T) == 4) {
+    if constexpr (std::is_same_v<T, float>) if (p.one) {
         CeFew d = {};
         d.w = a.w.p; d.x = a.x.p; d.count = V; d.n = 1; d.C = C; d.Cp = p.Cp;
         d.target = rows.target; d.scale2 = a.scale2; d.part = a.part; d.own = a.own;
@@ -1162,7 +1258,7 @@ static int ce_wide_stats(const CePlan &p, const void *x, const void *w, const Ce
 
 static int ce_forward(int dtype, const void *x, const void *w, const int64_t *target, int64_t n, int64_t V, int C, float scale, int64_t ignore,
                       int reduction, float *loss, float *lse, float *kept, char *ws, hipStream_t st) {
-    const CePlan p = ce_plan(n, V, C, dtype, false, false, false);
+    const CePlan p = ce_plan(n, V, C, dtype, ce_in_pieces(n, C, dtype), false, false, false);
     float *losses = reduction == 0 ? loss : reinterpret_cast<float *>(ws + p.rows);
     if (n > 0) {
         float2 *part = reinterpret_cast<float2 *>(ws + p.part);
@@ -1173,6 +1269,8 @@ static int ce_forward(int dtype, const void *x, const void *w, const int64_t *ta
             NarrowArgs a = ce_narrow_args(p, dtype, x, w, rows, V, C, scale, ws);
             a.part = part; a.own = own;
             rc = ce_narrow_forward(dtype, a, st);
+        } else if (p.pieces) {
+            rc = ce_wide_stats<pieces_t>(p, x, w, rows, V, C, scale, ws, st);
         } else {
             MVS_DTYPE_DISPATCH(dtype, T, rc = (ce_wide_stats<T>(p, x, w, rows, V, C, scale, ws, st)));
         }
@@ -1186,6 +1284,7 @@ static int ce_forward(int dtype, const void *x, const void *w, const int64_t *ta
 template <typename T>
 static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const CeRows &rows, const float *lse, const float *kept, const float *grad_loss,
                             int64_t V, int C, float scale, int reduction, void *grad_x, void *grad_w, char *ws, hipStream_t st) {
+    using O = typename Given<T>::type;
     const int step = kRowBytes / p.es;
     const int64_t n = rows.n;
     float *factors = reinterpret_cast<float *>(ws + p.factors);
@@ -1202,9 +1301,10 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
     a.dl = grad_x || p.few || (along && grad_w) ? ws + p.dl : nullptr;
     a.dlt = grad_w && !p.few && !along ? ws + p.dlt : nullptr;
     a.ld_dlt = p.np;
+    a.dl_plane = p.np * p.piece * 2;
     a.dl_step = along ? step : 1;      // (dW's product reads whole steps of rows; along: dl has p.np of them)
     // x^T once; ignored rows as zeros, whatever they hold
-    if (a.dlt) ce_transpose<T>(a.x.p, rows, !p.together, C, p.Cp, ws + p.xt, p.np, st);
+    if constexpr (!kPieces<T>) if (a.dlt) ce_transpose<T>(a.x.p, rows, !p.together, C, p.Cp, ws + p.xt, p.np, st);
     auto product = [&](CeProduct &d, auto a_along, auto b_along) {
         ce_tiles<T>(d.m, d.n, [&](auto x) {
             using X = decltype(x);
@@ -1225,7 +1325,7 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             a.tiles_m = ceil_div(count, X::BM); a.tiles_n = ceil_div(n, X::BN);
             ce_launch<X>(ce_grad_kernel<T, X>, a, dim3((unsigned)(a.tiles_m * a.tiles_n)), (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
         });
-        if (p.few) {
+        if constexpr (!kPieces<T>) if (p.few) {
             CeFew d = {};
             d.w = a.w.p; d.x = a.x.p; d.dl = a.dl; d.count = count; d.ld_dl = k;
             d.n = (int)n; d.C = C; d.Cp = p.Cp;
@@ -1247,7 +1347,7 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
                 ce_transpose<T>(a.w.p, table, false, C, p.Cp, ws + p.wt, k, st);
                 d.a = Operand{ws + p.wt, k * p.es, C};
             }
-            d.b = Operand{ws + p.dl, k * p.es, n};
+            d.b = Operand{ws + p.dl, k * p.es, n, a.dl_plane};
             d.steps = (int)(k / step);
             d.first_steps = (int)p.first_steps;
             d.m = C; d.n = n;
@@ -1260,27 +1360,29 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
             CeProduct d = {};
             d.steps = (int)(p.np / step);
             d.m = C; d.n = count;
-            d.out = static_cast<T *>(grad_w) + v0 * C;
+            d.out = static_cast<O *>(grad_w) + v0 * C;
             d.top = factors + 2 * n; d.factor = factor; d.count = rows.count;
             if constexpr (sizeof(T) == 2) {
                 if (along) {
                     d.a = a.x;
-                    d.b = Operand{ws + p.dl, k * p.es, p.np};
+                    d.b = Operand{ws + p.dl, k * p.es, p.np, a.dl_plane};
                     product(d, std::true_type(), std::true_type());
                     continue;
                 }
             }
-            d.a = Operand{ws + p.xt, p.np * p.es, C};
-            d.b = Operand{ws + p.dlt, p.np * p.es, count};
-            product(d, std::false_type(), std::false_type());
+            if constexpr (!kPieces<T>) {
+                d.a = Operand{ws + p.xt, p.np * p.es, C};
+                d.b = Operand{ws + p.dlt, p.np * p.es, count};
+                product(d, std::false_type(), std::false_type());
+            }
         }
     }
     if (grad_x && p.few)
-        hipLaunchKernelGGL((ce_few_finish_kernel<T>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 16)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
-                           p.parts, (int)n, C, p.c4, factors, few_factor, static_cast<T *>(grad_x));
+        hipLaunchKernelGGL((ce_few_finish_kernel<O>), dim3((unsigned)ceil_div(n * (p.c4 / 4), 16)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
+                           p.parts, (int)n, C, p.c4, factors, few_factor, static_cast<O *>(grad_x));
     else if (grad_x)
-        hipLaunchKernelGGL((ce_finish_kernel<T>), grid_of(ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
-                           p.first_steps, p.big, rows, C, p.c4, factors, factor, static_cast<T *>(grad_x));
+        hipLaunchKernelGGL((ce_finish_kernel<O>), grid_of(ceil_div(n * (p.c4 / 4), 256)), dim3(256), 0, st, reinterpret_cast<const float *>(ws + p.sums),
+                           p.first_steps, p.big, rows, C, p.c4, factors, factor, static_cast<O *>(grad_x));
     return check_launch("mvs_linear_ce_bwd");
 }
 
@@ -1295,7 +1397,9 @@ using namespace mvs;
 
 extern "C" size_t mvs_linear_ce_workspace_bytes(int64_t n, int64_t V, int C, int dtype, int backward, int need_x, int need_w) {
     if (n < 0 || V < 1 || C < 1 || dtype_size(dtype) == 0) return 0;
-    return ce_plan(n, V, C, dtype, backward != 0, need_x != 0, need_w != 0).total + 256;
+    const size_t plain = ce_plan(n, V, C, dtype, false, backward != 0, need_x != 0, need_w != 0).total;
+    const size_t pieces = ce_in_pieces(n, C, dtype) ? ce_plan(n, V, C, dtype, true, backward != 0, need_x != 0, need_w != 0).total : 0;
+    return (plain > pieces ? plain : pieces) + 256;
 }
 
 extern "C" int mvs_linear_ce_fwd(const void *x, const void *weight, int dtype, const int64_t *target, int64_t n, int64_t V, int C, float scale,
@@ -1327,7 +1431,8 @@ extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, c
         set_error("mvs_linear_ce_bwd: lse, kept, grad_loss and a gradient to compute are needed");
         return MVS_EINVAL;
     }
-    const CePlan p = ce_plan(n, V, C, dtype, true, grad_x != nullptr, grad_weight != nullptr);
+    // (rows with factors of their own need dl^T, which the pieces' products do without)
+    const CePlan p = ce_plan(n, V, C, dtype, reduction != 0 && ce_in_pieces(n, C, dtype), true, grad_x != nullptr, grad_weight != nullptr);
     char *ws = static_cast<char *>(workspace);
     const CeRows rows = ce_rows(p, target, n, ignore_index, nullptr, ws, as_stream(stream));
     if (p.narrow) {
@@ -1340,6 +1445,8 @@ extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, c
         a.factor = scale / (dtype == MVS_DTYPE_F16 ? GradUnit<f16_t>::value : 1.0f);
         return ce_narrow_backward(dtype, a, as_stream(stream));
     }
+    if (p.pieces)
+        return ce_wide_backward<pieces_t>(p, x, weight, rows, lse, kept, grad_loss, V, C, scale, reduction, grad_x, grad_weight, ws, as_stream(stream));
     MVS_DTYPE_DISPATCH(dtype, T, {
         return (ce_wide_backward<T>(p, x, weight, rows, lse, kept, grad_loss, V, C, scale, reduction, grad_x, grad_weight, ws, as_stream(stream)));
     });

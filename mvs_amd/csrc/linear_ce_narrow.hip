@@ -380,23 +380,6 @@ __global__ __launch_bounds__(256, 2) void narrow_grad_kernel(NarrowArgs a, float
         narrow_grad<X, true>(a, a.w, x, of_table % split.blocks_w, of_table / split.blocks_w, split.per_w, unit, log_unit, lds, row_stats);
 }
 
-// a value's pieces: 8 bits each, the first one cut instead of rounded where rounding would overflow
-template <typename E, int PL, typename T>
-__device__ __forceinline__ void pieces_of(T value, E (&p)[PL]) {
-    if constexpr (PL == 1) {
-        p[0] = value;
-    } else {
-        float v = value;
-        p[0] = from_float<E>(v);
-        if (__builtin_fabsf(v) > DtypeMax<E>::value && __builtin_fabsf(v) <= DtypeMax<float>::value) p[0].bits = (unsigned short)(__float_as_uint(v) >> 16);
-#pragma unroll
-        for (int q = 1; q < PL; ++q) {
-            v -= to_float(p[q - 1]);
-            p[q] = from_float<E>(v);
-        }
-    }
-}
-
 // Writes what the other kernels read of x (blockIdx.y = 0) and of the table (1): the rows in pieces and their transpose, 64 rows per
 // workgroup.  Backward: blockIdx.y = 2 works out the rows' factors (one workgroup).
 template <typename T, typename E, int PL>

@@ -2218,7 +2218,8 @@ def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduct
     all is 0 / 0 = NaN, its gradients zero); any other target outside [0, V) makes its row's loss and the gradients NaN.
     Products are summed in float32.  For 16-bit operands the backward pass rounds each logit's gradient to that type before its two
     products (half a unit in the last place of each term, of either sign); float32 operands keep 24 bits throughout (rows of at most
-    64 go through the matrix cores as three bfloat16 pieces: the sums are as exact, an Inf among them counts as a NaN).  Equal calls
+    64, and longer ones where there are more than 256, go through the matrix cores as three bfloat16 pieces: the sums are as exact, an
+    Inf among them counts as a NaN, and what is below 2^-133 is dropped).  Equal calls
     give equal bits."""
     _dtype_code(x, "linear_cross_entropy")
     if weight.dtype != x.dtype:

@@ -509,6 +509,57 @@ def test_linear_cross_entropy_of_a_single_row(C, dtype):
     gx, gw = torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, reduction="sum"), leaves)
     assert not torch.isfinite(gx).any() and not torch.isfinite(gw).any()
 
+@pytest.mark.parametrize("n,V,C", [(257, 100, 65), (300, 3001, 130), (1100, 777, 513), (2500, 6000, 700)])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_linear_cross_entropy_of_many_wide_float32_rows(reduction, n, V, C):
+    """float32 rows in three pieces, forward and backward (reduction 'none': its backward pass in float32)."""
+    x, w, t, _ = ce_case(n, V, C, torch.float32, seed=n)
+    for scale in (1.0, -3.0):
+        ce_check(x, w, t, scale, reduction=reduction)
+
+
+@pytest.mark.parametrize("n,V,C", [(257, 100, 65), (300, 3001, 130), (1100, 777, 513), (2500, 6000, 700)])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_linear_cross_entropy_float32_pieces_at_the_ends_of_the_range(reduction, n, V, C):
+    """Values that bfloat16 rounds to infinity, and ones whose last bits are below its least: a value is carried to within half of
+    2^-133, so a logit of x = 2^128 (1 - 2^-24) and w < 2^-127 is off by at most 2^128 2^-134 = 2^-6, in either pass; a loss by two of
+    those, an exponential by a factor of e^(2 2^-6).  (dW, some 2^128 times a probability, has sums that no float32 holds.)"""
+    _, _, t, _ = ce_case(n, V, C, torch.float32, seed=n)
+    big = torch.finfo(torch.float32).max
+    x = torch.zeros(n, C, device="cuda")
+    x[:, 0], x[:, 1] = big, 1e-30
+    w = torch.zeros(V, C, device="cuda")
+    w[:, 0], w[:, 1] = torch.arange(V, device="cuda") / V / big, 1e30
+    leaf = x.requires_grad_()
+    loss = ops.linear_cross_entropy(leaf, w, t, reduction=reduction)
+    gx, = torch.autograd.grad(loss.sum(), leaf)
+    kept = t >= 0
+    logits = x.detach().double() @ w.double().t()
+    lse = torch.logsumexp(logits, 1, keepdim=True)
+    want = torch.where(kept, (lse - logits.gather(1, t.clamp(min=0).unsqueeze(1))).squeeze(1), 0.0)
+    off = 2 * 2.0 ** -6 + 1e-4
+    if reduction == "none":
+        assert ((loss.detach().double() - want).abs() <= off).all()
+    else:
+        total, count = float(want.sum()), int(kept.sum())
+        assert abs(float(loss.detach()) - (total if reduction == "sum" else total / count)) <= off * (count if reduction == "sum" else 1)
+    p = torch.exp(logits - lse)
+    dl = p.clone()
+    dl[torch.arange(n, device="cuda"), t.clamp(min=0)] -= 1
+    g = kept.double().unsqueeze(1) / (int(kept.sum()) if reduction == "mean" else 1)
+    bound = (math.expm1(2 * 2.0 ** -6) + 1e-4) * (p * g) @ w.double().abs() + V * U * (dl.abs() * g) @ w.double().abs() + 2.0 ** -126
+    assert ((gx.double() - (dl * g) @ w.double()).abs() <= bound).all()
+
+
+def test_linear_cross_entropy_of_wide_float32_rows_in_pieces_of_the_table():
+    x, w, t, _ = ce_case(1025, (1 << 17) + 301, 100, torch.float32, seed=6)
+    ce_check(x, w, t, 2.0)
+    x[5, 7] = float("nan")
+    t[5] = -100
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    gx, gw = torch.autograd.grad(ops.linear_cross_entropy(*leaves, t), leaves)
+    assert torch.isfinite(gx).all() and torch.isfinite(gw).all() and (gx[5] == 0).all()
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n,V,C", [(600, 40001, 768), (9001, 700, 1000), (3000, 5000, 1096)])
 def test_linear_cross_entropy_on_large_tiles(n, V, C, dtype):
