@@ -732,7 +732,7 @@ int mvs_lookup_rows_bwd(const void *grad_out, int dtype, const int64_t *index, i
                         void *grad_table, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Softmax cross entropy of n rows against a table of V rows without the logits: l[i][v] = scale * <x[i], weight[v]>,
- * loss_i = logsumexp_v l[i][v] - l[i][target[i]].  x [n, C], weight [V, C] contiguous, of one type, 16-byte aligned; target int64.
+ * loss_i = logsumexp_v l[i][v] - l[i][target[i]].  x [n, C], weight [V, C] contiguous, of one type, 16-byte aligned, as the gradients; target int64.
  * A row whose target is ignore_index has loss 0 and no gradient, whatever x holds there; a target outside [0, V) otherwise makes
  * the row's loss NaN.  Products are summed in float32, losses are float32; float32 operands run on the float32 matrix pipe, rows of
  * at most 64 of them, and more than 256 longer rows, as three bfloat16 pieces (24 bits down to 2^-133; an Inf among them counts

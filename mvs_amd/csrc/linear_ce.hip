@@ -1421,6 +1421,10 @@ extern "C" int mvs_linear_ce_bwd(const void *x, const void *weight, int dtype, c
     const int rc = ce_check("mvs_linear_ce_bwd", x, weight, dtype, target, n, V, C, reduction, workspace, workspace_bytes,
                             mvs_linear_ce_workspace_bytes(n, V, C, dtype, 1, grad_x != nullptr, grad_weight != nullptr));
     if (rc != MVS_OK) return rc;
+    if (!aligned16(grad_x) || !aligned16(grad_weight)) {
+        set_error("mvs_linear_ce_bwd: the gradients are to be aligned to 16 bytes");
+        return MVS_EINVAL;
+    }
     if (n == 0) {
         if (grad_weight)
             hipLaunchKernelGGL(ce_zero_kernel, dim3(1024), dim3(256), 0, as_stream(stream), static_cast<unsigned short *>(grad_weight),

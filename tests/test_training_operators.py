@@ -140,6 +140,7 @@ def test_linear_ce_entry_points_refuse_bad_arguments(call):
     assert _ce(call, nbytes=64) == EWORKSPACE
     assert _ce("fwd", loss=None) == EINVAL
     assert _ce("bwd", g=None) == EINVAL and _ce("bwd", gx=None, gw=None) == EINVAL
+    assert _ce("bwd", gx=ODD) == EINVAL and _ce("bwd", gw=ODD) == EINVAL and "gradients" in _text()
 
 
 def test_linear_ce_workspace_keeps_no_logits():
