@@ -737,7 +737,8 @@ int mvs_lookup_rows_bwd(const void *grad_out, int dtype, const int64_t *index, i
  * the row's loss NaN.  Products are summed in float32, losses are float32; float32 operands run on the float32 matrix pipe, rows of
  * at most 64 of them, and more than 256 longer rows, as three bfloat16 pieces (24 bits down to 2^-133; an Inf among them counts
  * as a NaN).
- * reduction: 0 none (loss [n]), 1 mean over the rows kept (0 / 0 = NaN if there are none; gradients are then zero), 2 sum.
+ * reduction: 0 none (loss [n]), 1 mean over the rows kept (0 / 0 = NaN if there are none), 2 sum.  With no row
+ * kept the gradients are zero whatever grad_loss holds.
  * lse [n] (of the kept rows, in the backward pass's order) and kept [1] (their number, as a float) are for the backward pass.
  * Backward: grad_loss [n] (reduction 0) or [1]; grad_x [n, C] and grad_weight [V, C] in the operands' type, either may be NULL.
  * The logits are formed again, a piece of the table at a time; the workspace (mvs_linear_ce_workspace_bytes; backward != 0 for

@@ -56,14 +56,15 @@ __device__ __forceinline__ int64_t ce_count(const CeRows &r) { return r.count ? 
 __device__ __forceinline__ int64_t ce_original(const CeRows &r, int64_t i) { return r.map ? r.map[i] : i; }
 
 // g of the rows `first`, `first` + `step`, ... and their ratios to one number, which is the last: factors[i], factors[n + i],
-// factors[2 n].  One factor for all rows is that number, the ratios are 1; else it is the largest magnitude, which one workgroup
-// looks for first.  `tops`: a word of LDS per wave.
+// factors[2 n].  One factor for all rows is that number (0 if no row is kept, whatever comes from above: Inf times dW's empty sums
+// would be NaN), the ratios are 1; else it is the largest magnitude, which one workgroup looks for first.  `tops`: a word of LDS per
+// wave.
 __device__ __forceinline__ void ce_factors(const CeRows &rows, const float *__restrict__ grad_loss, const float *__restrict__ kept, int reduction,
                                            float *__restrict__ factors, int64_t first, int64_t step, float *tops) {
     const int64_t count = ce_count(rows);
     float top = 0.0f;
     if (reduction != 0) {
-        const float common = reduction == 2 ? grad_loss[0] : *kept > 0.0f ? grad_loss[0] / *kept : 0.0f;
+        const float common = !(*kept > 0.0f) ? 0.0f : reduction == 2 ? grad_loss[0] : grad_loss[0] / *kept;
         for (int64_t i = first; i < count; i += step) {
             const bool here = ce_kept(rows.target[i], rows.ignore) && common != 0.0f;
             factors[i] = here ? common : 0.0f;

@@ -2215,7 +2215,7 @@ def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduct
     loss, in float32 -- torch.nn.functional.cross_entropy(scale * x @ weight.T, target, ignore_index=..., reduction=...) without the
     [rows, V] tensor, forward or backward.  scale is one over a temperature.
     A row with target == ignore_index has loss 0 and leaves no trace in a gradient, whatever x holds there (the mean over no row at
-    all is 0 / 0 = NaN, its gradients zero); any other target outside [0, V) makes its row's loss and the gradients NaN.
+    all is 0 / 0 = NaN; the gradients of no row are zero, whatever comes from above); any other target outside [0, V) makes its row's loss and the gradients NaN.
     Products are summed in float32.  For 16-bit operands the backward pass rounds each logit's gradient to that type before its two
     products (half a unit in the last place of each term, of either sign); float32 operands keep 24 bits throughout (rows of at most
     64, and longer ones where there are more than 256, go through the matrix cores as three bfloat16 pieces: the sums are as exact, an
