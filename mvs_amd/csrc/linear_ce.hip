@@ -807,7 +807,7 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeFew a) {
     const int64_t v0 = (int64_t)blockIdx.x * kFewTable;
     const int rows = (int)min((int64_t)kFewTable, a.count - v0);
     const bool here = col < a.Cp;
-    float lse2 = INFINITY, ratio_w = 0.0f;      // (an ignored row: logits of 0, exponentials of -Inf)
+    float lse2 = 0.0f, ratio_w = 0.0f;
     int target = -1;
     bool kept = false;
     if constexpr (LOGITS) {
@@ -855,7 +855,8 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeFew a) {
             few_logits<T, VEC, BATCH>(p, x[0], a.threads, shares[b & 1], l);
 #pragma unroll
             for (int u = 0; u < BATCH; ++u) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(l[u], a.scale2, -lse2));
+                // (an ignored row has no gradient, whatever the table holds: a logit of 0 times Inf is NaN)
+                const float e = kept ? __builtin_amdgcn_exp2f(__builtin_fmaf(l[u], a.scale2, -lse2)) : 0.0f;
                 g[u][0] = v + u * subs == target ? e - 1.0f : e;
             }
         } else {

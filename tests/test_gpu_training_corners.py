@@ -26,3 +26,15 @@ def test_linear_cross_entropy_without_a_kept_row_has_no_gradient(n, C, upstream,
         gx, gw = torch.autograd.grad(loss, (x, w), torch.full_like(loss, upstream))
         assert (gx == 0).all() and (gw == 0).all(), reduction
         assert math.isnan(float(loss.detach())) if reduction == "mean" else (loss == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("C", [40, 200, 1024, 2056])
+def test_linear_cross_entropy_of_a_single_ignored_row_whatever_the_table_holds(C, bad, dtype):
+    x, w = randn(1, C, seed=1).to(dtype), randn(150, C, seed=2).to(dtype)
+    w[7], w[149, 3] = bad, bad
+    x, w = x.requires_grad_(), w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, torch.tensor([-100], device="cuda"), reduction="sum")
+    gx, gw = torch.autograd.grad(loss, (x, w))
+    assert float(loss.detach()) == 0 and (gx == 0).all() and (gw == 0).all()
