@@ -86,13 +86,8 @@ def matching_cells(depth, src_proj, ref_proj, mask=None):
     return cell.to(torch.int64)
 
 
-def feature_matching_loss(ref_fea, src_fea, ref_cells, src_cells, temperature=1.0):
-    """Cross entropy of finding a point's cell in the source view by its feature in the reference view: over the pairs (point) of
-    ref_cells, src_cells [B,P] (cell numbers y * w + x; -1 on either side: no such pair; a number beyond its map: NaN), the softmax of
-    <ref feature, source feature> / temperature over ALL cells of the source map, averaged over the pairs there are (NaN if there is
-    none).
-    ref_fea, src_fea [B,C,h,w]; differentiable in both.  The [P, h*w] scores are never stored (ops.linear_cross_entropy), several
-    points may share a cell (ops.lookup_rows)."""
+def matching_sums(ref_fea, src_fea, ref_cells, src_cells, temperature=1.0):
+    """feature_matching_loss as (sum over the pairs there are, their number): 0 of 0, with gradients of zero, where there is none."""
     B, C, h, w = src_fea.shape
     total = 0.0
     for b in range(B):
@@ -101,4 +96,15 @@ def feature_matching_loss(ref_fea, src_fea, ref_cells, src_cells, temperature=1.
         target = torch.where(paired, src_cells[b].masked_fill(ref_cells[b] >= rows[0].shape[0], h * w), -100)
         total = total + ops.linear_cross_entropy(ops.lookup_rows(rows[0], ref_cells[b]), rows[1], target, scale=1.0 / temperature,
                                                  reduction="sum")
-    return total / ((ref_cells >= 0) & (src_cells >= 0)).sum()
+    return total, ((ref_cells >= 0) & (src_cells >= 0)).sum()
+
+
+def feature_matching_loss(ref_fea, src_fea, ref_cells, src_cells, temperature=1.0):
+    """Cross entropy of finding a point's cell in the source view by its feature in the reference view: over the pairs (point) of
+    ref_cells, src_cells [B,P] (cell numbers y * w + x; -1 on either side: no such pair; a number beyond its map: NaN), the softmax of
+    <ref feature, source feature> / temperature over ALL cells of the source map, averaged over the pairs there are (NaN if there is
+    none, with gradients of zero).
+    ref_fea, src_fea [B,C,h,w]; differentiable in both.  The [P, h*w] scores are never stored (ops.linear_cross_entropy), several
+    points may share a cell (ops.lookup_rows)."""
+    total, pairs = matching_sums(ref_fea, src_fea, ref_cells, src_cells, temperature)
+    return total / pairs

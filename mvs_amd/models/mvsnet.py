@@ -24,7 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import ops
-from .module import ConvBnReLU, ConvBnReLU3D, feature_matching_loss, matching_cells
+from .module import ConvBnReLU, ConvBnReLU3D, matching_cells, matching_sums
 
 
 class FeatureNet(nn.Module):
@@ -560,9 +560,10 @@ class MVSNet(nn.Module):
     def matching_loss(self, imgs, proj_matrices, depth, mask=None, temperature=0.1):
         """Supervision of FeatureNet alone, from the depth the reference view is trained on: every reference cell with a depth has to
         find its cell in each source view among all of them (feature_matching_loss over matching_cells), averaged over the source
-        views.  imgs [B,V,3,H,W], proj_matrices [B,V,4,4], depth and mask [B,H/4,W/4].  Train on it first, or add it to mvsnet_loss (a
-        second pass of FeatureNet, which counts as one more update of its running statistics); training mode, FeatureNet's HIP
-        layers (each view with its own batch statistics, as in forward())."""
+        views that have such a pair: one that shows nothing of the reference view is left out, and without any pair the loss and
+        its gradients are 0.  imgs [B,V,3,H,W], proj_matrices [B,V,4,4], depth and mask [B,H/4,W/4].  Train on it first, or add it to
+        mvsnet_loss (a second pass of FeatureNet, which counts as one more update of its running statistics); training mode,
+        FeatureNet's HIP layers (each view with its own batch statistics, as in forward())."""
         if not (self.training and self.feature.hip_supported()):
             raise ops.MvsHipError("matching_loss: a training step on FeatureNet's HIP layers (model.train())")
         if imgs.shape[1] != proj_matrices.shape[1] or imgs.shape[1] < 2:
@@ -575,9 +576,10 @@ class MVSNet(nn.Module):
         fea = self.feature.forward_train_hip(imgs.transpose(0, 1).reshape(V * B, *imgs.shape[2:]), groups=V, act8=self.train_act8)
         fea = fea.reshape(V, B, *fea.shape[1:]).permute(0, 1, 4, 2, 3)             # [V,B,C,h,w] views of channels-last maps
         here = torch.arange(fea.shape[3] * fea.shape[4], device=fea.device).expand(B, -1)
-        losses = [feature_matching_loss(fea[0], fea[v], here, matching_cells(depth, proj_matrices[:, v], proj_matrices[:, 0], mask), temperature)
-                  for v in range(1, V)]
-        return torch.stack(losses).mean()
+        totals, pairs = zip(*[matching_sums(fea[0], fea[v], here, matching_cells(depth, proj_matrices[:, v], proj_matrices[:, 0], mask), temperature)
+                              for v in range(1, V)])
+        pairs = torch.stack(pairs)
+        return (torch.stack(totals) / pairs.clamp(min=1)).sum() / (pairs > 0).sum().clamp(min=1)
 
 
 def mvsnet_loss(depth_est, depth_gt, mask):

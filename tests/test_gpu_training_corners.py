@@ -1,10 +1,12 @@
 """Corners of the training operators that keep no large tensor, on the GPU."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from mvs_amd import ops
+from mvs_amd import ops, synth
+from mvs_amd.models import MVSNet, feature_matching_loss
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -38,3 +40,49 @@ def test_linear_cross_entropy_of_a_single_ignored_row_whatever_the_table_holds(C
     loss = ops.linear_cross_entropy(x, w, torch.tensor([-100], device="cuda"), reduction="sum")
     gx, gw = torch.autograd.grad(loss, (x, w))
     assert float(loss.detach()) == 0 and (gx == 0).all() and (gw == 0).all()
+
+
+def _scene(V=3, seed=5, H=128, W=160):
+    rng = np.random.default_rng(seed)
+    imgs = torch.from_numpy(synth.images(rng, 1, V, H, W)).cuda()
+    proj = torch.from_numpy(synth.proj_matrices(V, H // 4, W // 4)).cuda().expand(1, -1, -1, -1).contiguous()
+    gt = torch.from_numpy((synth.DTU_TARGET_Z + 20 * rng.standard_normal((1, H // 4, W // 4))).astype(np.float32)).cuda()
+    return imgs, proj, gt
+
+
+def _matching_step(imgs, proj, gt, mask=None):
+    torch.manual_seed(3)
+    model = MVSNet(refine=False).cuda().train()
+    loss = model.matching_loss(imgs, proj, gt, mask)
+    loss.backward()
+    return float(loss.detach()), {k: p.grad for k, p in model.feature.named_parameters()}
+
+
+@pytest.mark.parametrize("without", [1, 2])
+def test_matching_loss_leaves_out_a_view_without_a_pair(without):
+    """Every point behind that view's camera: the loss and the gradients are those of the other views."""
+    imgs, proj, gt = _scene()
+    proj[:, without, 2] *= -1
+    loss, grads = _matching_step(imgs, proj, gt)
+    rest = [v for v in range(3) if v != without]
+    want, wants = _matching_step(imgs[:, rest].contiguous(), proj[:, rest].contiguous(), gt)
+    # FeatureNet normalises each view by itself; its statistics may be rounded another way in a batch of three: logits of a few hundred
+    # move by their last bits, 1e-4 at most, and a probability by that part of it
+    assert math.isfinite(loss) and abs(loss - want) <= 1e-4 * want
+    for k in grads:
+        assert torch.isfinite(grads[k]).all() and float((grads[k] - wants[k]).norm()) <= 1e-3 * float(wants[k].norm()) + 1e-12, k
+
+
+def test_matching_loss_without_any_pair_is_zero():
+    imgs, proj, gt = _scene()
+    loss, grads = _matching_step(imgs, proj, gt, torch.zeros_like(gt))
+    assert loss == 0
+    for k in grads:
+        assert (grads[k] == 0).all(), k
+    # ... and the loss of a single pair of maps is 0 / 0, with gradients of zero
+    a, b = randn(1, 32, 8, 9, seed=1).requires_grad_(), randn(1, 32, 8, 9, seed=2).requires_grad_()
+    none = torch.full((1, 5), -1, device="cuda")
+    loss = feature_matching_loss(a, b, none, none)
+    assert math.isnan(float(loss.detach()))
+    for g in torch.autograd.grad(loss, (a, b)):
+        assert (g == 0).all()
