@@ -82,8 +82,8 @@ def matching_cells(depth, src_proj, ref_proj, mask=None):
     seen = (depth.reshape(B, h * w) > 0) & (p[..., 2] > 0) & (u >= 0) & (u <= w - 1) & (v >= 0) & (v <= h - 1)
     if mask is not None:
         seen = seen & (mask.reshape(B, h * w) > 0.5)
-    cell = torch.where(seen, v * w + u, torch.full_like(u, -1.0))
-    return cell.to(torch.int64)
+    u, v = (torch.where(seen, t, 0.0).to(torch.int64) for t in (u, v))      # (whole from here on: v * w + u may pass 2^24)
+    return (v * w + u).masked_fill(~seen, -1)
 
 
 def matching_sums(ref_fea, src_fea, ref_cells, src_cells, temperature=1.0):
