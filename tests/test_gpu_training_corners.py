@@ -86,3 +86,44 @@ def test_matching_loss_without_any_pair_is_zero():
     assert math.isnan(float(loss.detach()))
     for g in torch.autograd.grad(loss, (a, b)):
         assert (g == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [2, 4])
+def test_linear_cross_entropy_few_16_bit_rows_in_pieces(n, dtype):
+    """The rows that the one-pass kernel takes, against a table of more than 2^26 / n rows: a second piece, a short one, whose sums are
+    added to the first's."""
+    V, C = (1 << 26) // n + 777, 136
+    w = torch.empty(V, C, device="cuda", dtype=dtype)
+    spans = [slice(v, min(v + (1 << 22), V)) for v in range(0, V, 1 << 22)]
+    for s in spans:
+        w[s] = randn(s.stop - s.start, C, seed=s.start) * 0.1
+    t = torch.tensor([V - 1, (1 << 26) // n, 5, -100], device="cuda")[-n:]      # (n = 2: one row, of the second piece, and an ignored one)
+    t[0] = V - 1
+    x = (randn(n, C, seed=2) + 8 * w[t.clamp(min=0)].float()).to(dtype)
+    x[t < 0] = float("nan")
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    loss = ops.linear_cross_entropy(*leaves, t, reduction="sum")
+    gx, gw = torch.autograd.grad(loss, leaves)
+    keep = t >= 0
+    k, xd = int(keep.sum()), x.detach()[keep].double()
+    logits = torch.cat([xd @ w.detach()[s].double().t() for s in spans], 1)
+    lse = torch.logsumexp(logits, 1)
+    # A logit is off by `most` = (C + 4) u |x| |w|; a row's sum of exponentials by twice that part of it and one rounding for each of the
+    # terms that are added one after the other (a tile's, and every sixteenth tile); a probability by `rel` in all.  dl is rounded to
+    # the type (h; float16 carries it times 2^14: down to 2^-39), and so is each result.
+    u = 2.0 ** -24
+    most = (C + 4) * u * float(xd.abs().sum(1).max()) * float(w.detach().abs().max())
+    rel = math.expm1(2 * most) + (V / 128 / 16 + 300) * u
+    assert abs(float(loss.detach()) - float((lse - logits.gather(1, t[keep].unsqueeze(1)).squeeze(1)).sum())) <= k * (rel + 2 * u * float(lse.max()))
+    h, least = torch.finfo(dtype).eps / 2, 2.0 ** -39 if dtype == torch.float16 else 0.0
+    p = torch.exp(logits - lse.unsqueeze(1))
+    p[torch.arange(k, device="cuda"), t[keep]] -= 1
+    want = sum(p[:, s] @ w.detach()[s].double() for s in spans)
+    off = sum((p[:, s].abs() * (h + rel) + least) @ w.detach()[s].double().abs() for s in spans)
+    assert ((gx[keep].double() - want).abs() <= off + h * (want.abs() + off)).all() and (gx[~keep] == 0).all()
+    smallest = torch.finfo(dtype).smallest_normal
+    for s in (slice(0, 100), slice((1 << 26) // n // 256 * 256 - 300, V)):
+        want = p[:, s].t() @ xd
+        off = (p[:, s].abs() * (h + rel) + least).t() @ xd.abs()
+        assert ((gw[s].double() - want).abs() <= off + h * (want.abs() + off) + smallest).all()
