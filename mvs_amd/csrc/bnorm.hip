@@ -14,8 +14,8 @@
 // HELD (mvs_bn_train_*_act8_f32): the backward pass has x in 8 bits (act8.h) and the ReLU's mask as a bit per value.  The apply
 // pass of the forward writes both while it has x in registers: 1.16 bytes kept per value instead of 4, and the backward's two
 // passes read 1.16 + 4 bytes instead of 8.  The mask is the forward's own, not recomputed from the codes: within half a step of
-// the corner the codes do not know the sign, and a wrong mask bit costs the gradient its whole value there, where a rounded
-// x costs it a part in 250 of the projection term only.  Bound by memory: 3.9 million rows of 8 channels with a skip, forward 37
+// the corner the codes do not know the sign, and a wrong mask bit costs the gradient its whole value there, where a rounded x
+// (off by at most 1 / 127 of its block's largest magnitude) moves the projection term only.  Bound by memory: 3.9 million rows of 8 channels with a skip, forward 37
 // (statistics) + 64 us (apply: 416 MB, 6.5 TB/s), backward 57 (sums: 163 MB, 2.8 TB/s) + 47 us (apply: 288 MB, 6.1 TB/s).  The sums
 // are neither bound by float64 (sums of four terms in float32 first: no change) nor by loads under way (double-buffered rounds, 1024
 // threads: no change; three groups of 328000 rows 31 instead of 17 us with those).

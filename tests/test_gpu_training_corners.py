@@ -127,3 +127,39 @@ def test_linear_cross_entropy_few_16_bit_rows_in_pieces(n, dtype):
         want = p[:, s].t() @ xd
         off = (p[:, s].abs() * (h + rel) + least).t() @ xd.abs()
         assert ((gw[s].double() - want).abs() <= off + h * (want.abs() + off) + smallest).all()
+
+
+@pytest.mark.parametrize("route", ["f16", "f32 weight gradient", "bf16"])
+def test_variance_conv0_act8_gradients_are_those_of_the_rounded_volume(route, monkeypatch):
+    """The variance volume held in 8 bits: conv0's weight gradient is that of the volume read back, nothing else changes."""
+    if route != "f16":
+        monkeypatch.setenv("MVS_WGRAD_F16" if route == "f32 weight gradient" else "MVS_CONV0_F16", "0")
+    V, h, w, D = 3, 32, 40, 16
+    f0, w0 = randn(V, 1, 2, h, w, 16, seed=3) * 0.5, randn(8, 32, 3, 3, 3, seed=4) / 30
+    rts = ops.rot_trans_all(torch.from_numpy(synth.proj_matrices(V, h, w)).cuda(), "device")
+    dv = torch.from_numpy(synth.depth_values(D, interval=synth.sweep_interval(D))).cuda()
+    go = randn(1, D, h, w, 8, seed=5)
+    res = []
+    for act8 in (True, False):
+        f, k = f0.clone().requires_grad_(), w0.clone().requires_grad_()
+        y = ops.variance_conv0_autograd(f[0], f[1:], rts, dv, k, act8=act8)
+        res.append((y.detach(), *torch.autograd.grad(y, (f, k), go)))
+    (y8, gf8, gw8), (y, gf, gw) = res
+    # (the variance's backward pass ends in floating-point atomics: a sum of float32 terms in another order)
+    assert torch.equal(y8, y) and float((gf8 - gf).norm()) <= 1e-5 * float(gf.norm())
+    with torch.no_grad():
+        var = ops.costvol_variance_c16(f0[0].contiguous(), f0[1:].contiguous(), rts, dv, False, out_c8=True,
+                                       absmax_out=ops.absmax_block(f0.device) if route != "bf16" else None)
+        back = ops.act8_dequantize(ops.act8_quantize(var))
+    blocks = torch.nn.functional.pad(var.reshape(-1), (0, -var.numel() % 32)).view(-1, 32)
+    off = torch.nn.functional.pad((back - var).reshape(-1), (0, -var.numel() % 32)).view(-1, 32)
+    assert (off.abs() <= blocks.abs().amax(1, keepdim=True) / 127).all()      # half a step of its block's scale
+
+    def weight_gradient(volume):      # [B, D, H, C / 8, W, 8], in 64 bits on the CPU
+        x = volume.double().cpu().permute(0, 3, 5, 1, 2, 4).reshape(1, 32, D, h, w)
+        return torch.nn.grad.conv3d_weight(x, (8, 32, 3, 3, 3), go.double().cpu().permute(0, 4, 1, 2, 3), padding=1)
+    rounded, full = weight_gradient(back), weight_gradient(var)
+    # two-piece and float32 products of D h w terms: below 1e-5 of the norm, where the volume's rounding moves it by far more
+    for got, want in ((gw8, rounded), (gw, full)):
+        assert float((got.double().cpu() - want).norm()) <= 1e-5 * float(want.norm())
+    assert float((rounded - full).norm()) > 1e-4 * float(full.norm())
