@@ -7,6 +7,7 @@ import torch
 
 from mvs_amd import ops, synth
 from mvs_amd.models import MVSNet, feature_matching_loss
+from product_pieces import LOW_PIECES, PAIRS, SCALE, gradient_bound, gradient_case, gradient_errors, logit_case
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -163,3 +164,28 @@ def test_variance_conv0_act8_gradients_are_those_of_the_rounded_volume(route, mo
     for got, want in ((gw8, rounded), (gw, full)):
         assert float((got.double().cpu() - want).norm()) <= 1e-5 * float(want.norm())
     assert float((rounded - full).norm()) > 1e-4 * float(full.norm())
+
+
+# (the last three: 256 x 256 tiles in the logits', in dW's and in dx's product)
+@pytest.mark.parametrize("n,V,C", LOW_PIECES + [(200, 119, 130), (5000, 12004, 130), (600, 48016, 768), (9001, 811, 1000)])
+def test_linear_cross_entropy_float32_logits_of_the_low_pieces(n, V, C):
+    """tests/test_training_corners.py: any of the low pieces' products left out moves a logit by more than 1."""
+    for which in PAIRS[:3]:
+        x, w, logits = (t.cuda() for t in logit_case(which, n, V, C))
+        t = torch.arange(n, device="cuda") * 7 % V
+        loss = ops.linear_cross_entropy(x, w, t, scale=SCALE, reduction="none")
+        logits = SCALE * logits[0].double()
+        want = torch.logsumexp(logits, 0) - logits[t]
+        # exact products; a logit of at most 9, rounded once or twice, and the sum of V exponentials
+        assert float((loss.double() - want).abs().max()) <= 4 * 9 * 2.0 ** -24 + (V / 128 + 160) * 2.0 ** -24 + 4 * 16 * 2.0 ** -24, which
+
+
+@pytest.mark.parametrize("n,V,C", LOW_PIECES + [(200, 119, 130), (5000, 12004, 130), (600, 48016, 768), (9001, 811, 1000)])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_linear_cross_entropy_float32_gradients_keep_24_bits(reduction, n, V, C):
+    x, w, of_x, of_w = gradient_case(n, V, C)
+    t = torch.full((n,), V - 1)
+    leaves = [x.cuda().requires_grad_(), w.cuda().requires_grad_()]
+    loss = ops.linear_cross_entropy(*leaves, t.cuda(), reduction=reduction)
+    gx, gw = torch.autograd.grad(loss, leaves, torch.full_like(loss, float(n) if reduction == "mean" else 1.0))
+    assert gradient_errors(V, gx.cpu(), gw.cpu(), t, of_x, of_w) <= gradient_bound(V)
