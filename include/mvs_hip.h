@@ -742,9 +742,11 @@ int mvs_lookup_rows_bwd(const void *grad_out, int dtype, const int64_t *index, i
  * lse [n] (of the kept rows, in the backward pass's order) and kept [1] (their number, as a float) are for the backward pass.
  * Backward: grad_loss [n] (reduction 0) or [1]; grad_x [n, C] and grad_weight [V, C] in the operands' type, either may be NULL.
  * The logits are formed again, a piece of the table at a time; the workspace (mvs_linear_ce_workspace_bytes; backward != 0 for
- * the backward pass, with need_x / need_w for the gradients asked for) holds a piece's gradient, transposes of the operands' size
- * and partial sums.  No atomics: equal calls give equal bits.  At most 2^29 rows of either kind (2^23 rows of x where a row is
- * longer than 64 float32 or 128 16-bit values), C at most 2^20. */
+ * the backward pass, with need_x / need_w for the gradients asked for) holds a piece's gradient (2^26 values; float32 in pieces 2^27
+ * of 6 bytes; more beyond 2^18 rows of x) and its transpose, the kept rows of x, partial sums, and a copy of the table where its rows
+ * are not whole 128-byte steps (narrow rows: 32 values) or, 1.5 times its size, go in pieces.  No atomics: equal calls give equal
+ * bits.  At most 2^29 rows of either kind (2^23 rows of x where a row is longer than 64 float32 or 128 16-bit values), C at most
+ * 2^20. */
 size_t mvs_linear_ce_workspace_bytes(int64_t n, int64_t V, int C, int dtype, int backward, int need_x, int need_w);
 int mvs_linear_ce_fwd(const void *x, const void *weight, int dtype, const int64_t *target, int64_t n, int64_t V, int C, float scale,
                       int64_t ignore_index, int reduction, float *loss, float *lse, float *kept, void *workspace,

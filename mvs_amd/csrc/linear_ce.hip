@@ -2,10 +2,13 @@
 //
 //   forward    a tile of logits lives in the matrix cores' accumulators and leaves as one (max, sum of exponentials) per row and
 //              tile; a second launch joins a row's tiles.  2 N V C operations, (N + V) C elements read.
-//   backward   dl = (p - 1[t]) g needs the logits again: a piece of the table at a time (N * piece <= 2^26, so that what it writes
-//              stays in the last-level cache), one launch forms the tile's logits once more and writes dl, rounded to the operands'
-//              type; two products follow, dx += dl W and dW = dl^T x.  6 N V C operations: 8 in all, of which 6 are the
-//              definition's and 2 buy the N V logits not being kept.
+//   backward   dl = (p - 1[t]) g needs the logits again: a piece of the table at a time, one launch forms the tile's logits once more
+//              and writes dl, rounded to the operands' type; two products follow, dx += dl W and dW = dl^T x.  6 N V C operations: 8
+//              in all, of which 6 are the definition's and 2 buy the N V logits not being kept.
+//              A piece is 2^26 / N rows of the table: 16-bit dl is then 128 MB, which stays in the last-level cache, float32 256 MB,
+//              with a dl^T of that size beside it where the products need one.  float32 in pieces takes 2^27 / N rows, 805 MB in
+//              three planes: its products want a full chip more than the cache.  256 rows at the least, so that beyond 2^18 rows of x
+//              dl grows with N.
 //
 // All four products are one kernel shape, C[m][n] = sum_k A[m][k] B[n][k].  A workgroup owns a BM x BN tile and walks k in 128-byte
 // steps: both operands go from memory to LDS by DMA, two stages, the 16-byte chunks of a row exchanged by a few bits of its number so

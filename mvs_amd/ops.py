@@ -2215,12 +2215,19 @@ def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduct
     loss, in float32 -- torch.nn.functional.cross_entropy(scale * x @ weight.T, target, ignore_index=..., reduction=...) without the
     [rows, V] tensor, forward or backward.  scale is one over a temperature.
     A row with target == ignore_index has loss 0 and leaves no trace in a gradient, whatever x holds there (the mean over no row at
-    all is 0 / 0 = NaN; the gradients of no row are zero, whatever comes from above); any other target outside [0, V) makes its row's loss and the gradients NaN.
+    all is 0 / 0 = NaN; the gradients of no row are zero, whatever comes from above); any other target outside [0, V) makes its row's
+    loss and the gradients NaN.
     Products are summed in float32.  For 16-bit operands the backward pass rounds each logit's gradient to that type before its two
-    products (half a unit in the last place of each term, of either sign); float32 operands keep 24 bits throughout (rows of at most
-    64, and longer ones where there are more than 256, go through the matrix cores as three bfloat16 pieces: the sums are as exact, an
-    Inf among them counts as a NaN, and what is below 2^-133 is dropped).  Equal calls
-    give equal bits."""
+    products (half a unit in the last place of each term, of either sign: 8192 x 128000 x 2048 bfloat16 gradients are 0.0020 of their
+    norm from the exact ones, where rounding the results alone costs 0.0017); float32 operands keep 24 bits throughout (rows of at
+    most 64, and longer ones where there are more than 256, go through the matrix cores as three bfloat16 pieces: the sums are as
+    exact, an Inf among them counts as a NaN, and what is below 2^-133 is dropped).  Equal calls give equal bits.
+    Memory besides operands and gradients, for the length of a pass.  Rows longer than 64 float32 or 128 16-bit values: forward 8 bytes
+    for a row of x and 128 rows of the table, backward a piece of the logits' gradient, 2^26 values at most (float32 in pieces 2^27 of
+    6 bytes; more for over 2^18 rows of x), and its transpose where the products need one.  Shorter rows: partial sums of the
+    gradients instead, about 110 MB where there is much to do.  In either pass the kept rows of x, and a copy of the table where its
+    rows are not whole steps of 128 bytes (shorter rows: 32 values), in float32 in pieces always and of 1.5 times its size.  (8192 x
+    128000 x 2048, logits of 4.2 GB: bfloat16 67 and 403 MB, float32 1.7 and 2.5 GB beside a table of 1 GB.)"""
     _dtype_code(x, "linear_cross_entropy")
     if weight.dtype != x.dtype:
         raise MvsHipError(f"linear_cross_entropy: x is {x.dtype}, weight {weight.dtype}")
