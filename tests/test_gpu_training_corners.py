@@ -189,3 +189,78 @@ def test_linear_cross_entropy_float32_gradients_keep_24_bits(reduction, n, V, C)
     loss = ops.linear_cross_entropy(*leaves, t.cuda(), reduction=reduction)
     gx, gw = torch.autograd.grad(loss, leaves, torch.full_like(loss, float(n) if reduction == "mean" else 1.0))
     assert gradient_errors(V, gx.cpu(), gw.cpu(), t, of_x, of_w) <= gradient_bound(V)
+
+
+def _poison(value):
+    """What the allocator hands out next has held `value`."""
+    blocks = [torch.full((n,), value, device="cuda") for n in (1 << 26, 1 << 22, 1 << 18, 1 << 14, 1 << 10, 64) for _ in range(4)]
+    torch.cuda.synchronize()
+    del blocks
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_training_operators_give_equal_bits_whatever_memory_held_and_on_two_streams(dtype):
+    cases = []
+    for n, V, C in ((1, 700, 200), (4, 700, 200), (16, 300, 136), (100, 700, 200), (300, 5001, 200), (1000, 700, 48)):
+        x, w = randn(n, C, seed=n).to(dtype).requires_grad_(), randn(V, C, seed=n + 1).to(dtype).requires_grad_()
+        t = torch.arange(n, device="cuda") * 7 % V
+        t[1::3] = -100
+
+        def loss(x=x, w=w, t=t):
+            value = ops.linear_cross_entropy(x, w, t, scale=0.3)
+            return (value.detach(), *torch.autograd.grad(value, (x, w)))
+        cases.append(loss)
+    for n, rows, C in ((50, 1000, 33), (9000, 70, 64), (40000, 5000, 8)):
+        table, index = randn(rows, C, seed=n).to(dtype).requires_grad_(), (torch.rand(n, device="cuda") ** 3 * rows).long()
+        g = randn(n, C, seed=n + 1).to(dtype)
+        cases.append(lambda table=table, index=index, g=g: torch.autograd.grad(ops.lookup_rows(table, index, 0.7), table, g))
+    a = randn(777, 33, seed=1).to(dtype)
+    cases.append(lambda: (ops.act8_dequantize(ops.act8_quantize(a)),))
+    side = torch.cuda.Stream()
+    for i, case in enumerate(cases):
+        want = case()
+        for value in (float("nan"), 3e38):
+            _poison(value)
+            assert all(torch.equal(p, q) for p, q in zip(case(), want)), (i, value)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            there = [case() for _ in range(3)]
+        here = [case() for _ in range(3)]
+        torch.cuda.synchronize()
+        for got in there + here:
+            assert all(torch.equal(p, q) for p, q in zip(got, want)), i
+
+
+def test_matching_loss_captured_and_replayed():
+    """... with another number of pairs each time, a view without any among them."""
+    bufs = [*_scene(H=256, W=320), torch.ones(1, 64, 80, device="cuda")]
+    torch.manual_seed(3)
+    model = MVSNet(refine=False).cuda().train()
+    weights = list(model.feature.parameters())
+
+    def step():
+        loss = model.matching_loss(*bufs)
+        return [loss.detach(), *torch.autograd.grad(loss, weights)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="relaxed"):
+        out = step()
+    for seed in range(6, 12):
+        imgs, proj, gt = _scene(seed=seed, H=256, W=320)
+        if seed % 3 == 1:
+            proj[:, 1, 2] *= -1
+        mask = (torch.rand(gt.shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda") < 0.3 * (seed % 4)).float()
+        for b, v in zip(bufs, (imgs, proj, gt, mask)):
+            b.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = step()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and (float(want[0]) == 0) == (seed % 4 == 0), seed
+        for g, w in zip(got[1:], want[1:]):      # (the convolutions' weight gradients end in floating-point atomics)
+            assert torch.isfinite(w).all() and float((g - w).norm()) <= 1e-5 * float(w.norm()), seed
