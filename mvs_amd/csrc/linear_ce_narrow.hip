@@ -17,9 +17,13 @@
 // products.  dl is split the same way in the registers.
 //
 // Operations: 10 N V C forward and backward (the logits three times) instead of 8, all on chip.  A 32 x 32 block of logits costs a
-// wave 24 + 24 matrix instructions of 16 cycles (float32, C = 32, a gradient) and about as many cycles of exponentials and splitting,
-// so the gradients are bound by both pipes at once: of 14336 x 20480 x 32 float32 they take 377 us, the matrix cores busy 54 % of it
-// and the vector unit 67 %; the statistics 118 us.  919 x 20480 x 32: gradients 36 us, statistics 14 us, the copies in pieces 7 us a pass.
+// wave 24 + 24 matrix instructions of 16 cycles (float32, C = 32, a gradient) and about as many cycles of exponentials and splitting.
+// Neither pipe is full: of 14336 x 20480 x 32 float32 the gradients take 387 us, the matrix cores busy 52 % of it and the vector unit
+// 64 %, the statistics 119 us at 37 and 64 %.  A wave goes through product, exponentials, splitting and second product in order, and
+// the 2.3 to 2.6 waves a SIMD holds (LDS of two stages, registers of the fragments) do not hide each other's: 37 to 47 % of their
+// cycles wait to issue.  919 x 20480 x 32: gradients 35 us, statistics 14 us, the copies in pieces 7 us a pass.  16 bits have one
+// plane: 20480 x 20480 x 32 bfloat16 gradients 205 us, statistics 119 us -- the float32 ones' time, it is the exponentials'; C = 128
+// 454 and 147 us, 950 and 730 TFLOP/s.
 #include "linear_ce.h"
 
 namespace mvs {
