@@ -36,6 +36,8 @@ __device__ __forceinline__ unsigned pack2(float a, float b, f16_t) {
 }
 __device__ __forceinline__ float low_of(unsigned p, bf16_t) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_of(unsigned p, bf16_t) { return __uint_as_float(p & 0xffff0000u); }
+__device__ __forceinline__ float low_of(unsigned p, f16_t) { return (float)__builtin_bit_cast(_Float16, (unsigned short)p); }
+__device__ __forceinline__ float high_of(unsigned p, f16_t) { return (float)__builtin_bit_cast(_Float16, (unsigned short)(p >> 16)); }
 
 // largest finite value of a type
 template <typename T> struct DtypeMax;

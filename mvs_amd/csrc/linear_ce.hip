@@ -30,6 +30,9 @@
 // one in both passes, so a row's p sum to one).  16-bit dl: float16 carries it times 2^14 (|p - 1| <= 1: no overflow, and p down to
 // 4e-9 keeps a normal number's precision), the row's gradient factor is applied after the product in float32 (dx) or, relative to
 // the largest one, before the rounding (dW) -- 1 / N of a mean never reaches a 16-bit number.
+// The tiles round dl to the operands' type: of two pieces the two products would take their 6.5 ms twice, of 13 in all (8192 x 128000 x
+// 2048 bfloat16), where the gradients are 0.0020 of their norm from the exact ones and rounding the results alone makes it 0.0017.
+// Few rows keep it in float32, narrow ones in two pieces: there it is little beside what is read.
 #include <type_traits>
 
 #include "linear_ce.h"
@@ -456,7 +459,8 @@ __global__ __launch_bounds__(1024) void ce_factors_kernel(CeRows rows, const flo
     ce_factors(rows, grad_loss, kept, reduction, factors, (int64_t)blockIdx.x * 1024 + threadIdx.x, (int64_t)gridDim.x * 1024, tops);
 }
 
-template <typename T, typename X>
+// FLOATS: dl is left as float32 (few rows)
+template <typename T, typename X, bool FLOATS = false>
 __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
     extern __shared__ __align__(1024) char lds[];
     const int64_t rows = ce_count(a.rows);
@@ -515,6 +519,9 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
                 if (n < dl_rows && m < a.ld_dl)
 #pragma unroll
                     for (int q = 0; q < 3; ++q) put(static_cast<char *>(a.dl) + q * a.dl_plane + (n * a.ld_dl + m) * 2, out[q]);
+            } else if constexpr (FLOATS) {
+                const f32x4_t out = kept ? acc[i][j] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                if (n < dl_rows && m < a.ld_dl) *reinterpret_cast<f32x4_t *>(static_cast<float *>(a.dl) + n * a.ld_dl + m) = out;
             } else {
                 Pack<T, 4> out;
 #pragma unroll
@@ -527,7 +534,7 @@ __global__ __launch_bounds__(X::THREADS) void ce_grad_kernel(CeArgs a) {
             }
         }
     }
-    if (kPieces<T> || !a.dlt) return;
+    if (kPieces<T> || FLOATS || !a.dlt) return;
     __syncthreads();
     constexpr int PER16 = 16 / (int)sizeof(T), CHUNKS = X::BN / PER16;
     for (int c = threadIdx.x; c < X::BM * CHUNKS; c += X::THREADS) {
@@ -703,7 +710,8 @@ constexpr int kFewTable = 64;
 // 388 against 368.  float32, whose tiles need W^T: sixteen 172 against 242.
 static int ce_few_rows(int es) { return es == 2 ? 4 : 16; }
 struct CeFew {
-    const void *w, *x, *dl;
+    const void *w, *x;
+    const float *dl;                    // (float32 whatever the operands are: it is little beside the table)
     int64_t count, ld_dl;               // table rows of the piece; elements per row of dl
     int n, C, Cp, threads;              // threads per table row, a power of two
     const float *ratio, *top;
@@ -823,7 +831,7 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeFew a) {
         }
     } else for (int i = tid; i < kFewTable * NR; i += 256) {
         const int v = i / NR, r = i % NR;
-        d[v][r] = v < rows && r < a.n ? to_float(static_cast<const T *>(a.dl)[r * a.ld_dl + v0 + v]) : 0.0f;
+        d[v][r] = v < rows && r < a.n ? a.dl[r * a.ld_dl + v0 + v] : 0.0f;
     }
     float x[NR][VEC], dx[NR][VEC];
 #pragma unroll
@@ -1078,7 +1086,7 @@ static CePlan ce_plan(int64_t n, int64_t V, int C, int dtype, bool pieces, bool 
         p.np = round_up(n, step);
         p.factors = take((size_t)(2 * n + 1) * 4);
         if (p.few) {
-            p.dl = take((size_t)n * p.piece * p.es);
+            p.dl = take((size_t)n * p.piece * 4);
             p.parts = (int)ceil_div(V < p.piece ? V : p.piece, kFewTable);
             if (need_x) p.sums = take((size_t)p.parts * n * p.c4 * 4);
         } else {
@@ -1324,14 +1332,16 @@ static int ce_wide_backward(const CePlan &p, const void *x, const void *w, const
         a.w.p = w_rows + v0 * p.Cp * p.es;
         a.w.rows = count;
         a.v0 = v0; a.v_count = count; a.ld_dl = k;
-        if (!logits) ce_tiles<T>(count, n, [&](auto x) {
+        auto gradient = [&](auto x, auto kernel) {
             using X = decltype(x);
             a.tiles_m = ceil_div(count, X::BM); a.tiles_n = ceil_div(n, X::BN);
-            ce_launch<X>(ce_grad_kernel<T, X>, a, dim3((unsigned)(a.tiles_m * a.tiles_n)), (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
-        });
+            ce_launch<X>(kernel, a, dim3((unsigned)(a.tiles_m * a.tiles_n)), (size_t)X::BM * (X::BN * sizeof(T) + 16), st);
+        };
+        if constexpr (!kPieces<T>) if (p.few && !logits) gradient(Tile128(), ce_grad_kernel<T, Tile128, true>);
+        if (!p.few) ce_tiles<T>(count, n, [&](auto x) { gradient(x, ce_grad_kernel<T, decltype(x)>); });
         if constexpr (!kPieces<T>) if (p.few) {
             CeFew d = {};
-            d.w = a.w.p; d.x = a.x.p; d.dl = a.dl; d.count = count; d.ld_dl = k;
+            d.w = a.w.p; d.x = a.x.p; d.dl = static_cast<const float *>(a.dl); d.count = count; d.ld_dl = k;
             d.n = (int)n; d.C = C; d.Cp = p.Cp;
             d.ratio = factors + n; d.top = factors + 2 * n; d.factor = few_factor;
             if (logits) { d.lse2 = lse; d.target = rows.target; d.ignore = rows.ignore; d.v0 = v0; d.scale2 = a.scale2; }

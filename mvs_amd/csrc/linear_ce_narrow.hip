@@ -14,7 +14,10 @@
 //
 // float32 runs on the bfloat16 pipe: a value is three bfloat16 pieces of 8 bits each (24 in all: nothing is dropped), a product six
 // of the nine piece products -- the others are below 2^-24 of it -- summed in float32.  16 times the float32 pipe's rate over six
-// products.  dl is split the same way in the registers.
+// products.  dl is split the same way in the registers.  For 16-bit operands dl is two pieces of their type, 16 bits at the least: a
+// row's dl sum to 0, so where the table's rows have much in common the gradient is what is left of sums far larger than itself, and
+// half a unit of 8 or 11 bits in each dl shows there (4096 x 17296 x 8 bfloat16: dx 1.75 times as far from the exact one as with
+// float32 dl).
 //
 // Operations: 10 N V C forward and backward (the logits three times) instead of 8, all on chip.  A 32 x 32 block of logits costs a
 // wave 24 + 24 matrix instructions of 16 cycles (float32, C = 32, a gradient) and about as many cycles of exponentials and splitting.
@@ -22,8 +25,8 @@
 // 64 %, the statistics 119 us at 37 and 64 %.  A wave goes through product, exponentials, splitting and second product in order, and
 // the 2.3 to 2.6 waves a SIMD holds (LDS of two stages, registers of the fragments) do not hide each other's: 37 to 47 % of their
 // cycles wait to issue.  919 x 20480 x 32: gradients 35 us, statistics 14 us, the copies in pieces 7 us a pass.  16 bits have one
-// plane: 20480 x 20480 x 32 bfloat16 gradients 205 us, statistics 119 us -- the float32 ones' time, it is the exponentials'; C = 128
-// 454 and 147 us, 950 and 730 TFLOP/s.
+// plane, and two pieces of dl: 20480 x 20480 x 32 bfloat16 gradients 286 us (205 with one piece), statistics 119 us -- the float32 ones'
+// time, it is the exponentials'; C = 128 617 (454) and 150 us.
 #include "linear_ce.h"
 
 namespace mvs {
@@ -33,6 +36,7 @@ template <typename E_, int PL_, int KS_>
 struct Narrow {
     using E = E_;
     static constexpr int PL = PL_, KS = KS_;
+    static constexpr int DL = PL == 3 ? 3 : 2;                   // pieces of dl
     static constexpr int CT = KS * 2;                            // 16-column tiles of the result
     static constexpr int MR = PL * KS >= 6 ? 32 : 64;            // rows of the moving operand per stage (two workgroups' stages fit a CU)
     static constexpr int RG = MR / 16, HALVES = MR / 32;
@@ -54,6 +58,17 @@ __device__ __forceinline__ void mma_planes(f32x4_t &c, const u32x4_t (&a)[PL], c
         mma_e(c, a[0], b[1], E());
     }
     mma_e(c, a[0], b[0], E());
+}
+
+// c += a b for the pieces that dl is carried in: float32's three as above, 16-bit operands' two against their one plane
+template <typename E, int PL, int DL>
+__device__ __forceinline__ void mma_dl(f32x4_t &c, const u32x4_t (&a)[PL], const u32x4_t (&d)[DL]) {
+    if constexpr (PL == 3) {
+        mma_planes<E, PL>(c, a, d);
+    } else {
+        mma_e(c, a[0], d[1], E());
+        mma_e(c, a[0], d[0], E());
+    }
 }
 
 // LDS holds sub-tiles of rows of 64 bytes, two rows to a 128-byte line, the eight 16-byte chunks of a line exchanged by the line's
@@ -124,20 +139,19 @@ __device__ __forceinline__ void narrow_first(const char *stage, int block, int l
         }
 }
 
-// eight values of a lane, as they lie, as a fragment of each plane
-template <typename E, int PL>
-__device__ __forceinline__ void narrow_pieces(const f32x4_t &lo, const f32x4_t &hi, u32x4_t (&d)[PL]) {
+// eight values of a lane, as they lie, as a fragment of each of their pieces
+template <typename E, int DL>
+__device__ __forceinline__ void narrow_pieces(const f32x4_t &lo, const f32x4_t &hi, u32x4_t (&d)[DL]) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         float v0 = w < 2 ? lo[w * 2] : hi[w * 2 - 4], v1 = w < 2 ? lo[w * 2 + 1] : hi[w * 2 - 3];
-        d[0][w] = pack2(v0, v1, E());
-        if constexpr (PL == 3) {
-            v0 -= low_of(d[0][w], E());
-            v1 -= high_of(d[0][w], E());
-            d[1][w] = pack2(v0, v1, E());
-            v0 -= low_of(d[1][w], E());
-            v1 -= high_of(d[1][w], E());
-            d[2][w] = pack2(v0, v1, E());
+#pragma unroll
+        for (int q = 0; q < DL; ++q) {
+            d[q][w] = pack2(v0, v1, E());
+            if (q + 1 < DL) {
+                v0 -= low_of(d[q][w], E());
+                v1 -= high_of(d[q][w], E());
+            }
         }
     }
 }
@@ -343,16 +357,16 @@ __device__ __forceinline__ void narrow_grad(const NarrowArgs &a, const NarrowOpe
                             if (mh + i * 16 + group * 4 + r >= rows) s[i][0][r] = s[i][1][r] = 0.0f;
                 }
             }
-            u32x4_t d[2][X::PL];
+            u32x4_t d[2][X::DL];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) narrow_pieces<typename X::E, X::PL>(s[0][j], s[1][j], d[j]);
+            for (int j = 0; j < 2; ++j) narrow_pieces<typename X::E, X::DL>(s[0][j], s[1][j], d[j]);
 #pragma unroll
             for (int c = 0; c < X::CT; ++c) {
                 u32x4_t f[X::PL];
 #pragma unroll
                 for (int q = 0; q < X::PL; ++q) f[q] = narrow_frag(trans + (q * X::HALVES + half) * X::CT * 1024, c, lane_at);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) mma_planes<typename X::E, X::PL>(out[c][j], f, d[j]);
+                for (int j = 0; j < 2; ++j) mma_dl<typename X::E, X::PL, X::DL>(out[c][j], f, d[j]);
             }
         }
     }

@@ -2217,9 +2217,10 @@ def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduct
     A row with target == ignore_index has loss 0 and leaves no trace in a gradient, whatever x holds there (the mean over no row at
     all is 0 / 0 = NaN; the gradients of no row are zero, whatever comes from above); any other target outside [0, V) makes its row's
     loss and the gradients NaN.
-    Products are summed in float32.  For 16-bit operands the backward pass rounds each logit's gradient to that type before its two
-    products (half a unit in the last place of each term, of either sign: 8192 x 128000 x 2048 bfloat16 gradients are 0.0020 of their
-    norm from the exact ones, where rounding the results alone costs 0.0017); float32 operands keep 24 bits throughout (rows of at
+    Products are summed in float32.  For more than four rows of more than 128 16-bit values the backward pass rounds each logit's
+    gradient to their type before its two products (half a unit in the last place of each term, of either sign: 8192 x 128000 x 2048
+    bfloat16 gradients are 0.0020 of their norm from the exact ones, where rounding the results alone costs 0.0017); other 16-bit
+    rows keep 16 bits of it at the least, float32 operands keep 24 bits throughout (rows of at
     most 64, and longer ones where there are more than 256, go through the matrix cores as three bfloat16 pieces: the sums are as
     exact, an Inf among them counts as a NaN, and what is below 2^-133 is dropped).  Equal calls give equal bits.
     Memory besides operands and gradients, for the length of a pass.  Rows longer than 64 float32 or 128 16-bit values: forward 8 bytes

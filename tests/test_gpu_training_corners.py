@@ -264,3 +264,38 @@ def test_matching_loss_captured_and_replayed():
         assert torch.equal(got[0], want[0]) and (float(want[0]) == 0) == (seed % 4 == 0), seed
         for g, w in zip(got[1:], want[1:]):      # (the convolutions' weight gradients end in floating-point atomics)
             assert torch.isfinite(w).all() and float((g - w).norm()) <= 1e-5 * float(w.norm()), seed
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,V,C", [(300, 300, 8), (1021, 511, 8), (50, 200, 33), (400, 300, 128), (130, 511, 100), (2, 300, 130), (3, 511, 1024), (4, 301, 257)])
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_linear_cross_entropy_of_narrow_or_few_16_bit_rows_keeps_the_logits_gradient(reduction, n, V, C, dtype):
+    """A table around a common value: what a row's gradients of the logits, which sum to 0, make of it cancels, and what they are rounded
+    to would show.  Sixteenths throughout, so that a logit is a sum of exact products without a rounding."""
+    x, w = (torch.round(4 * randn(n, C, seed=n)) / 16).to(dtype), (2 + torch.round(4 * randn(V, C, seed=n + 1)) / 16).to(dtype)
+    t = torch.arange(n, device="cuda") * 7 % V
+    t[1::5] = -100
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    loss = ops.linear_cross_entropy(*leaves, t, reduction=reduction)
+    g = 0.5 + torch.rand(n, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda") if reduction == "none" else torch.ones((), device="cuda")
+    gx, gw = torch.autograd.grad(loss, leaves, g)
+    kept = (t >= 0).nonzero().squeeze(1)
+    xd, wd = x.detach()[kept].double(), w.detach().double()
+    l = xd @ wd.t()
+    p = torch.exp(l - torch.logsumexp(l, 1, keepdim=True))
+    dl = p.clone()
+    dl[torch.arange(len(kept), device="cuda"), t[kept]] -= 1
+    factor = (g.double()[kept] if reduction == "none" else torch.ones(len(kept), dtype=torch.float64, device="cuda")).unsqueeze(1)
+    # A logit is rounded with its scale and again as an exponent, 4 u of it; a probability is off by twice the largest of a row's and its
+    # sum's roundings, (V / 128 + 160) u.  Each logit's gradient keeps 16 bits at the least (float16: down to 2^-39; with factors of its own a
+    # row's come to the largest one's before that).  Sums of V or n float32 products, and the result rounded once.
+    u, h = 2.0 ** -24, torch.finfo(dtype).eps / 2
+    off_l = 4 * u * l.abs().amax(1, keepdim=True)
+    off = p * (2 * off_l + 2 * (V / 128 + 160) * u) + 2.0 ** -16 * dl.abs() + (2.0 ** -38 if dtype == torch.float16 else 0.0)
+    least = torch.finfo(dtype).smallest_normal * h
+    dx, off_x = (dl * factor) @ wd, ((off + (V + 8) * u * dl.abs()) * factor) @ wd.abs()
+    dw, off_w = (dl * factor).t() @ xd, ((off + (n + 8) * u * dl.abs()) * factor).t() @ xd.abs()
+    over_x = ((gx[kept].double() - dx).abs() / (off_x + h * (dx.abs() + off_x) + least)).max()
+    over_w = ((gw.double() - dw).abs() / (off_w + h * (dw.abs() + off_w) + least)).max()
+    assert float(over_x) <= 1 and float(over_w) <= 1, (float(over_x), float(over_w))
+    assert (gx[t < 0] == 0).all()
