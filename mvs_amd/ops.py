@@ -2219,10 +2219,11 @@ def linear_cross_entropy(x, weight, target, scale=1.0, ignore_index=-100, reduct
     loss and the gradients NaN.
     Products are summed in float32.  For more than four rows of more than 128 16-bit values the backward pass rounds each logit's
     gradient to their type before its two products (half a unit in the last place of each term, of either sign: 8192 x 128000 x 2048
-    bfloat16 gradients are 0.0020 of their norm from the exact ones, where rounding the results alone costs 0.0017); other 16-bit
-    rows keep 16 bits of it at the least, float32 operands keep 24 bits throughout (rows of at
-    most 64, and longer ones where there are more than 256, go through the matrix cores as three bfloat16 pieces: the sums are as
-    exact, an Inf among them counts as a NaN, and what is below 2^-133 is dropped).  Equal calls give equal bits.
+    bfloat16 gradients are 0.0020 of their norm from the exact ones, where rounding the results alone costs 0.0017; in x's gradient it
+    is half a unit of terms that sum to less where the table's rows have much in common); other 16-bit rows keep 16 bits of it at the
+    least, float32 operands 24 bits throughout (rows of at most 64, and longer ones where there are more than 256, go through the
+    matrix cores as three bfloat16 pieces: the sums are as exact, an Inf among them counts as a NaN, and what is below 2^-133 is
+    dropped).  Equal calls give equal bits.
     Memory besides operands and gradients, for the length of a pass.  Rows longer than 64 float32 or 128 16-bit values: forward 8 bytes
     for a row of x and 128 rows of the table, backward a piece of the logits' gradient, 2^26 values at most (float32 in pieces 2^27 of
     6 bytes; more for over 2^18 rows of x), and its transpose where the products need one.  Shorter rows: partial sums of the
